@@ -303,6 +303,70 @@ int rngd_attn_decode(const float* q, const void* kc, const void* vc, const int32
 int rngd_attn_decode_noalloc(const float* q, const void* kc, const void* vc, const int32_t* pos, int B,
                              int Bcap, int NH, int NKV, int HD, int S, float* ao, rngd_stream_t stream);
 
+/* ------------------------------------------------ paged 4-bit KV cache
+ * The reference keeps its cache in bf16 lanes of a fixed width (src/rngd_pd/engines/
+ * decode_batch.py:300-420).  These entries hold it in pages of 64 positions at 5 bits a value, so that
+ * sequences of unequal length share one pool and the beams of a search share the pages they have in
+ * common.  pool: [L][P][NKV][4][20*HD] bytes (rngd-pd_b200/csrc/kv4.cuh gives the layout of a block),
+ * layers layer_bytes apart, 16-byte aligned; HD 64 or 128.  table: int32 [B][ld_table] page ids of each
+ * sequence, page k holding positions 64k .. 64k+63; an id outside [0, P) stands for no page (nothing is
+ * stored there, nothing is seen there).  All arrays are device memory.  dtype: of k, v, q and out. */
+#define RNGD_DT_BF16 0
+#define RNGD_DT_F16 1
+#define RNGD_DT_F32 2
+/* Quantises rows [L][B][T][NKV] of K and V (HD values each, contiguous; strides of the four dimensions
+ * in elements) into positions start[b] + t, t < count[b] (NULL: T).  Magnitudes are held to 16384; a
+ * group of 32 with a NaN reads back as NaN.  Rows of one call must not fall on one position. */
+int rngd_kv4_store(void* pool, size_t layer_bytes, int P, int NKV, int HD, int L, const int32_t* table, int ld_table,
+                   const int32_t* start, const int32_t* count, int B, int T, const void* k, const int64_t* k_strides,
+                   const void* v, const int64_t* v_strides, int dtype, rngd_stream_t stream);
+/* The values that positions start[b] + t stand for -> k, v [L][B][T][NKV][HD]; zeros for t >= count[b]
+ * and where there is no page. */
+int rngd_kv4_load(const void* pool, size_t layer_bytes, int P, int NKV, int HD, int L, const int32_t* table,
+                  int ld_table, const int32_t* start, const int32_t* count, int B, int T, void* k, void* v, int dtype,
+                  rngd_stream_t stream);
+/* Attention of the last T tokens of each sequence over its pages of one layer (pool: that layer's).
+ * q, out: [B][T][NH] rows of HD contiguous values, strides of the three dimensions in elements.
+ * lens[b]: positions held, the T tokens' own among them: token t is at i = lens[b] - T + t and sees
+ * positions j <= i that lie in the window (j > i - window; 0: no window) or are sinks (j < sinks).
+ * A token that sees nothing gives zeros.  workspace: rngd_kv4_attn_workspace() bytes, 16-byte aligned,
+ * any content, not shared by calls that may overlap. */
+int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out, const int64_t* out_strides, int dtype,
+                  const void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table, const int32_t* lens,
+                  int B, int T, int NH, int window, int sinks, float scale, void* workspace, size_t workspace_bytes,
+                  rngd_stream_t stream);
+int rngd_kv4_attn_workspace(int B, int T, int NH, int NKV, int HD, int ld_table, size_t* bytes);
+/* Sequences and their pages.  ref: int32 [P] holders of each page (0: free); table: [R][ld_table]; lens: [R].
+ * Fork: row r goes on as row parents[r] (NULL: as itself; < 0: it ends and lets go of its pages).  A last
+ * page that is partly filled belongs to one row alone afterwards: the lowest row keeps it if none but
+ * these rows hold it, the others get a copy (all L layers, the filled blocks).  Then each row gets pages
+ * for `room` more positions.  Free pages are given lowest first, in the order of rows.  The new state
+ * goes to new_ref / new_table / new_lens (other buffers); the pool changes in pages that were free or
+ * were let go.  *short_out: pages that could not be given (-1 in the table).  R <= 1024. */
+int rngd_kv4_fork(void* pool, size_t layer_bytes, int L, int P, int NKV, int HD, const int32_t* ref,
+                  const int32_t* table, int ld_table, const int32_t* lens, int R, const int32_t* parents, int room,
+                  int32_t* new_ref, int32_t* new_table, int32_t* new_lens, int32_t* short_out, void* workspace,
+                  size_t workspace_bytes, rngd_stream_t stream);
+int rngd_kv4_fork_workspace(int R, int ld_table, size_t* bytes);
+/* Compaction: the n pages that are held move into places 0 .. n-1 (the k-th held page from place n on
+ * into the k-th free place below n; the rest stay), with their counts and table entries.  *live: n. */
+int rngd_kv4_compact(void* pool, size_t layer_bytes, int L, int P, int NKV, int HD, const int32_t* ref,
+                     const int32_t* table, int ld_table, int R, int32_t* new_ref, int32_t* new_table, int32_t* live,
+                     void* workspace, size_t workspace_bytes, rngd_stream_t stream);
+int rngd_kv4_compact_workspace(int P, size_t* bytes);
+
+/* ------------------------------------------------------------ beam search
+ * The reference decodes greedily (greedy_tokens, src/rngd_pd/engines/decode_batch.py:162-171).  Selection
+ * of a search: rows are groups of W beams; of a group's W*V continuations the W with the largest
+ * scores[r] + log_softmax(logits[r])[v], equal ones by the lowest r*V + v (within a row by the larger
+ * logit first).  A beam that is done has one continuation, eos, at its own score.  NaN scores count as
+ * -inf.  logits: [R] rows of V, ld elements apart.  Out, best first, [R/W][W]: scores, parents (rows),
+ * tokens, done (the parent's, or token == eos; eos < 0: none).  W <= 32, W <= V. */
+int rngd_beam_select(const void* logits, int dtype, int64_t ld, int R, int V, int W, const float* scores,
+                     const uint8_t* done, int eos, float* out_scores, int32_t* parents, int32_t* tokens,
+                     uint8_t* out_done, void* workspace, size_t workspace_bytes, rngd_stream_t stream);
+int rngd_beam_workspace(int R, int V, int W, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,61 @@
+// Paged 4-bit KV cache: the layout of a block and what a code stands for.
+//
+// A page holds 64 positions of one layer: [NKV][4 blocks][20 * HD bytes], a block being 16
+// positions of one kv head.  Along the head dimension every 32 values share two fp16 numbers
+// (s, c); a 4-bit code u stands for fp16(s * (16 + u) + c).  With NG = HD / 32 a block is
+//   K codes   [16 keys][t 0..3][j 0..NG-1][4 B]        nibble e of the word: dimension 32 j + 8 t + e
+//   V codes   [2][g 0..7][8 keys][j 0..NG-1][2 B]      nibble e of the half word: dimension 32 j + 4 g + e
+//   K scales  [16 keys][NG][s, c]
+//   V scales  [2][4 key pairs][NG][s of both keys, c of both keys]
+// K words sit where lane t of a matrix fragment row reads its NG words with one load, V half words
+// where lane (g, t) reads keys 2t and 2t + 1 with one load and all rows of a fragment share a group.
+// The 16 in the value comes from the decoding: a code or-ed into the upper mantissa bits of fp16 16.0
+// is 16 + u exactly, so one fused multiply-add per pair of values finishes it, and c = fp16(min - 16 s)
+// is held to s / 64.  5 bits a value in all.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "tc.cuh"
+
+namespace rngd {
+
+constexpr int kPage = 64;    // positions of a page
+constexpr int kBlk = 16;     // positions of a block
+constexpr int kGrp = 32;     // values that share a scale
+constexpr float kKvMax = 16384.0f;  // magnitudes are held to this, so that c stays finite in fp16
+
+enum : int { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
+
+__host__ __device__ constexpr int kv4_block_bytes(int HD) { return 20 * HD; }
+__host__ __device__ constexpr size_t kv4_page_bytes(int NKV, int HD) { return (size_t)NKV * 4 * 20 * HD; }
+
+// Byte offsets inside a block of the 4-dimension unit `l` (dimensions 4l .. 4l+3) of position `key`.
+template <int HD>
+__device__ __forceinline__ int k_unit(int key, int l) {
+  constexpr int NG = HD / 32;
+  return key * (HD / 2) + ((((l & 7) >> 1) * NG + (l >> 3)) << 2) + ((l & 1) << 1);
+}
+template <int HD>
+__device__ __forceinline__ int v_unit(int key, int l) {
+  constexpr int NG = HD / 32;
+  return 8 * HD + (((key >> 3) * 8 + (l & 7)) * 8 + (key & 7)) * (2 * NG) + ((l >> 3) << 1);
+}
+template <int HD>
+__device__ __forceinline__ int k_scale(int key, int j) {  // s, c: 4 bytes
+  return 16 * HD + (key * (HD / 32) + j) * 4;
+}
+template <int HD>
+__device__ __forceinline__ int v_scale(int key, int j) {  // s at +0, c at +4
+  return 18 * HD + (((key >> 3) * 4 + ((key & 7) >> 1)) * (HD / 32) + j) * 8 + (key & 1) * 2;
+}
+
+// Four codes -> the four values they stand for.
+__device__ __forceinline__ void kv4_values(uint32_t unit, __half s, __half c, __half* out) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const __half x = __ushort_as_half((unsigned short)(0x4C00u | (((unit >> (4 * e)) & 15u) << 6)));
+    out[e] = __hfma(x, s, c);
+  }
+}
+
+}  // namespace rngd

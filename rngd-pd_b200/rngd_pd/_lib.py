@@ -128,6 +128,22 @@ _sig("rngd_attn_decode", _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.
      ctypes.c_int, ctypes.c_int, _vp, _vp, _vp)
 _sig("rngd_attn_decode_noalloc", _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
      ctypes.c_int, ctypes.c_int, _vp, _vp)
+_int, _sz = ctypes.c_int, ctypes.c_size_t
+_i64p = ctypes.POINTER(ctypes.c_int64)
+_sig("rngd_kv4_store", _vp, _sz, _int, _int, _int, _int, _vp, _int, _vp, _vp, _int, _int, _vp, _i64p, _vp, _i64p,
+     _int, _vp)
+_sig("rngd_kv4_load", _vp, _sz, _int, _int, _int, _int, _vp, _int, _vp, _vp, _int, _int, _vp, _vp, _int, _vp)
+_sig("rngd_kv4_attn", _vp, _i64p, _vp, _i64p, _int, _vp, _int, _int, _int, _vp, _int, _vp, _int, _int, _int, _int,
+     _int, ctypes.c_float, _vp, _sz, _vp)
+_sig("rngd_kv4_attn_workspace", _int, _int, _int, _int, _int, _int, _szp)
+_sig("rngd_kv4_fork", _vp, _sz, _int, _int, _int, _int, _vp, _vp, _int, _vp, _int, _vp, _int, _vp, _vp, _vp, _vp,
+     _vp, _sz, _vp)
+_sig("rngd_kv4_fork_workspace", _int, _int, _szp)
+_sig("rngd_kv4_compact", _vp, _sz, _int, _int, _int, _int, _vp, _vp, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp)
+_sig("rngd_kv4_compact_workspace", _int, _szp)
+_sig("rngd_beam_select", _vp, _int, ctypes.c_int64, _int, _int, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _sz,
+     _vp)
+_sig("rngd_beam_workspace", _int, _int, _int, _szp)
 
 
 def last_error():
@@ -178,6 +194,30 @@ def decode_attn_workspace(model, Bcap, S):
     out = ctypes.c_size_t(0)
     call("rngd_decode_attn_workspace", ctypes.byref(model), Bcap, S, ctypes.byref(out))
     return out.value
+
+
+def workspace_bytes(name, *args):
+    """Bytes that the workspace query `name` answers for these sizes."""
+    out = ctypes.c_size_t(0)
+    call(name, *args, ctypes.byref(out))
+    return out.value
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def device_of(dev):
+    """Context in which the GPU `dev` is current (nothing to do where it already is)."""
+    import torch
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def exported_symbols():

@@ -1,0 +1,48 @@
+"""Beam search's selection over beams and vocabulary.
+
+The reference decodes greedily (greedy_tokens, src/rngd_pd/engines/decode_batch.py:162-171); this is the same
+step for a search that keeps the W best continuations of each prompt.  The parents it returns are what
+rngd_pd.kv4.fork takes to reorder the sequences.
+"""
+import torch
+
+from rngd_pd import _lib
+
+MAX_BEAMS = 32
+_DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def select(logits, scores, done, beams, eos=-1):
+    """Of each group's beams x V continuations the `beams` best by scores + log_softmax(logits).
+
+    logits: [R, V] bfloat16, float16 or float32 (rows may lie apart), rows g * beams .. of group g;
+    scores: float32 [R], the beams' own; done: bool [R].  A beam that is done goes on with `eos` alone, at its own
+    score (eos < 0: none ends, and a beam that is done is lost).  Equal scores: the lowest row, then the lowest
+    token (within a row the larger logit first).  NaN counts as -inf.
+    Returns, best first, [R / beams, beams]: scores float32, parents int32 (rows), tokens int32, done bool."""
+    if logits.dim() != 2 or logits.dtype not in _DT or not logits.is_cuda:
+        raise ValueError(f"logits must be a CUDA matrix of bfloat16, float16 or float32, got {tuple(logits.shape)} "
+                         f"{logits.dtype} on {logits.device}")
+    R, V = logits.shape
+    dev = logits.device
+    if not 1 <= beams <= MAX_BEAMS or R % beams:
+        raise ValueError(f"beams={beams}: 1..{MAX_BEAMS}, and {R} rows must be whole groups")
+    if V < beams or V * beams >= 2 ** 31 or (V > 1 and logits.stride(1) != 1) or (R > 1 and logits.stride(0) < V):
+        raise ValueError(f"logits {tuple(logits.shape)} strides {logits.stride()}: rows must be contiguous, at least "
+                         f"{beams} wide and not overlap")
+    for name, t, dt in (("scores", scores, torch.float32), ("done", done, torch.bool)):
+        if t.dtype != dt or tuple(t.shape) != (R,) or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dt} [{R}] tensor on {dev}, got {tuple(t.shape)} {t.dtype}")
+    if eos >= V:
+        raise ValueError(f"eos={eos} outside the vocabulary of {V}")
+    with _lib.device_of(dev):
+        shape = (R // beams, beams)
+        out = torch.empty(shape, dtype=torch.float32, device=dev)
+        parents, tokens = torch.empty((2,) + shape, dtype=torch.int32, device=dev).unbind(0)
+        ended = torch.empty(shape, dtype=torch.bool, device=dev)
+        need = _lib.workspace_bytes("rngd_beam_workspace", R, V, beams)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.call("rngd_beam_select", logits.data_ptr(), _DT[logits.dtype], logits.stride(0), R, V, beams,
+                  scores.data_ptr(), done.data_ptr(), eos, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                  ended.data_ptr(), ws.data_ptr(), need, _lib.stream_handle())
+    return out, parents, tokens, ended

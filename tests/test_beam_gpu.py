@@ -1,0 +1,134 @@
+"""Beam selection on the GPU against a plain numpy form in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from tests import kv4_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _check(logits, scores, done, W, eos):
+    """The choice has to be the plain form's wherever 64 bits tell its candidates apart by more than fp32 may blur."""
+    from rngd_pd import beam
+    out = beam.select(logits.cuda(), scores.cuda(), done.cuda(), W, eos)
+    x = logits.double().numpy()
+    best, parent, token, ended, every = ref.select(x, scores.double().numpy(), done.numpy(), W, eos)
+    got = [t.cpu().numpy() for t in out]
+    V = x.shape[1]
+    # score = cum + (x - lse): lse to 16 roundings of 2^-23 of itself, then two roundings of the magnitudes met
+    fin = np.isfinite(x) & (np.abs(x) < 1e30)
+    big = np.abs(np.where(fin, x, 0)).max() + np.log(V) + np.abs(np.where(np.isfinite(scores.numpy()), scores.numpy(), 0)).max()
+    tol = 24 * 2.0 ** -23 * (big + 1)
+    at = (got[1] - W * np.arange(len(best))[:, None]) * V + got[2]
+    assert got[1].dtype == np.int32 and got[2].dtype == np.int32 and got[3].dtype == np.bool_
+    assert (at >= 0).all() and (at < W * V).all()
+    assert all(len(set(row)) == W for row in at.tolist())
+    picked = np.take_along_axis(every, at, 1)
+    inf = np.isinf(best)
+    assert np.array_equal(inf, np.isinf(picked)) and np.array_equal(got[0][inf], picked[inf].astype(np.float32))
+    assert np.all(np.abs(got[0][~inf] - picked[~inf]) <= tol) and np.all(np.abs(best[~inf] - picked[~inf]) <= 2 * tol)
+    srt = -np.sort(-every, axis=1)[:, :W + 1]
+    with np.errstate(invalid="ignore"):
+        gap = np.abs(np.diff(srt, axis=1))  # nan between two -inf
+    clear = np.ones(best.shape, bool)
+    close = gap <= 2 * tol
+    clear &= ~close[:, :W] if close.shape[1] >= W else ~np.pad(close, ((0, 0), (0, W - close.shape[1])))
+    clear[:, 1:] &= ~close[:, :W - 1]
+    assert np.array_equal(got[1][clear], parent[clear]) and np.array_equal(got[2][clear], token[clear])
+    assert np.array_equal(got[3], done.numpy()[got[1]] | (got[2] == eos))
+    return got, (best, parent, token, ended), clear
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("G,W,V", [(1, 1, 1), (1, 1, 7), (2, 4, 4), (3, 4, 1000), (1, 5, 32003), (2, 8, 8192),
+                                   (1, 32, 8193), (5, 3, 16385), (2, 16, 40001), (1, 32, 32)])
+def test_select_matches_the_plain_form(dt, G, W, V):
+    g = torch.Generator().manual_seed(V + W)
+    logits = (3 * torch.randn(G * W, V, generator=g)).to(DT[dt])
+    scores = -5 + 2 * torch.randn(G * W, generator=g)
+    for n_done in {0, W // 2, W}:
+        done = (torch.arange(G * W) % W) < n_done
+        _, _, clear = _check(logits, scores, done, W, V // 2)
+        if n_done == 0 and dt == "fp32" and V >= 1000:
+            assert clear.mean() > 0.9
+
+
+def test_ties_go_to_the_lowest_row_and_token():
+    from rngd_pd import beam
+    G, W, V = 2, 4, 20000
+    logits = torch.zeros(G * W, V)
+    logits[:, 700] = 2.0
+    logits[:, 19999] = 2.0
+    out = beam.select(logits.cuda(), torch.zeros(G * W).cuda(), torch.zeros(G * W, dtype=torch.bool).cuda(), W)
+    assert out[1].tolist() == [[0, 0, 1, 1], [4, 4, 5, 5]] and out[2].tolist() == [[700, 19999] * 2] * 2
+    logits[:] = -1.0
+    out = beam.select(logits.cuda(), torch.zeros(G * W).cuda(), torch.zeros(G * W, dtype=torch.bool).cuda(), W)
+    assert out[1].tolist() == [[0] * 4, [4] * 4] and out[2].tolist() == [[0, 1, 2, 3]] * 2
+
+
+def test_first_step_from_one_live_beam():
+    """Beams at -inf have no continuation while others have any."""
+    g = torch.Generator().manual_seed(3)
+    logits = torch.randn(8, 500, generator=g)
+    scores = torch.tensor([0.0, -np.inf, -np.inf, -np.inf] * 2)
+    got, want, _ = _check(logits, scores, torch.zeros(8, dtype=torch.bool), 4, -1)
+    assert got[1].tolist() == [[0] * 4, [4] * 4]
+
+
+def test_masked_infinite_and_nan_logits():
+    g = torch.Generator().manual_seed(4)
+    logits = torch.randn(12, 9000, generator=g)
+    scores = torch.randn(12, generator=g)
+    logits[0] = -np.inf                  # a row without continuation
+    logits[1, 5] = np.nan                # a row that is lost
+    logits[2, 7] = np.inf                # another
+    logits[3, 100:] = -np.inf
+    logits[4:8] = -np.inf                # a whole group without continuation: the lowest places
+    logits[9, ::2] = torch.finfo(torch.float32).min
+    logits[10] = torch.finfo(torch.float32).min
+    got, want, _ = _check(logits, scores, torch.zeros(12, dtype=torch.bool), 4, 3)
+    assert np.isinf(got[0][1]).all() and got[2][1].tolist() == [0, 1, 2, 3] and got[1][1].tolist() == [4] * 4
+    assert (got[1][0] == 3).all()
+    # done beams whose own score is -inf, or without an eos, are lost too
+    done = torch.ones(12, dtype=torch.bool)
+    got, want, _ = _check(logits, torch.full((12,), -np.inf), done, 4, 3)
+    assert got[2].tolist() == [[0, 1, 2, 3]] * 3
+    got, want, _ = _check(logits, scores, done, 4, -1)
+    assert got[2].tolist() == [[0, 1, 2, 3]] * 3
+
+
+def test_done_beams_keep_their_score():
+    logits = torch.zeros(4, 1000)
+    scores = torch.tensor([-3.0, -1.0, -50.0, -2.0])
+    done = torch.tensor([True, False, True, True])
+    got, want, _ = _check(logits, scores, done, 4, 17)
+    assert got[0][0, :2].tolist() == [-2.0, -3.0] and got[1][0, :2].tolist() == [3, 0]
+    assert got[2][0, :2].tolist() == [17, 17] and got[3][0, :2].all()
+
+
+def test_rows_apart_and_odd_addresses():
+    from rngd_pd import beam
+    g = torch.Generator().manual_seed(5)
+    for dt in DT.values():
+        big = torch.randn(6, 5003, generator=g).to(dt).cuda()
+        view = big[:, 1:4999]
+        scores, done = torch.randn(6, generator=g).cuda(), torch.zeros(6, dtype=torch.bool, device="cuda")
+        a = beam.select(view, scores, done, 3, 5)
+        b = beam.select(view.contiguous(), scores, done, 3, 5)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_select_refusals():
+    from rngd_pd import beam
+    x, s, d = torch.zeros(4, 100, device="cuda"), torch.zeros(4, device="cuda"), torch.zeros(4, dtype=torch.bool, device="cuda")
+    for f in (lambda: beam.select(x.cpu(), s, d, 2), lambda: beam.select(x, s, d, 3), lambda: beam.select(x, s, d, 0),
+              lambda: beam.select(x.double(), s, d, 2), lambda: beam.select(x[:, :1], s, d, 2),
+              lambda: beam.select(x.t(), s, d, 2), lambda: beam.select(x, s.double(), d, 2),
+              lambda: beam.select(x, s, d.int(), 2), lambda: beam.select(x, s[:2], d, 2),
+              lambda: beam.select(x, s, d, 2, 100), lambda: beam.select(x[:1].expand(4, 100), s, d, 2)):
+        with pytest.raises(ValueError):
+            f()
+    assert beam.select(x[:0], s[:0], d[:0], 2)[0].shape == (0, 2)
