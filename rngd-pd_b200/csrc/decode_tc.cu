@@ -1158,10 +1158,11 @@ int rngd::read_status_decode(int* st, int reset) {
 
 extern "C" int rngd_device_status(int* status, int reset) {
   RNGD_REQUIRE(status != nullptr, "device_status: null output");
-  int st = 0, sp = 0, sa = 0;
+  int st = 0, sp = 0, sa = 0, s4 = 0;
   RNGD_TRY(read_status_decode(&st, reset));
   RNGD_TRY(read_status_prefill(&sp, reset));
   RNGD_TRY(read_status_attn(&sa, reset));
-  *status = st != 0 ? st : (sp != 0 ? sp : sa);
+  RNGD_TRY(read_status_kv4(&s4, reset));
+  *status = st != 0 ? st : (sp != 0 ? sp : (sa != 0 ? sa : s4));
   return RNGD_OK;
 }

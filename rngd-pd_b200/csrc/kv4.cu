@@ -1,17 +1,10 @@
-// Paged 4-bit KV cache (layout in kv4.cuh): storing rows into pages, reading them back, and the
-// attention of a few query tokens over the pages of each stream.
+// Paged 4-bit KV cache (layout in kv4.cuh): storing rows into pages and reading them back.
 //
 // The reference keeps its cache in bf16 lanes of a fixed width (src/rngd_pd/engines/decode_batch.py:
 // 300-420); this cache holds the same rows in pages, at 5 bits a value.
 #include "kv4.cuh"
 
 namespace rngd {
-
-__device__ __forceinline__ float load1(const void* p, size_t i, int dt) {
-  if (dt == DT_F32) return ((const float*)p)[i];
-  if (dt == DT_BF16) return bf2f(((const uint16_t*)p)[i]);
-  return __half2float(((const __half*)p)[i]);
-}
 
 // min and max that keep a NaN
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -138,16 +131,6 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(StoreArgs a) {
   }
 }
 
-__device__ __forceinline__ void store1(void* p, size_t i, int dt, float v) {
-  if (dt == DT_F32) {
-    ((float*)p)[i] = v;
-  } else if (dt == DT_BF16) {
-    ((uint16_t*)p)[i] = f2bf_bits(v);
-  } else {
-    ((__half*)p)[i] = __float2half_rn(v);
-  }
-}
-
 // The inverse: rows of positions -> values [L][B][T][NKV][HD], zeros where nothing is stored.
 template <int HD>
 __global__ void __launch_bounds__(256) kv4_load_kernel(StoreArgs a, void* ko, void* vo) {
@@ -170,90 +153,6 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(StoreArgs a, void* ko, vo
 #pragma unroll
     for (int e = 0; e < 4; e++) store1(w ? vo : ko, (size_t)r * HD + 4 * l + e, a.dt, __half2float(o[e]));
   }
-}
-
-struct AttnArgs {
-  const void* q;
-  void* out;
-  long qs[3], os[3];  // strides in elements: stream, token, head
-  int dt, B, T, NH, NKV, P, ld_table, window, sinks;
-  const uint8_t* pool;
-  const int32_t* table;
-  const int32_t* lens;
-  float scale;
-};
-
-// One CTA per (stream, token, query head): the warps take positions in turn, each with its own
-// running maximum and sum, joined at the end.
-template <int HD>
-__global__ void __launch_bounds__(128) kv4_attn_kernel(AttnArgs a) {
-  constexpr int LPR = HD / 4, SUB = 32 / LPR, NW = 4;
-  __shared__ float sm[NW * SUB][2];
-  __shared__ float so[NW * SUB][HD];
-  const int h = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
-  const int w = threadIdx.x / 32, l = threadIdx.x % LPR, sub = threadIdx.x % 32 / LPR;
-  const int kvh = h / (a.NH / a.NKV);
-  const int i = a.lens[b] - a.T + t;
-  float q[4];
-#pragma unroll
-  for (int e = 0; e < 4; e++)
-    q[e] = load1(a.q, (size_t)(b * a.qs[0] + t * a.qs[1] + h * a.qs[2]) + 4 * l + e, a.dt) * a.scale;
-  float m = -INFINITY, z = 0.0f, o[4] = {};
-  for (int j0 = 0; j0 <= i; j0 += NW * SUB) {
-    const int j = j0 + w * SUB + sub;
-    bool seen = j <= i && (a.window == 0 || j > i - a.window || j < a.sinks) && j / kPage < a.ld_table;
-    int page = -1;
-    if (seen) page = a.table[(size_t)b * a.ld_table + j / kPage];
-    seen = seen && page >= 0 && page < a.P;
-    const uint8_t* blk = a.pool + (((size_t)max(page, 0) * a.NKV + kvh) * 4 + ((j & 63) >> 4)) * kv4_block_bytes(HD);
-    const int key = j & 15;
-    __half x[4] = {};
-    float s = 0.0f;
-    if (seen) {
-      const __half* d = (const __half*)(blk + k_scale<HD>(key, l >> 3));
-      kv4_values(*(const uint16_t*)(blk + k_unit<HD>(key, l)), d[0], d[1], x);
-#pragma unroll
-      for (int e = 0; e < 4; e++) s = fmaf(q[e], __half2float(x[e]), s);
-    }
-#pragma unroll
-    for (int k = 1; k < LPR; k <<= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    if (seen) {
-      const __half* d = (const __half*)(blk + v_scale<HD>(key, l >> 3));
-      kv4_values(*(const uint16_t*)(blk + v_unit<HD>(key, l)), d[0], d[2], x);
-      const float mn = fmaxf(m, s);
-      const float f = m == mn ? 1.0f : expf(m - mn), p = s == mn ? 1.0f : expf(s - mn);
-      z = fmaf(z, f, p);
-#pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = fmaf(o[e], f, p * __half2float(x[e]));
-      m = mn;
-    }
-  }
-  if (l == 0) {
-    sm[w * SUB + sub][0] = m;
-    sm[w * SUB + sub][1] = z;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; e++) so[w * SUB + sub][4 * l + e] = o[e];
-  __syncthreads();
-  if (threadIdx.x < HD) {
-    float M = -INFINITY, Z = 0.0f, O = 0.0f;
-    for (int k = 0; k < NW * SUB; k++) M = fmaxf(M, sm[k][0]);
-    for (int k = 0; k < NW * SUB; k++) {
-      if (sm[k][1] == 0.0f) continue;
-      const float f = sm[k][0] == M ? 1.0f : expf(sm[k][0] - M);
-      Z = fmaf(sm[k][1], f, Z);
-      O = fmaf(so[k][threadIdx.x], f, O);
-    }
-    store1(a.out, (size_t)(b * a.os[0] + t * a.os[1] + h * a.os[2]) + threadIdx.x, a.dt, Z == 0.0f ? 0.0f : O / Z);
-  }
-}
-
-static int check_pool(const char* what, const void* pool, size_t layer_bytes, int P, int NKV, int HD) {
-  RNGD_REQUIRE(pool != nullptr && ((uintptr_t)pool & 15) == 0 && (layer_bytes & 15) == 0,
-               "%s: the pool must be 16-byte aligned", what);
-  RNGD_REQUIRE(HD == 64 || HD == 128, "%s: built for HD 64 and 128, not %d", what, HD);
-  RNGD_REQUIRE(P >= 1 && NKV >= 1 && NKV <= 1024, "%s: P=%d NKV=%d", what, P, NKV);
-  return RNGD_OK;
 }
 
 static int store_args(const char* what, StoreArgs* a, void* pool, size_t layer_bytes, int P, int NKV, int HD, int L,
@@ -323,51 +222,4 @@ extern "C" int rngd_kv4_load(const void* pool, size_t layer_bytes, int P, int NK
   else
     kv4_load_kernel<64><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a, k, v);
   return check_launch("kv4_load_kernel");
-}
-
-extern "C" int rngd_kv4_attn_workspace(int B, int T, int NH, int NKV, int HD, int ld_table, size_t* bytes) {
-  RNGD_REQUIRE(bytes && B >= 0 && T >= 0 && NH >= 1 && NKV >= 1 && ld_table >= 0, "kv4_attn_workspace: bad argument");
-  *bytes = 0;
-  (void)HD;
-  return RNGD_OK;
-}
-
-extern "C" int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out, const int64_t* out_strides, int dtype,
-                             const void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table,
-                             const int32_t* lens, int B, int T, int NH, int window, int sinks, float scale,
-                             void* workspace, size_t workspace_bytes, rngd_stream_t stream) {
-  RNGD_TRY(check_pool("kv4_attn", pool, 0, P, NKV, HD));
-  RNGD_REQUIRE(dtype >= DT_BF16 && dtype <= DT_F32, "kv4_attn: data type %d", dtype);
-  RNGD_REQUIRE(B >= 0 && T >= 0 && NH >= 1 && NH % NKV == 0 && ld_table >= 0,
-               "kv4_attn: B=%d T=%d NH=%d must be a multiple of NKV=%d, table width %d", B, T, NH, NKV, ld_table);
-  RNGD_REQUIRE(window >= 0 && sinks >= 0, "kv4_attn: window=%d sinks=%d", window, sinks);
-  if (B == 0 || T == 0) return RNGD_OK;
-  RNGD_REQUIRE(q && out && q_strides && out_strides && lens && (table || ld_table == 0), "kv4_attn: null pointer");
-  AttnArgs a = {};
-  a.q = q;
-  a.out = out;
-  for (int i = 0; i < 3; i++) {
-    a.qs[i] = (long)q_strides[i];
-    a.os[i] = (long)out_strides[i];
-  }
-  a.dt = dtype;
-  a.B = B;
-  a.T = T;
-  a.NH = NH;
-  a.NKV = NKV;
-  a.P = P;
-  a.ld_table = ld_table;
-  a.window = window;
-  a.sinks = sinks;
-  a.pool = (const uint8_t*)pool;
-  a.table = table;
-  a.lens = lens;
-  a.scale = scale;
-  (void)workspace;
-  (void)workspace_bytes;
-  if (HD == 128)
-    kv4_attn_kernel<128><<<dim3(NH, T, B), 128, 0, (cudaStream_t)stream>>>(a);
-  else
-    kv4_attn_kernel<64><<<dim3(NH, T, B), 128, 0, (cudaStream_t)stream>>>(a);
-  return check_launch("kv4_attn_kernel");
 }

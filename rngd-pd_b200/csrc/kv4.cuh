@@ -58,4 +58,28 @@ __device__ __forceinline__ void kv4_values(uint32_t unit, __half s, __half c, __
   }
 }
 
+__device__ __forceinline__ float load1(const void* p, size_t i, int dt) {
+  if (dt == DT_F32) return ((const float*)p)[i];
+  if (dt == DT_BF16) return bf2f(((const uint16_t*)p)[i]);
+  return __half2float(((const __half*)p)[i]);
+}
+
+__device__ __forceinline__ void store1(void* p, size_t i, int dt, float v) {
+  if (dt == DT_F32) {
+    ((float*)p)[i] = v;
+  } else if (dt == DT_BF16) {
+    ((uint16_t*)p)[i] = f2bf_bits(v);
+  } else {
+    ((__half*)p)[i] = __float2half_rn(v);
+  }
+}
+
+static inline int check_pool(const char* what, const void* pool, size_t layer_bytes, int P, int NKV, int HD) {
+  RNGD_REQUIRE(pool != nullptr && ((uintptr_t)pool & 15) == 0 && (layer_bytes & 15) == 0,
+               "%s: the pool must be 16-byte aligned", what);
+  RNGD_REQUIRE(HD == 64 || HD == 128, "%s: built for HD 64 and 128, not %d", what, HD);
+  RNGD_REQUIRE(P >= 1 && NKV >= 1 && NKV <= 1024, "%s: P=%d NKV=%d", what, P, NKV);
+  return RNGD_OK;
+}
+
 }  // namespace rngd

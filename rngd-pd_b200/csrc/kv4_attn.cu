@@ -1,0 +1,775 @@
+// Attention of a few query tokens over the paged 4-bit KV cache (layout in kv4.cuh).
+//
+// The reference attends over bf16 lanes (src/rngd_pd/kernels/decode_batch.py:73-91); the cache read here
+// takes 5 bits a value, and positions may be limited to a window and a few first ones (sinks).
+#include "kv4.cuh"
+
+namespace rngd {
+
+// ------------------------------------------------------------------------------------ attention
+// o = softmax(scale q K^T) V over the pages of each stream, on the warp-level tensor cores.
+//
+// Work is cut into units of 32 positions of a (stream, kv head, row tile), laid end to end, and every
+// warp (a CTA of its own) takes an equal contiguous run of them, whatever the lengths: a long stream is
+// split over many warps, many short streams share one.  A segment (all units of one (stream, kv head,
+// row tile)) that one warp holds whole is written at once; a cut one leaves its pieces as records
+// (maximum, sum, unnormalised output), which a second kernel joins in the order of the positions.
+//
+// Units arrive by bulk copy (a unit is one contiguous run of 2 blocks) in a ring of stages.  The lane
+// whose turn it is looks its unit up 32 units ahead (stream by search in the prefix sums, page id) and
+// issues the copy itself.
+//
+// A block's codes go straight from shared memory into matrix fragments: or-ing a code into the upper
+// mantissa bits of fp16 16.0 gives 16 + u, and one fused multiply-add per pair of values by the group's
+// (s, c) gives the value, exactly as it is defined.  S = K q^T has the keys as its 16 rows and 8 columns
+// for the query rows that share the kv head; O^T = V^T P has 16 dimensions as its rows.  q enters as
+// fp16 scaled by a power of two (exact for 16-bit q), fp32 q as fp16 hi + lo, and P as hi + lo, so that
+// the result keeps fp32 accuracy.  With up to 4 rows the lo halves take the columns that would stay
+// empty (COLS: hi in columns 0..3, lo in 4..7, one matrix instruction for both); with more they are
+// products of their own into the same accumulators.  Probabilities are held as 2^(x - m + 8), x the
+// score in units of log 2 and m a running maximum that is only moved when a score exceeds it by 6:
+// fp16 then holds them to 2^-35 of the largest, and the output is rescaled rarely.
+constexpr int kUnit = 32;
+constexpr int kAttnStreams = 1024;  // streams of one launch
+constexpr float kPBias = 8.0f, kPMax = 14.0f;
+
+__device__ int g_status_kv4 = 0;
+
+struct AttnArgs {
+  const void* q;
+  void* out;
+  long qs[3], os[3];  // strides in elements: stream, token, head
+  int dt, qvec, B, T, NH, NKV, G, RT, P, ld_table, window, sinks;
+  const uint8_t* pool;
+  const int32_t* table;
+  const int32_t* lens;
+  float scale;
+  int* pre;     // [B + 1] prefix sums of units, for the joining kernel
+  float* rec;   // [warps][2][rows][HD + 2]
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+               "{%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+
+// The four pairs (nibble i of the low half, nibble i of the high half) of w -> values.
+__device__ __forceinline__ void decode_word(uint32_t w, __half2 s, __half2 c, uint32_t (&v)[4]) {
+  v[0] = h2u(__hfma2(u2h(((w << 6) & 0x03C003C0u) | 0x4C004C00u), s, c));
+  v[1] = h2u(__hfma2(u2h(((w << 2) & 0x03C003C0u) | 0x4C004C00u), s, c));
+  v[2] = h2u(__hfma2(u2h(((w >> 2) & 0x03C003C0u) | 0x4C004C00u), s, c));
+  v[3] = h2u(__hfma2(u2h(((w >> 6) & 0x03C003C0u) | 0x4C004C00u), s, c));
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// What a stream of n positions has to look at: units [0, su) hold sinks before the window, units
+// [start, end) the window.
+struct Span {
+  int su, start, end;
+  __device__ __forceinline__ int units() const { return su + end - start; }
+  __device__ __forceinline__ int at(int x) const { return x < su ? x : start + x - su; }
+};
+__device__ __forceinline__ Span span_of(int n, const AttnArgs& a) {
+  Span s;
+  const int held = min(max(n, 0), a.ld_table * kPage);
+  const int low = a.window > 0 ? max(0, max(n - a.T, 0) - a.window + 1) : 0;
+  s.end = (held + kUnit - 1) / kUnit;
+  s.su = min((min(a.sinks, low) + kUnit - 1) / kUnit, s.end);
+  s.start = min(max(low / kUnit, s.su), s.end);
+  return s;
+}
+
+// Prefix sums over the streams of one launch, by one warp: pre[b] = units before stream b.
+__device__ __forceinline__ void prefix_units(const AttnArgs& a, int* lens, int* pre) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int b = b0 + lane;
+    const int n = b < a.B ? a.lens[b] : 0;
+    int x = b < a.B ? span_of(n, a).units() * a.NKV * a.RT : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (b < a.B) {
+      lens[b] = n;
+      pre[b + 1] = base + x;
+    }
+    base += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) pre[0] = 0;
+  __syncwarp();
+}
+
+// One unit, as its lane looked it up.
+struct Unit {
+  int seg;    // (stream * NKV + kv head) * RT + row tile
+  int pos;    // first position | blocks to read (0..2) | 4: every row sees every position
+  size_t off; // of its first block in the pool
+};
+
+template <int HD>
+__device__ __forceinline__ Unit look_up(int x, const AttnArgs& a, const int* lens, const int* pre) {
+  int lo = 0, hi = a.B - 1;  // pre[lo] <= x < pre[hi + 1]
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  const int b = lo, n = lens[b], per = a.NKV * a.RT;
+  const Span s = span_of(n, a);
+  const int ub = s.units(), rem = x - pre[b], sg = rem / ub;
+  const int p0 = s.at(rem - sg * ub) * kUnit;
+  const int held = min(n, a.ld_table * kPage);
+  const int page = a.table[(size_t)b * a.ld_table + p0 / kPage];
+  int blocks = page >= 0 && page < a.P ? min(2, (held - p0 + kBlk - 1) / kBlk) : 0;
+  const bool all = p0 + kUnit <= held && p0 + kUnit - 1 <= n - a.T &&
+                   (a.window == 0 || p0 > n - 1 - a.window || p0 + kUnit <= a.sinks);
+  Unit u;
+  u.seg = b * per + sg;
+  u.pos = p0 | blocks | (all ? 4 : 0);
+  u.off = (((size_t)max(page, 0) * a.NKV + sg / a.RT) * 4 + ((p0 & (kPage - 1)) >> 4)) * kv4_block_bytes(HD);
+  return u;
+}
+
+// Eight consecutive elements of q as fp32.
+__device__ __forceinline__ void load_q8(const AttnArgs& a, size_t at, float* x) {
+  if (!a.qvec) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = load1(a.q, at + e, a.dt);
+  } else if (a.dt == DT_F32) {
+    const float4 u = __ldg((const float4*)((const float*)a.q + at)), v = __ldg((const float4*)((const float*)a.q + at) + 1);
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+  } else {
+    const uint4 u = __ldg((const uint4*)((const uint16_t*)a.q + at));
+    if (a.dt == DT_BF16) {
+      unpack8(u, x);
+    } else {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float2 f = __half22float2(u2h(w[e]));
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+      }
+    }
+  }
+}
+
+// How the halves of q and P are laid out: see above.  Q16 and Q32 differ in whether q has a lo half.
+enum : int { COLS = 0, Q16 = 1, Q32 = 2 };
+
+// One warp's state for a segment.  NT tiles of 8 columns; a column is a query row, or with COLS the hi
+// (columns 0..3) or lo (4..7) half of one.  Lane = 4 g + t as in the fragments.
+template <int HD, int NT, int MODE>
+struct Rows {
+  static constexpr int NG = HD / 32;
+  static constexpr bool SPLIT = MODE == COLS;
+  static constexpr int CPT = SPLIT ? 4 : 8;  // rows of a column tile
+  static constexpr int QL = MODE == Q32 ? NT : 1;
+  uint32_t qf[NT][NG][4], ql[QL][NG][4];
+  float o[NT][NG][2][4];
+  float f[NT][2], mb[NT][2], l[NT][2];  // of columns 2t, 2t + 1 (rows 2 (t & 1), + 1 with SPLIT)
+  int i[NT][2];                         // their positions, -1: none
+
+  __device__ __forceinline__ void begin(const AttnArgs& a, int seg, int n) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV;
+    const int R = a.T * a.G;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int r = (rt * NT + nt) * CPT + (SPLIT ? g & 3 : g);
+      float x[NG][8];
+      float mx = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        if (r < R) {
+          load_q8(a, (size_t)(b * a.qs[0] + r / a.G * a.qs[1] + (kvh * a.G + r % a.G) * a.qs[2]) + 32 * j + 8 * t, x[j]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[j][e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[j][e]));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // scale by the power of two that brings the largest into [2^10, 2^11)
+      const int ex = min(max((int)(__float_as_uint(mx) >> 23), 40), 254);
+      const float up = __uint_as_float((uint32_t)(264 - ex) << 23);
+      const float fc = a.scale * 1.4426950408889634f * (1.0f / up);
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+          const float x0 = x[j][p] * up, x1 = x[j][p + 4] * up;
+          const uint32_t hi = pack_h2(x0, x1);
+          qf[nt][j][p] = hi;
+          if constexpr (MODE != Q16) {
+            const float2 hf = __half22float2(u2h(hi));
+            const uint32_t lo = pack_h2(x0 - hf.x, x1 - hf.y);
+            if constexpr (SPLIT) {
+              if (g >= 4) qf[nt][j][p] = lo;
+            } else {
+              ql[nt][j][p] = lo;
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[nt][j][e][k] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int col = (SPLIT ? 2 * (t & 1) : 2 * t) + e;
+        f[nt][e] = __shfl_sync(0xffffffffu, fc, 4 * col);
+        const int rr = (rt * NT + nt) * CPT + col;
+        i[nt][e] = rr < R ? n - a.T + rr / a.G : -1;
+        mb[nt][e] = 1e30f;
+        l[nt][e] = 0.0f;
+      }
+    }
+  }
+
+  // A block of 16 positions from p0 on; EDGE: some rows do not see some of them, and what lies past the
+  // stream's end may be anything.
+  template <bool EDGE>
+  __device__ __forceinline__ void block(const uint8_t* blk, int p0, int held, const AttnArgs& a) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float c[NT][4] = {};
+    {
+      uint32_t w0[NG], w1[NG], s0[NG], s1[NG];
+      if constexpr (NG == 4) {
+        const uint4 x = *(const uint4*)(blk + g * 64 + t * 16), y = *(const uint4*)(blk + (g + 8) * 64 + t * 16);
+        w0[0] = x.x; w0[1] = x.y; w0[2] = x.z; w0[3] = x.w;
+        w1[0] = y.x; w1[1] = y.y; w1[2] = y.z; w1[3] = y.w;
+        const uint4 u = *(const uint4*)(blk + 16 * HD + g * 16), v = *(const uint4*)(blk + 16 * HD + (g + 8) * 16);
+        s0[0] = u.x; s0[1] = u.y; s0[2] = u.z; s0[3] = u.w;
+        s1[0] = v.x; s1[1] = v.y; s1[2] = v.z; s1[3] = v.w;
+      } else {
+        const uint2 x = *(const uint2*)(blk + g * 32 + t * 8), y = *(const uint2*)(blk + (g + 8) * 32 + t * 8);
+        w0[0] = x.x; w0[1] = x.y;
+        w1[0] = y.x; w1[1] = y.y;
+        const uint2 u = *(const uint2*)(blk + 16 * HD + g * 8), v = *(const uint2*)(blk + 16 * HD + (g + 8) * 8);
+        s0[0] = u.x; s0[1] = u.y;
+        s1[0] = v.x; s1[1] = v.y;
+      }
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        uint32_t x[4], y[4];
+        decode_word(w0[j], __low2half2(u2h(s0[j])), __high2half2(u2h(s0[j])), x);
+        decode_word(w1[j], __low2half2(u2h(s1[j])), __high2half2(u2h(s1[j])), y);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          mma_f16(c[nt], x[0], y[0], x[1], y[1], qf[nt][j][0], qf[nt][j][1]);
+          mma_f16(c[nt], x[2], y[2], x[3], y[3], qf[nt][j][2], qf[nt][j][3]);
+          if constexpr (MODE == Q32) {
+            mma_f16(c[nt], x[0], y[0], x[1], y[1], ql[nt][j][0], ql[nt][j][1]);
+            mma_f16(c[nt], x[2], y[2], x[3], y[3], ql[nt][j][2], ql[nt][j][3]);
+          }
+        }
+      }
+    }
+    // V's scales of keys 2t, 2t + 1 (h = 0) and 2t + 8, 2t + 9 (h = 1)
+    uint32_t vs[2][NG], vc[2][NG];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint8_t* sp = blk + 18 * HD + (h * 4 + t) * NG * 8;
+#pragma unroll
+      for (int j = 0; j < NG; j += 2) {
+        const uint4 x = *(const uint4*)(sp + j * 8);
+        vs[h][j] = x.x; vc[h][j] = x.y; vs[h][j + 1] = x.z; vc[h][j + 1] = x.w;
+      }
+    }
+    uint32_t bad = 0;  // keys whose V holds a NaN
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        bool n0 = false, n1 = false;
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+          n0 |= (vs[h][j] & 0x7FFFu) > 0x7C00u;
+          n1 |= (vs[h][j] >> 16 & 0x7FFFu) > 0x7C00u;
+        }
+        const int k0 = p0 + 8 * h + 2 * t;
+        const bool z0 = n0 || k0 >= held, z1 = n1 || k0 + 1 >= held;
+        const uint32_t keep = (z0 ? 0u : 0xFFFFu) | (z1 ? 0u : 0xFFFF0000u);
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+          vs[h][j] &= keep;
+          vc[h][j] &= keep;
+        }
+        const uint32_t b0 = __ballot_sync(0xffffffffu, n0) & 15u, b1 = __ballot_sync(0xffffffffu, n1) & 15u;
+#pragma unroll
+        for (int k = 0; k < 4; k++) bad |= (b0 >> k & 1u) << (8 * h + 2 * k) | (b1 >> k & 1u) << (8 * h + 2 * k + 1);
+      }
+    }
+    uint32_t pb[NT][2], pl[SPLIT ? 1 : NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      // scores of this lane: keys kk[], columns e
+      constexpr int NK = SPLIT ? 1 : 2;
+      float x[NK][2];
+      int kk[NK];
+      if constexpr (SPLIT) {  // t < 2: key g, else key g + 8
+        const float r0 = __shfl_xor_sync(0xffffffffu, t < 2 ? c[nt][2] : c[nt][0], 2);
+        const float r1 = __shfl_xor_sync(0xffffffffu, t < 2 ? c[nt][3] : c[nt][1], 2);
+        x[0][0] = (t < 2 ? c[nt][0] : c[nt][2]) + r0;
+        x[0][1] = (t < 2 ? c[nt][1] : c[nt][3]) + r1;
+        kk[0] = t < 2 ? g : g + 8;
+      } else {
+        x[0][0] = c[nt][0];
+        x[0][1] = c[nt][1];
+        x[1][0] = c[nt][2];
+        x[1][1] = c[nt][3];
+        kk[0] = g;
+        kk[1] = g + 8;
+      }
+#pragma unroll
+      for (int k = 0; k < NK; k++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) x[k][e] *= f[nt][e];
+      if constexpr (EDGE) {
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int j = p0 + kk[k];
+            const bool seen = j <= i[nt][e] && j < held && (a.window == 0 || j > i[nt][e] - a.window || j < a.sinks);
+            if (bad >> kk[k] & 1u) x[k][e] = __uint_as_float(0x7FFFFFFFu);
+            if (!seen) x[k][e] = -INFINITY;
+          }
+      }
+      float y[NK][2];
+      bool over = false;
+#pragma unroll
+      for (int k = 0; k < NK; k++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          y[k][e] = x[k][e] + mb[nt][e];
+          over |= y[k][e] > kPMax;
+        }
+      if (__any_sync(0xffffffffu, over)) {  // move the maxima
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float m = x[0][e];
+          if constexpr (NK == 2) m = fmaxf(m, x[NK - 1][e]);
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+          if constexpr (SPLIT) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const float nb = fminf(mb[nt][e], kPBias - m);
+          const float al = ex2(nb - mb[nt][e]);
+          mb[nt][e] = nb;
+          l[nt][e] *= al;
+#pragma unroll
+          for (int j = 0; j < NG; j++)
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+              o[nt][j][q][e] *= al;
+              o[nt][j][q][e + 2] *= al;
+            }
+#pragma unroll
+          for (int k = 0; k < NK; k++) y[k][e] = x[k][e] + nb;
+        }
+      }
+      float p[NK][2];
+#pragma unroll
+      for (int k = 0; k < NK; k++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          p[k][e] = ex2(y[k][e]);
+          l[nt][e] += p[k][e];
+        }
+      if constexpr (SPLIT) {
+        const uint32_t hi = pack_h2(p[0][0], p[0][1]);
+        const float2 hf = __half22float2(u2h(hi));
+        const uint32_t lo = pack_h2(p[0][0] - hf.x, p[0][1] - hf.y);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, t < 2 ? lo : hi, 2);
+        pb[nt][0] = movmatrix(t < 2 ? hi : other);
+        pb[nt][1] = movmatrix(t < 2 ? other : lo);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const uint32_t hi = pack_h2(p[k][0], p[k][1]);
+          const float2 hf = __half22float2(u2h(hi));
+          pb[nt][k] = movmatrix(hi);
+          pl[nt][k] = movmatrix(pack_h2(p[k][0] - hf.x, p[k][1] - hf.y));
+        }
+      }
+    }
+    // O^T += V^T P
+    {
+      uint32_t wa[2][NG / 2], wb[2][NG / 2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if constexpr (NG == 4) {
+          const uint4 x = *(const uint4*)(blk + 8 * HD + h * 512 + g * 64 + t * 16);
+          wa[h][0] = x.x; wa[h][1] = x.y; wb[h][0] = x.z; wb[h][1] = x.w;
+        } else {
+          const uint2 x = *(const uint2*)(blk + 8 * HD + h * 256 + g * 32 + t * 8);
+          wa[h][0] = x.x; wb[h][0] = x.y;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        uint32_t x[4], y[4];
+        const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
+        decode_word(__byte_perm(wa[0][j / 2], wb[0][j / 2], sel), u2h(vs[0][j]), u2h(vc[0][j]), x);
+        decode_word(__byte_perm(wa[1][j / 2], wb[1][j / 2], sel), u2h(vs[1][j]), u2h(vc[1][j]), y);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          mma_f16(o[nt][j][0], x[0], x[1], y[0], y[1], pb[nt][0], pb[nt][1]);
+          mma_f16(o[nt][j][1], x[2], x[3], y[2], y[3], pb[nt][0], pb[nt][1]);
+          if constexpr (!SPLIT) {
+            mma_f16(o[nt][j][0], x[0], x[1], y[0], y[1], pl[nt][0], pl[nt][1]);
+            mma_f16(o[nt][j][1], x[2], x[3], y[2], y[3], pl[nt][0], pl[nt][1]);
+          }
+        }
+      }
+    }
+  }
+
+  // The segment's piece is done: to `out` (whole) or to a record.
+  __device__ __forceinline__ void end(const AttnArgs& a, int seg, bool whole, float* rec) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV;
+    const int R = a.T * a.G;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float ls = l[nt][e];
+#pragma unroll
+        for (int w = SPLIT ? 2 : 4; w < 32; w <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, w);
+        const int col = (SPLIT ? 2 * (t & 1) : 2 * t) + e;
+        const int rl = nt * CPT + col, r = rt * NT * CPT + rl;
+        const float inv = ls > 0.0f ? 1.0f / ls : (ls == 0.0f ? 0.0f : ls);
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+          float v[4] = {o[nt][j][0][e], o[nt][j][0][e + 2], o[nt][j][1][e], o[nt][j][1][e + 2]};
+          if constexpr (SPLIT) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], 2);
+          }
+          if (SPLIT && (j & 1) != (t >> 1)) continue;
+          if (whole) {
+            if (r < R) {
+              const size_t at = (size_t)(b * a.os[0] + r / a.G * a.os[1] + (kvh * a.G + r % a.G) * a.os[2]) + 32 * j + 4 * g;
+#pragma unroll
+              for (int k = 0; k < 4; k++) store1(a.out, at + k, a.dt, v[k] * inv);
+            }
+          } else {
+            *(float4*)(rec + (size_t)rl * (HD + 4) + 32 * j + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        if (!whole && g == 0 && (!SPLIT || t < 2)) {
+          rec[(size_t)rl * (HD + 4) + HD] = mb[nt][e];
+          rec[(size_t)rl * (HD + 4) + HD + 1] = ls;
+        }
+      }
+  }
+};
+
+template <int HD>
+__host__ __device__ constexpr int attn_stages() { return HD == 128 ? 3 : 5; }
+template <int HD>
+__host__ __device__ constexpr int attn_smem(int B) { return attn_stages<HD>() * 2 * kv4_block_bytes(HD) + 64 + (2 * B + 1) * 4; }
+
+template <int HD, int NT, int MODE>
+__global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 ? 16 : 12)) kv4_attn_kernel(AttnArgs a) {
+  constexpr int ST = attn_stages<HD>(), BLK = kv4_block_bytes(HD);
+  extern __shared__ __align__(128) uint8_t sm[];
+  uint64_t* bar = (uint64_t*)(sm + ST * 2 * BLK);
+  int* s_len = (int*)(bar + 8);
+  int* s_pre = s_len + a.B;
+  const int lane = threadIdx.x;
+  if (lane == 0) {
+    for (int s = 0; s < ST; s++) mbar_init(bar + s, 1);
+    fence_mbar_init();
+  }
+  prefix_units(a, s_len, s_pre);
+  if (blockIdx.x == 0)
+    for (int b = lane; b <= a.B; b += 32) a.pre[b] = s_pre[b];
+  const int N = s_pre[a.B];
+  const int W = min((int)gridDim.x, N);  // warps with work: every one of them has a unit
+  grid_dep_launch();
+  if ((int)blockIdx.x >= W) return;
+  const int x0 = (int)((long)N * blockIdx.x / W), x1 = (int)((long)N * (blockIdx.x + 1) / W);
+  Unit mine, next;  // of units (u & ~31) + lane, for the reader and for the issuer
+  mine = next = look_up<HD>(min(x0 + lane, x1 - 1), a, s_len, s_pre);
+  auto issue = [&](int k) {  // the k-th unit of this warp
+    if (lane == (k & 31)) {
+      uint64_t* b = bar + k % ST;
+      const uint32_t bytes = (next.pos & 3) * BLK;
+      mbar_arrive_expect_tx(b, bytes);
+      if (bytes) bulk_load(sm + k % ST * 2 * BLK, a.pool + next.off, bytes, b);
+    }
+  };
+  const int n = x1 - x0;
+  for (int k = 0; k < ST - 1 && k < n; k++) issue(k);
+  Rows<HD, NT, MODE> rows;
+  constexpr int RPT = NT * (MODE == COLS ? 4 : 8);
+  int seg = -1, held = 0;
+  bool ok = true;
+  float* rec = a.rec + (size_t)blockIdx.x * 2 * RPT * (HD + 4);
+  int seg0 = 0, seg1 = 0;  // the segment's units
+  auto finish = [&]() {
+    const bool whole = seg0 >= x0 && seg1 <= x1;
+    rows.end(a, seg, whole, rec + (seg0 < x0 ? 0 : (size_t)RPT * (HD + 4)));
+  };
+  int k = 0;
+  for (; k < n; k++) {
+    if ((k & 31) == 0 && k > 0) mine = next;
+    const int ahead = k + ST - 1;
+    if (ahead < n) {
+      if ((ahead & 31) == 0) next = look_up<HD>(min(x0 + ahead + lane, x1 - 1), a, s_len, s_pre);
+      issue(ahead);
+    }
+    const int sg = __shfl_sync(0xffffffffu, mine.seg, k & 31), pos = __shfl_sync(0xffffffffu, mine.pos, k & 31);
+    if (sg != seg) {
+      if (seg >= 0) finish();
+      seg = sg;
+      const int per = a.NKV * a.RT, b = seg / per, ub = (s_pre[b + 1] - s_pre[b]) / per;
+      seg0 = s_pre[b] + seg % per * ub;
+      seg1 = seg0 + ub;
+      held = min(s_len[b], a.ld_table * kPage);
+      rows.begin(a, seg, s_len[b]);
+    }
+    if (ok) ok = mbar_wait(bar + k % ST, (k / ST) & 1, ST_TMA_WAIT, &g_status_kv4);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    const int p0 = pos & ~7, blocks = pos & 3;
+    const uint8_t* st = sm + k % ST * 2 * BLK;
+    if (pos & 4) {
+      if (blocks) {
+        rows.template block<false>(st, p0, held, a);
+        rows.template block<false>(st + BLK, p0 + kBlk, held, a);
+      }
+    } else {
+      for (int i = 0; i < blocks; i++) rows.template block<true>(st + i * BLK, p0 + i * kBlk, held, a);
+    }
+    __syncwarp();
+  }
+  if (!ok) {  // give up, once the copies in flight are in (waited for with a limit too)
+    for (int i = k; i < min(k + ST, n); i++) mbar_wait(bar + i % ST, (i / ST) & 1, ST_TMA_WAIT, &g_status_kv4);
+    return;
+  }
+  finish();
+}
+
+// Joins the pieces of cut segments; one CTA per (segment, row).
+template <int HD>
+__global__ void __launch_bounds__(128) kv4_join_kernel(AttnArgs a, int grid, int rows_per_tile) {
+  __shared__ float s_m[4], s_l[4];
+  __shared__ float s_o[4][HD];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int seg = blockIdx.x, rl = blockIdx.y;
+  const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV, per = a.NKV * a.RT;
+  const int r = rt * rows_per_tile + rl;
+  if (r >= a.T * a.G) return;
+  grid_dep_wait();
+  const int p0 = a.pre[b], p1 = a.pre[b + 1], N = a.pre[a.B];
+  const int ub = (p1 - p0) / per;
+  const int seg0 = p0 + seg % per * ub, seg1 = seg0 + ub;
+  constexpr int D = HD / 32;
+  float v[D];
+#pragma unroll
+  for (int d = 0; d < D; d++) v[d] = 0.0f;
+  float inv = 0.0f;
+  if (ub > 0) {
+    const int W = min(grid, N);
+    const int w0 = owner_of(seg0, N, W), w1 = owner_of(seg1 - 1, N, W);
+    if (w0 == w1) return;  // written whole
+    auto record = [&](int x) {
+      return a.rec + ((size_t)(2 * x + (x == w0 ? 1 : 0)) * rows_per_tile + rl) * (HD + 4);
+    };
+    // mb = 8 - m: the smallest is the largest maximum
+    float mb = 1e30f;
+    for (int x = w0 + threadIdx.x; x <= w1; x += 128) mb = fminf(mb, __ldcg(record(x) + HD));
+    mb = -warp_max(-mb);
+    if (lane == 0) s_m[w] = mb;
+    __syncthreads();
+    mb = fminf(fminf(s_m[0], s_m[1]), fminf(s_m[2], s_m[3]));
+    float l = 0.0f;
+#pragma unroll 4
+    for (int x = w0 + w; x <= w1; x += 4) {
+      const float* rc = record(x);
+      const float f = ex2(mb - __ldcg(rc + HD));
+      l = fmaf(__ldcg(rc + HD + 1), f, l);
+#pragma unroll
+      for (int d = 0; d < D; d++) v[d] = fmaf(__ldcg(rc + lane + 32 * d), f, v[d]);
+    }
+    if (lane == 0) s_l[w] = l;
+#pragma unroll
+    for (int d = 0; d < D; d++) s_o[w][lane + 32 * d] = v[d];
+    __syncthreads();
+    l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+    inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    if (w != 0) return;
+#pragma unroll
+    for (int d = 0; d < D; d++)
+      v[d] = s_o[0][lane + 32 * d] + s_o[1][lane + 32 * d] + s_o[2][lane + 32 * d] + s_o[3][lane + 32 * d];
+  }
+  if (w != 0) return;
+  const size_t at = (size_t)(b * a.os[0] + r / a.G * a.os[1] + (kvh * a.G + r % a.G) * a.os[2]);
+#pragma unroll
+  for (int d = 0; d < D; d++) store1(a.out, at + lane + 32 * d, a.dt, v[d] * inv);
+}
+
+// How a call is laid out over the GPU.
+struct AttnPlan {
+  int NT, mode, RT, rows, warps;
+  size_t pre_bytes, bytes;
+};
+
+typedef void (*AttnKernel)(AttnArgs);
+template <int HD>
+static AttnKernel attn_kernel(int NT, int mode) {
+  if (mode == COLS) return kv4_attn_kernel<HD, 1, COLS>;
+  if (mode == Q16) return NT == 1 ? kv4_attn_kernel<HD, 1, Q16> : kv4_attn_kernel<HD, 2, Q16>;
+  return NT == 1 ? kv4_attn_kernel<HD, 1, Q32> : kv4_attn_kernel<HD, 2, Q32>;
+}
+
+// Warps that fit one SM at a time (registers, shared memory), remembered per kernel and size class of
+// the shared memory.
+static int attn_per_sm(int HD, int NT, int mode, int B, int* out) {
+  static std::atomic<int> known[2][2][3][kAttnStreams / 32 + 1];
+  const int cls = (B + 31) / 32;
+  std::atomic<int>& slot = known[HD == 128][NT - 1][mode][cls];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n == 0) {
+    const AttnKernel k = HD == 128 ? attn_kernel<128>(NT, mode) : attn_kernel<64>(NT, mode);
+    const int smem = HD == 128 ? attn_smem<128>(32 * cls) : attn_smem<64>(32 * cls);
+    RNGD_TRY(check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, 32, smem), "occupancy(kv4_attn_kernel)"));
+    if (n < 1) n = 1;
+    slot.store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return RNGD_OK;
+}
+
+static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, AttnPlan* p) {
+  RNGD_REQUIRE(HD == 64 || HD == 128, "kv4_attn: built for HD 64 and 128, not %d", HD);
+  RNGD_REQUIRE(dtype >= DT_BF16 && dtype <= DT_F32, "kv4_attn: data type %d", dtype);
+  RNGD_REQUIRE(B >= 0 && T >= 0 && NKV >= 1 && NH >= 1 && NH % NKV == 0 && ld_table >= 0,
+               "kv4_attn: B=%d T=%d NH=%d must be a multiple of NKV=%d, table width %d", B, T, NH, NKV, ld_table);
+  const int Bl = B < kAttnStreams ? B : kAttnStreams;  // streams of one launch
+  const long R = (long)T * (NH / NKV);
+  p->mode = R <= 4 ? COLS : (dtype == DT_F32 ? Q32 : Q16);
+  const long cpt = p->mode == COLS ? 4 : 8, tiles = (R + cpt - 1) / cpt;
+  RNGD_REQUIRE(R < (1l << 24), "kv4_attn: %ld query rows of a kv head", R);
+  p->NT = tiles > 1 ? 2 : 1;
+  p->RT = (int)((tiles + p->NT - 1) / p->NT);
+  p->rows = p->NT * (int)cpt;
+  const long units = (long)Bl * NKV * p->RT * ld_table * (kPage / kUnit);
+  RNGD_REQUIRE(units < (1l << 31) && (long)Bl * NKV * p->RT < (1l << 31), "kv4_attn: %ld units of work", units);
+  int per = 1;
+  RNGD_TRY(attn_per_sm(HD, p->NT, p->mode, Bl, &per));
+  const long most = (long)num_sms() * per;
+  p->warps = (int)(units < 1 ? 1 : (units < most ? units : most));
+  p->pre_bytes = ((size_t)(Bl + 1) * 4 + 15) / 16 * 16;
+  p->bytes = p->pre_bytes + (size_t)p->warps * 2 * p->rows * (HD + 4) * 4;
+  return RNGD_OK;
+}
+
+int read_status_kv4(int* st, int reset) {
+  RNGD_TRY(check_cuda(cudaMemcpyFromSymbol(st, g_status_kv4, sizeof(int)), "read device status"));
+  if (reset) {
+    const int zero = 0;
+    RNGD_TRY(check_cuda(cudaMemcpyToSymbol(g_status_kv4, &zero, sizeof(int)), "reset device status"));
+  }
+  return RNGD_OK;
+}
+
+}  // namespace rngd
+
+using namespace rngd;
+
+extern "C" int rngd_kv4_attn_workspace(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, size_t* bytes) {
+  RNGD_REQUIRE(bytes != nullptr, "kv4_attn_workspace: null output");
+  AttnPlan p;
+  RNGD_TRY(attn_plan(dtype, B, T, NH, NKV, HD, ld_table, &p));
+  *bytes = p.bytes;
+  return RNGD_OK;
+}
+
+extern "C" int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out, const int64_t* out_strides, int dtype,
+                             const void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table,
+                             const int32_t* lens, int B, int T, int NH, int window, int sinks, float scale,
+                             void* workspace, size_t workspace_bytes, rngd_stream_t stream) {
+  RNGD_TRY(check_pool("kv4_attn", pool, 0, P, NKV, HD));
+  AttnPlan p;
+  RNGD_TRY(attn_plan(dtype, B, T, NH, NKV, HD, ld_table, &p));
+  RNGD_REQUIRE(window >= 0 && sinks >= 0, "kv4_attn: window=%d sinks=%d", window, sinks);
+  if (B == 0 || T == 0) return RNGD_OK;
+  RNGD_REQUIRE(q && out && q_strides && out_strides && lens && (table || ld_table == 0), "kv4_attn: null pointer");
+  RNGD_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.bytes,
+               "kv4_attn: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, p.bytes);
+  const int esz = dtype == DT_F32 ? 4 : 2;
+  AttnArgs a = {};
+  bool vec = ((uintptr_t)q & 15) == 0;
+  for (int i = 0; i < 3; i++) {
+    a.qs[i] = (long)q_strides[i];
+    a.os[i] = (long)out_strides[i];
+    vec = vec && a.qs[i] * esz % 16 == 0;
+  }
+  a.qvec = vec;
+  a.dt = dtype;
+  a.T = T;
+  a.NH = NH;
+  a.NKV = NKV;
+  a.G = NH / NKV;
+  a.RT = p.RT;
+  a.P = P;
+  a.ld_table = ld_table;
+  a.window = window;
+  a.sinks = sinks;
+  a.pool = (const uint8_t*)pool;
+  a.scale = scale;
+  a.pre = (int*)workspace;
+  a.rec = (float*)((uint8_t*)workspace + p.pre_bytes);
+  cudaStream_t s = (cudaStream_t)stream;
+  for (int b0 = 0; b0 < B; b0 += kAttnStreams) {
+    a.B = B - b0 < kAttnStreams ? B - b0 : kAttnStreams;
+    a.q = (const uint8_t*)q + (long)b0 * a.qs[0] * esz;
+    a.out = (uint8_t*)out + (long)b0 * a.os[0] * esz;
+    a.table = table + (size_t)b0 * ld_table;
+    a.lens = lens + b0;
+    if (HD == 128)
+      attn_kernel<128>(p.NT, p.mode)<<<p.warps, 32, attn_smem<128>(a.B), s>>>(a);
+    else
+      attn_kernel<64>(p.NT, p.mode)<<<p.warps, 32, attn_smem<64>(a.B), s>>>(a);
+    RNGD_TRY(check_launch("kv4_attn_kernel"));
+    const dim3 grid(a.B * a.NKV * a.RT, p.rows);
+    RNGD_TRY(launch_pdl(HD == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, grid, dim3(128), 0, s, "kv4_join_kernel", a,
+                        p.warps, p.rows));
+  }
+  return RNGD_OK;
+}

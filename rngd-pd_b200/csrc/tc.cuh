@@ -255,6 +255,7 @@ static int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sm
 int read_status_decode(int* st, int reset);
 int read_status_prefill(int* st, int reset);
 int read_status_attn(int* st, int reset);
+int read_status_kv4(int* st, int reset);
 size_t attn_fused_scratch_units(int Bcap, int NKV, int S);
 
 // Shared host helpers (decode_tc.cu): SM count, cached tensor maps for weight

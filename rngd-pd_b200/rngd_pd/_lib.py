@@ -135,7 +135,7 @@ _sig("rngd_kv4_store", _vp, _sz, _int, _int, _int, _int, _vp, _int, _vp, _vp, _i
 _sig("rngd_kv4_load", _vp, _sz, _int, _int, _int, _int, _vp, _int, _vp, _vp, _int, _int, _vp, _vp, _int, _vp)
 _sig("rngd_kv4_attn", _vp, _i64p, _vp, _i64p, _int, _vp, _int, _int, _int, _vp, _int, _vp, _int, _int, _int, _int,
      _int, ctypes.c_float, _vp, _sz, _vp)
-_sig("rngd_kv4_attn_workspace", _int, _int, _int, _int, _int, _int, _szp)
+_sig("rngd_kv4_attn_workspace", _int, _int, _int, _int, _int, _int, _int, _szp)
 _sig("rngd_kv4_fork", _vp, _sz, _int, _int, _int, _int, _vp, _vp, _int, _vp, _int, _vp, _int, _vp, _vp, _vp, _vp,
      _vp, _sz, _vp)
 _sig("rngd_kv4_fork_workspace", _int, _int, _szp)

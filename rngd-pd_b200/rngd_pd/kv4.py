@@ -145,7 +145,7 @@ def attention(q, pool, table, lens, window=0, sinks=0, scale=None, out=None):
             out = torch.empty((B, T, NH, HD), dtype=q.dtype, device=dev)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {dev}, got {tuple(out.shape)} {out.dtype}")
-        need = _lib.workspace_bytes("rngd_kv4_attn_workspace", B, T, NH, NKV, HD, width)
+        need = _lib.workspace_bytes("rngd_kv4_attn_workspace", _DT[q.dtype], B, T, NH, NKV, HD, width)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _lib.call("rngd_kv4_attn", qp, _I64x3(*q.stride()[:3]), _rows("out", out, 4), _I64x3(*out.stride()[:3]),
                   _DT[q.dtype], pool.data_ptr(), P, NKV, HD, _i32("table", table, (B, width), dev), width,
