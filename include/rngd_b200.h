@@ -335,7 +335,8 @@ int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out, const int6
                   const void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table, const int32_t* lens,
                   int B, int T, int NH, int window, int sinks, float scale, void* workspace, size_t workspace_bytes,
                   rngd_stream_t stream);
-int rngd_kv4_attn_workspace(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, size_t* bytes);
+int rngd_kv4_attn_workspace(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, int window, int sinks,
+                            size_t* bytes);
 /* Sequences and their pages.  ref: int32 [P] holders of each page (0: free); table: [R][ld_table]; lens: [R].
  * Fork: row r goes on as row parents[r] (NULL: as itself; < 0: it ends and lets go of its pages).  A last
  * page that is partly filled belongs to one row alone afterwards: the lowest row keeps it if none but

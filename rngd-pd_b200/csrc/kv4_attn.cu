@@ -72,12 +72,19 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 
+// (a & m) | o as one instruction: left to itself the compiler moves the mask ahead of the shift and
+// takes a third one (15% of the kernel's time).
+__device__ __forceinline__ uint32_t lop_ao(uint32_t a, uint32_t m, uint32_t o) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(m), "r"(o));
+  return r;
+}
 // The four pairs (nibble i of the low half, nibble i of the high half) of w -> values.
 __device__ __forceinline__ void decode_word(uint32_t w, __half2 s, __half2 c, uint32_t (&v)[4]) {
-  v[0] = h2u(__hfma2(u2h(((w << 6) & 0x03C003C0u) | 0x4C004C00u), s, c));
-  v[1] = h2u(__hfma2(u2h(((w << 2) & 0x03C003C0u) | 0x4C004C00u), s, c));
-  v[2] = h2u(__hfma2(u2h(((w >> 2) & 0x03C003C0u) | 0x4C004C00u), s, c));
-  v[3] = h2u(__hfma2(u2h(((w >> 6) & 0x03C003C0u) | 0x4C004C00u), s, c));
+  v[0] = h2u(__hfma2(u2h(lop_ao(w << 6, 0x03C003C0u, 0x4C004C00u)), s, c));
+  v[1] = h2u(__hfma2(u2h(lop_ao(w << 2, 0x03C003C0u, 0x4C004C00u)), s, c));
+  v[2] = h2u(__hfma2(u2h(lop_ao(w >> 2, 0x03C003C0u, 0x4C004C00u)), s, c));
+  v[3] = h2u(__hfma2(u2h(lop_ao(w >> 6, 0x03C003C0u, 0x4C004C00u)), s, c));
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -135,25 +142,31 @@ struct Unit {
 };
 
 template <int HD>
+__device__ __forceinline__ Unit unit_at(const AttnArgs& a, int b, int kvh, int at, int n, int held) {
+  const int p0 = at * kUnit;
+  const int page = a.table[(size_t)b * a.ld_table + p0 / kPage];
+  const int blocks = page >= 0 && page < a.P ? min(2, (held - p0 + kBlk - 1) / kBlk) : 0;
+  const bool all = p0 + kUnit <= held && p0 + kUnit - 1 <= n - a.T &&
+                   (a.window == 0 || p0 > n - 1 - a.window || p0 + kUnit <= a.sinks);
+  Unit u;
+  u.seg = 0;
+  u.pos = p0 | blocks | (all ? 4 : 0);
+  u.off = (((size_t)max(page, 0) * a.NKV + kvh) * 4 + ((p0 & (kPage - 1)) >> 4)) * kv4_block_bytes(HD);
+  return u;
+}
+
+template <int HD>
 __device__ __forceinline__ Unit look_up(int x, const AttnArgs& a, const int* lens, const int* pre) {
   int lo = 0, hi = a.B - 1;  // pre[lo] <= x < pre[hi + 1]
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (pre[mid] <= x) lo = mid; else hi = mid - 1;
   }
-  const int b = lo, n = lens[b], per = a.NKV * a.RT;
+  const int n = lens[lo], per = a.NKV * a.RT;
   const Span s = span_of(n, a);
-  const int ub = s.units(), rem = x - pre[b], sg = rem / ub;
-  const int p0 = s.at(rem - sg * ub) * kUnit;
-  const int held = min(n, a.ld_table * kPage);
-  const int page = a.table[(size_t)b * a.ld_table + p0 / kPage];
-  int blocks = page >= 0 && page < a.P ? min(2, (held - p0 + kBlk - 1) / kBlk) : 0;
-  const bool all = p0 + kUnit <= held && p0 + kUnit - 1 <= n - a.T &&
-                   (a.window == 0 || p0 > n - 1 - a.window || p0 + kUnit <= a.sinks);
-  Unit u;
-  u.seg = b * per + sg;
-  u.pos = p0 | blocks | (all ? 4 : 0);
-  u.off = (((size_t)max(page, 0) * a.NKV + sg / a.RT) * 4 + ((p0 & (kPage - 1)) >> 4)) * kv4_block_bytes(HD);
+  const int ub = s.units(), rem = x - pre[lo], sg = rem / ub;
+  Unit u = unit_at<HD>(a, lo, sg / a.RT, s.at(rem - sg * ub), n, min(n, a.ld_table * kPage));
+  u.seg = lo * per + sg;
   return u;
 }
 
@@ -258,132 +271,176 @@ struct Rows {
     }
   }
 
-  // A block of 16 positions from p0 on; EDGE: some rows do not see some of them, and what lies past the
-  // stream's end may be anything.
-  template <bool EDGE>
-  __device__ __forceinline__ void block(const uint8_t* blk, int p0, int held, const AttnArgs& a) {
+  // S += K q^T of one block.
+  __device__ __forceinline__ void scores(const uint8_t* blk, float (&c)[NT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float c[NT][4] = {};
-    {
-      uint32_t w0[NG], w1[NG], s0[NG], s1[NG];
-      if constexpr (NG == 4) {
-        const uint4 x = *(const uint4*)(blk + g * 64 + t * 16), y = *(const uint4*)(blk + (g + 8) * 64 + t * 16);
-        w0[0] = x.x; w0[1] = x.y; w0[2] = x.z; w0[3] = x.w;
-        w1[0] = y.x; w1[1] = y.y; w1[2] = y.z; w1[3] = y.w;
-        const uint4 u = *(const uint4*)(blk + 16 * HD + g * 16), v = *(const uint4*)(blk + 16 * HD + (g + 8) * 16);
-        s0[0] = u.x; s0[1] = u.y; s0[2] = u.z; s0[3] = u.w;
-        s1[0] = v.x; s1[1] = v.y; s1[2] = v.z; s1[3] = v.w;
-      } else {
-        const uint2 x = *(const uint2*)(blk + g * 32 + t * 8), y = *(const uint2*)(blk + (g + 8) * 32 + t * 8);
-        w0[0] = x.x; w0[1] = x.y;
-        w1[0] = y.x; w1[1] = y.y;
-        const uint2 u = *(const uint2*)(blk + 16 * HD + g * 8), v = *(const uint2*)(blk + 16 * HD + (g + 8) * 8);
-        s0[0] = u.x; s0[1] = u.y;
-        s1[0] = v.x; s1[1] = v.y;
-      }
+    uint32_t w0[NG], w1[NG], s0[NG], s1[NG];
+    if constexpr (NG == 4) {
+      const uint4 x = *(const uint4*)(blk + g * 64 + t * 16), y = *(const uint4*)(blk + (g + 8) * 64 + t * 16);
+      w0[0] = x.x; w0[1] = x.y; w0[2] = x.z; w0[3] = x.w;
+      w1[0] = y.x; w1[1] = y.y; w1[2] = y.z; w1[3] = y.w;
+      const uint4 u = *(const uint4*)(blk + 16 * HD + g * 16), v = *(const uint4*)(blk + 16 * HD + (g + 8) * 16);
+      s0[0] = u.x; s0[1] = u.y; s0[2] = u.z; s0[3] = u.w;
+      s1[0] = v.x; s1[1] = v.y; s1[2] = v.z; s1[3] = v.w;
+    } else {
+      const uint2 x = *(const uint2*)(blk + g * 32 + t * 8), y = *(const uint2*)(blk + (g + 8) * 32 + t * 8);
+      w0[0] = x.x; w0[1] = x.y;
+      w1[0] = y.x; w1[1] = y.y;
+      const uint2 u = *(const uint2*)(blk + 16 * HD + g * 8), v = *(const uint2*)(blk + 16 * HD + (g + 8) * 8);
+      s0[0] = u.x; s0[1] = u.y;
+      s1[0] = v.x; s1[1] = v.y;
+    }
 #pragma unroll
-      for (int j = 0; j < NG; j++) {
-        uint32_t x[4], y[4];
-        decode_word(w0[j], __low2half2(u2h(s0[j])), __high2half2(u2h(s0[j])), x);
-        decode_word(w1[j], __low2half2(u2h(s1[j])), __high2half2(u2h(s1[j])), y);
+    for (int j = 0; j < NG; j++) {
+      uint32_t x[4], y[4];
+      decode_word(w0[j], __low2half2(u2h(s0[j])), __high2half2(u2h(s0[j])), x);
+      decode_word(w1[j], __low2half2(u2h(s1[j])), __high2half2(u2h(s1[j])), y);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          mma_f16(c[nt], x[0], y[0], x[1], y[1], qf[nt][j][0], qf[nt][j][1]);
-          mma_f16(c[nt], x[2], y[2], x[3], y[3], qf[nt][j][2], qf[nt][j][3]);
-          if constexpr (MODE == Q32) {
-            mma_f16(c[nt], x[0], y[0], x[1], y[1], ql[nt][j][0], ql[nt][j][1]);
-            mma_f16(c[nt], x[2], y[2], x[3], y[3], ql[nt][j][2], ql[nt][j][3]);
-          }
+      for (int nt = 0; nt < NT; nt++) {
+        mma_f16(c[nt], x[0], y[0], x[1], y[1], qf[nt][j][0], qf[nt][j][1]);
+        mma_f16(c[nt], x[2], y[2], x[3], y[3], qf[nt][j][2], qf[nt][j][3]);
+        if constexpr (MODE == Q32) {
+          mma_f16(c[nt], x[0], y[0], x[1], y[1], ql[nt][j][0], ql[nt][j][1]);
+          mma_f16(c[nt], x[2], y[2], x[3], y[3], ql[nt][j][2], ql[nt][j][3]);
         }
       }
     }
-    // V's scales of keys 2t, 2t + 1 (h = 0) and 2t + 8, 2t + 9 (h = 1)
-    uint32_t vs[2][NG], vc[2][NG];
+  }
+
+  // The pairs of keys (2t, 2t + 1) and (2t + 8, 2t + 9) of a block, as bits of four, whose V is NaN.
+  __device__ __forceinline__ uint32_t nan_values(const uint8_t* blk) {
+    const int t = threadIdx.x & 3;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        const uint32_t s = *(const uint32_t*)(blk + 18 * HD + ((h * 4 + t) * NG + j) * 8);
+        bad |= ((s & 0x7FFFu) > 0x7C00u ? 1u : 0u) << (2 * h);
+        bad |= ((s >> 16 & 0x7FFFu) > 0x7C00u ? 2u : 0u) << (2 * h);
+      }
+    return bad;
+  }
+
+  // O^T += V^T P of one block; the keys of `drop` (bits as above) are left out.
+  template <bool EDGE>
+  __device__ __forceinline__ void output(const uint8_t* blk, const uint32_t (&pb)[NT][2],
+                                         const uint32_t (&pl)[SPLIT ? 1 : NT][2], uint32_t drop) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint32_t wa[2][NG / 2], wb[2][NG / 2], vs[2][NG], vc[2][NG];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
+      if constexpr (NG == 4) {
+        const uint4 x = *(const uint4*)(blk + 8 * HD + h * 512 + g * 64 + t * 16);
+        wa[h][0] = x.x; wa[h][1] = x.y; wb[h][0] = x.z; wb[h][1] = x.w;
+      } else {
+        const uint2 x = *(const uint2*)(blk + 8 * HD + h * 256 + g * 32 + t * 8);
+        wa[h][0] = x.x; wb[h][0] = x.y;
+      }
       const uint8_t* sp = blk + 18 * HD + (h * 4 + t) * NG * 8;
 #pragma unroll
       for (int j = 0; j < NG; j += 2) {
         const uint4 x = *(const uint4*)(sp + j * 8);
         vs[h][j] = x.x; vc[h][j] = x.y; vs[h][j + 1] = x.z; vc[h][j + 1] = x.w;
       }
-    }
-    uint32_t bad = 0;  // keys whose V holds a NaN
-    if constexpr (EDGE) {
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        bool n0 = false, n1 = false;
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-          n0 |= (vs[h][j] & 0x7FFFu) > 0x7C00u;
-          n1 |= (vs[h][j] >> 16 & 0x7FFFu) > 0x7C00u;
-        }
-        const int k0 = p0 + 8 * h + 2 * t;
-        const bool z0 = n0 || k0 >= held, z1 = n1 || k0 + 1 >= held;
-        const uint32_t keep = (z0 ? 0u : 0xFFFFu) | (z1 ? 0u : 0xFFFF0000u);
+      if constexpr (EDGE) {
+        const uint32_t d = drop >> (2 * h), keep = (d & 1u ? 0u : 0xFFFFu) | (d & 2u ? 0u : 0xFFFF0000u);
 #pragma unroll
         for (int j = 0; j < NG; j++) {
           vs[h][j] &= keep;
           vc[h][j] &= keep;
         }
-        const uint32_t b0 = __ballot_sync(0xffffffffu, n0) & 15u, b1 = __ballot_sync(0xffffffffu, n1) & 15u;
-#pragma unroll
-        for (int k = 0; k < 4; k++) bad |= (b0 >> k & 1u) << (8 * h + 2 * k) | (b1 >> k & 1u) << (8 * h + 2 * k + 1);
       }
     }
-    uint32_t pb[NT][2], pl[SPLIT ? 1 : NT][2];
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+      uint32_t x[4], y[4];
+      const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
+      decode_word(__byte_perm(wa[0][j / 2], wb[0][j / 2], sel), u2h(vs[0][j]), u2h(vc[0][j]), x);
+      decode_word(__byte_perm(wa[1][j / 2], wb[1][j / 2], sel), u2h(vs[1][j]), u2h(vc[1][j]), y);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        mma_f16(o[nt][j][0], x[0], x[1], y[0], y[1], pb[nt][0], pb[nt][1]);
+        mma_f16(o[nt][j][1], x[2], x[3], y[2], y[3], pb[nt][0], pb[nt][1]);
+        if constexpr (!SPLIT) {
+          mma_f16(o[nt][j][0], x[0], x[1], y[0], y[1], pl[nt][0], pl[nt][1]);
+          mma_f16(o[nt][j][1], x[2], x[3], y[2], y[3], pl[nt][0], pl[nt][1]);
+        }
+      }
+    }
+  }
+
+  // A unit: the two blocks at blk, positions from p0 on.  EDGE: some rows do not see some of them, and
+  // what lies past the stream's end (position held) may be anything.
+  template <bool EDGE>
+  __device__ __forceinline__ void unit(const uint8_t* blk, int p0, int held, const AttnArgs& a) {
+    constexpr int BLK = kv4_block_bytes(HD);
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float c[2][NT][4] = {};
+    scores(blk, c[0]);
+    scores(blk + BLK, c[1]);
+    uint32_t drop[2] = {0u, 0u}, bad = 0;  // bad: a bit for each of the 32 keys
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        uint32_t nan = nan_values(blk + b * BLK);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int key = 16 * b + 8 * (k >> 1) + 2 * t + (k & 1);
+          if (p0 + key >= held) {
+            drop[b] |= 1u << k;
+            nan &= ~(1u << k);
+          }
+          const uint32_t v = __ballot_sync(0xffffffffu, nan >> k & 1u) & 15u;
+#pragma unroll
+          for (int tt = 0; tt < 4; tt++) bad |= (v >> tt & 1u) << (16 * b + 8 * (k >> 1) + 2 * tt + (k & 1));
+        }
+        drop[b] |= nan;
+      }
+    }
+    uint32_t pb[2][NT][2], pl[2][SPLIT ? 1 : NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      // scores of this lane: keys kk[], columns e
-      constexpr int NK = SPLIT ? 1 : 2;
-      float x[NK][2];
-      int kk[NK];
-      if constexpr (SPLIT) {  // t < 2: key g, else key g + 8
-        const float r0 = __shfl_xor_sync(0xffffffffu, t < 2 ? c[nt][2] : c[nt][0], 2);
-        const float r1 = __shfl_xor_sync(0xffffffffu, t < 2 ? c[nt][3] : c[nt][1], 2);
-        x[0][0] = (t < 2 ? c[nt][0] : c[nt][2]) + r0;
-        x[0][1] = (t < 2 ? c[nt][1] : c[nt][3]) + r1;
-        kk[0] = t < 2 ? g : g + 8;
+      // this lane's scores: of key key0 + 8 k (+ 16 b) in columns e; COLS: block t / 2 alone
+      constexpr int NB = SPLIT ? 1 : 2;
+      float x[NB][2][2];
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float r = __shfl_xor_sync(0xffffffffu, t < 2 ? c[1][nt][i] : c[0][nt][i], 2);
+          x[0][i >> 1][i & 1] = (t < 2 ? c[0][nt][i] : c[1][nt][i]) + r;
+        }
       } else {
-        x[0][0] = c[nt][0];
-        x[0][1] = c[nt][1];
-        x[1][0] = c[nt][2];
-        x[1][1] = c[nt][3];
-        kk[0] = g;
-        kk[1] = g + 8;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i >> 2][i >> 1 & 1][i & 1] = c[i >> 2][nt][i & 3];
       }
-#pragma unroll
-      for (int k = 0; k < NK; k++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) x[k][e] *= f[nt][e];
-      if constexpr (EDGE) {
-#pragma unroll
-        for (int k = 0; k < NK; k++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const int j = p0 + kk[k];
-            const bool seen = j <= i[nt][e] && j < held && (a.window == 0 || j > i[nt][e] - a.window || j < a.sinks);
-            if (bad >> kk[k] & 1u) x[k][e] = __uint_as_float(0x7FFFFFFFu);
-            if (!seen) x[k][e] = -INFINITY;
-          }
-      }
-      float y[NK][2];
+      float y[NB][2][2];
       bool over = false;
 #pragma unroll
-      for (int k = 0; k < NK; k++)
+      for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          y[k][e] = x[k][e] + mb[nt][e];
-          over |= y[k][e] > kPMax;
-        }
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float& v = y[b][k][e];
+            if constexpr (EDGE) {
+              const int key = (SPLIT ? 16 * (t >> 1) : 16 * b) + g + 8 * k, j = p0 + key, i_ = i[nt][e];
+              const bool seen = j <= i_ && j < held && (a.window == 0 || j > i_ - a.window || j < a.sinks);
+              x[b][k][e] = !seen ? -INFINITY : (bad >> key & 1u) ? __uint_as_float(0x7FFFFFFFu) : x[b][k][e] * f[nt][e];
+              v = x[b][k][e] + mb[nt][e];
+            } else {
+              v = fmaf(x[b][k][e], f[nt][e], mb[nt][e]);
+            }
+            over |= v > kPMax;
+          }
       if (__any_sync(0xffffffffu, over)) {  // move the maxima
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          float m = x[0][e];
-          if constexpr (NK == 2) m = fmaxf(m, x[NK - 1][e]);
+          const float fe = EDGE ? 1.0f : f[nt][e];
+          float m = fmaxf(x[0][0][e] * fe, x[0][1][e] * fe);
+          if constexpr (NB == 2) m = fmaxf(m, fmaxf(x[NB - 1][0][e] * fe, x[NB - 1][1][e] * fe));
 #pragma unroll
-          for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-          if constexpr (SPLIT) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          for (int w = SPLIT ? 2 : 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
           const float nb = fminf(mb[nt][e], kPBias - m);
           const float al = ex2(nb - mb[nt][e]);
           mb[nt][e] = nb;
@@ -396,64 +453,33 @@ struct Rows {
               o[nt][j][q][e + 2] *= al;
             }
 #pragma unroll
-          for (int k = 0; k < NK; k++) y[k][e] = x[k][e] + nb;
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) y[b][k][e] = fmaf(x[b][k][e], fe, nb);
         }
       }
-      float p[NK][2];
 #pragma unroll
-      for (int k = 0; k < NK; k++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          p[k][e] = ex2(y[k][e]);
-          l[nt][e] += p[k][e];
-        }
-      if constexpr (SPLIT) {
-        const uint32_t hi = pack_h2(p[0][0], p[0][1]);
-        const float2 hf = __half22float2(u2h(hi));
-        const uint32_t lo = pack_h2(p[0][0] - hf.x, p[0][1] - hf.y);
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, t < 2 ? lo : hi, 2);
-        pb[nt][0] = movmatrix(t < 2 ? hi : other);
-        pb[nt][1] = movmatrix(t < 2 ? other : lo);
-      } else {
+      for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-          const uint32_t hi = pack_h2(p[k][0], p[k][1]);
+          const float p0_ = ex2(y[b][k][0]), p1_ = ex2(y[b][k][1]);
+          l[nt][0] += p0_;
+          l[nt][1] += p1_;
+          const uint32_t hi = pack_h2(p0_, p1_);
           const float2 hf = __half22float2(u2h(hi));
-          pb[nt][k] = movmatrix(hi);
-          pl[nt][k] = movmatrix(pack_h2(p[k][0] - hf.x, p[k][1] - hf.y));
-        }
-      }
-    }
-    // O^T += V^T P
-    {
-      uint32_t wa[2][NG / 2], wb[2][NG / 2];
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if constexpr (NG == 4) {
-          const uint4 x = *(const uint4*)(blk + 8 * HD + h * 512 + g * 64 + t * 16);
-          wa[h][0] = x.x; wa[h][1] = x.y; wb[h][0] = x.z; wb[h][1] = x.w;
-        } else {
-          const uint2 x = *(const uint2*)(blk + 8 * HD + h * 256 + g * 32 + t * 8);
-          wa[h][0] = x.x; wb[h][0] = x.y;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NG; j++) {
-        uint32_t x[4], y[4];
-        const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
-        decode_word(__byte_perm(wa[0][j / 2], wb[0][j / 2], sel), u2h(vs[0][j]), u2h(vc[0][j]), x);
-        decode_word(__byte_perm(wa[1][j / 2], wb[1][j / 2], sel), u2h(vs[1][j]), u2h(vc[1][j]), y);
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          mma_f16(o[nt][j][0], x[0], x[1], y[0], y[1], pb[nt][0], pb[nt][1]);
-          mma_f16(o[nt][j][1], x[2], x[3], y[2], y[3], pb[nt][0], pb[nt][1]);
-          if constexpr (!SPLIT) {
-            mma_f16(o[nt][j][0], x[0], x[1], y[0], y[1], pl[nt][0], pl[nt][1]);
-            mma_f16(o[nt][j][1], x[2], x[3], y[2], y[3], pl[nt][0], pl[nt][1]);
+          const uint32_t lo = pack_h2(p0_ - hf.x, p1_ - hf.y);
+          if constexpr (SPLIT) {  // lanes t < 2 hold block 0 and give hi (columns 0..3), the others block 1 and lo
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, t < 2 ? lo : hi, 2);
+            pb[0][nt][k] = movmatrix(t < 2 ? hi : other);
+            pb[1][nt][k] = movmatrix(t < 2 ? other : lo);
+          } else {
+            pb[b][nt][k] = movmatrix(hi);
+            pl[b][nt][k] = movmatrix(lo);
           }
         }
-      }
     }
+    output<EDGE>(blk, pb[0], pl[0], drop[0]);
+    output<EDGE>(blk + BLK, pb[1], pl[1], drop[1]);
   }
 
   // The segment's piece is done: to `out` (whole) or to a record.
@@ -498,12 +524,12 @@ struct Rows {
 };
 
 template <int HD>
-__host__ __device__ constexpr int attn_stages() { return HD == 128 ? 3 : 5; }
+__host__ __device__ constexpr int attn_stages() { return HD == 128 ? 2 : 4; }
 template <int HD>
 __host__ __device__ constexpr int attn_smem(int B) { return attn_stages<HD>() * 2 * kv4_block_bytes(HD) + 64 + (2 * B + 1) * 4; }
 
 template <int HD, int NT, int MODE>
-__global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 ? 16 : 12)) kv4_attn_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? (MODE == COLS ? 16 : 12) : 8) : (NT == 1 ? 16 : 12)) kv4_attn_kernel(AttnArgs a) {
   constexpr int ST = attn_stages<HD>(), BLK = kv4_block_bytes(HD);
   extern __shared__ __align__(128) uint8_t sm[];
   uint64_t* bar = (uint64_t*)(sm + ST * 2 * BLK);
@@ -514,6 +540,7 @@ __global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 
     for (int s = 0; s < ST; s++) mbar_init(bar + s, 1);
     fence_mbar_init();
   }
+  grid_dep_wait();
   prefix_units(a, s_len, s_pre);
   if (blockIdx.x == 0)
     for (int b = lane; b <= a.B; b += 32) a.pre[b] = s_pre[b];
@@ -567,13 +594,11 @@ __global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 
     if (!ok) break;
     const int p0 = pos & ~7, blocks = pos & 3;
     const uint8_t* st = sm + k % ST * 2 * BLK;
-    if (pos & 4) {
-      if (blocks) {
-        rows.template block<false>(st, p0, held, a);
-        rows.template block<false>(st + BLK, p0 + kBlk, held, a);
-      }
-    } else {
-      for (int i = 0; i < blocks; i++) rows.template block<true>(st + i * BLK, p0 + i * kBlk, held, a);
+    if (blocks) {
+      if (pos & 4)
+        rows.template unit<false>(st, p0, held, a);
+      else
+        rows.template unit<true>(st, p0, held, a);
     }
     __syncwarp();
   }
@@ -584,68 +609,182 @@ __global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 
   finish();
 }
 
-// Joins the pieces of cut segments; one CTA per (segment, row).
+// Weighted sum of records: 2^(m - M) of each, as mb = 8 - m.
+template <int D>
+struct Joined {
+  float mb, l, v[D];
+  __device__ __forceinline__ void clear() {
+    mb = 1e30f;
+    l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D; d++) v[d] = 0.0f;
+  }
+  __device__ __forceinline__ void add(float mb2, float l2, const float* v2) {
+    const float nb = fminf(mb, mb2), f = ex2(nb - mb), f2 = ex2(nb - mb2);
+    mb = nb;
+    l = fmaf(l2, f2, l * f);
+#pragma unroll
+    for (int d = 0; d < D; d++) v[d] = fmaf(v2[d], f2, v[d] * f);
+  }
+  __device__ __forceinline__ float inverse() const { return l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); }
+};
+
+// Joins the pieces of cut segments.  A CTA takes rows blockIdx.y * rows_cta .. of a segment, `parts`
+// warps to a row, each every parts-th record; a lane holds HD / 32 consecutive dimensions.
+constexpr int kJoinWarps = 16, kJoinBatch = 6;
 template <int HD>
-__global__ void __launch_bounds__(128) kv4_join_kernel(AttnArgs a, int grid, int rows_per_tile) {
-  __shared__ float s_m[4], s_l[4];
-  __shared__ float s_o[4][HD];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int seg = blockIdx.x, rl = blockIdx.y;
+__global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(AttnArgs a, int grid, int rows_per_tile, int parts) {
+  constexpr int D = HD / 32;
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+  __shared__ float s_o[kJoinWarps][HD];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, part = w % parts;
+  const int seg = blockIdx.x, rl = blockIdx.y * (blockDim.x / 32 / parts) + w / parts;
   const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV, per = a.NKV * a.RT;
   const int r = rt * rows_per_tile + rl;
-  if (r >= a.T * a.G) return;
+  const bool row = rl < rows_per_tile && r < a.T * a.G;
   grid_dep_wait();
   const int p0 = a.pre[b], p1 = a.pre[b + 1], N = a.pre[a.B];
   const int ub = (p1 - p0) / per;
-  const int seg0 = p0 + seg % per * ub, seg1 = seg0 + ub;
-  constexpr int D = HD / 32;
-  float v[D];
-#pragma unroll
-  for (int d = 0; d < D; d++) v[d] = 0.0f;
-  float inv = 0.0f;
+  Joined<D> x;
+  x.clear();
   if (ub > 0) {
-    const int W = min(grid, N);
-    const int w0 = owner_of(seg0, N, W), w1 = owner_of(seg1 - 1, N, W);
-    if (w0 == w1) return;  // written whole
-    auto record = [&](int x) {
-      return a.rec + ((size_t)(2 * x + (x == w0 ? 1 : 0)) * rows_per_tile + rl) * (HD + 4);
-    };
-    // mb = 8 - m: the smallest is the largest maximum
-    float mb = 1e30f;
-    for (int x = w0 + threadIdx.x; x <= w1; x += 128) mb = fminf(mb, __ldcg(record(x) + HD));
-    mb = -warp_max(-mb);
-    if (lane == 0) s_m[w] = mb;
-    __syncthreads();
-    mb = fminf(fminf(s_m[0], s_m[1]), fminf(s_m[2], s_m[3]));
-    float l = 0.0f;
-#pragma unroll 4
-    for (int x = w0 + w; x <= w1; x += 4) {
-      const float* rc = record(x);
-      const float f = ex2(mb - __ldcg(rc + HD));
-      l = fmaf(__ldcg(rc + HD + 1), f, l);
+    const int seg0 = p0 + seg % per * ub, W = min(grid, N);
+    const int w0 = owner_of(seg0, N, W), n = owner_of(seg0 + ub - 1, N, W) - w0 + 1;
+    if (n == 1) return;  // written whole
+    const size_t step = (size_t)2 * rows_per_tile * (HD + 4);
+    const float* rec = a.rec + (size_t)w0 * step + (size_t)(row ? rl : 0) * (HD + 4);
+    for (int i = part; i < n; i += kJoinBatch * parts) {
+      float mb[kJoinBatch], l[kJoinBatch], v[kJoinBatch][D];
 #pragma unroll
-      for (int d = 0; d < D; d++) v[d] = fmaf(__ldcg(rc + lane + 32 * d), f, v[d]);
+      for (int k = 0; k < kJoinBatch; k++) {
+        const int ii = i + k * parts;
+        if (ii >= n) break;
+        const float* rc = rec + ii * step + (ii == 0 ? (size_t)rows_per_tile * (HD + 4) : 0);
+        const float2 ml = __ldcg((const float2*)(rc + HD));
+        mb[k] = ml.x;
+        l[k] = ml.y;
+        if constexpr (D == 4) {
+          const float4 u = __ldcg((const float4*)rc + lane);
+          v[k][0] = u.x; v[k][1] = u.y; v[k][2] = u.z; v[k][3] = u.w;
+        } else {
+          const float2 u = __ldcg((const float2*)rc + lane);
+          v[k][0] = u.x; v[k][1] = u.y;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; k++)
+        if (i + k * parts < n) x.add(mb[k], l[k], v[k]);
     }
-    if (lane == 0) s_l[w] = l;
+    if (parts > 1) {
+      if (lane == 0) {
+        s_m[w] = x.mb;
+        s_l[w] = x.l;
+      }
 #pragma unroll
-    for (int d = 0; d < D; d++) s_o[w][lane + 32 * d] = v[d];
-    __syncthreads();
-    l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-    inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-    if (w != 0) return;
+      for (int d = 0; d < D; d++) s_o[w][lane * D + d] = x.v[d];
+      __syncthreads();
+      if (part != 0) return;
+      for (int k = 1; k < min(n, parts); k++) {
+        float v[D];
 #pragma unroll
-    for (int d = 0; d < D; d++)
-      v[d] = s_o[0][lane + 32 * d] + s_o[1][lane + 32 * d] + s_o[2][lane + 32 * d] + s_o[3][lane + 32 * d];
+        for (int d = 0; d < D; d++) v[d] = s_o[w + k][lane * D + d];
+        x.add(s_m[w + k], s_l[w + k], v);
+      }
+    }
   }
-  if (w != 0) return;
-  const size_t at = (size_t)(b * a.os[0] + r / a.G * a.os[1] + (kvh * a.G + r % a.G) * a.os[2]);
+  if (part != 0 || !row) return;
+  const float inv = x.inverse();
+  const size_t at = (size_t)(b * a.os[0] + r / a.G * a.os[1] + (kvh * a.G + r % a.G) * a.os[2]) + lane * D;
 #pragma unroll
-  for (int d = 0; d < D; d++) store1(a.out, at + lane + 32 * d, a.dt, v[d] * inv);
+  for (int d = 0; d < D; d++) store1(a.out, at + d, a.dt, x.v[d] * inv);
+}
+
+// The same for sequences that are known to be short: one CTA holds a segment, its warps take the units
+// in turn and join through shared memory, so that one launch is all there is.
+template <int HD, int NT, int MODE>
+__host__ __device__ constexpr int whole_warps() {  // as many as the registers allow
+  return HD == 128 && NT == 2 ? 8 : (NT == 2 || (HD == 128 && MODE == Q32) ? 12 : 16);
+}
+template <int HD, int NT, int MODE>
+__host__ __device__ constexpr int whole_smem(int warps) {
+  const int ring = warps * 2 * 2 * kv4_block_bytes(HD), rec = warps * NT * (MODE == COLS ? 4 : 8) * (HD + 4) * 4;
+  return (ring > rec ? ring : rec) + warps * 16;
+}
+template <int HD, int NT, int MODE>
+__global__ void __launch_bounds__(32 * whole_warps<HD, NT, MODE>()) kv4_attn_whole_kernel(AttnArgs a) {
+  constexpr int BLK = kv4_block_bytes(HD), ST = 2, RPT = NT * (MODE == COLS ? 4 : 8);
+  extern __shared__ __align__(128) uint8_t sm[];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  uint8_t* ring = sm + w * ST * 2 * BLK;
+  uint64_t* bar = (uint64_t*)(sm + whole_smem<HD, NT, MODE>(warps) - warps * 16) + w * 2;
+  if (lane < ST) mbar_init(bar + lane, 1);
+  fence_mbar_init();
+  __syncwarp();
+  grid_dep_wait();
+  const int seg = blockIdx.x;
+  const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV;
+  const int n = a.lens[b], held = min(max(n, 0), a.ld_table * kPage);
+  const Span sp = span_of(n, a);
+  const int U = sp.units(), mine = U > w ? (U - w + warps - 1) / warps : 0;
+  Rows<HD, NT, MODE> rows;
+  Unit next = {}, cur;  // of this warp's units (k & ~31) + lane, for the issuer and for the reader
+  auto issue = [&](int k) {
+    if ((k & 31) == 0) next = unit_at<HD>(a, b, kvh, sp.at(w + min(k + lane, mine - 1) * warps), n, held);
+    if (lane == (k & 31)) {
+      const uint32_t bytes = (next.pos & 3) * BLK;
+      mbar_arrive_expect_tx(bar + (k & 1), bytes);
+      if (bytes) bulk_load(ring + (k & 1) * 2 * BLK, a.pool + next.off, bytes, bar + (k & 1));
+    }
+  };
+  for (int k = 0; k < min(mine, 2); k++) issue(k);
+  cur = next;
+  rows.begin(a, seg, n);
+  bool ok = true;
+  int k = 0;
+  for (; k < mine; k++) {
+    if ((k & 31) == 0 && k > 0) cur = next;
+    const int ps = __shfl_sync(0xffffffffu, cur.pos, k & 31);
+    ok = __all_sync(0xffffffffu, mbar_wait(bar + (k & 1), (k >> 1) & 1, ST_TMA_WAIT, &g_status_kv4));
+    if (!ok) break;
+    const uint8_t* st = ring + (k & 1) * 2 * BLK;
+    if (ps & 3) {
+      if (ps & 4)
+        rows.template unit<false>(st, ps & ~7, held, a);
+      else
+        rows.template unit<true>(st, ps & ~7, held, a);
+    }
+    __syncwarp();
+    if (k + 2 < mine) issue(k + 2);
+  }
+  if (!ok)  // give up, once the copies in flight are in (waited for with a limit too)
+    for (int i = k; i < min(k + 2, mine); i++) mbar_wait(bar + (i & 1), (i >> 1) & 1, ST_TMA_WAIT, &g_status_kv4);
+  float* rec = (float*)sm;
+  __syncthreads();
+  const int parts = min(U, warps);
+  if (w < parts) rows.end(a, seg, false, rec + (size_t)w * RPT * (HD + 4));
+  __syncthreads();
+  // four dimensions of a row per thread
+  for (int i = threadIdx.x; i < RPT * (HD / 4); i += blockDim.x) {
+    const int rl = i / (HD / 4), d = i % (HD / 4) * 4, r = rt * RPT + rl;
+    if (r >= a.T * a.G) break;
+    Joined<4> x;
+    x.clear();
+    for (int k = 0; k < parts; k++) {
+      const float* rc = rec + ((size_t)k * RPT + rl) * (HD + 4);
+      const float4 u = *(const float4*)(rc + d);
+      const float v[4] = {u.x, u.y, u.z, u.w};
+      x.add(rc[HD], rc[HD + 1], v);
+    }
+    const float inv = x.inverse();
+    const size_t at = (size_t)(b * a.os[0] + r / a.G * a.os[1] + (kvh * a.G + r % a.G) * a.os[2]) + d;
+#pragma unroll
+    for (int e = 0; e < 4; e++) store1(a.out, at + e, a.dt, x.v[e] * inv);
+  }
 }
 
 // How a call is laid out over the GPU.
 struct AttnPlan {
-  int NT, mode, RT, rows, warps;
+  int NT, mode, RT, rows, warps, whole;  // whole: warps of a CTA per segment, 0: equal runs of units
   size_t pre_bytes, bytes;
 };
 
@@ -655,6 +794,22 @@ static AttnKernel attn_kernel(int NT, int mode) {
   if (mode == COLS) return kv4_attn_kernel<HD, 1, COLS>;
   if (mode == Q16) return NT == 1 ? kv4_attn_kernel<HD, 1, Q16> : kv4_attn_kernel<HD, 2, Q16>;
   return NT == 1 ? kv4_attn_kernel<HD, 1, Q32> : kv4_attn_kernel<HD, 2, Q32>;
+}
+
+template <int HD, int NT, int MODE>
+static int launch_whole(const AttnArgs& a, int warps, cudaStream_t s) {
+  static std::atomic<unsigned long long> smem_set{0};
+  RNGD_TRY(set_smem_limit_once((const void*)kv4_attn_whole_kernel<HD, NT, MODE>, whole_smem<HD, NT, MODE>(whole_warps<HD, NT, MODE>()),
+                               &smem_set, "cudaFuncSetAttribute(kv4_attn_whole_kernel)"));
+  return launch_pdl(kv4_attn_whole_kernel<HD, NT, MODE>, dim3(a.B * a.NKV * a.RT), dim3(32 * warps),
+                    whole_smem<HD, NT, MODE>(warps), s, "kv4_attn_whole_kernel", a);
+}
+template <int HD>
+static int launch_whole(const AttnArgs& a, const AttnPlan& p, cudaStream_t s) {
+  if (p.mode == COLS) return launch_whole<HD, 1, COLS>(a, p.whole, s);
+  if (p.mode == Q16)
+    return p.NT == 1 ? launch_whole<HD, 1, Q16>(a, p.whole, s) : launch_whole<HD, 2, Q16>(a, p.whole, s);
+  return p.NT == 1 ? launch_whole<HD, 1, Q32>(a, p.whole, s) : launch_whole<HD, 2, Q32>(a, p.whole, s);
 }
 
 // Warps that fit one SM at a time (registers, shared memory), remembered per kernel and size class of
@@ -675,11 +830,13 @@ static int attn_per_sm(int HD, int NT, int mode, int B, int* out) {
   return RNGD_OK;
 }
 
-static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, AttnPlan* p) {
+static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, int window, int sinks,
+                     AttnPlan* p) {
   RNGD_REQUIRE(HD == 64 || HD == 128, "kv4_attn: built for HD 64 and 128, not %d", HD);
   RNGD_REQUIRE(dtype >= DT_BF16 && dtype <= DT_F32, "kv4_attn: data type %d", dtype);
   RNGD_REQUIRE(B >= 0 && T >= 0 && NKV >= 1 && NH >= 1 && NH % NKV == 0 && ld_table >= 0,
                "kv4_attn: B=%d T=%d NH=%d must be a multiple of NKV=%d, table width %d", B, T, NH, NKV, ld_table);
+  RNGD_REQUIRE(window >= 0 && sinks >= 0, "kv4_attn: window=%d sinks=%d", window, sinks);
   const int Bl = B < kAttnStreams ? B : kAttnStreams;  // streams of one launch
   const long R = (long)T * (NH / NKV);
   p->mode = R <= 4 ? COLS : (dtype == DT_F32 ? Q32 : Q16);
@@ -688,14 +845,32 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
   p->NT = tiles > 1 ? 2 : 1;
   p->RT = (int)((tiles + p->NT - 1) / p->NT);
   p->rows = p->NT * (int)cpt;
-  const long units = (long)Bl * NKV * p->RT * ld_table * (kPage / kUnit);
+  // units of the longest segment there can be
+  long most_u = (long)ld_table * (kPage / kUnit);
+  if (window > 0) {
+    const long w = ((long)window + T - 2) / kUnit + 2 + ((long)sinks + kUnit - 1) / kUnit;
+    most_u = most_u < w ? most_u : w;
+  }
+  const int cap = HD == 128 && p->NT == 2 ? 8 : (p->NT == 2 || (HD == 128 && p->mode == Q32) ? 12 : 16);
+  // One CTA per segment saves the joining kernel (and its launch) but leaves a long stream to one SM.  Streams
+  // of one length, 32/8 heads of 128, us in a graph, whole against runs: 1x387 8.2 and 9.9, 1x1000 10.8 and
+  // 10.3, 1x2000 14.7 and 10.4; 16x300 7.8 and 15.3, 16x4000 23.6 and 31.9; 64x1000 23.5 and 34.6, 64x5000
+  // 90.5 and 91.2.  A CTA has no more warps than let all CTAs run at once (64x300: 12.0 us, 28.7 without).
+  const long segs = (long)Bl * NKV * p->RT;
+  p->whole = 0;
+  if (most_u <= 48 || (most_u <= 128 && segs >= 64)) {
+    long w = segs < 1 ? 1 : (long)num_sms() * 16 / segs;
+    w = w < 2 ? 2 : (w < cap ? w : cap);
+    p->whole = (int)(most_u < 1 ? 1 : (most_u < w ? most_u : w));
+  }
+  const long units = (long)Bl * NKV * p->RT * most_u;
   RNGD_REQUIRE(units < (1l << 31) && (long)Bl * NKV * p->RT < (1l << 31), "kv4_attn: %ld units of work", units);
   int per = 1;
   RNGD_TRY(attn_per_sm(HD, p->NT, p->mode, Bl, &per));
   const long most = (long)num_sms() * per;
   p->warps = (int)(units < 1 ? 1 : (units < most ? units : most));
   p->pre_bytes = ((size_t)(Bl + 1) * 4 + 15) / 16 * 16;
-  p->bytes = p->pre_bytes + (size_t)p->warps * 2 * p->rows * (HD + 4) * 4;
+  p->bytes = p->whole ? 16 : p->pre_bytes + (size_t)p->warps * 2 * p->rows * (HD + 4) * 4;
   return RNGD_OK;
 }
 
@@ -712,10 +887,11 @@ int read_status_kv4(int* st, int reset) {
 
 using namespace rngd;
 
-extern "C" int rngd_kv4_attn_workspace(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, size_t* bytes) {
+extern "C" int rngd_kv4_attn_workspace(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, int window,
+                                       int sinks, size_t* bytes) {
   RNGD_REQUIRE(bytes != nullptr, "kv4_attn_workspace: null output");
   AttnPlan p;
-  RNGD_TRY(attn_plan(dtype, B, T, NH, NKV, HD, ld_table, &p));
+  RNGD_TRY(attn_plan(dtype, B, T, NH, NKV, HD, ld_table, window, sinks, &p));
   *bytes = p.bytes;
   return RNGD_OK;
 }
@@ -726,8 +902,7 @@ extern "C" int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out,
                              void* workspace, size_t workspace_bytes, rngd_stream_t stream) {
   RNGD_TRY(check_pool("kv4_attn", pool, 0, P, NKV, HD));
   AttnPlan p;
-  RNGD_TRY(attn_plan(dtype, B, T, NH, NKV, HD, ld_table, &p));
-  RNGD_REQUIRE(window >= 0 && sinks >= 0, "kv4_attn: window=%d sinks=%d", window, sinks);
+  RNGD_TRY(attn_plan(dtype, B, T, NH, NKV, HD, ld_table, window, sinks, &p));
   if (B == 0 || T == 0) return RNGD_OK;
   RNGD_REQUIRE(q && out && q_strides && out_strides && lens && (table || ld_table == 0), "kv4_attn: null pointer");
   RNGD_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.bytes,
@@ -762,14 +937,20 @@ extern "C" int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out,
     a.out = (uint8_t*)out + (long)b0 * a.os[0] * esz;
     a.table = table + (size_t)b0 * ld_table;
     a.lens = lens + b0;
-    if (HD == 128)
-      attn_kernel<128>(p.NT, p.mode)<<<p.warps, 32, attn_smem<128>(a.B), s>>>(a);
-    else
-      attn_kernel<64>(p.NT, p.mode)<<<p.warps, 32, attn_smem<64>(a.B), s>>>(a);
-    RNGD_TRY(check_launch("kv4_attn_kernel"));
-    const dim3 grid(a.B * a.NKV * a.RT, p.rows);
-    RNGD_TRY(launch_pdl(HD == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, grid, dim3(128), 0, s, "kv4_join_kernel", a,
-                        p.warps, p.rows));
+    if (p.whole) {
+      RNGD_TRY(HD == 128 ? launch_whole<128>(a, p, s) : launch_whole<64>(a, p, s));
+      continue;
+    }
+    const AttnKernel k = HD == 128 ? attn_kernel<128>(p.NT, p.mode) : attn_kernel<64>(p.NT, p.mode);
+    RNGD_TRY(launch_pdl(k, dim3(p.warps), dim3(32), HD == 128 ? attn_smem<128>(a.B) : attn_smem<64>(a.B), s,
+                        "kv4_attn_kernel", a));
+    // few segments have many records each: a CTA per row, its records shared by 16 warps; many segments: a CTA
+    // for all rows of one (64x5000: 105 us with 16 warps a row, 91 us so)
+    const int segs = a.B * NKV * p.RT;
+    const bool few = segs * p.rows <= 4 * num_sms();
+    const int parts = few ? kJoinWarps : (p.rows <= 8 ? 2 : 1);
+    RNGD_TRY(launch_pdl(HD == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, dim3(segs, few ? p.rows : 1),
+                        dim3(32 * (few ? kJoinWarps : p.rows * parts)), 0, s, "kv4_join_kernel", a, p.warps, p.rows, parts));
   }
   return RNGD_OK;
 }

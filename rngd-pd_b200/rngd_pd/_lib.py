@@ -5,6 +5,7 @@ built ``_rngd_b200.so`` raises, and every call that returns a negative status
 raises ``RngdError`` with the library's own message.
 """
 import ctypes
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -135,7 +136,7 @@ _sig("rngd_kv4_store", _vp, _sz, _int, _int, _int, _int, _vp, _int, _vp, _vp, _i
 _sig("rngd_kv4_load", _vp, _sz, _int, _int, _int, _int, _vp, _int, _vp, _vp, _int, _int, _vp, _vp, _int, _vp)
 _sig("rngd_kv4_attn", _vp, _i64p, _vp, _i64p, _int, _vp, _int, _int, _int, _vp, _int, _vp, _int, _int, _int, _int,
      _int, ctypes.c_float, _vp, _sz, _vp)
-_sig("rngd_kv4_attn_workspace", _int, _int, _int, _int, _int, _int, _int, _szp)
+_sig("rngd_kv4_attn_workspace", _int, _int, _int, _int, _int, _int, _int, _int, _int, _szp)
 _sig("rngd_kv4_fork", _vp, _sz, _int, _int, _int, _int, _vp, _vp, _int, _vp, _int, _vp, _int, _vp, _vp, _vp, _vp,
      _vp, _sz, _vp)
 _sig("rngd_kv4_fork_workspace", _int, _int, _szp)
@@ -196,11 +197,25 @@ def decode_attn_workspace(model, Bcap, S):
     return out.value
 
 
+@functools.lru_cache(maxsize=4096)
 def workspace_bytes(name, *args):
-    """Bytes that the workspace query `name` answers for these sizes."""
+    """Bytes that the workspace query `name` answers for these sizes (they depend on nothing else)."""
     out = ctypes.c_size_t(0)
     call(name, *args, ctypes.byref(out))
     return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def i64_array(values):
+    """A C array of these numbers (strides)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def raw_stream(index):
+    """cudaStream_t of the current stream of GPU `index`, as a number: what stream_handle() wraps, at a
+    fraction of its time (the small operators are called hundreds of times a step)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class _Here:

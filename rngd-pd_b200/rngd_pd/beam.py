@@ -10,6 +10,12 @@ from rngd_pd import _lib
 
 MAX_BEAMS = 32
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_select = _lib.lib.rngd_beam_select
+
+
+def _vector(name, t, dt, n, dev):
+    if t.dtype is not dt or t.shape != (n,) or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dt} [{n}] tensor on {dev}, got {tuple(t.shape)} {t.dtype}")
 
 
 def select(logits, scores, done, beams, eos=-1):
@@ -30,19 +36,19 @@ def select(logits, scores, done, beams, eos=-1):
     if V < beams or V * beams >= 2 ** 31 or (V > 1 and logits.stride(1) != 1) or (R > 1 and logits.stride(0) < V):
         raise ValueError(f"logits {tuple(logits.shape)} strides {logits.stride()}: rows must be contiguous, at least "
                          f"{beams} wide and not overlap")
-    for name, t, dt in (("scores", scores, torch.float32), ("done", done, torch.bool)):
-        if t.dtype != dt or tuple(t.shape) != (R,) or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dt} [{R}] tensor on {dev}, got {tuple(t.shape)} {t.dtype}")
+    _vector("scores", scores, torch.float32, R, dev)
+    _vector("done", done, torch.bool, R, dev)
     if eos >= V:
         raise ValueError(f"eos={eos} outside the vocabulary of {V}")
     with _lib.device_of(dev):
         shape = (R // beams, beams)
         out = torch.empty(shape, dtype=torch.float32, device=dev)
-        parents, tokens = torch.empty((2,) + shape, dtype=torch.int32, device=dev).unbind(0)
+        parents = torch.empty(shape, dtype=torch.int32, device=dev)
+        tokens = torch.empty_like(parents)
         ended = torch.empty(shape, dtype=torch.bool, device=dev)
         need = _lib.workspace_bytes("rngd_beam_workspace", R, V, beams)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("rngd_beam_select", logits.data_ptr(), _DT[logits.dtype], logits.stride(0), R, V, beams,
-                  scores.data_ptr(), done.data_ptr(), eos, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
-                  ended.data_ptr(), ws.data_ptr(), need, _lib.stream_handle())
+        _lib.check(_select(logits.data_ptr(), _DT[logits.dtype], logits.stride(0), R, V, beams, scores.data_ptr(),
+                           done.data_ptr(), eos, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                           ended.data_ptr(), ws.data_ptr(), need, _lib.raw_stream(dev.index)))
     return out, parents, tokens, ended

@@ -14,9 +14,6 @@ Everything lives on the pool's GPU; calls are queued on the current stream and w
 be captured into a CUDA graph.  As with torch's own operators, a tensor made on another stream has to be
 ordered before the call by the caller (and kept alive with record_stream).  Nothing falls back to the CPU.
 """
-import ctypes
-import math
-
 import torch
 
 from rngd_pd import _lib
@@ -26,7 +23,10 @@ GROUP = 32    # values that share a scale
 HEAD_DIMS = (64, 128)
 
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_I64x3, _I64x4 = ctypes.c_int64 * 3, ctypes.c_int64 * 4
+_INT_MAX = 2 ** 31 - 1
+_check = _lib.check
+_store, _load, _attn = _lib.lib.rngd_kv4_store, _lib.lib.rngd_kv4_load, _lib.lib.rngd_kv4_attn
+_fork, _compact = _lib.lib.rngd_kv4_fork, _lib.lib.rngd_kv4_compact
 
 
 def page_bytes(n_kv, head_dim):
@@ -49,32 +49,33 @@ def empty_state(rows, width, pages, device="cuda"):
 
 def _pool_dims(pool, layers):
     """(L, P, NKV, HD, bytes between layers) of a pool, or of one layer's where `layers` is false."""
-    want = 5 if layers else 4
-    if pool.dim() != want or pool.dtype != torch.uint8 or not pool.is_cuda:
-        raise ValueError(f"pool must be a {want}-dimensional uint8 CUDA tensor, got {tuple(pool.shape)} {pool.dtype} "
-                         f"on {pool.device}")
-    P, NKV, four, blk = pool.shape[-4:]
+    shape = pool.shape
+    if len(shape) != (5 if layers else 4) or pool.dtype is not torch.uint8 or not pool.is_cuda:
+        raise ValueError(f"pool must be a {5 if layers else 4}-dimensional uint8 CUDA tensor, got {tuple(shape)} "
+                         f"{pool.dtype} on {pool.device}")
+    P, NKV, four, blk = shape[-4:]
     HD = blk // 20
     if four != 4 or blk % 20 or HD not in HEAD_DIMS:
-        raise ValueError(f"pool {tuple(pool.shape)}: the last dimensions must be [pages, kv heads, 4, 20 * head_dim]")
-    if pool.stride()[-4:] != (NKV * 4 * blk, 4 * blk, blk, 1):
+        raise ValueError(f"pool {tuple(shape)}: the last dimensions must be [pages, kv heads, 4, 20 * head_dim]")
+    if not pool.is_contiguous() and pool.stride()[-4:] != (NKV * 4 * blk, 4 * blk, blk, 1):
         raise ValueError("pool: a layer's pages must be contiguous")
-    return pool.shape[0] if layers else 1, P, NKV, HD, pool.stride(0) if layers else 0
+    return (shape[0], P, NKV, HD, pool.stride(0)) if layers else (1, P, NKV, HD, 0)
 
 
 def _i32(name, t, shape, dev):
-    if t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != dev or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 {tuple(shape)} tensor on {dev}, got {tuple(t.shape)} "
                          f"{t.dtype} on {t.device}")
     return t.data_ptr()
 
 
 def _rows(name, t, dims):
-    """A tensor of rows whose last dimension is contiguous -> (pointer, strides of the others)."""
-    if t.dim() != dims or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    """A tensor of rows whose last dimension is contiguous -> (pointer, strides)."""
+    st = t.stride()
+    if len(st) != dims or (st[-1] != 1 and t.shape[-1] > 1):
         raise ValueError(f"{name} must have {dims} dimensions, the last one contiguous, got {tuple(t.shape)} "
-                         f"strides {t.stride()}")
-    return t.data_ptr()
+                         f"strides {st}")
+    return t.data_ptr(), _lib.i64_array(st)
 
 
 def store(pool, table, start, k, v, count=None):
@@ -87,17 +88,19 @@ def store(pool, table, start, k, v, count=None):
     if k.dim() == 4:
         k, v = k.unsqueeze(0), v.unsqueeze(0)
     dev = pool.device
-    if k.dim() != 5 or k.shape != v.shape or k.shape[0] != L or k.shape[3:] != (NKV, HD):
+    shape = k.shape
+    if len(shape) != 5 or v.shape != shape or shape[0] != L or shape[3] != NKV or shape[4] != HD:
         raise ValueError(f"k and v must be [{L}, streams, tokens, {NKV}, {HD}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype not in _DT or v.dtype != k.dtype or k.device != dev or v.device != dev:
+    if k.dtype not in _DT or v.dtype is not k.dtype or k.device != dev or v.device != dev:
         raise ValueError(f"k and v must be bfloat16, float16 or float32 on {dev}, got {k.dtype} and {v.dtype}")
-    B, T = k.shape[1:3]
-    kp, vp = _rows("k", k, 5), _rows("v", v, 5)
+    B, T = shape[1], shape[2]
+    kp, ks = _rows("k", k, 5)
+    vp, vs = _rows("v", v, 5)
+    width = table.shape[-1]
     with _lib.device_of(dev):
-        _lib.call("rngd_kv4_store", pool.data_ptr(), layer, P, NKV, HD, L,
-                  _i32("table", table, (B, table.shape[-1]), dev), table.shape[-1], _i32("start", start, (B,), dev),
-                  None if count is None else _i32("count", count, (B,), dev), B, T, kp, _I64x4(*k.stride()[:4]), vp,
-                  _I64x4(*v.stride()[:4]), _DT[k.dtype], _lib.stream_handle())
+        _check(_store(pool.data_ptr(), layer, P, NKV, HD, L, _i32("table", table, (B, width), dev), width,
+                      _i32("start", start, (B,), dev), None if count is None else _i32("count", count, (B,), dev), B, T,
+                      kp, ks, vp, vs, _DT[k.dtype], _lib.raw_stream(dev.index)))
 
 
 def load(pool, table, start, tokens, count=None, dtype=torch.float16):
@@ -109,16 +112,17 @@ def load(pool, table, start, tokens, count=None, dtype=torch.float16):
     dev = pool.device
     if dtype not in _DT:
         raise ValueError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-    B, tokens = table.shape[0], int(tokens)
+    B, width = table.shape
     if tokens < 0:
         raise ValueError(f"tokens={tokens}")
+    shape = (L, B, tokens, NKV, HD) if layers else (B, tokens, NKV, HD)
     with _lib.device_of(dev):
-        k, v = torch.empty((2, L, B, tokens, NKV, HD), dtype=dtype, device=dev).unbind(0)
-        _lib.call("rngd_kv4_load", pool.data_ptr(), layer, P, NKV, HD, L, _i32("table", table, (B, table.shape[-1]), dev),
-                  table.shape[-1], _i32("start", start, (B,), dev),
-                  None if count is None else _i32("count", count, (B,), dev), B, tokens, k.data_ptr(), v.data_ptr(),
-                  _DT[dtype], _lib.stream_handle())
-    return (k, v) if layers else (k[0], v[0])
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = torch.empty_like(k)
+        _check(_load(pool.data_ptr(), layer, P, NKV, HD, L, _i32("table", table, (B, width), dev), width,
+                     _i32("start", start, (B,), dev), None if count is None else _i32("count", count, (B,), dev), B,
+                     tokens, k.data_ptr(), v.data_ptr(), _DT[dtype], _lib.raw_stream(dev.index)))
+    return k, v
 
 
 def attention(q, pool, table, lens, window=0, sinks=0, scale=None, out=None):
@@ -130,27 +134,29 @@ def attention(q, pool, table, lens, window=0, sinks=0, scale=None, out=None):
     does not see, and what lies where there is no page, has no part in the result.  A token that sees nothing gives
     zeros.  scale: 1 / sqrt(HD) by default.  Returns [B, T, NH, HD] of q's type, in `out` where given."""
     _, P, NKV, HD, _ = _pool_dims(pool, False)
-    dev = pool.device
-    qp = _rows("q", q, 4)
-    B, T, NH, _ = q.shape
-    if q.shape[3] != HD or NH % NKV or NH == 0:
+    dev, dt = pool.device, q.dtype
+    qp, qs = _rows("q", q, 4)
+    B, T, NH, D = q.shape
+    if D != HD or NH % NKV or NH == 0:
         raise ValueError(f"q {tuple(q.shape)} does not fit a pool of {NKV} kv heads of {HD}")
-    if q.dtype not in _DT or q.device != dev:
-        raise ValueError(f"q must be bfloat16, float16 or float32 on {dev}, got {q.dtype} on {q.device}")
+    if dt not in _DT or q.device != dev:
+        raise ValueError(f"q must be bfloat16, float16 or float32 on {dev}, got {dt} on {q.device}")
     if window < 0 or sinks < 0:
         raise ValueError(f"window={window} and sinks={sinks} must not be negative")
     width = table.shape[-1]
+    window, sinks = min(window, _INT_MAX), min(sinks, _INT_MAX)
     with _lib.device_of(dev):
         if out is None:
-            out = torch.empty((B, T, NH, HD), dtype=q.dtype, device=dev)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
-            raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {dev}, got {tuple(out.shape)} {out.dtype}")
-        need = _lib.workspace_bytes("rngd_kv4_attn_workspace", _DT[q.dtype], B, T, NH, NKV, HD, width)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype is not dt or out.device != dev:
+            raise ValueError(f"out must be {tuple(q.shape)} {dt} on {dev}, got {tuple(out.shape)} {out.dtype}")
+        op, os = _rows("out", out, 4)
+        need = _lib.workspace_bytes("rngd_kv4_attn_workspace", _DT[dt], B, T, NH, NKV, HD, width, window,
+                                     sinks)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("rngd_kv4_attn", qp, _I64x3(*q.stride()[:3]), _rows("out", out, 4), _I64x3(*out.stride()[:3]),
-                  _DT[q.dtype], pool.data_ptr(), P, NKV, HD, _i32("table", table, (B, width), dev), width,
-                  _i32("lens", lens, (B,), dev), B, T, NH, min(int(window), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1),
-                  1.0 / math.sqrt(HD) if scale is None else scale, ws.data_ptr(), need, _lib.stream_handle())
+        _check(_attn(qp, qs, op, os, _DT[dt], pool.data_ptr(), P, NKV, HD, _i32("table", table, (B, width), dev), width,
+                     _i32("lens", lens, (B,), dev), B, T, NH, window, sinks,
+                     HD ** -0.5 if scale is None else scale, ws.data_ptr(), need, _lib.raw_stream(dev.index)))
     return out
 
 
@@ -172,10 +178,10 @@ def fork(pool, ref, table, lens, parents=None, room=0):
         short = torch.empty(1, dtype=torch.int32, device=dev)
         need = _lib.workspace_bytes("rngd_kv4_fork_workspace", R, width)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("rngd_kv4_fork", pool.data_ptr(), layer, L, P, NKV, HD, rp, tp, width, lp, R,
-                  None if parents is None else _i32("parents", parents, (R,), dev), int(room), new_ref.data_ptr(),
-                  new_table.data_ptr(), new_lens.data_ptr(), short.data_ptr(), ws.data_ptr(), need,
-                  _lib.stream_handle())
+        _check(_fork(pool.data_ptr(), layer, L, P, NKV, HD, rp, tp, width, lp, R,
+                     None if parents is None else _i32("parents", parents, (R,), dev), room, new_ref.data_ptr(),
+                     new_table.data_ptr(), new_lens.data_ptr(), short.data_ptr(), ws.data_ptr(), need,
+                     _lib.raw_stream(dev.index)))
     return new_ref, new_table, new_lens, short
 
 
@@ -192,6 +198,6 @@ def compact(pool, ref, table):
         live = torch.empty(1, dtype=torch.int32, device=dev)
         need = _lib.workspace_bytes("rngd_kv4_compact_workspace", P)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("rngd_kv4_compact", pool.data_ptr(), layer, L, P, NKV, HD, rp, tp, width, R, new_ref.data_ptr(),
-                  new_table.data_ptr(), live.data_ptr(), ws.data_ptr(), need, _lib.stream_handle())
+        _check(_compact(pool.data_ptr(), layer, L, P, NKV, HD, rp, tp, width, R, new_ref.data_ptr(),
+                        new_table.data_ptr(), live.data_ptr(), ws.data_ptr(), need, _lib.raw_stream(dev.index)))
     return new_ref, new_table, live
