@@ -17,52 +17,36 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float held_to(float x) { return min_nan(max_nan(x, -kKvMax), kKvMax); }
 
-// fp16 of the exact number whose fp32 rounding is x and whose remainder has the sign of `rest`: rounding
-// twice would be off by one in the last place where x falls between two fp16 numbers, so a number that
-// is not x exactly is first cut to fp32 with its last bit set (a sticky bit, 13 bits below fp16's last).
-__device__ __forceinline__ __half half_once(float x, float rest) {
-  uint32_t b = __float_as_uint(x);
-  if (rest != 0.0f && (b & 0x7FFFFFFFu) != 0u) b = (b - ((rest < 0.0f) != (x < 0.0f) ? 1u : 0u)) | 1u;
-  return __float2half_rn(__uint_as_float(b));
-}
-// a - b = d + e exactly (two-sum)
-__device__ __forceinline__ float sub_exact(float a, float b, float* e) {
-  const float d = __fsub_rn(a, b), bb = __fsub_rn(a, d);
-  *e = __fadd_rn(__fsub_rn(a, __fadd_rn(d, bb)), __fsub_rn(bb, b));
-  return d;
+// s and c of a group, in fp32 and each rounded to fp16; NaN for a group with a NaN, s = 0 for a constant
+// one.
+__device__ __forceinline__ __half2 group_scale(float lo, float hi) {
+  const __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+  return __halves2half2(s, __float2half_rn(__fsub_rn(lo, 16.0f * __half2float(s))));
 }
 
-// Four values of a lane, eight lanes to a group of 32 -> codes, s, c.  s and c are rounded once, the
-// quotients in fp32; a group with a NaN gets s = c = NaN, a constant group s = 0.
-__device__ __forceinline__ uint32_t quantise4(const float* xin, __half* s, __half* c) {
-  float x[4];
+// Codes of four values as 16 bits: (x - c) / s rounded to the nearest, ties to even, in fp32.  The
+// quotient is taken by an approximate reciprocal (to 2^-16 of a step) and by a true division only where
+// that comes within 2^-13 of a tie.
+__device__ __forceinline__ uint32_t codes4(const float* x, float s, float c, float inv) {
+  if (!(s > 0.0f)) return 0;
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+  float n[4];
+  bool near = false;
 #pragma unroll
-  for (int e = 0; e < 4; e++) x[e] = min_nan(max_nan(xin[e], -kKvMax), kKvMax);
-  float lo = min_nan(min_nan(x[0], x[1]), min_nan(x[2], x[3]));
-  float hi = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  for (int e = 0; e < 4; e++) {
+    const float q = fmaf(__fsub_rn(x[e], c), inv, -16.0f);
+    n[e] = __fsub_rn(__fadd_rn(q, kMagic), kMagic);
+    near |= !(fabsf(q - n[e]) < 0.5f - 0x1p-13f);
   }
-  float e;
-  const float d = sub_exact(hi, lo, &e);
-  const float q = __fdiv_rn(d, 15.0f);
-  *s = half_once(q, __fadd_rn(fmaf(-q, 15.0f, d), e));
-  const float sf = __half2float(*s);
-  const float b = sub_exact(lo, 16.0f * sf, &e);
-  *c = half_once(b, e);
-  const float cf = __half2float(*c);
-  uint32_t unit = 0;
-  if (sf > 0.0f) {
+  if (near) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float t = rintf(__fdiv_rn(__fsub_rn(x[e], cf), sf)) - 16.0f;
-      unit |= (uint32_t)fminf(fmaxf(t, 0.0f), 15.0f) << (4 * e);
-    }
+    for (int e = 0; e < 4; e++) n[e] = rintf(__fdiv_rn(__fsub_rn(x[e], c), s)) - 16.0f;
   }
-  return unit;
+#pragma unroll
+  for (int e = 0; e < 4; e++) n[e] = fminf(fmaxf(n[e], 0.0f), 15.0f);
+  return __float_as_uint(fmaf(n[3], 4096.0f, fmaf(n[2], 256.0f, fmaf(n[1], 16.0f, n[0]))) + 8388608.0f) & 0xFFFFu;
 }
 
 struct StoreArgs {
@@ -78,80 +62,355 @@ struct StoreArgs {
   int dt;
 };
 
-// The block of (layer, stream, token, head) and the position in it; null where there is none.
+// Storing is done in groups of 8 positions that lie in one half of a block, HD / 4 lanes to a group (a
+// warp, or half of one with HD = 64), four dimensions a lane: K's and V's codes of such a group are
+// 4 * HD contiguous bytes each, its scales HD each.  The eight lanes of a scale group reduce the minima
+// and maxima of the eight rows together (each ends up with one row), so that s and c are worked out once
+// per row instead of in every lane.
 template <int HD>
-__device__ __forceinline__ uint8_t* locate(const StoreArgs& a, int l, int b, int t, int h, int* key) {
-  const int n = a.count != nullptr ? min(a.count[b], a.T) : a.T;
-  if (t >= n) return nullptr;
-  const int pos = a.start[b] + t;
-  if (pos < 0 || pos / kPage >= a.ld_table) return nullptr;
-  const int page = a.table[(size_t)b * a.ld_table + pos / kPage];
-  if (page < 0 || page >= a.P) return nullptr;
-  *key = pos & (kBlk - 1);
-  return a.pool + l * a.layer_bytes +
-         (((size_t)page * a.NKV + h) * 4 + ((pos & (kPage - 1)) >> 4)) * kv4_block_bytes(HD);
+struct Group {
+  uint8_t* blk;  // null: nowhere
+  int half;      // which half of the block
+  int t0;        // token of the group's first position (may be negative)
+  int n;         // tokens of the stream
+  int layer, b, h;
+  __device__ __forceinline__ bool has(int r) const { return blk != nullptr && t0 + r >= 0 && t0 + r < n; }
+};
+template <int HD>
+__device__ __forceinline__ Group<HD> group_of(const StoreArgs& a, int groups, long i) {
+  Group<HD> g;
+  g.h = (int)(i % a.NKV);
+  i /= a.NKV;
+  const int k = (int)(i % groups);
+  i /= groups;
+  g.b = (int)(i % a.B);
+  g.layer = (int)(i / a.B);
+  g.blk = nullptr;
+  g.n = g.t0 = g.half = 0;
+  if (g.layer >= a.L) return g;
+  g.n = a.count != nullptr ? min(a.count[g.b], a.T) : a.T;
+  const int start = a.start[g.b], pos = (start & ~7) + 8 * k;  // of the group; start may be negative
+  g.t0 = pos - start;
+  g.half = (pos & 8) >> 3;
+  if (pos < 0 || g.t0 >= g.n || pos / kPage >= a.ld_table) return g;
+  const int page = a.table[(size_t)g.b * a.ld_table + pos / kPage];
+  if (page < 0 || page >= a.P) return g;
+  g.blk = a.pool + g.layer * a.layer_bytes +
+          (((size_t)page * a.NKV + g.h) * 4 + ((pos & (kPage - 1)) >> 4)) * kv4_block_bytes(HD);
+  return g;
 }
 
-// One row (a position of a kv head) per HD / 4 lanes, four dimensions a lane.
-template <int HD>
-__global__ void __launch_bounds__(256) kv4_store_kernel(StoreArgs a) {
-  constexpr int LPR = HD / 4;
-  const long rows = (long)a.L * a.B * a.T * a.NKV;
-  const long r = ((long)blockIdx.x * 256 + threadIdx.x) / LPR;
-  const int l = threadIdx.x % LPR;
-  const bool in = r < rows;
-  const long rr = in ? r : 0;
-  const int h = (int)(rr % a.NKV), t = (int)(rr / a.NKV % a.T), b = (int)(rr / a.NKV / a.T % a.B);
-  const int layer = (int)(rr / a.NKV / a.T / a.B);
-  int key = 0;
-  uint8_t* blk = in ? locate<HD>(a, layer, b, t, h, &key) : nullptr;
+template <int DT, bool VEC>
+struct Raw4 {  // four elements as loaded
+  uint32_t w[DT == DT_F32 ? 4 : 2];
+  __device__ __forceinline__ void load(const void* p, size_t at) {
+    if constexpr (DT == DT_F32) {
+      const uint32_t* q = (const uint32_t*)p + at;
+      if constexpr (VEC) {
+        const uint4 u = *(const uint4*)q;
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+      } else {
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
-    const long* st = w ? a.vs : a.ks;
-    const size_t at = (size_t)(layer * st[0] + b * st[1] + t * st[2] + h * st[3]) + 4 * l;
+        for (int e = 0; e < 4; e++) w[e] = q[e];
+      }
+    } else {
+      const uint16_t* q = (const uint16_t*)p + at;
+      if constexpr (VEC) {
+        const uint2 u = *(const uint2*)q;
+        w[0] = u.x; w[1] = u.y;
+      } else {
+        w[0] = (uint32_t)q[0] | (uint32_t)q[1] << 16;
+        w[1] = (uint32_t)q[2] | (uint32_t)q[3] << 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float* x) const {
+    if constexpr (DT == DT_F32) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = __uint_as_float(w[e]);
+    } else if constexpr (DT == DT_BF16) {
+      x[0] = bf_lo(w[0]); x[1] = bf_hi(w[0]); x[2] = bf_lo(w[1]); x[3] = bf_hi(w[1]);
+    } else {
+      const float2 u = __half22float2(*(const __half2*)&w[0]), v = __half22float2(*(const __half2*)&w[1]);
+      x[0] = u.x; x[1] = u.y; x[2] = v.x; x[3] = v.y;
+    }
+  }
+};
+
+// Eight rows of one tensor -> this lane's units of the rows, and (s, c) of row l & 7.
+template <int DT, bool VEC>
+__device__ __forceinline__ __half2 quantise8(const Raw4<DT, VEC> (&raw)[8], int l, uint32_t (&unit)[8]) {
+  float lo[8], hi[8];
+#pragma unroll
+  for (int r = 0; r < 8; r++) {
     float x[4];
+    raw[r].get(x);
+    lo[r] = min_nan(min_nan(x[0], x[1]), min_nan(x[2], x[3]));
+    hi[r] = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+  }
 #pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = blk ? load1(w ? a.v : a.k, at + e, a.dt) : 0.0f;
-    __half s, c;
-    const uint32_t unit = quantise4(x, &s, &c);
-    if (blk != nullptr) {
-      *(uint16_t*)(blk + (w ? v_unit<HD>(key, l) : k_unit<HD>(key, l))) = (uint16_t)unit;
-      if ((l & 7) == 0) {
-        if (w) {
-          __half* d = (__half*)(blk + v_scale<HD>(key, l >> 3));
-          d[0] = s;
-          d[2] = c;
-        } else {
-          __half* d = (__half*)(blk + k_scale<HD>(key, l >> 3));
-          d[0] = s;
-          d[1] = c;
+  for (int o = 4; o > 0; o >>= 1) {
+    const bool up = (l & o) != 0;
+#pragma unroll
+    for (int r = 0; r < o; r++) {
+      const float a = __shfl_xor_sync(0xffffffffu, up ? lo[r] : lo[r + o], o);
+      const float b = __shfl_xor_sync(0xffffffffu, up ? hi[r] : hi[r + o], o);
+      lo[r] = min_nan(up ? lo[r + o] : lo[r], a);
+      hi[r] = max_nan(up ? hi[r + o] : hi[r], b);
+    }
+  }
+  const bool wild = __any_sync(0xffffffffu, !(lo[0] >= -kKvMax && hi[0] <= kKvMax));
+  const __half2 sc = wild ? group_scale(held_to(lo[0]), held_to(hi[0])) : group_scale(lo[0], hi[0]);
+  const uint32_t bits = *(const uint32_t*)&sc;
+#pragma unroll
+  for (int r = 0; r < 8; r++) {
+    const uint32_t u = __shfl_sync(0xffffffffu, bits, r, 8);
+    const float2 f = __half22float2(*(const __half2*)&u);
+    float x[4];
+    raw[r].get(x);
+    if (wild) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = held_to(x[e]);
+    }
+    unit[r] = codes4(x, f.x, f.y, __fdividef(1.0f, f.x));
+  }
+  return sc;
+}
+
+template <int HD, int DT, bool VEC>
+__global__ void __launch_bounds__(128) kv4_store_kernel(StoreArgs a, int groups) {
+  constexpr int LPG = HD / 4, NG = HD / 32;
+  const long i = ((long)blockIdx.x * 128 + threadIdx.x) / LPG;
+  const int l = threadIdx.x % LPG;
+  const Group<HD> g = group_of<HD>(a, groups, i);
+  if (__all_sync(0xffffffffu, g.blk == nullptr)) return;
+  Raw4<DT, VEC> k[8], v[8];
+  const size_t ka = (size_t)(g.layer * a.ks[0] + g.b * a.ks[1] + g.t0 * a.ks[2] + g.h * a.ks[3]) + 4 * l;
+  const size_t va = (size_t)(g.layer * a.vs[0] + g.b * a.vs[1] + g.t0 * a.vs[2] + g.h * a.vs[3]) + 4 * l;
+#pragma unroll
+  for (int r = 0; r < 8; r++) {
+#pragma unroll
+    for (uint32_t& w : k[r].w) w = 0;
+#pragma unroll
+    for (uint32_t& w : v[r].w) w = 0;
+    if (g.has(r)) {
+      k[r].load(a.k, ka + (size_t)(r * a.ks[2]));
+      v[r].load(a.v, va + (size_t)(r * a.vs[2]));
+    }
+  }
+  uint32_t unit[8];
+  const int r0 = l & 7, j = l >> 3;
+  {
+    const __half2 sc = quantise8<DT, VEC>(k, l, unit);
+    uint8_t* rows = g.blk + g.half * 4 * HD;  // of the group's first position
+    if (g.has(r0)) *(__half2*)(g.blk + k_scale<HD>(g.half * 8 + r0, j)) = sc;
+    // a word is two lanes' units: even lanes put together the even rows', odd lanes the odd rows'
+#pragma unroll
+    for (int r = 0; r < 8; r += 2) {
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, l & 1 ? unit[r] : unit[r + 1], 1);
+      const int mine = r + (l & 1);
+      if (g.has(mine))
+        *(uint32_t*)(rows + mine * (HD / 2) + (((l & 7) >> 1) * NG + j) * 4) = l & 1 ? o | unit[r + 1] << 16 : unit[r] | o << 16;
+    }
+  }
+  {
+    const __half2 sc = quantise8<DT, VEC>(v, l, unit);
+    {
+      const uint32_t s = __half_as_ushort(__low2half(sc)), c = __half_as_ushort(__high2half(sc));
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, l & 1 ? s : c, 1);
+      uint8_t* p = g.blk + v_scale<HD>(g.half * 8 + (r0 & 6), j);
+      if (g.has(r0) && g.has(r0 ^ 1)) {
+        *(uint32_t*)(p + (l & 1) * 4) = l & 1 ? o | c << 16 : s | o << 16;
+      } else if (g.has(r0)) {
+        *(uint16_t*)(p + (l & 1) * 2) = (uint16_t)s;
+        *(uint16_t*)(p + 4 + (l & 1) * 2) = (uint16_t)c;
+      }
+    }
+    // pairs of keys, exchanged among the NG lanes that hold the groups of one g: lane j gets the pairs
+    // j (HD 128), or j and j + 2 (HD 64), of all groups
+    uint32_t pr[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) pr[q] = unit[2 * q] | unit[2 * q + 1] << 16;
+    uint8_t* p = g.blk + 8 * HD + (g.half * 8 + (l & 7)) * 8 * (2 * NG);
+    if constexpr (NG == 4) {
+      // after both exchanges pr[x] is group x's units of pair j
+#pragma unroll
+      for (int q = 0; q < 2; q++) {  // with lane j ^ 2: keep pairs of own half
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, j & 2 ? pr[q] : pr[q + 2], 16);
+        const uint32_t m = j & 2 ? pr[q + 2] : pr[q];
+        pr[q] = j & 2 ? o : m;      // from groups 0/1
+        pr[q + 2] = j & 2 ? m : o;  // from groups 2/3
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 2; q++) {  // with lane j ^ 1
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, j & 1 ? pr[2 * q] : pr[2 * q + 1], 8);
+        const uint32_t m = j & 1 ? pr[2 * q + 1] : pr[2 * q];
+        w[2 * q] = j & 1 ? o : m;
+        w[2 * q + 1] = j & 1 ? m : o;
+      }
+      const uint2 a0 = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+      const uint2 a1 = make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+      const bool h0 = g.has(2 * j), h1 = g.has(2 * j + 1);
+      if (h0 && h1) {
+        *(uint4*)(p + j * 16) = make_uint4(a0.x, a0.y, a1.x, a1.y);
+      } else if (h0) {
+        *(uint2*)(p + j * 16) = a0;
+      } else if (h1) {
+        *(uint2*)(p + j * 16 + 8) = a1;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2; q++) {  // lane j = 0 takes pairs 0 and 2, lane 1 pairs 1 and 3
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, j ? pr[2 * q] : pr[2 * q + 1], 8);
+        const uint32_t m = j ? pr[2 * q + 1] : pr[2 * q];
+        const uint32_t u0 = j ? o : m, u1 = j ? m : o;  // of groups 0 and 1
+        const uint32_t a0 = __byte_perm(u0, u1, 0x5410), a1 = __byte_perm(u0, u1, 0x7632);
+        const int pair = 2 * q + j;
+        const bool h0 = g.has(2 * pair), h1 = g.has(2 * pair + 1);
+        if (h0 && h1) {
+          *(uint2*)(p + pair * 8) = make_uint2(a0, a1);
+        } else if (h0) {
+          *(uint32_t*)(p + pair * 8) = a0;
+        } else if (h1) {
+          *(uint32_t*)(p + pair * 8 + 4) = a1;
         }
       }
     }
   }
 }
 
-// The inverse: rows of positions -> values [L][B][T][NKV][HD], zeros where nothing is stored.
-template <int HD>
-__global__ void __launch_bounds__(256) kv4_load_kernel(StoreArgs a, void* ko, void* vo) {
-  constexpr int LPR = HD / 4;
-  const long rows = (long)a.L * a.B * a.T * a.NKV;
-  const long r = ((long)blockIdx.x * 256 + threadIdx.x) / LPR;
-  const int l = threadIdx.x % LPR;
-  if (r >= rows) return;
-  const int h = (int)(r % a.NKV), t = (int)(r / a.NKV % a.T), b = (int)(r / a.NKV / a.T % a.B);
-  const int layer = (int)(r / a.NKV / a.T / a.B);
-  int key = 0;
-  const uint8_t* blk = locate<HD>(a, layer, b, t, h, &key);
+// Eight fp16 values, or their half of four, to the output type; VEC: 16-byte aligned rows.
+template <int DT, int N>
+__device__ __forceinline__ void put(void* p, size_t at, const uint32_t (&w)[N]) {  // 2 N values
+  if constexpr (DT == DT_F16) {
+    __half* q = (__half*)p + at;
+    if constexpr (N == 4) *(uint4*)q = make_uint4(w[0], w[1], w[2], w[3]);
+    else *(uint2*)q = make_uint2(w[0], w[1]);
+  } else {
+    float x[2 * N];
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
-    __half o[4] = {};
-    if (blk != nullptr) {
-      const __half* d = (const __half*)(blk + (w ? v_scale<HD>(key, l >> 3) : k_scale<HD>(key, l >> 3)));
-      kv4_values(*(const uint16_t*)(blk + (w ? v_unit<HD>(key, l) : k_unit<HD>(key, l))), d[0], d[w ? 2 : 1], o);
+    for (int i = 0; i < N; i++) {
+      const float2 f = __half22float2(*(const __half2*)&w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
     }
+    if constexpr (DT == DT_F32) {
+      float* q = (float*)p + at;
 #pragma unroll
-    for (int e = 0; e < 4; e++) store1(w ? vo : ko, (size_t)r * HD + 4 * l + e, a.dt, __half2float(o[e]));
+      for (int i = 0; i < N / 2; i++) ((float4*)q)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    } else {
+      uint16_t* q = (uint16_t*)p + at;
+      uint32_t b[N];
+#pragma unroll
+      for (int i = 0; i < N; i++) b[i] = (uint32_t)f2bf_bits(x[2 * i]) | (uint32_t)f2bf_bits(x[2 * i + 1]) << 16;
+      if constexpr (N == 4) *(uint4*)q = make_uint4(b[0], b[1], b[2], b[3]);
+      else *(uint2*)q = make_uint2(b[0], b[1]);
+    }
+  }
+}
+
+// The inverse, by the same groups of 8 positions; rows outside the cache become zeros.
+template <int HD, int DT>
+__global__ void __launch_bounds__(128) kv4_load_kernel(StoreArgs a, int groups, void* ko, void* vo) {
+  constexpr int LPG = HD / 4, NG = HD / 32;
+  const long i = ((long)blockIdx.x * 128 + threadIdx.x) / LPG;
+  const int l = threadIdx.x % LPG;
+  const Group<HD> g = group_of<HD>(a, groups, i);
+  if (g.layer >= a.L) return;
+  // row of token t0 + r
+  auto row = [&](int r) { return ((((size_t)g.layer * a.B + g.b) * a.T + (g.t0 + r)) * a.NKV + g.h) * HD; };
+  auto want = [&](int r) { return g.t0 + r >= 0 && g.t0 + r < a.T; };
+  if constexpr (NG == 4) {
+    {
+      const int r = l >> 2, t = l & 3, key = g.half * 8 + r;
+      uint4 w = make_uint4(0, 0, 0, 0), sc = w;
+      if (g.has(r)) {
+        w = *(const uint4*)(g.blk + key * 64 + t * 16);
+        sc = *(const uint4*)(g.blk + 16 * HD + key * 16);
+      }
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w}, ss[4] = {sc.x, sc.y, sc.z, sc.w};
+      if (want(r)) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          uint32_t v[4];
+          decode_word(ww[j], __low2half2(*(const __half2*)&ss[j]), __high2half2(*(const __half2*)&ss[j]), v);
+          const uint32_t o[4] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                                 __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)};
+          put<DT>(ko, row(r) + 32 * j + 8 * t, o);
+        }
+      }
+    }
+    {
+      const int gg = l >> 2, t = l & 3;
+      const bool h0 = g.has(2 * t), h1 = g.has(2 * t + 1);
+      uint4 w = make_uint4(0, 0, 0, 0), s0 = w, s1 = w;
+      if (h0 || h1) {
+        w = *(const uint4*)(g.blk + 8 * HD + g.half * 512 + gg * 64 + t * 16);
+        const uint8_t* sp = g.blk + 18 * HD + (g.half * 4 + t) * 32;
+        s0 = *(const uint4*)sp;
+        s1 = *(const uint4*)(sp + 16);
+      }
+      const uint32_t keep = (h0 ? 0xFFFFu : 0u) | (h1 ? 0xFFFF0000u : 0u);
+      const uint32_t vs[4] = {s0.x & keep, s0.z & keep, s1.x & keep, s1.z & keep};
+      const uint32_t vc[4] = {s0.y & keep, s0.w & keep, s1.y & keep, s1.w & keep};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        uint32_t v[4];
+        decode_word(j < 2 ? __byte_perm(w.x, w.z, j & 1 ? 0x7632 : 0x5410) : __byte_perm(w.y, w.w, j & 1 ? 0x7632 : 0x5410),
+                    *(const __half2*)&vs[j], *(const __half2*)&vc[j], v);
+        const uint32_t o0[2] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410)};
+        const uint32_t o1[2] = {__byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)};
+        if (want(2 * t)) put<DT>(vo, row(2 * t) + 32 * j + 4 * gg, o0);
+        if (want(2 * t + 1)) put<DT>(vo, row(2 * t + 1) + 32 * j + 4 * gg, o1);
+      }
+    }
+  } else {
+    {
+      const int r = l >> 1, t2 = (l & 1) * 2, key = g.half * 8 + r;  // words of t2 and t2 + 1
+      uint4 w = make_uint4(0, 0, 0, 0);
+      uint2 sc = make_uint2(0, 0);
+      if (g.has(r)) {
+        w = *(const uint4*)(g.blk + key * 32 + t2 * 8);
+        sc = *(const uint2*)(g.blk + 16 * HD + key * 8);
+      }
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w}, ss[2] = {sc.x, sc.y};
+      if (want(r)) {
+#pragma unroll
+        for (int x = 0; x < 4; x++) {  // t = t2 + x / 2, j = x & 1
+          uint32_t v[4];
+          decode_word(ww[x], __low2half2(*(const __half2*)&ss[x & 1]), __high2half2(*(const __half2*)&ss[x & 1]), v);
+          const uint32_t o[4] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                                 __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)};
+          put<DT>(ko, row(r) + 32 * (x & 1) + 8 * (t2 + x / 2), o);
+        }
+      }
+    }
+    {
+      const int gg = l >> 1;
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        const int t = (l & 1) + 2 * y;
+        const bool h0 = g.has(2 * t), h1 = g.has(2 * t + 1);
+        uint2 w = make_uint2(0, 0);
+        uint4 s0 = make_uint4(0, 0, 0, 0);
+        if (h0 || h1) {
+          w = *(const uint2*)(g.blk + 8 * HD + g.half * 256 + gg * 32 + t * 8);
+          s0 = *(const uint4*)(g.blk + 18 * HD + (g.half * 4 + t) * 16);
+        }
+        const uint32_t keep = (h0 ? 0xFFFFu : 0u) | (h1 ? 0xFFFF0000u : 0u);
+        const uint32_t vs[2] = {s0.x & keep, s0.z & keep}, vc[2] = {s0.y & keep, s0.w & keep};
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          uint32_t v[4];
+          decode_word(__byte_perm(w.x, w.y, j ? 0x7632 : 0x5410), *(const __half2*)&vs[j], *(const __half2*)&vc[j], v);
+          const uint32_t o0[2] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410)};
+          const uint32_t o1[2] = {__byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)};
+          if (want(2 * t)) put<DT>(vo, row(2 * t) + 32 * j + 4 * gg, o0);
+          if (want(2 * t + 1)) put<DT>(vo, row(2 * t + 1) + 32 * j + 4 * gg, o1);
+        }
+      }
+    }
   }
 }
 
@@ -196,14 +455,22 @@ extern "C" int rngd_kv4_store(void* pool, size_t layer_bytes, int P, int NKV, in
     a.ks[i] = (long)k_strides[i];
     a.vs[i] = (long)v_strides[i];
   }
-  const long rows = (long)L * B * T * NKV;
-  if (rows == 0) return RNGD_OK;
-  const long blocks = (rows * (HD / 4) + 255) / 256;
-  RNGD_REQUIRE(blocks < (1l << 31), "kv4_store: %ld rows in one call", rows);
-  if (HD == 128)
-    kv4_store_kernel<128><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
-  else
-    kv4_store_kernel<64><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
+  if (B == 0 || T == 0) return RNGD_OK;
+  const int groups = (T + 14) / 8;  // groups of 8 aligned positions that T positions can touch
+  const long blocks = ((long)L * B * groups * NKV * (HD / 4) + 127) / 128;
+  RNGD_REQUIRE(blocks < (1l << 31), "kv4_store: %ld groups of rows in one call", blocks);
+  const int lane_bytes = dtype == DT_F32 ? 16 : 8, esz = lane_bytes / 4;
+  bool vec = ((uintptr_t)k | (uintptr_t)v) % lane_bytes == 0;
+  for (int i = 0; i < 4; i++) vec = vec && a.ks[i] * esz % lane_bytes == 0 && a.vs[i] * esz % lane_bytes == 0;
+  typedef void (*Kernel)(StoreArgs, int);
+  static const Kernel kernels[2][3][2] = {
+      {{kv4_store_kernel<64, DT_BF16, false>, kv4_store_kernel<64, DT_BF16, true>},
+       {kv4_store_kernel<64, DT_F16, false>, kv4_store_kernel<64, DT_F16, true>},
+       {kv4_store_kernel<64, DT_F32, false>, kv4_store_kernel<64, DT_F32, true>}},
+      {{kv4_store_kernel<128, DT_BF16, false>, kv4_store_kernel<128, DT_BF16, true>},
+       {kv4_store_kernel<128, DT_F16, false>, kv4_store_kernel<128, DT_F16, true>},
+       {kv4_store_kernel<128, DT_F32, false>, kv4_store_kernel<128, DT_F32, true>}}};
+  kernels[HD == 128][dtype][vec]<<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a, groups);
   return check_launch("kv4_store_kernel");
 }
 
@@ -213,13 +480,15 @@ extern "C" int rngd_kv4_load(const void* pool, size_t layer_bytes, int P, int NK
   StoreArgs a;
   RNGD_TRY(store_args("kv4_load", &a, (void*)pool, layer_bytes, P, NKV, HD, L, table, ld_table, start, count, B, T, k,
                       v, dtype));
-  const long rows = (long)L * B * T * NKV;
-  if (rows == 0) return RNGD_OK;
-  const long blocks = (rows * (HD / 4) + 255) / 256;
-  RNGD_REQUIRE(blocks < (1l << 31), "kv4_load: %ld rows in one call", rows);
-  if (HD == 128)
-    kv4_load_kernel<128><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a, k, v);
-  else
-    kv4_load_kernel<64><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a, k, v);
+  if (B == 0 || T == 0) return RNGD_OK;
+  RNGD_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "kv4_load: k and v must be 16-byte aligned");
+  const int groups = (T + 14) / 8;
+  const long blocks = ((long)L * B * groups * NKV * (HD / 4) + 127) / 128;
+  RNGD_REQUIRE(blocks < (1l << 31), "kv4_load: %ld groups of rows in one call", blocks);
+  typedef void (*Kernel)(StoreArgs, int, void*, void*);
+  static const Kernel kernels[2][3] = {
+      {kv4_load_kernel<64, DT_BF16>, kv4_load_kernel<64, DT_F16>, kv4_load_kernel<64, DT_F32>},
+      {kv4_load_kernel<128, DT_BF16>, kv4_load_kernel<128, DT_F16>, kv4_load_kernel<128, DT_F32>}};
+  kernels[HD == 128][dtype]<<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a, groups, k, v);
   return check_launch("kv4_load_kernel");
 }

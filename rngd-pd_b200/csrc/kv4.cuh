@@ -2,7 +2,8 @@
 //
 // A page holds 64 positions of one layer: [NKV][4 blocks][20 * HD bytes], a block being 16
 // positions of one kv head.  Along the head dimension every 32 values share two fp16 numbers
-// (s, c); a 4-bit code u stands for fp16(s * (16 + u) + c).  With NG = HD / 32 a block is
+// (s, c); a 4-bit code u stands for fp16(s * (16 + u) + c).  Storing takes s = fp16((max - min) * (1 / 15)),
+// c = fp16(min - 16 s) and u = rint((x - c) / s) - 16 held to 0..15, each step in fp32.  With NG = HD / 32 a block is
 //   K codes   [16 keys][t 0..3][j 0..NG-1][4 B]        nibble e of the word: dimension 32 j + 8 t + e
 //   V codes   [2][g 0..7][8 keys][j 0..NG-1][2 B]      nibble e of the half word: dimension 32 j + 4 g + e
 //   K scales  [16 keys][NG][s, c]
@@ -29,17 +30,7 @@ enum : int { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
 __host__ __device__ constexpr int kv4_block_bytes(int HD) { return 20 * HD; }
 __host__ __device__ constexpr size_t kv4_page_bytes(int NKV, int HD) { return (size_t)NKV * 4 * 20 * HD; }
 
-// Byte offsets inside a block of the 4-dimension unit `l` (dimensions 4l .. 4l+3) of position `key`.
-template <int HD>
-__device__ __forceinline__ int k_unit(int key, int l) {
-  constexpr int NG = HD / 32;
-  return key * (HD / 2) + ((((l & 7) >> 1) * NG + (l >> 3)) << 2) + ((l & 1) << 1);
-}
-template <int HD>
-__device__ __forceinline__ int v_unit(int key, int l) {
-  constexpr int NG = HD / 32;
-  return 8 * HD + (((key >> 3) * 8 + (l & 7)) * 8 + (key & 7)) * (2 * NG) + ((l >> 3) << 1);
-}
+// Byte offsets of a scale inside a block.
 template <int HD>
 __device__ __forceinline__ int k_scale(int key, int j) {  // s, c: 4 bytes
   return 16 * HD + (key * (HD / 32) + j) * 4;
@@ -49,13 +40,22 @@ __device__ __forceinline__ int v_scale(int key, int j) {  // s at +0, c at +4
   return 18 * HD + (((key >> 3) * 4 + ((key & 7) >> 1)) * (HD / 32) + j) * 8 + (key & 1) * 2;
 }
 
-// Four codes -> the four values they stand for.
-__device__ __forceinline__ void kv4_values(uint32_t unit, __half s, __half c, __half* out) {
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const __half x = __ushort_as_half((unsigned short)(0x4C00u | (((unit >> (4 * e)) & 15u) << 6)));
-    out[e] = __hfma(x, s, c);
-  }
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+
+// (a & m) | o as one instruction: left to itself the compiler moves the mask ahead of the shift and
+// takes a third one (15% of the kernel's time).
+__device__ __forceinline__ uint32_t lop_ao(uint32_t a, uint32_t m, uint32_t o) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(m), "r"(o));
+  return r;
+}
+// The four pairs (nibble i of the low half, nibble i of the high half) of w -> values.
+__device__ __forceinline__ void decode_word(uint32_t w, __half2 s, __half2 c, uint32_t (&v)[4]) {
+  v[0] = h2u(__hfma2(u2h(lop_ao(w << 6, 0x03C003C0u, 0x4C004C00u)), s, c));
+  v[1] = h2u(__hfma2(u2h(lop_ao(w << 2, 0x03C003C0u, 0x4C004C00u)), s, c));
+  v[2] = h2u(__hfma2(u2h(lop_ao(w >> 2, 0x03C003C0u, 0x4C004C00u)), s, c));
+  v[3] = h2u(__hfma2(u2h(lop_ao(w >> 6, 0x03C003C0u, 0x4C004C00u)), s, c));
 }
 
 __device__ __forceinline__ float load1(const void* p, size_t i, int dt) {

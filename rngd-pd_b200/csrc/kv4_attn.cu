@@ -69,24 +69,6 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
-
-// (a & m) | o as one instruction: left to itself the compiler moves the mask ahead of the shift and
-// takes a third one (15% of the kernel's time).
-__device__ __forceinline__ uint32_t lop_ao(uint32_t a, uint32_t m, uint32_t o) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(m), "r"(o));
-  return r;
-}
-// The four pairs (nibble i of the low half, nibble i of the high half) of w -> values.
-__device__ __forceinline__ void decode_word(uint32_t w, __half2 s, __half2 c, uint32_t (&v)[4]) {
-  v[0] = h2u(__hfma2(u2h(lop_ao(w << 6, 0x03C003C0u, 0x4C004C00u)), s, c));
-  v[1] = h2u(__hfma2(u2h(lop_ao(w << 2, 0x03C003C0u, 0x4C004C00u)), s, c));
-  v[2] = h2u(__hfma2(u2h(lop_ao(w >> 2, 0x03C003C0u, 0x4C004C00u)), s, c));
-  v[3] = h2u(__hfma2(u2h(lop_ao(w >> 6, 0x03C003C0u, 0x4C004C00u)), s, c));
-}
-
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                    smem_u32(dst)),

@@ -5,13 +5,16 @@ PAGE = 64
 
 
 def encode(x):
-    """x [..., HD] float64 -> codes [..., HD], s, c [..., HD / 32] (float64 holding fp16 numbers)."""
+    """x [..., HD] -> codes [..., HD], s, c [..., HD / 32] (float64 holding fp16 numbers), and how far each quotient is
+    from a tie.  s and c are formed in fp32 and rounded to fp16, as the format has it; the rest is in 64 bits."""
     x = np.clip(x, -16384.0, 16384.0)  # keeps NaN
     g = x.reshape(*x.shape[:-1], -1, 32)
     lo, hi = g.min(-1), g.max(-1)
     with np.errstate(all="ignore"):
-        s = ((hi - lo) / 15).astype(np.float16).astype(np.float64)
-        c = (lo - 16 * s).astype(np.float16).astype(np.float64)
+        lo4, hi4 = lo.astype(np.float32), hi.astype(np.float32)
+        s4 = ((hi4 - lo4) * (np.float32(1) / np.float32(15))).astype(np.float16)
+        c4 = (lo4 - np.float32(16) * s4.astype(np.float32)).astype(np.float16)
+        s, c = s4.astype(np.float64), c4.astype(np.float64)
         t = (g - c[..., None]) / s[..., None] - 16
         u = np.where(s[..., None] > 0, np.clip(np.rint(t), 0, 15), 0)
         tie = np.where(s[..., None] > 0, np.abs(t - np.floor(t) - 0.5), 1.0)  # distance from a tie, in steps
