@@ -26,27 +26,33 @@ __device__ __forceinline__ __half2 group_scale(float lo, float hi) {
   return __halves2half2(s, __float2half_rn(__fsub_rn(lo, 16.0f * __half2float(s))));
 }
 
-// Codes of four values as 16 bits: (x - c) / s rounded to the nearest, ties to even, in fp32.  The
-// quotient is taken by an approximate reciprocal (to 2^-16 of a step) and by a true division only where
-// that comes within 2^-13 of a tie.
-__device__ __forceinline__ uint32_t codes4(const float* x, float s, float c, float inv) {
-  if (!(s > 0.0f)) return 0;
-  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
-  float n[4];
-  bool near = false;
+// (x - c) / s rounded to the nearest, ties to even, in fp32, held to a code.
+__device__ __noinline__ uint32_t codes4_slow(float x0, float x1, float x2, float x3, float s, float c) {
+  const float x[4] = {x0, x1, x2, x3};
+  uint32_t unit = 0;
+  for (int e = 0; e < 4; e++) {
+    const float n = rintf(__fdiv_rn(__fsub_rn(x[e], c), s)) - 16.0f;
+    unit |= (uint32_t)fminf(fmaxf(n, 0.0f), 15.0f) << (4 * e);
+  }
+  return unit;
+}
+
+// Codes of four values as 16 bits.  inv ~ 1 / s and k ~ -c / s - 16 give the quotient to 2^-14 of a step
+// as long as |k| <= 512, and c and s lie near enough to the group's ends then (s >= 2^-17) that no code
+// leaves 0..15; whatever comes within 2^-12 of a tie, and other groups, take the true quotient.
+__device__ __forceinline__ uint32_t codes4(const float* x, float s, float c, float inv, float k) {
+  if (!(s > 0.0f)) return 0;  // a constant group, or one with a NaN
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, in the low bits
+  uint32_t m[4];
+  float off = 0.0f;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    const float q = fmaf(__fsub_rn(x[e], c), inv, -16.0f);
-    n[e] = __fsub_rn(__fadd_rn(q, kMagic), kMagic);
-    near |= !(fabsf(q - n[e]) < 0.5f - 0x1p-13f);
+    const float q = fmaf(x[e], inv, k), n = __fadd_rn(q, kMagic);
+    m[e] = __float_as_uint(n);
+    off = fmaxf(off, fabsf(__fsub_rn(q, __fsub_rn(n, kMagic))));
   }
-  if (near) {
-#pragma unroll
-    for (int e = 0; e < 4; e++) n[e] = rintf(__fdiv_rn(__fsub_rn(x[e], c), s)) - 16.0f;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; e++) n[e] = fminf(fmaxf(n[e], 0.0f), 15.0f);
-  return __float_as_uint(fmaf(n[3], 4096.0f, fmaf(n[2], 256.0f, fmaf(n[1], 16.0f, n[0]))) + 8388608.0f) & 0xFFFFu;
+  if (!(off < 0.5f - 0x1p-12f && s >= 0x1p-17f && fabsf(k) <= 512.0f)) return codes4_slow(x[0], x[1], x[2], x[3], s, c);
+  return (m[0] + m[1] * 16u + m[2] * 256u + m[3] * 4096u) & 0xFFFFu;
 }
 
 struct StoreArgs {
@@ -137,42 +143,88 @@ struct Raw4 {  // four elements as loaded
   }
 };
 
-// Eight rows of one tensor -> this lane's units of the rows, and (s, c) of row l & 7.
-template <int DT, bool VEC>
-__device__ __forceinline__ __half2 quantise8(const Raw4<DT, VEC> (&raw)[8], int l, uint32_t (&unit)[8]) {
-  float lo[8], hi[8];
+// The least of some values and of their negatives, as the bits that shuffles move: two 16-bit numbers in
+// a word, or two floats.  A NaN stays.
+template <int DT>
+struct Ends {
+  uint32_t w[DT == DT_F32 ? 2 : 1];
+  __device__ __forceinline__ void least(const Ends& o) {
+    if constexpr (DT == DT_F32) {
 #pragma unroll
-  for (int r = 0; r < 8; r++) {
-    float x[4];
-    raw[r].get(x);
-    lo[r] = min_nan(min_nan(x[0], x[1]), min_nan(x[2], x[3]));
-    hi[r] = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+      for (int i = 0; i < 2; i++) w[i] = __float_as_uint(min_nan(__uint_as_float(w[i]), __uint_as_float(o.w[i])));
+    } else {
+      w[0] = min2(w[0], o.w[0]);
+    }
   }
+  static __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (DT == DT_BF16)
+      asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+      asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  template <bool VEC>
+  __device__ __forceinline__ void of(const Raw4<DT, VEC>& x) {
+    if constexpr (DT == DT_F32) {
+      float v[4];
+      x.get(v);
+      w[0] = __float_as_uint(min_nan(min_nan(v[0], v[1]), min_nan(v[2], v[3])));
+      w[1] = __float_as_uint(-max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])));
+    } else {
+      const uint32_t a = min2(x.w[0], x.w[1]), b = min2(x.w[0] ^ 0x80008000u, x.w[1] ^ 0x80008000u);
+      w[0] = min2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+    }
+  }
+  __device__ __forceinline__ float2 get() const {  // lo, hi
+    if constexpr (DT == DT_F32) return make_float2(__uint_as_float(w[0]), -__uint_as_float(w[1]));
+    if constexpr (DT == DT_BF16) return make_float2(bf_lo(w[0]), -bf_hi(w[0]));
+    const float2 f = __half22float2(*(const __half2*)&w[0]);
+    return make_float2(f.x, -f.y);
+  }
+};
+
+// Eight rows of one tensor -> this lane's units of the rows, and (s, c) of row l & 7.  there: the rows
+// that any lane of the warp holds (one of them, when a decode step appends).
+template <int DT, bool VEC>
+__device__ __forceinline__ __half2 quantise8(const Raw4<DT, VEC> (&raw)[8], int l, uint32_t there,
+                                             uint32_t (&unit)[8]) {
+  Ends<DT> e[8];
+#pragma unroll
+  for (int r = 0; r < 8; r++) e[r].of(raw[r]);
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) {
     const bool up = (l & o) != 0;
 #pragma unroll
     for (int r = 0; r < o; r++) {
-      const float a = __shfl_xor_sync(0xffffffffu, up ? lo[r] : lo[r + o], o);
-      const float b = __shfl_xor_sync(0xffffffffu, up ? hi[r] : hi[r + o], o);
-      lo[r] = min_nan(up ? lo[r + o] : lo[r], a);
-      hi[r] = max_nan(up ? hi[r + o] : hi[r], b);
+      Ends<DT> other;
+#pragma unroll
+      for (int i = 0; i < (DT == DT_F32 ? 2 : 1); i++) {
+        other.w[i] = __shfl_xor_sync(0xffffffffu, up ? e[r].w[i] : e[r + o].w[i], o);
+        e[r].w[i] = up ? e[r + o].w[i] : e[r].w[i];
+      }
+      e[r].least(other);
     }
   }
-  const bool wild = __any_sync(0xffffffffu, !(lo[0] >= -kKvMax && hi[0] <= kKvMax));
-  const __half2 sc = wild ? group_scale(held_to(lo[0]), held_to(hi[0])) : group_scale(lo[0], hi[0]);
+  const float2 ends = e[0].get();
+  const bool wild = __any_sync(0xffffffffu, !(ends.x >= -kKvMax && ends.y <= kKvMax));
+  const __half2 sc = wild ? group_scale(held_to(ends.x), held_to(ends.y)) : group_scale(ends.x, ends.y);
   const uint32_t bits = *(const uint32_t*)&sc;
 #pragma unroll
   for (int r = 0; r < 8; r++) {
+    unit[r] = 0;
+    if (!(there >> r & 1u)) continue;
     const uint32_t u = __shfl_sync(0xffffffffu, bits, r, 8);
     const float2 f = __half22float2(*(const __half2*)&u);
     float x[4];
     raw[r].get(x);
     if (wild) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = held_to(x[e]);
+      for (int i = 0; i < 4; i++) x[i] = held_to(x[i]);
     }
-    unit[r] = codes4(x, f.x, f.y, __fdividef(1.0f, f.x));
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(f.x));
+    unit[r] = codes4(x, f.x, f.y, inv, fmaf(-f.y, inv, -16.0f));
   }
   return sc;
 }
@@ -198,10 +250,13 @@ __global__ void __launch_bounds__(128) kv4_store_kernel(StoreArgs a, int groups)
       v[r].load(a.v, va + (size_t)(r * a.vs[2]));
     }
   }
-  uint32_t unit[8];
+  uint32_t unit[8], there = 0;
+#pragma unroll
+  for (int r = 0; r < 8; r++) there |= g.has(r) ? 1u << r : 0u;
+  there = __reduce_or_sync(0xffffffffu, there);
   const int r0 = l & 7, j = l >> 3;
   {
-    const __half2 sc = quantise8<DT, VEC>(k, l, unit);
+    const __half2 sc = quantise8<DT, VEC>(k, l, there, unit);
     uint8_t* rows = g.blk + g.half * 4 * HD;  // of the group's first position
     if (g.has(r0)) *(__half2*)(g.blk + k_scale<HD>(g.half * 8 + r0, j)) = sc;
     // a word is two lanes' units: even lanes put together the even rows', odd lanes the odd rows'
@@ -214,7 +269,7 @@ __global__ void __launch_bounds__(128) kv4_store_kernel(StoreArgs a, int groups)
     }
   }
   {
-    const __half2 sc = quantise8<DT, VEC>(v, l, unit);
+    const __half2 sc = quantise8<DT, VEC>(v, l, there, unit);
     {
       const uint32_t s = __half_as_ushort(__low2half(sc)), c = __half_as_ushort(__high2half(sc));
       const uint32_t o = __shfl_xor_sync(0xffffffffu, l & 1 ? s : c, 1);

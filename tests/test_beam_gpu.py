@@ -121,6 +121,23 @@ def test_rows_apart_and_odd_addresses():
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_a_vocabulary_too_large_for_the_list():
+    """Many chunks of many beams: the candidates are taken one after the other."""
+    g = torch.Generator().manual_seed(6)
+    logits = 3 * torch.randn(32, 500009, generator=g)
+    _, _, clear = _check(logits, -5 + torch.randn(32, generator=g), torch.arange(32) == 3, 32, 77)
+    assert clear.mean() > 0.9
+
+
+def test_equal_logits_in_many_places():
+    """The bound falls on a value that many places share: rows of few distinct values, and of two."""
+    g = torch.Generator().manual_seed(7)
+    for V in (2048, 9000, 40003):
+        logits = torch.randint(0, 40, (6, V), generator=g).float() / 8
+        logits[3:] = torch.randint(0, 2, (3, V), generator=g).float()
+        _check(logits, torch.tensor([0.0, -0.3, -0.7, 0.0, -0.1, -0.2]), torch.zeros(6, dtype=torch.bool), 3, 1)
+
+
 def test_select_refusals():
     from rngd_pd import beam
     x, s, d = torch.zeros(4, 100, device="cuda"), torch.zeros(4, device="cuda"), torch.zeros(4, dtype=torch.bool, device="cuda")
