@@ -366,7 +366,7 @@ int rngd_kv4_compact_workspace(int P, size_t* bytes);
 int rngd_beam_select(const void* logits, int dtype, int64_t ld, int R, int V, int W, const float* scores,
                      const uint8_t* done, int eos, float* out_scores, int32_t* parents, int32_t* tokens,
                      uint8_t* out_done, void* workspace, size_t workspace_bytes, rngd_stream_t stream);
-int rngd_beam_workspace(int R, int V, int W, size_t* bytes);
+int rngd_beam_workspace(int dtype, int R, int V, int W, size_t* bytes);
 
 #ifdef __cplusplus
 }

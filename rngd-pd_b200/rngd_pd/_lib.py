@@ -144,7 +144,7 @@ _sig("rngd_kv4_compact", _vp, _sz, _int, _int, _int, _int, _vp, _vp, _int, _int,
 _sig("rngd_kv4_compact_workspace", _int, _szp)
 _sig("rngd_beam_select", _vp, _int, ctypes.c_int64, _int, _int, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _sz,
      _vp)
-_sig("rngd_beam_workspace", _int, _int, _int, _szp)
+_sig("rngd_beam_workspace", _int, _int, _int, _int, _szp)
 
 
 def last_error():

@@ -46,7 +46,7 @@ def select(logits, scores, done, beams, eos=-1):
         parents = torch.empty(shape, dtype=torch.int32, device=dev)
         tokens = torch.empty_like(parents)
         ended = torch.empty(shape, dtype=torch.bool, device=dev)
-        need = _lib.workspace_bytes("rngd_beam_workspace", R, V, beams)
+        need = _lib.workspace_bytes("rngd_beam_workspace", _DT[logits.dtype], R, V, beams)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _lib.check(_select(logits.data_ptr(), _DT[logits.dtype], logits.stride(0), R, V, beams, scores.data_ptr(),
                            done.data_ptr(), eos, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),

@@ -129,6 +129,38 @@ def test_a_vocabulary_too_large_for_the_list():
     assert clear.mean() > 0.9
 
 
+@pytest.mark.parametrize("order", ["up", "down", "late", "steps"])
+def test_long_rows_whose_best_come_late(order):
+    """Many rows, each CTA goes through several chunks: rising logits fill the list of candidates again and again."""
+    W, R, V = 16, 320, 100003
+    g = torch.Generator().manual_seed(8)
+    base = torch.linspace(-20, 20, V)
+    if order == "up":
+        logits = base.repeat(R, 1) + 0.001 * torch.rand(R, 1, generator=g)
+    elif order == "down":
+        logits = base.flip(0).repeat(R, 1) + 0.001 * torch.rand(R, 1, generator=g)
+    elif order == "late":
+        logits = torch.randn(R, V, generator=g)
+        logits[:, 60000:] += 30
+    else:
+        logits = (torch.arange(V) // 3000).float().repeat(R, 1) / 4
+    _check(logits, torch.linspace(-3, 0, R), torch.zeros(R, dtype=torch.bool), W, 1)
+
+
+@pytest.mark.parametrize("keep", [1, 5, 40])
+def test_vocabulary_masked_to_a_few_tokens(keep):
+    """All but a few logits at -inf, anywhere in the row."""
+    W, R, V = 16, 320, 70001
+    g = torch.Generator().manual_seed(keep)
+    logits = torch.full((R, V), -np.inf)
+    at = torch.stack([torch.randperm(V, generator=g)[:keep] for _ in range(R)])
+    logits.scatter_(1, at, torch.randn(R, keep, generator=g))
+    _check(logits, torch.randn(R, generator=g), torch.arange(R) % 40 == 3, W, 1)
+    scores = torch.full((R,), -np.inf)
+    scores[::W] = 0.0
+    _check(logits, scores, torch.zeros(R, dtype=torch.bool), W, -1)
+
+
 def test_equal_logits_in_many_places():
     """The bound falls on a value that many places share: rows of few distinct values, and of two."""
     g = torch.Generator().manual_seed(7)
