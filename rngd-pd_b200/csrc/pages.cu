@@ -22,11 +22,14 @@ struct ForkArgs {
   int32_t* new_table;
   int32_t* new_lens;
   int32_t* short_out;
-  Move* moves;  // [R], blocks = 0: none
+  int* n_moves;
+  Move* moves;  // [R]
+  int* list;    // [R * (1 + ld)] free pages
   int P, R, ld, room;
 };
 
 constexpr int kMetaThreads = 1024;
+constexpr int kForkCtas = 8;  // one cluster
 
 // Exclusive prefix sum over the CTA; *total gets the sum.
 __device__ __forceinline__ int block_scan(int v, int* s_warp, int* total) {
@@ -54,29 +57,51 @@ __device__ __forceinline__ int block_scan(int v, int* s_warp, int* total) {
   return x - v + (w > 0 ? s_warp[w - 1] : 0);
 }
 
-// One CTA of 1024 threads, one thread per row for what is decided row by row.
-__global__ void __launch_bounds__(kMetaThreads) kv4_fork_kernel(ForkArgs a) {
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One cluster: its CTAs share the tables (counts go up and down by whole-number atomics), the first one
+// then decides row by row, a thread to each.  Latency is what it takes: two rounds of dependent loads over
+// the tables and a walk through the free pages.
+__global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads) kv4_fork_kernel(ForkArgs a) {
   __shared__ int s_warp[32];
-  __shared__ int s_tail[kMetaThreads];
-  const int tid = threadIdx.x;
-  for (int p = tid; p < a.P; p += kMetaThreads) a.new_ref[p] = a.ref[p];
-  if (tid == 0) *a.short_out = 0;
-  __syncthreads();
-  const long cells = (long)a.R * a.ld;
-  for (long i = tid; i < cells; i += kMetaThreads) {
-    const int r = (int)(i / a.ld), col = (int)(i % a.ld);
-    const int old = a.table[i];
-    if (old >= 0 && old < a.P) atomicAdd(a.new_ref + old, -1);
-    const int par = a.parents != nullptr ? a.parents[r] : r;
-    int now = -1;
-    if (par >= 0 && par < a.R && col < (a.lens[par] + kPage - 1) / kPage) now = a.table[(size_t)par * a.ld + col];
-    if (now >= a.P) now = -1;
-    a.new_table[i] = now;
-    if (now >= 0) atomicAdd(a.new_ref + now, 1);
+  __shared__ __align__(16) int s_tail[kMetaThreads];
+  const int tid = threadIdx.x, all = kForkCtas * kMetaThreads, me = blockIdx.x * kMetaThreads + tid;
+  grid_dep_wait();
+  for (int p = me; p < a.P; p += all) a.new_ref[p] = a.ref[p];
+  cluster_sync();
+  const int cells = a.R * a.ld;
+  for (int i0 = me; i0 < cells; i0 += 4 * all) {
+    int old[4], now[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int i = i0 + k * all;
+      old[k] = now[k] = -1;
+      if (i < cells) {
+        const int r = i / a.ld, col = i - r * a.ld;
+        old[k] = a.table[i];
+        const int par = a.parents != nullptr ? a.parents[r] : r;
+        if (par >= 0 && par < a.R && col < (a.lens[par] + kPage - 1) / kPage) now[k] = a.table[par * a.ld + col];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int i = i0 + k * all;
+      if (i < cells) {
+        if (now[k] < 0 || now[k] >= a.P) now[k] = -1;
+        if (old[k] < 0 || old[k] >= a.P) old[k] = -1;
+        a.new_table[i] = now[k];
+        if (old[k] != now[k]) {  // a page that stays needs no counting
+          if (old[k] >= 0) atomicAdd(a.new_ref + old[k], -1);
+          if (now[k] >= 0) atomicAdd(a.new_ref + now[k], 1);
+        }
+      }
+    }
   }
   __threadfence();
-  __syncthreads();
-  // rows
+  cluster_sync();
+  if (blockIdx.x != 0) return;
   const int r = tid;
   int len = 0, n = 0, last = 0, tail = -1, over = 0;
   if (r < a.R) {
@@ -85,71 +110,80 @@ __global__ void __launch_bounds__(kMetaThreads) kv4_fork_kernel(ForkArgs a) {
     len = on ? max(a.lens[par], 0) : 0;
     a.new_lens[r] = len;
     n = min((len + kPage - 1) / kPage, a.ld);
-    const int want = on ? (len + a.room + kPage - 1) / kPage : 0;
+    const int want = on ? (int)(((long)len + a.room + kPage - 1) / kPage) : 0;
     last = max(n, min(want, a.ld));
     over = max(want - last, 0);
-    if (on && len % kPage != 0 && n > 0 && (len + kPage - 1) / kPage <= a.ld) tail = a.new_table[(size_t)r * a.ld + n - 1];
+    if (on && len % kPage != 0 && n > 0 && (len + kPage - 1) / kPage <= a.ld) tail = __ldcg(a.new_table + r * a.ld + n - 1);
   }
   s_tail[tid] = tail;
   __syncthreads();
   bool copy = false;
   if (tail >= 0) {
-    int same = 0;
-    bool lower = false;
-    for (int k = 0; k < a.R; k++)
-      if (s_tail[k] == tail) {
-        same++;
-        lower |= k < r;
+    const int held = __ldcg(a.new_ref + tail);
+    if (held > 1) {
+      int same = 0, lower = 0;
+      for (int k = 0; k < a.R; k += 4) {
+        const int4 t = *(const int4*)(s_tail + k);
+        const int h0 = t.x == tail, h1 = t.y == tail, h2 = t.z == tail, h3 = t.w == tail;
+        same += h0 + h1 + h2 + h3;
+        lower |= (h0 & (k < r)) | (h1 & (k + 1 < r)) | (h2 & (k + 2 < r)) | (h3 & (k + 3 < r));
       }
-    copy = lower || __ldcg(a.new_ref + tail) > same;
+      copy = lower || held > same;
+    }
   }
-  int need;
+  int need, got;
   const int base = block_scan((copy ? 1 : 0) + last - n, s_warp, &need);
-  // the `need` lowest free pages, in order: the page with rank k answers request k, so each row
-  // finds its own by reading the list back
-  __shared__ int s_have;
-  if (tid == 0) s_have = 0;
-  __syncthreads();
-  int* list = (int*)(a.moves + a.R);  // [need] at most R * (1 + ld)
-  for (int p0 = 0; p0 < a.P; p0 += kMetaThreads) {
-    const int have = s_have;
-    if (have >= need) break;
-    const int p = p0 + tid;
-    const bool free = p < a.P && __ldcg(a.new_ref + p) == 0;
-    int got;
-    const int at = have + block_scan(free ? 1 : 0, s_warp, &got);
-    if (free && at < need) list[at] = p;
-    if (tid == 0) s_have = have + got;
-    __syncthreads();
+  // the `need` lowest free pages: the one of rank k answers request k
+  int have = 0;
+  for (int p0 = 0; p0 < a.P && have < need; p0 += 4 * kMetaThreads) {
+    int free = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int p = p0 + 4 * tid + k;
+      free |= p < a.P && __ldcg(a.new_ref + p) == 0 ? 1 << k : 0;
+    }
+    int at = have + block_scan(__popc(free), s_warp, &got);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (free >> k & 1) {
+        if (at < need) a.list[at] = p0 + 4 * tid + k;
+        at++;
+      }
+    have += got;
   }
   __threadfence();
   __syncthreads();
-  const int have = min(s_have, need);
+  have = min(have, need);
+  Move mv = {0, 0, 0};
   if (r < a.R) {
     int k = base;
-    Move mv = {0, 0, 0};
     if (copy) {
-      const int p = k < have ? __ldcg(list + k) : -1;
+      const int p = k < have ? __ldcg(a.list + k) : -1;
       k++;
-      a.new_table[(size_t)r * a.ld + n - 1] = p;
+      a.new_table[r * a.ld + n - 1] = p;
       atomicAdd(a.new_ref + tail, -1);
       if (p >= 0) {
-        atomicAdd(a.new_ref + p, 1);
+        a.new_ref[p] = 1;
         mv = {tail, p, (len % kPage + kBlk - 1) / kBlk};
       } else {
         over++;
       }
     }
     for (int c = n; c < last; c++, k++) {
-      const int p = k < have ? __ldcg(list + k) : -1;
-      a.new_table[(size_t)r * a.ld + c] = p;
+      const int p = k < have ? __ldcg(a.list + k) : -1;
+      a.new_table[r * a.ld + c] = p;
       if (p >= 0)
-        atomicAdd(a.new_ref + p, 1);
+        a.new_ref[p] = 1;
       else
         over++;
     }
-    a.moves[r] = mv;
-    if (over) atomicAdd(a.short_out, over);
+  }
+  const int m = block_scan(mv.blocks > 0, s_warp, &got);
+  if (mv.blocks > 0) a.moves[m] = mv;
+  block_scan(over, s_warp, &over);
+  if (tid == 0) {
+    *a.n_moves = got;
+    *a.short_out = over;
   }
 }
 
@@ -159,37 +193,38 @@ struct CompactArgs {
   int32_t* new_ref;
   int32_t* new_table;
   int32_t* live_out;
+  int* n_moves;
   Move* moves;    // [P]
-  int32_t* n_moves;
   int32_t* map;   // [P]
   int P;
-  long cells;
+  int cells;
 };
 
-// One CTA: counts the live pages (n), pairs the k-th live page from n on with the k-th free place
-// below n, and rewrites counts and tables.
+// One CTA: counts the live pages (n), pairs the k-th live page from n on with the k-th free place below n,
+// and rewrites counts and tables.  A thread has a run of pages of its own, so that one prefix sum counts
+// them all.
 __global__ void __launch_bounds__(kMetaThreads) kv4_compact_kernel(CompactArgs a) {
   __shared__ int s_warp[32];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, run = (a.P + kMetaThreads - 1) / kMetaThreads;
+  const int q0 = min(tid * run, a.P), q1 = min(q0 + run, a.P);
+  grid_dep_wait();
   int c = 0, n;
   for (int p = tid; p < a.P; p += kMetaThreads) c += a.ref[p] > 0;
   block_scan(c, s_warp, &n);
-  int srcs = 0, dsts = 0;
-  for (int p0 = 0; p0 < a.P; p0 += kMetaThreads) {
-    const int p = p0 + tid;
-    const int rf = p < a.P ? a.ref[p] : 0;
-    const bool src = p < a.P && p >= n && rf > 0, dst = p < min(n, a.P) && rf <= 0;
-    int got;
-    int at = block_scan(src, s_warp, &got);
-    if (src) a.moves[srcs + at].src = p;
-    srcs += got;
-    at = block_scan(dst, s_warp, &got);
-    if (dst) a.moves[dsts + at].dst = p;
-    dsts += got;
-    if (p < a.P) {
-      a.map[p] = p;
-      a.new_ref[p] = rf;
-    }
+  int src = 0, dst = 0, srcs, dsts;
+  for (int p = q0; p < q1; p++) {
+    const bool live = a.ref[p] > 0;
+    src += live && p >= n;
+    dst += !live && p < n;
+  }
+  src = block_scan(src, s_warp, &srcs);
+  dst = block_scan(dst, s_warp, &dsts);
+  for (int p = q0; p < q1; p++) {
+    const int rf = a.ref[p];
+    if (rf > 0 && p >= n) a.moves[src++].src = p;
+    if (rf <= 0 && p < n) a.moves[dst++].dst = p;
+    a.map[p] = p;
+    a.new_ref[p] = rf;
   }
   __threadfence();
   __syncthreads();
@@ -206,27 +241,40 @@ __global__ void __launch_bounds__(kMetaThreads) kv4_compact_kernel(CompactArgs a
   }
   __threadfence();
   __syncthreads();
-  for (long i = tid; i < a.cells; i += kMetaThreads) {
+  grid_dep_launch();
+#pragma unroll 4
+  for (int i = tid; i < a.cells; i += kMetaThreads) {
     const int p = a.table[i];
     a.new_table[i] = p >= 0 && p < a.P ? __ldcg(a.map + p) : -1;
   }
 }
 
-// Copies pages, one (move, layer, head) per warp and turn.  `n` (device) or `fixed` gives the number
-// of moves.
+// Copies pages: a warp takes 2560 bytes of a (move, layer, head) at a time, five loads in flight a lane.
+constexpr int kCopyVecs = 160;
 __global__ void __launch_bounds__(256) kv4_copy_kernel(uint8_t* pool, size_t layer_bytes, int L, int NKV, int blk_bytes,
-                                                       const Move* moves, const int32_t* n, int fixed) {
+                                                       const Move* moves, const int* n_moves) {
   const int lane = threadIdx.x & 31;
   const long warp = ((long)blockIdx.x * 256 + threadIdx.x) >> 5, warps = (long)gridDim.x * 8;
-  const long units = (long)(n != nullptr ? *n : fixed) * L * NKV;
+  const int blk_vecs = blk_bytes / 16, subs = 4 * blk_vecs / kCopyVecs;
+  grid_dep_wait();
+  const long units = (long)*n_moves * L * NKV * subs;
   for (long u = warp; u < units; u += warps) {
-    const Move mv = moves[u / NKV / L];
-    const int h = (int)(u % NKV), l = (int)(u / NKV % L);
-    uint8_t* base = pool + l * layer_bytes;
+    uint32_t x = (uint32_t)(u % ((long)L * NKV * subs));
+    const Move mv = moves[u / ((long)L * NKV * subs)];
+    const int sub = (int)(x % subs);
+    x /= subs;
+    const int h = (int)(x % NKV), l = (int)(x / NKV);
+    const int vecs = mv.blocks * blk_vecs - sub * kCopyVecs;  // from this part's start on
+    uint8_t* base = pool + l * layer_bytes + (size_t)sub * kCopyVecs * 16;
     const uint4* s = (const uint4*)(base + ((size_t)mv.src * NKV + h) * 4 * blk_bytes);
     uint4* d = (uint4*)(base + ((size_t)mv.dst * NKV + h) * 4 * blk_bytes);
-    const int words = mv.blocks * blk_bytes / 16;
-    for (int i = lane; i < words; i += 32) d[i] = s[i];
+    uint4 v[5];
+#pragma unroll
+    for (int k = 0; k < 5; k++)
+      if (lane + 32 * k < vecs) v[k] = __ldcs(s + lane + 32 * k);
+#pragma unroll
+    for (int k = 0; k < 5; k++)
+      if (lane + 32 * k < vecs) __stcs(d + lane + 32 * k, v[k]);
   }
 }
 
@@ -240,13 +288,22 @@ static int check_pages(const char* what, const void* pool, size_t layer_bytes, i
   return RNGD_OK;
 }
 
+// The copies of up to `most` moves; how many there are is known on the device alone.
+static int launch_copy(uint8_t* pool, size_t layer_bytes, int L, int NKV, int HD, const Move* moves, const int* n_moves,
+                       int most, cudaStream_t s) {
+  const long units = (long)most * L * NKV * (4 * kv4_block_bytes(HD) / 16 / kCopyVecs), blocks = (units + 7) / 8;
+  const long cap = (long)num_sms() * 8;
+  return launch_pdl(kv4_copy_kernel, dim3((unsigned)(blocks < cap ? blocks : cap)), dim3(256), 0, s, "kv4_copy_kernel", pool,
+                    layer_bytes, L, NKV, kv4_block_bytes(HD), moves, n_moves);
+}
+
 }  // namespace rngd
 
 using namespace rngd;
 
 extern "C" int rngd_kv4_fork_workspace(int R, int ld_table, size_t* bytes) {
   RNGD_REQUIRE(bytes && R >= 0 && ld_table >= 0, "kv4_fork_workspace: bad argument");
-  *bytes = (size_t)R * sizeof(Move) + (size_t)R * (1 + ld_table) * 4;
+  *bytes = 16 + (size_t)R * sizeof(Move) + (size_t)R * (1 + ld_table) * 4;
   return RNGD_OK;
 }
 
@@ -263,17 +320,14 @@ extern "C" int rngd_kv4_fork(void* pool, size_t layer_bytes, int L, int P, int N
   size_t need;
   RNGD_TRY(rngd_kv4_fork_workspace(R, ld_table, &need));
   RNGD_REQUIRE(workspace_bytes >= need, "kv4_fork: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  ForkArgs a = {ref, table, lens, parents, new_ref, new_table, new_lens, short_out, (Move*)workspace, P, R, ld_table,
-                room};
+  int* n_moves = (int*)workspace;
+  Move* moves = (Move*)((uint8_t*)workspace + 16);
+  ForkArgs a = {ref, table, lens, parents, new_ref, new_table, new_lens, short_out, n_moves, moves, (int*)(moves + R),
+                P, R, ld_table, room};
   cudaStream_t s = (cudaStream_t)stream;
-  kv4_fork_kernel<<<1, kMetaThreads, 0, s>>>(a);
-  RNGD_TRY(check_launch("kv4_fork_kernel"));
+  RNGD_TRY(launch_pdl(kv4_fork_kernel, dim3(kForkCtas), dim3(kMetaThreads), 0, s, "kv4_fork_kernel", a));
   if (R == 0) return RNGD_OK;
-  const long units = (long)R * L * NKV;
-  const long blocks = (units + 7) / 8;
-  kv4_copy_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, s>>>(
-      (uint8_t*)pool, layer_bytes, L, NKV, kv4_block_bytes(HD), a.moves, nullptr, R);
-  return check_launch("kv4_copy_kernel");
+  return launch_copy((uint8_t*)pool, layer_bytes, L, NKV, HD, moves, n_moves, R, s);
 }
 
 extern "C" int rngd_kv4_compact_workspace(int P, size_t* bytes) {
@@ -293,13 +347,11 @@ extern "C" int rngd_kv4_compact(void* pool, size_t layer_bytes, int L, int P, in
   size_t need;
   RNGD_TRY(rngd_kv4_compact_workspace(P, &need));
   RNGD_REQUIRE(workspace_bytes >= need, "kv4_compact: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  int32_t* n_moves = (int32_t*)workspace;
+  int* n_moves = (int*)workspace;
   Move* moves = (Move*)((uint8_t*)workspace + 16);
   int32_t* map = (int32_t*)(moves + P);
-  CompactArgs a = {ref, table, new_ref, new_table, live, moves, n_moves, map, P, cells};
+  CompactArgs a = {ref, table, new_ref, new_table, live, n_moves, moves, map, P, (int)cells};
   cudaStream_t s = (cudaStream_t)stream;
-  kv4_compact_kernel<<<1, kMetaThreads, 0, s>>>(a);
-  RNGD_TRY(check_launch("kv4_compact_kernel"));
-  kv4_copy_kernel<<<148 * 8, 256, 0, s>>>((uint8_t*)pool, layer_bytes, L, NKV, kv4_block_bytes(HD), moves, n_moves, 0);
-  return check_launch("kv4_copy_kernel");
+  RNGD_TRY(launch_pdl(kv4_compact_kernel, dim3(1), dim3(kMetaThreads), 0, s, "kv4_compact_kernel", a));
+  return launch_copy((uint8_t*)pool, layer_bytes, L, NKV, HD, moves, n_moves, P, s);
 }
