@@ -337,6 +337,22 @@ int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out, const int6
                   rngd_stream_t stream);
 int rngd_kv4_attn_workspace(int dtype, int B, int T, int NH, int NKV, int HD, int ld_table, int window, int sinks,
                             size_t* bytes);
+/* The decode step's layers [layer0, layer1) over a paged 4-bit cache instead of io's lanes: as rngd_decode_layers,
+ * but each stream b appends at io->pos[b] to the pages of table row b and attends over them, with an optional
+ * window and sinks.  io's kcache, vcache, Bcap, S and lanes are not used.  pool: layer0's first page. */
+typedef struct rngd_kv4 {
+  void* pool;            /* layers layer_bytes apart */
+  size_t layer_bytes;
+  int32_t P, ld_table;   /* pages of the pool, width of the tables */
+  const int32_t* table;  /* device [B][ld_table] */
+  int32_t window, sinks; /* as in rngd_kv4_attn */
+  void* rows;            /* bf16 [2][16][NKV][HD] scratch: the step's new rows */
+  void* workspace;       /* rngd_decode_kv4_workspace() bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} rngd_kv4_t;
+int rngd_decode_layers_kv4(const rngd_model_t* m, const rngd_decode_io_t* io, const rngd_kv4_t* kv, int layer0,
+                           int layer1, rngd_stream_t stream);
+int rngd_decode_kv4_workspace(const rngd_model_t* m, int B, int ld_table, int window, int sinks, size_t* bytes);
 /* Sequences and their pages.  ref: int32 [P] holders of each page (0: free); table: [R][ld_table]; lens: [R].
  * Fork: row r goes on as row parents[r] (NULL: as itself; < 0: it ends and lets go of its pages).  A last
  * page that is partly filled belongs to one row alone afterwards: the lowest row keeps it if none but

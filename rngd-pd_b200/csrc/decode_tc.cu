@@ -85,6 +85,7 @@ struct GemmArgs {
   uint16_t* vc;
   const int32_t* lanes;  // [B] cache lane of each stream, nullptr = stream b -> lane b
   int NH, NKV, S;
+  int kv_rows;  // 1: kc and vc are the new rows alone, [B][NKV][128] (S = 1), whatever their position
   // RESID: x += y; act_next = hi/lo(x * w_next); ss_out = per-tile sums of squares of x
   float* x;
   int ldx;
@@ -515,17 +516,17 @@ __device__ __forceinline__ void epilogue_phase(const GemmArgs& a, const Ring& R,
             if (b < a.B) {
               if (head < a.NH) {
                 a.q[(size_t)b * a.ldq + n] = o[i];
-              } else if (p >= 0 && p < a.S) {
-                a.kc[(((size_t)R.s_lane[b] * a.NKV + (head - a.NH)) * a.S + p) * 128 + r] = f2bf_bits(o[i]);
+              } else if (const int at = a.kv_rows ? 0 : p; p >= 0 && at < a.S) {
+                a.kc[(((size_t)R.s_lane[b] * a.NKV + (head - a.NH)) * a.S + at) * 128 + r] = f2bf_bits(o[i]);
               }
             }
           }
         } else {
 #pragma unroll
           for (int i = 0; i < SPG; i++) {
-            const int b = sb + i, p = R.s_pos[b];
-            if (b < a.B && p >= 0 && p < a.S)
-              a.vc[(((size_t)R.s_lane[b] * a.NKV + (head - a.NH - a.NKV)) * a.S + p) * 128 + r] = f2bf_bits(y[i]);
+            const int b = sb + i, p = R.s_pos[b], at = a.kv_rows ? 0 : p;
+            if (b < a.B && p >= 0 && at < a.S)
+              a.vc[(((size_t)R.s_lane[b] * a.NKV + (head - a.NH - a.NKV)) * a.S + at) * 128 + r] = f2bf_bits(y[i]);
           }
         }
       } else if constexpr (EPI == EPI_SWIGLU) {
@@ -871,6 +872,11 @@ int launch_attn_decode_act(const float* q, int ldq, const void* kc, const void* 
                            const int32_t* lanes, int B,
                            int NH, int NKV, int HD, int S, float* part, void* act, int ld_act, cudaStream_t s);
 int launch_embed(const void* emb, const int32_t* toks, int H, int V, float* x, int B, cudaStream_t s);
+int launch_kv4_decode_store(void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table, const int32_t* pos,
+                            int B, const void* k, const void* v, cudaStream_t s);
+int launch_kv4_decode_attn(const float* q, const void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table,
+                           const int32_t* pos, int B, int NH, int window, int sinks, void* act, int ld_act,
+                           void* workspace, size_t workspace_bytes, cudaStream_t s);
 
 // scratch sizes of one GEMM shape under the stream-K split
 static void shape_workspace(int N, int K, size_t* pf, size_t* ct) {
@@ -1060,6 +1066,56 @@ extern "C" int rngd_decode_layers(const rngd_model_t* m, const rngd_decode_io_t*
     if (l + 1 < layer1)
       RNGD_TRY(launch_skgemm<EPI_QKV>(m->wqkv, m->L, l + 1, NQKV, H, io->act, ld_act,
                                       layer_args(m, io, layer0, l + 1, 0, off), s));
+  }
+  return RNGD_OK;
+}
+
+extern "C" int rngd_decode_kv4_workspace(const rngd_model_t* m, int B, int ld_table, int window, int sinks, size_t* bytes) {
+  RNGD_REQUIRE(m && bytes, "decode_kv4_workspace: null argument");
+  return rngd_kv4_attn_workspace(RNGD_DT_F32, B, 1, m->NH, m->NKV, m->HD, ld_table, window, sinks, bytes);
+}
+
+// The layers of rngd_decode_layers over the paged 4-bit cache: the QKV GEMM leaves the new rows in bf16, a
+// kernel stores them in the pages, the attention reads the pages and writes the O projection's operand.
+extern "C" int rngd_decode_layers_kv4(const rngd_model_t* m, const rngd_decode_io_t* io_in, const rngd_kv4_t* kv,
+                                      int layer0, int layer1, rngd_stream_t stream) {
+  RNGD_REQUIRE(m && io_in && kv, "decode_layers_kv4: null argument");
+  RNGD_REQUIRE(kv->pool && kv->rows && (kv->table || kv->ld_table == 0) && kv->ld_table >= 0,
+               "decode_layers_kv4: null buffer");
+  rngd_decode_io_t io = *io_in;  // the cache of the checks and of the GEMM's epilogue: the new rows
+  const size_t row_elems = (size_t)MAXB * m->NKV * m->HD;
+  io.kcache = kv->rows;
+  io.vcache = (uint16_t*)kv->rows + row_elems;
+  io.Bcap = MAXB;
+  io.S = 128;
+  io.lanes = nullptr;
+  RNGD_TRY(check_tc_io(m, &io));
+  RNGD_REQUIRE(0 <= layer0 && layer0 <= layer1 && layer1 <= m->L, "decode_layers_kv4: layers [%d, %d) outside [0, %d)",
+               layer0, layer1, m->L);
+  if (layer0 == layer1) return RNGD_OK;
+  cudaStream_t s = (cudaStream_t)stream;
+  const int H = m->H, Mi = m->M, QN = m->NH * m->HD, KN = m->NKV * m->HD, NQKV = QN + 2 * KN;
+  const int ld_act = H > QN ? H : QN;
+  size_t off[5], pf, ct;
+  decode_shapes(m, off, &pf, &ct);
+  auto qkv = [&](int l) {
+    GemmArgs a = layer_args(m, &io, layer0, l, 0, off);
+    a.kc = (uint16_t*)io.kcache;
+    a.vc = (uint16_t*)io.vcache;
+    a.S = 1;
+    a.kv_rows = 1;
+    return launch_skgemm<EPI_QKV>(m->wqkv, m->L, l, NQKV, H, io.act, ld_act, a, s);
+  };
+  for (int l = layer0; l < layer1; l++) {
+    uint8_t* pool = (uint8_t*)kv->pool + (size_t)(l - layer0) * kv->layer_bytes;
+    RNGD_TRY(qkv(l));
+    RNGD_TRY(launch_kv4_decode_store(pool, kv->P, m->NKV, m->HD, kv->table, kv->ld_table, io.pos, io.B, io.kcache,
+                                     io.vcache, s));
+    RNGD_TRY(launch_kv4_decode_attn(io.q, pool, kv->P, m->NKV, m->HD, kv->table, kv->ld_table, io.pos, io.B, m->NH,
+                                    kv->window, kv->sinks, io.act_o, QN, kv->workspace, kv->workspace_bytes, s));
+    RNGD_TRY(launch_skgemm<EPI_RESID>(m->wo, m->L, l, H, QN, io.act_o, QN, layer_args(m, &io, layer0, l, 1, off), s));
+    RNGD_TRY(launch_skgemm<EPI_SWIGLU>(m->wgu, m->L, l, 2 * Mi, H, io.act, ld_act, layer_args(m, &io, layer0, l, 2, off), s));
+    RNGD_TRY(launch_skgemm<EPI_RESID>(m->wd, m->L, l, H, Mi, io.act2, Mi, layer_args(m, &io, layer0, l, 3, off), s));
   }
   return RNGD_OK;
 }

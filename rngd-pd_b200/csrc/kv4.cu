@@ -234,6 +234,8 @@ __global__ void __launch_bounds__(128) kv4_store_kernel(StoreArgs a, int groups)
   constexpr int LPG = HD / 4, NG = HD / 32;
   const long i = ((long)blockIdx.x * 128 + threadIdx.x) / LPG;
   const int l = threadIdx.x % LPG;
+  grid_dep_wait();
+  grid_dep_launch();
   const Group<HD> g = group_of<HD>(a, groups, i);
   if (__all_sync(0xffffffffu, g.blk == nullptr)) return;
   Raw4<DT, VEC> k[8], v[8];
@@ -371,6 +373,7 @@ __global__ void __launch_bounds__(128) kv4_load_kernel(StoreArgs a, int groups, 
   constexpr int LPG = HD / 4, NG = HD / 32;
   const long i = ((long)blockIdx.x * 128 + threadIdx.x) / LPG;
   const int l = threadIdx.x % LPG;
+  grid_dep_wait();
   const Group<HD> g = group_of<HD>(a, groups, i);
   if (g.layer >= a.L) return;
   // row of token t0 + r
@@ -494,6 +497,35 @@ static int store_args(const char* what, StoreArgs* a, void* pool, size_t layer_b
   return RNGD_OK;
 }
 
+static int launch_store(const StoreArgs& a, int HD, cudaStream_t s) {
+  if (a.B == 0 || a.T == 0) return RNGD_OK;
+  const int groups = (a.T + 14) / 8;  // groups of 8 aligned positions that T positions can touch
+  const long blocks = ((long)a.L * a.B * groups * a.NKV * (HD / 4) + 127) / 128;
+  RNGD_REQUIRE(blocks < (1l << 31), "kv4_store: %ld groups of rows in one call", blocks);
+  const int lane_bytes = a.dt == DT_F32 ? 16 : 8, esz = lane_bytes / 4;
+  bool vec = ((uintptr_t)a.k | (uintptr_t)a.v) % lane_bytes == 0;
+  for (int i = 0; i < 4; i++) vec = vec && a.ks[i] * esz % lane_bytes == 0 && a.vs[i] * esz % lane_bytes == 0;
+  typedef void (*Kernel)(StoreArgs, int);
+  static const Kernel kernels[2][3][2] = {
+      {{kv4_store_kernel<64, DT_BF16, false>, kv4_store_kernel<64, DT_BF16, true>},
+       {kv4_store_kernel<64, DT_F16, false>, kv4_store_kernel<64, DT_F16, true>},
+       {kv4_store_kernel<64, DT_F32, false>, kv4_store_kernel<64, DT_F32, true>}},
+      {{kv4_store_kernel<128, DT_BF16, false>, kv4_store_kernel<128, DT_BF16, true>},
+       {kv4_store_kernel<128, DT_F16, false>, kv4_store_kernel<128, DT_F16, true>},
+       {kv4_store_kernel<128, DT_F32, false>, kv4_store_kernel<128, DT_F32, true>}}};
+  return launch_pdl(kernels[HD == 128][a.dt][vec], dim3((unsigned)blocks), dim3(128), 0, s, "kv4_store_kernel", a, groups);
+}
+
+// One layer's new tokens of the decode step: rows [B][NKV][HD] bf16 to position pos[b].
+int launch_kv4_decode_store(void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table, const int32_t* pos,
+                            int B, const void* k, const void* v, cudaStream_t s) {
+  StoreArgs a;
+  RNGD_TRY(store_args("decode_layers_kv4", &a, pool, 0, P, NKV, HD, 1, table, ld_table, pos, nullptr, B, 1, k, v, DT_BF16));
+  a.ks[1] = a.vs[1] = (long)NKV * HD;
+  a.ks[3] = a.vs[3] = HD;
+  return launch_store(a, HD, s);
+}
+
 }  // namespace rngd
 
 using namespace rngd;
@@ -510,23 +542,7 @@ extern "C" int rngd_kv4_store(void* pool, size_t layer_bytes, int P, int NKV, in
     a.ks[i] = (long)k_strides[i];
     a.vs[i] = (long)v_strides[i];
   }
-  if (B == 0 || T == 0) return RNGD_OK;
-  const int groups = (T + 14) / 8;  // groups of 8 aligned positions that T positions can touch
-  const long blocks = ((long)L * B * groups * NKV * (HD / 4) + 127) / 128;
-  RNGD_REQUIRE(blocks < (1l << 31), "kv4_store: %ld groups of rows in one call", blocks);
-  const int lane_bytes = dtype == DT_F32 ? 16 : 8, esz = lane_bytes / 4;
-  bool vec = ((uintptr_t)k | (uintptr_t)v) % lane_bytes == 0;
-  for (int i = 0; i < 4; i++) vec = vec && a.ks[i] * esz % lane_bytes == 0 && a.vs[i] * esz % lane_bytes == 0;
-  typedef void (*Kernel)(StoreArgs, int);
-  static const Kernel kernels[2][3][2] = {
-      {{kv4_store_kernel<64, DT_BF16, false>, kv4_store_kernel<64, DT_BF16, true>},
-       {kv4_store_kernel<64, DT_F16, false>, kv4_store_kernel<64, DT_F16, true>},
-       {kv4_store_kernel<64, DT_F32, false>, kv4_store_kernel<64, DT_F32, true>}},
-      {{kv4_store_kernel<128, DT_BF16, false>, kv4_store_kernel<128, DT_BF16, true>},
-       {kv4_store_kernel<128, DT_F16, false>, kv4_store_kernel<128, DT_F16, true>},
-       {kv4_store_kernel<128, DT_F32, false>, kv4_store_kernel<128, DT_F32, true>}}};
-  kernels[HD == 128][dtype][vec]<<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a, groups);
-  return check_launch("kv4_store_kernel");
+  return launch_store(a, HD, (cudaStream_t)stream);
 }
 
 extern "C" int rngd_kv4_load(const void* pool, size_t layer_bytes, int P, int NKV, int HD, int L,
@@ -544,6 +560,6 @@ extern "C" int rngd_kv4_load(const void* pool, size_t layer_bytes, int P, int NK
   static const Kernel kernels[2][3] = {
       {kv4_load_kernel<64, DT_BF16>, kv4_load_kernel<64, DT_F16>, kv4_load_kernel<64, DT_F32>},
       {kv4_load_kernel<128, DT_BF16>, kv4_load_kernel<128, DT_F16>, kv4_load_kernel<128, DT_F32>}};
-  kernels[HD == 128][dtype]<<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a, groups, k, v);
-  return check_launch("kv4_load_kernel");
+  return launch_pdl(kernels[HD == 128][dtype], dim3((unsigned)blocks), dim3(128), 0, (cudaStream_t)stream, "kv4_load_kernel", a,
+                    groups, k, v);
 }

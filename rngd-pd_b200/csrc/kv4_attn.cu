@@ -39,6 +39,8 @@ struct AttnArgs {
   const void* q;
   void* out;
   long qs[3], os[3];  // strides in elements: stream, token, head
+  long lo_off;        // 0: out is of q's type; else bf16, hi at its place and lo (out - hi) so far behind
+  int len_add;        // positions held beyond lens[b]
   int dt, qvec, B, T, NH, NKV, G, RT, P, ld_table, window, sinks;
   const uint8_t* pool;
   const int32_t* table;
@@ -47,6 +49,16 @@ struct AttnArgs {
   int* pre;     // [B + 1] prefix sums of units, for the joining kernel
   float* rec;   // [warps][2][rows][HD + 2]
 };
+
+__device__ __forceinline__ void put_out(const AttnArgs& a, size_t at, float v) {
+  if (a.lo_off == 0) {
+    store1(a.out, at, a.dt, v);
+  } else {
+    const uint16_t hi = f2bf_bits(v);
+    ((uint16_t*)a.out)[at] = hi;
+    ((uint16_t*)a.out)[at + a.lo_off] = f2bf_bits(v - bf2f(hi));
+  }
+}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
@@ -99,7 +111,7 @@ __device__ __forceinline__ void prefix_units(const AttnArgs& a, int* lens, int* 
   int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < a.B ? a.lens[b] : 0;
+    const int n = b < a.B ? a.lens[b] + a.len_add : 0;
     int x = b < a.B ? span_of(n, a).units() * a.NKV * a.RT : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -491,7 +503,7 @@ struct Rows {
             if (r < R) {
               const size_t at = (size_t)(b * a.os[0] + r / a.G * a.os[1] + (kvh * a.G + r % a.G) * a.os[2]) + 32 * j + 4 * g;
 #pragma unroll
-              for (int k = 0; k < 4; k++) store1(a.out, at + k, a.dt, v[k] * inv);
+              for (int k = 0; k < 4; k++) put_out(a, at + k, v[k] * inv);
             }
           } else {
             *(float4*)(rec + (size_t)rl * (HD + 4) + 32 * j + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
@@ -678,7 +690,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(AttnArgs a, i
   const float inv = x.inverse();
   const size_t at = (size_t)(b * a.os[0] + r / a.G * a.os[1] + (kvh * a.G + r % a.G) * a.os[2]) + lane * D;
 #pragma unroll
-  for (int d = 0; d < D; d++) store1(a.out, at + d, a.dt, x.v[d] * inv);
+  for (int d = 0; d < D; d++) put_out(a, at + d, x.v[d] * inv);
 }
 
 // The same for sequences that are known to be short: one CTA holds a segment, its warps take the units
@@ -703,9 +715,10 @@ __global__ void __launch_bounds__(32 * whole_warps<HD, NT, MODE>()) kv4_attn_who
   fence_mbar_init();
   __syncwarp();
   grid_dep_wait();
+  grid_dep_launch();
   const int seg = blockIdx.x;
   const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV;
-  const int n = a.lens[b], held = min(max(n, 0), a.ld_table * kPage);
+  const int n = a.lens[b] + a.len_add, held = min(max(n, 0), a.ld_table * kPage);
   const Span sp = span_of(n, a);
   const int U = sp.units(), mine = U > w ? (U - w + warps - 1) / warps : 0;
   Rows<HD, NT, MODE> rows;
@@ -760,7 +773,7 @@ __global__ void __launch_bounds__(32 * whole_warps<HD, NT, MODE>()) kv4_attn_who
     const float inv = x.inverse();
     const size_t at = (size_t)(b * a.os[0] + r / a.G * a.os[1] + (kvh * a.G + r % a.G) * a.os[2]) + d;
 #pragma unroll
-    for (int e = 0; e < 4; e++) store1(a.out, at + e, a.dt, x.v[e] * inv);
+    for (int e = 0; e < 4; e++) put_out(a, at + e, x.v[e] * inv);
   }
 }
 
@@ -856,6 +869,74 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
   return RNGD_OK;
 }
 
+// The attention of one launch's arguments, streams in groups of kAttnStreams.
+static int launch_kv4_attn(AttnArgs a, const AttnPlan& p, int B, int HD, void* workspace, cudaStream_t s) {
+  const int esz = a.dt == DT_F32 ? 4 : 2, osz = a.lo_off != 0 ? 2 : esz;
+  bool vec = ((uintptr_t)a.q & 15) == 0;
+  for (int i = 0; i < 3; i++) vec = vec && a.qs[i] * esz % 16 == 0;
+  a.qvec = vec;
+  a.G = a.NH / a.NKV;
+  a.RT = p.RT;
+  a.pre = (int*)workspace;
+  a.rec = (float*)((uint8_t*)workspace + p.pre_bytes);
+  const AttnArgs all = a;
+  for (int b0 = 0; b0 < B; b0 += kAttnStreams) {
+    a.B = B - b0 < kAttnStreams ? B - b0 : kAttnStreams;
+    a.q = (const uint8_t*)all.q + (long)b0 * a.qs[0] * esz;
+    a.out = (uint8_t*)all.out + (long)b0 * a.os[0] * osz;
+    a.table = all.table + (size_t)b0 * a.ld_table;
+    a.lens = all.lens + b0;
+    if (p.whole) {
+      RNGD_TRY(HD == 128 ? launch_whole<128>(a, p, s) : launch_whole<64>(a, p, s));
+      continue;
+    }
+    const AttnKernel k = HD == 128 ? attn_kernel<128>(p.NT, p.mode) : attn_kernel<64>(p.NT, p.mode);
+    RNGD_TRY(launch_pdl(k, dim3(p.warps), dim3(32), HD == 128 ? attn_smem<128>(a.B) : attn_smem<64>(a.B), s,
+                        "kv4_attn_kernel", a));
+    // few segments have many records each: a CTA per row, its records shared by 16 warps; many segments: a CTA
+    // for all rows of one (64x5000: 105 us with 16 warps a row, 91 us so)
+    const int segs = a.B * a.NKV * p.RT;
+    const bool few = segs * p.rows <= 4 * num_sms();
+    const int parts = few ? kJoinWarps : (p.rows <= 8 ? 2 : 1);
+    RNGD_TRY(launch_pdl(HD == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, dim3(segs, few ? p.rows : 1),
+                        dim3(32 * (few ? kJoinWarps : p.rows * parts)), 0, s, "kv4_join_kernel", a, p.warps, p.rows, parts));
+  }
+  return RNGD_OK;
+}
+
+// One layer's attention of the decode step: q fp32 [B][NH * HD], the new tokens at pos[b] (stored already),
+// out as the hi / lo rows of the O projection's operand (16 streams apart).
+int launch_kv4_decode_attn(const float* q, const void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table,
+                           const int32_t* pos, int B, int NH, int window, int sinks, void* act, int ld_act,
+                           void* workspace, size_t workspace_bytes, cudaStream_t s) {
+  RNGD_TRY(check_pool("decode_layers_kv4", pool, 0, P, NKV, HD));
+  AttnPlan p;
+  RNGD_TRY(attn_plan(DT_F32, B, 1, NH, NKV, HD, ld_table, window, sinks, &p));
+  RNGD_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.bytes,
+               "decode_layers_kv4: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, p.bytes);
+  AttnArgs a = {};
+  a.q = q;
+  a.out = act;
+  a.qs[0] = a.qs[1] = (long)NH * HD;
+  a.os[0] = a.os[1] = ld_act;
+  a.qs[2] = a.os[2] = HD;
+  a.lo_off = 16l * ld_act;
+  a.len_add = 1;
+  a.dt = DT_F32;
+  a.T = 1;
+  a.NH = NH;
+  a.NKV = NKV;
+  a.P = P;
+  a.ld_table = ld_table;
+  a.window = window;
+  a.sinks = sinks;
+  a.pool = (const uint8_t*)pool;
+  a.table = table;
+  a.lens = pos;
+  a.scale = 1.0f / sqrtf((float)HD);
+  return launch_kv4_attn(a, p, B, HD, workspace, s);
+}
+
 int read_status_kv4(int* st, int reset) {
   RNGD_TRY(check_cuda(cudaMemcpyFromSymbol(st, g_status_kv4, sizeof(int)), "read device status"));
   if (reset) {
@@ -889,50 +970,24 @@ extern "C" int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out,
   RNGD_REQUIRE(q && out && q_strides && out_strides && lens && (table || ld_table == 0), "kv4_attn: null pointer");
   RNGD_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.bytes,
                "kv4_attn: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, p.bytes);
-  const int esz = dtype == DT_F32 ? 4 : 2;
   AttnArgs a = {};
-  bool vec = ((uintptr_t)q & 15) == 0;
+  a.q = q;
+  a.out = out;
   for (int i = 0; i < 3; i++) {
     a.qs[i] = (long)q_strides[i];
     a.os[i] = (long)out_strides[i];
-    vec = vec && a.qs[i] * esz % 16 == 0;
   }
-  a.qvec = vec;
   a.dt = dtype;
   a.T = T;
   a.NH = NH;
   a.NKV = NKV;
-  a.G = NH / NKV;
-  a.RT = p.RT;
   a.P = P;
   a.ld_table = ld_table;
   a.window = window;
   a.sinks = sinks;
   a.pool = (const uint8_t*)pool;
+  a.table = table;
+  a.lens = lens;
   a.scale = scale;
-  a.pre = (int*)workspace;
-  a.rec = (float*)((uint8_t*)workspace + p.pre_bytes);
-  cudaStream_t s = (cudaStream_t)stream;
-  for (int b0 = 0; b0 < B; b0 += kAttnStreams) {
-    a.B = B - b0 < kAttnStreams ? B - b0 : kAttnStreams;
-    a.q = (const uint8_t*)q + (long)b0 * a.qs[0] * esz;
-    a.out = (uint8_t*)out + (long)b0 * a.os[0] * esz;
-    a.table = table + (size_t)b0 * ld_table;
-    a.lens = lens + b0;
-    if (p.whole) {
-      RNGD_TRY(HD == 128 ? launch_whole<128>(a, p, s) : launch_whole<64>(a, p, s));
-      continue;
-    }
-    const AttnKernel k = HD == 128 ? attn_kernel<128>(p.NT, p.mode) : attn_kernel<64>(p.NT, p.mode);
-    RNGD_TRY(launch_pdl(k, dim3(p.warps), dim3(32), HD == 128 ? attn_smem<128>(a.B) : attn_smem<64>(a.B), s,
-                        "kv4_attn_kernel", a));
-    // few segments have many records each: a CTA per row, its records shared by 16 warps; many segments: a CTA
-    // for all rows of one (64x5000: 105 us with 16 warps a row, 91 us so)
-    const int segs = a.B * NKV * p.RT;
-    const bool few = segs * p.rows <= 4 * num_sms();
-    const int parts = few ? kJoinWarps : (p.rows <= 8 ? 2 : 1);
-    RNGD_TRY(launch_pdl(HD == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, dim3(segs, few ? p.rows : 1),
-                        dim3(32 * (few ? kJoinWarps : p.rows * parts)), 0, s, "kv4_join_kernel", a, p.warps, p.rows, parts));
-  }
-  return RNGD_OK;
+  return launch_kv4_attn(a, p, B, HD, workspace, (cudaStream_t)stream);
 }

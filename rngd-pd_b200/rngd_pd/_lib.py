@@ -62,6 +62,13 @@ class PrefillIO(ctypes.Structure):
                 ("partial", _vp), ("counters", _vp), ("operand_lo", _i32)]
 
 
+class Kv4(ctypes.Structure):
+    """rngd_kv4_t"""
+    _fields_ = [("pool", _vp), ("layer_bytes", ctypes.c_size_t), ("P", _i32), ("ld_table", _i32), ("table", _vp),
+                ("window", _i32), ("sinks", _i32), ("rows", _vp), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 def _sig(name, *args):
     f = getattr(lib, name)
     f.argtypes = list(args)
@@ -137,6 +144,9 @@ _sig("rngd_kv4_load", _vp, _sz, _int, _int, _int, _int, _vp, _int, _vp, _vp, _in
 _sig("rngd_kv4_attn", _vp, _i64p, _vp, _i64p, _int, _vp, _int, _int, _int, _vp, _int, _vp, _int, _int, _int, _int,
      _int, ctypes.c_float, _vp, _sz, _vp)
 _sig("rngd_kv4_attn_workspace", _int, _int, _int, _int, _int, _int, _int, _int, _int, _szp)
+_KVP = ctypes.POINTER(Kv4)
+_sig("rngd_decode_layers_kv4", _MP, _IOP, _KVP, _int, _int, _vp)
+_sig("rngd_decode_kv4_workspace", _MP, _int, _int, _int, _int, _szp)
 _sig("rngd_kv4_fork", _vp, _sz, _int, _int, _int, _int, _vp, _vp, _int, _vp, _int, _vp, _int, _vp, _vp, _vp, _vp,
      _vp, _sz, _vp)
 _sig("rngd_kv4_fork_workspace", _int, _int, _szp)
