@@ -623,7 +623,7 @@ extern "C" int rngd_beam_select(const void* logits, int dtype, int64_t ld, int R
   BeamPlan p;
   RNGD_TRY(beam_plan(dtype, R, V, W, &p));
   RNGD_REQUIRE(R % W == 0, "beam_select: %d rows are not whole groups of %d beams", R, W);
-  RNGD_REQUIRE(V >= W && (long)V * W < (1l << 31), "beam_select: vocabulary of %d", V);
+  RNGD_REQUIRE(V >= W && V < (1 << 30) && (long)V * W < (1l << 31), "beam_select: vocabulary of %d", V);
   RNGD_REQUIRE(ld >= V || R <= 1, "beam_select: rows of %d logits %ld apart", V, (long)ld);
   if (R == 0) return RNGD_OK;
   RNGD_REQUIRE(logits && scores && done && out_scores && parents && tokens && out_done && workspace,

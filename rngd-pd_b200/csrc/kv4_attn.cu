@@ -189,21 +189,40 @@ __device__ __forceinline__ void load_q8(const AttnArgs& a, size_t at, float* x) 
   }
 }
 
-// How the halves of q and P are laid out: see above.  Q16 and Q32 differ in whether q has a lo half.
-enum : int { COLS = 0, Q16 = 1, Q32 = 2 };
+// How the halves of q and P are laid out (see above), for 16-bit and for fp32 q.  Matrix instructions cut
+// their sums off instead of rounding them; for fp32 q, whose results show it, scores are summed in fp32
+// from one short chain per 32 dimensions, and the output is moved every kFlush units from the matrix
+// accumulators to fp32 sums in shared memory (65000 positions: 5e-7 off instead of 3e-6; 8x40000: 90 us
+// instead of 84).
+enum : int { COLS = 0, Q16 = 1, Q32 = 2, COLS32 = 3 };
+constexpr int kFlush = 4;
 
 // One warp's state for a segment.  NT tiles of 8 columns; a column is a query row, or with COLS the hi
 // (columns 0..3) or lo (4..7) half of one.  Lane = 4 g + t as in the fragments.
 template <int HD, int NT, int MODE>
 struct Rows {
   static constexpr int NG = HD / 32;
-  static constexpr bool SPLIT = MODE == COLS;
+  static constexpr bool SPLIT = MODE == COLS || MODE == COLS32, FLUSH = MODE == Q32 || MODE == COLS32;
   static constexpr int CPT = SPLIT ? 4 : 8;  // rows of a column tile
   static constexpr int QL = MODE == Q32 ? NT : 1;
   uint32_t qf[NT][NG][4], ql[QL][NG][4];
   float o[NT][NG][2][4];
   float f[NT][2], mb[NT][2], l[NT][2];  // of columns 2t, 2t + 1 (rows 2 (t & 1), + 1 with SPLIT)
   int i[NT][2];                         // their positions, -1: none
+  float* acc;                           // this lane's sums of o, 32 floats apart (FLUSH)
+  int since;                            // units since they were last added to
+
+  template <class F>
+  __device__ __forceinline__ void each_sum(F f) {  // f(sum, its part in o, its column e)
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int j = 0; j < NG; j++)
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) f(acc[(((nt * NG + j) * 2 + q) * 4 + k) * 32], o[nt][j][q][k], nt, k & 1);
+  }
 
   __device__ __forceinline__ void begin(const AttnArgs& a, int seg, int n) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -238,7 +257,7 @@ struct Rows {
           const float x0 = x[j][p] * up, x1 = x[j][p + 4] * up;
           const uint32_t hi = pack_h2(x0, x1);
           qf[nt][j][p] = hi;
-          if constexpr (MODE != Q16) {
+          if constexpr (MODE != Q16) {  // 16-bit q has a lo half of zeros
             const float2 hf = __half22float2(u2h(hi));
             const uint32_t lo = pack_h2(x0 - hf.x, x1 - hf.y);
             if constexpr (SPLIT) {
@@ -262,6 +281,10 @@ struct Rows {
         mb[nt][e] = 1e30f;
         l[nt][e] = 0.0f;
       }
+    }
+    if constexpr (FLUSH) {
+      since = 0;
+      each_sum([](float& sum, float&, int, int) { sum = 0.0f; });
     }
   }
 
@@ -291,11 +314,17 @@ struct Rows {
       decode_word(w1[j], __low2half2(u2h(s1[j])), __high2half2(u2h(s1[j])), y);
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        mma_f16(c[nt], x[0], y[0], x[1], y[1], qf[nt][j][0], qf[nt][j][1]);
-        mma_f16(c[nt], x[2], y[2], x[3], y[3], qf[nt][j][2], qf[nt][j][3]);
-        if constexpr (MODE == Q32) {
-          mma_f16(c[nt], x[0], y[0], x[1], y[1], ql[nt][j][0], ql[nt][j][1]);
-          mma_f16(c[nt], x[2], y[2], x[3], y[3], ql[nt][j][2], ql[nt][j][3]);
+        float t[4] = {};
+        float(&d)[4] = FLUSH ? t : c[nt];
+        if constexpr (MODE == Q32) {  // the small products first
+          mma_f16(d, x[0], y[0], x[1], y[1], ql[nt][j][0], ql[nt][j][1]);
+          mma_f16(d, x[2], y[2], x[3], y[3], ql[nt][j][2], ql[nt][j][3]);
+        }
+        mma_f16(d, x[0], y[0], x[1], y[1], qf[nt][j][0], qf[nt][j][1]);
+        mma_f16(d, x[2], y[2], x[3], y[3], qf[nt][j][2], qf[nt][j][3]);
+        if constexpr (FLUSH) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) c[nt][k] += t[k];
         }
       }
     }
@@ -446,6 +475,10 @@ struct Rows {
               o[nt][j][q][e] *= al;
               o[nt][j][q][e + 2] *= al;
             }
+          if constexpr (FLUSH)
+            each_sum([&](float& sum, float&, int t_, int e_) {
+              if (t_ == nt && e_ == e) sum *= al;
+            });
 #pragma unroll
           for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -474,6 +507,15 @@ struct Rows {
     }
     output<EDGE>(blk, pb[0], pl[0], drop[0]);
     output<EDGE>(blk + BLK, pb[1], pl[1], drop[1]);
+    if constexpr (FLUSH) {
+      if (++since == kFlush) {
+        since = 0;
+        each_sum([](float& sum, float& part, int, int) {
+          sum += part;
+          part = 0.0f;
+        });
+      }
+    }
   }
 
   // The segment's piece is done: to `out` (whole) or to a record.
@@ -481,6 +523,7 @@ struct Rows {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV;
     const int R = a.T * a.G;
+    if constexpr (FLUSH) each_sum([](float& sum, float& part, int, int) { part += sum; });
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -519,14 +562,18 @@ struct Rows {
 
 template <int HD>
 __host__ __device__ constexpr int attn_stages() { return HD == 128 ? 2 : 4; }
+// Bytes of a warp's fp32 sums.
+__host__ __device__ constexpr int sum_bytes(int HD, int NT, int mode) { return mode == Q32 || mode == COLS32 ? NT * HD * 8 * 4 : 0; }
 template <int HD>
-__host__ __device__ constexpr int attn_smem(int B) { return attn_stages<HD>() * 2 * kv4_block_bytes(HD) + 64 + (2 * B + 1) * 4; }
+__host__ __device__ constexpr int attn_smem(int B, int NT, int mode) {
+  return attn_stages<HD>() * 2 * kv4_block_bytes(HD) + sum_bytes(HD, NT, mode) + 64 + (2 * B + 1) * 4;
+}
 
 template <int HD, int NT, int MODE>
 __global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? (MODE == COLS ? 16 : 12) : 8) : (NT == 1 ? 16 : 12)) kv4_attn_kernel(AttnArgs a) {
   constexpr int ST = attn_stages<HD>(), BLK = kv4_block_bytes(HD);
   extern __shared__ __align__(128) uint8_t sm[];
-  uint64_t* bar = (uint64_t*)(sm + ST * 2 * BLK);
+  uint64_t* bar = (uint64_t*)(sm + ST * 2 * BLK + sum_bytes(HD, NT, MODE));
   int* s_len = (int*)(bar + 8);
   int* s_pre = s_len + a.B;
   const int lane = threadIdx.x;
@@ -555,8 +602,9 @@ __global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? (MODE == COLS ? 16 
   };
   const int n = x1 - x0;
   for (int k = 0; k < ST - 1 && k < n; k++) issue(k);
+  constexpr int RPT = Rows<HD, NT, MODE>::CPT * NT;
   Rows<HD, NT, MODE> rows;
-  constexpr int RPT = NT * (MODE == COLS ? 4 : 8);
+  rows.acc = (float*)(sm + ST * 2 * BLK) + lane;
   int seg = -1, held = 0;
   bool ok = true;
   float* rec = a.rec + (size_t)blockIdx.x * 2 * RPT * (HD + 4);
@@ -697,20 +745,21 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(AttnArgs a, i
 // in turn and join through shared memory, so that one launch is all there is.
 template <int HD, int NT, int MODE>
 __host__ __device__ constexpr int whole_warps() {  // as many as the registers allow
-  return HD == 128 && NT == 2 ? 8 : (NT == 2 || (HD == 128 && MODE == Q32) ? 12 : 16);
+  return HD == 128 && NT == 2 ? 8 : (NT == 2 || (HD == 128 && (MODE == Q32 || MODE == COLS32)) ? 12 : 16);
 }
 template <int HD, int NT, int MODE>
 __host__ __device__ constexpr int whole_smem(int warps) {
-  const int ring = warps * 2 * 2 * kv4_block_bytes(HD), rec = warps * NT * (MODE == COLS ? 4 : 8) * (HD + 4) * 4;
-  return (ring > rec ? ring : rec) + warps * 16;
+  const int ring = warps * 2 * 2 * kv4_block_bytes(HD), rec = warps * NT * Rows<HD, NT, MODE>::CPT * (HD + 4) * 4;
+  return (ring > rec ? ring : rec) + warps * (16 + sum_bytes(HD, NT, MODE));
 }
 template <int HD, int NT, int MODE>
 __global__ void __launch_bounds__(32 * whole_warps<HD, NT, MODE>()) kv4_attn_whole_kernel(AttnArgs a) {
-  constexpr int BLK = kv4_block_bytes(HD), ST = 2, RPT = NT * (MODE == COLS ? 4 : 8);
+  constexpr int BLK = kv4_block_bytes(HD), ST = 2, RPT = NT * Rows<HD, NT, MODE>::CPT;
   extern __shared__ __align__(128) uint8_t sm[];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
   uint8_t* ring = sm + w * ST * 2 * BLK;
-  uint64_t* bar = (uint64_t*)(sm + whole_smem<HD, NT, MODE>(warps) - warps * 16) + w * 2;
+  uint8_t* tail = sm + whole_smem<HD, NT, MODE>(warps) - warps * (16 + sum_bytes(HD, NT, MODE));
+  uint64_t* bar = (uint64_t*)(tail + warps * sum_bytes(HD, NT, MODE)) + w * 2;
   if (lane < ST) mbar_init(bar + lane, 1);
   fence_mbar_init();
   __syncwarp();
@@ -722,6 +771,7 @@ __global__ void __launch_bounds__(32 * whole_warps<HD, NT, MODE>()) kv4_attn_who
   const Span sp = span_of(n, a);
   const int U = sp.units(), mine = U > w ? (U - w + warps - 1) / warps : 0;
   Rows<HD, NT, MODE> rows;
+  rows.acc = (float*)(tail + w * sum_bytes(HD, NT, MODE)) + lane;
   Unit next = {}, cur;  // of this warp's units (k & ~31) + lane, for the issuer and for the reader
   auto issue = [&](int k) {
     if ((k & 31) == 0) next = unit_at<HD>(a, b, kvh, sp.at(w + min(k + lane, mine - 1) * warps), n, held);
@@ -787,6 +837,7 @@ typedef void (*AttnKernel)(AttnArgs);
 template <int HD>
 static AttnKernel attn_kernel(int NT, int mode) {
   if (mode == COLS) return kv4_attn_kernel<HD, 1, COLS>;
+  if (mode == COLS32) return kv4_attn_kernel<HD, 1, COLS32>;
   if (mode == Q16) return NT == 1 ? kv4_attn_kernel<HD, 1, Q16> : kv4_attn_kernel<HD, 2, Q16>;
   return NT == 1 ? kv4_attn_kernel<HD, 1, Q32> : kv4_attn_kernel<HD, 2, Q32>;
 }
@@ -802,6 +853,7 @@ static int launch_whole(const AttnArgs& a, int warps, cudaStream_t s) {
 template <int HD>
 static int launch_whole(const AttnArgs& a, const AttnPlan& p, cudaStream_t s) {
   if (p.mode == COLS) return launch_whole<HD, 1, COLS>(a, p.whole, s);
+  if (p.mode == COLS32) return launch_whole<HD, 1, COLS32>(a, p.whole, s);
   if (p.mode == Q16)
     return p.NT == 1 ? launch_whole<HD, 1, Q16>(a, p.whole, s) : launch_whole<HD, 2, Q16>(a, p.whole, s);
   return p.NT == 1 ? launch_whole<HD, 1, Q32>(a, p.whole, s) : launch_whole<HD, 2, Q32>(a, p.whole, s);
@@ -810,13 +862,13 @@ static int launch_whole(const AttnArgs& a, const AttnPlan& p, cudaStream_t s) {
 // Warps that fit one SM at a time (registers, shared memory), remembered per kernel and size class of
 // the shared memory.
 static int attn_per_sm(int HD, int NT, int mode, int B, int* out) {
-  static std::atomic<int> known[2][2][3][kAttnStreams / 32 + 1];
+  static std::atomic<int> known[2][2][4][kAttnStreams / 32 + 1];
   const int cls = (B + 31) / 32;
   std::atomic<int>& slot = known[HD == 128][NT - 1][mode][cls];
   int n = slot.load(std::memory_order_relaxed);
   if (n == 0) {
     const AttnKernel k = HD == 128 ? attn_kernel<128>(NT, mode) : attn_kernel<64>(NT, mode);
-    const int smem = HD == 128 ? attn_smem<128>(32 * cls) : attn_smem<64>(32 * cls);
+    const int smem = HD == 128 ? attn_smem<128>(32 * cls, NT, mode) : attn_smem<64>(32 * cls, NT, mode);
     RNGD_TRY(check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, 32, smem), "occupancy(kv4_attn_kernel)"));
     if (n < 1) n = 1;
     slot.store(n, std::memory_order_relaxed);
@@ -834,8 +886,8 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
   RNGD_REQUIRE(window >= 0 && sinks >= 0, "kv4_attn: window=%d sinks=%d", window, sinks);
   const int Bl = B < kAttnStreams ? B : kAttnStreams;  // streams of one launch
   const long R = (long)T * (NH / NKV);
-  p->mode = R <= 4 ? COLS : (dtype == DT_F32 ? Q32 : Q16);
-  const long cpt = p->mode == COLS ? 4 : 8, tiles = (R + cpt - 1) / cpt;
+  p->mode = R <= 4 ? (dtype == DT_F32 ? COLS32 : COLS) : (dtype == DT_F32 ? Q32 : Q16);
+  const long cpt = R <= 4 ? 4 : 8, tiles = (R + cpt - 1) / cpt;
   RNGD_REQUIRE(R < (1l << 24), "kv4_attn: %ld query rows of a kv head", R);
   p->NT = tiles > 1 ? 2 : 1;
   p->RT = (int)((tiles + p->NT - 1) / p->NT);
@@ -846,7 +898,7 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
     const long w = ((long)window + T - 2) / kUnit + 2 + ((long)sinks + kUnit - 1) / kUnit;
     most_u = most_u < w ? most_u : w;
   }
-  const int cap = HD == 128 && p->NT == 2 ? 8 : (p->NT == 2 || (HD == 128 && p->mode == Q32) ? 12 : 16);
+  const int cap = HD == 128 && p->NT == 2 ? 8 : (p->NT == 2 || (HD == 128 && (p->mode == Q32 || p->mode == COLS32)) ? 12 : 16);
   // One CTA per segment saves the joining kernel (and its launch) but leaves a long stream to one SM.  Streams
   // of one length, 32/8 heads of 128, us in a graph, whole against runs: 1x387 8.2 and 9.9, 1x1000 10.8 and
   // 10.3, 1x2000 14.7 and 10.4; 16x300 7.8 and 15.3, 16x4000 23.6 and 31.9; 64x1000 23.5 and 34.6, 64x5000
@@ -854,7 +906,7 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
   const long segs = (long)Bl * NKV * p->RT;
   p->whole = 0;
   if (most_u <= 48 || (most_u <= 128 && segs >= 64)) {
-    long w = segs < 1 ? 1 : (long)num_sms() * 16 / segs;
+    long w = segs < 1 ? 1 : (long)num_sms() * cap / segs;  // cap warps fill an SM
     w = w < 2 ? 2 : (w < cap ? w : cap);
     p->whole = (int)(most_u < 1 ? 1 : (most_u < w ? most_u : w));
   }
@@ -865,7 +917,7 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
   const long most = (long)num_sms() * per;
   p->warps = (int)(units < 1 ? 1 : (units < most ? units : most));
   p->pre_bytes = ((size_t)(Bl + 1) * 4 + 15) / 16 * 16;
-  p->bytes = p->whole ? 16 : p->pre_bytes + (size_t)p->warps * 2 * p->rows * (HD + 4) * 4;
+  p->bytes = p->whole ? 0 : p->pre_bytes + (size_t)p->warps * 2 * p->rows * (HD + 4) * 4;
   return RNGD_OK;
 }
 
@@ -891,7 +943,7 @@ static int launch_kv4_attn(AttnArgs a, const AttnPlan& p, int B, int HD, void* w
       continue;
     }
     const AttnKernel k = HD == 128 ? attn_kernel<128>(p.NT, p.mode) : attn_kernel<64>(p.NT, p.mode);
-    RNGD_TRY(launch_pdl(k, dim3(p.warps), dim3(32), HD == 128 ? attn_smem<128>(a.B) : attn_smem<64>(a.B), s,
+    RNGD_TRY(launch_pdl(k, dim3(p.warps), dim3(32), HD == 128 ? attn_smem<128>(a.B, p.NT, p.mode) : attn_smem<64>(a.B, p.NT, p.mode), s,
                         "kv4_attn_kernel", a));
     // few segments have many records each: a CTA per row, its records shared by 16 warps; many segments: a CTA
     // for all rows of one (64x5000: 105 us with 16 warps a row, 91 us so)
@@ -912,7 +964,7 @@ int launch_kv4_decode_attn(const float* q, const void* pool, int P, int NKV, int
   RNGD_TRY(check_pool("decode_layers_kv4", pool, 0, P, NKV, HD));
   AttnPlan p;
   RNGD_TRY(attn_plan(DT_F32, B, 1, NH, NKV, HD, ld_table, window, sinks, &p));
-  RNGD_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.bytes,
+  RNGD_REQUIRE(p.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.bytes),
                "decode_layers_kv4: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, p.bytes);
   AttnArgs a = {};
   a.q = q;
@@ -968,7 +1020,7 @@ extern "C" int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out,
   RNGD_TRY(attn_plan(dtype, B, T, NH, NKV, HD, ld_table, window, sinks, &p));
   if (B == 0 || T == 0) return RNGD_OK;
   RNGD_REQUIRE(q && out && q_strides && out_strides && lens && (table || ld_table == 0), "kv4_attn: null pointer");
-  RNGD_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.bytes,
+  RNGD_REQUIRE(p.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.bytes),
                "kv4_attn: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, p.bytes);
   AttnArgs a = {};
   a.q = q;

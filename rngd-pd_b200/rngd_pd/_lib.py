@@ -228,23 +228,6 @@ def raw_stream(index):
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-class _Here:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def device_of(dev):
-    """Context in which the GPU `dev` is current (nothing to do where it already is)."""
-    import torch
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-
 def exported_symbols():
     """Names declared in include/rngd_b200.h, for the ABI completeness test."""
     return [n for n in dir(lib) if n.startswith("rngd_")]

@@ -40,15 +40,17 @@ def select(logits, scores, done, beams, eos=-1):
     _vector("done", done, torch.bool, R, dev)
     if eos >= V:
         raise ValueError(f"eos={eos} outside the vocabulary of {V}")
-    with _lib.device_of(dev):
-        shape = (R // beams, beams)
-        out = torch.empty(shape, dtype=torch.float32, device=dev)
-        parents = torch.empty(shape, dtype=torch.int32, device=dev)
-        tokens = torch.empty_like(parents)
-        ended = torch.empty(shape, dtype=torch.bool, device=dev)
-        need = _lib.workspace_bytes("rngd_beam_workspace", _DT[logits.dtype], R, V, beams)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.check(_select(logits.data_ptr(), _DT[logits.dtype], logits.stride(0), R, V, beams, scores.data_ptr(),
-                           done.data_ptr(), eos, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
-                           ended.data_ptr(), ws.data_ptr(), need, _lib.raw_stream(dev.index)))
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return select(logits, scores, done, beams, eos)
+    shape = (R // beams, beams)
+    out = torch.empty(shape, dtype=torch.float32, device=dev)
+    parents = torch.empty(shape, dtype=torch.int32, device=dev)
+    tokens = torch.empty_like(parents)
+    ended = torch.empty(shape, dtype=torch.bool, device=dev)
+    need = _lib.workspace_bytes("rngd_beam_workspace", _DT[logits.dtype], R, V, beams)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.check(_select(logits.data_ptr(), _DT[logits.dtype], logits.stride(0), R, V, beams, scores.data_ptr(),
+                       done.data_ptr(), eos, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                       ended.data_ptr(), ws.data_ptr(), need, _lib.raw_stream(dev.index)))
     return out, parents, tokens, ended

@@ -47,6 +47,11 @@ def empty_state(rows, width, pages, device="cuda"):
     return (torch.zeros(pages, **i32), torch.full((rows, width), -1, **i32), torch.zeros(rows, **i32))
 
 
+def _elsewhere(dev):
+    """Whether another GPU than the tensors' is current (the calls below then start over with theirs)."""
+    return dev.index != torch.cuda.current_device()
+
+
 def _pool_dims(pool, layers):
     """(L, P, NKV, HD, bytes between layers) of a pool, or of one layer's where `layers` is false."""
     shape = pool.shape
@@ -97,10 +102,12 @@ def store(pool, table, start, k, v, count=None):
     kp, ks = _rows("k", k, 5)
     vp, vs = _rows("v", v, 5)
     width = table.shape[-1]
-    with _lib.device_of(dev):
-        _check(_store(pool.data_ptr(), layer, P, NKV, HD, L, _i32("table", table, (B, width), dev), width,
-                      _i32("start", start, (B,), dev), None if count is None else _i32("count", count, (B,), dev), B, T,
-                      kp, ks, vp, vs, _DT[k.dtype], _lib.raw_stream(dev.index)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return store(pool if pool.dim() == 5 else pool.unsqueeze(0), table, start, k, v, count)
+    _check(_store(pool.data_ptr(), layer, P, NKV, HD, L, _i32("table", table, (B, width), dev), width,
+                  _i32("start", start, (B,), dev), None if count is None else _i32("count", count, (B,), dev), B, T,
+                  kp, ks, vp, vs, _DT[k.dtype], _lib.raw_stream(dev.index)))
 
 
 def load(pool, table, start, tokens, count=None, dtype=torch.float16):
@@ -116,12 +123,14 @@ def load(pool, table, start, tokens, count=None, dtype=torch.float16):
     if tokens < 0:
         raise ValueError(f"tokens={tokens}")
     shape = (L, B, tokens, NKV, HD) if layers else (B, tokens, NKV, HD)
-    with _lib.device_of(dev):
-        k = torch.empty(shape, dtype=dtype, device=dev)
-        v = torch.empty_like(k)
-        _check(_load(pool.data_ptr(), layer, P, NKV, HD, L, _i32("table", table, (B, width), dev), width,
-                     _i32("start", start, (B,), dev), None if count is None else _i32("count", count, (B,), dev), B,
-                     tokens, k.data_ptr(), v.data_ptr(), _DT[dtype], _lib.raw_stream(dev.index)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return load(pool, table, start, tokens, count, dtype)
+    k = torch.empty(shape, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    _check(_load(pool.data_ptr(), layer, P, NKV, HD, L, _i32("table", table, (B, width), dev), width,
+                 _i32("start", start, (B,), dev), None if count is None else _i32("count", count, (B,), dev), B,
+                 tokens, k.data_ptr(), v.data_ptr(), _DT[dtype], _lib.raw_stream(dev.index)))
     return k, v
 
 
@@ -131,8 +140,8 @@ def attention(q, pool, table, lens, window=0, sinks=0, scale=None, out=None):
     q: [B, T, NH, HD] bfloat16, float16 or float32 (any strides, the last dimension contiguous), NH a multiple of
     the pool's kv heads; pool: one layer's.  Token t of sequence b stands at i = lens[b] - T + t (its own key and
     value are stored already) and sees positions j <= i with j > i - window (0: no window) or j < sinks; what it
-    does not see, and what lies where there is no page, has no part in the result.  A token that sees nothing gives
-    zeros.  scale: 1 / sqrt(HD) by default.  Returns [B, T, NH, HD] of q's type, in `out` where given."""
+    does not see, and what lies where there is no page, has no part in the result, NaN included.  A token that sees
+    nothing gives zeros; one that sees a NaN gives NaN, at least in the dimensions concerned.  scale: 1 / sqrt(HD) by default.  Returns [B, T, NH, HD] of q's type, in `out` where given."""
     _, P, NKV, HD, _ = _pool_dims(pool, False)
     dev, dt = pool.device, q.dtype
     qp, qs = _rows("q", q, 4)
@@ -145,18 +154,20 @@ def attention(q, pool, table, lens, window=0, sinks=0, scale=None, out=None):
         raise ValueError(f"window={window} and sinks={sinks} must not be negative")
     width = table.shape[-1]
     window, sinks = min(window, _INT_MAX), min(sinks, _INT_MAX)
-    with _lib.device_of(dev):
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != q.shape or out.dtype is not dt or out.device != dev:
-            raise ValueError(f"out must be {tuple(q.shape)} {dt} on {dev}, got {tuple(out.shape)} {out.dtype}")
-        op, os = _rows("out", out, 4)
-        need = _lib.workspace_bytes("rngd_kv4_attn_workspace", _DT[dt], B, T, NH, NKV, HD, width, window,
-                                     sinks)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _check(_attn(qp, qs, op, os, _DT[dt], pool.data_ptr(), P, NKV, HD, _i32("table", table, (B, width), dev), width,
-                     _i32("lens", lens, (B,), dev), B, T, NH, window, sinks,
-                     HD ** -0.5 if scale is None else scale, ws.data_ptr(), need, _lib.raw_stream(dev.index)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return attention(q, pool, table, lens, window, sinks, scale, out)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype is not dt or out.device != dev:
+        raise ValueError(f"out must be {tuple(q.shape)} {dt} on {dev}, got {tuple(out.shape)} {out.dtype}")
+    op, os = _rows("out", out, 4)
+    need = _lib.workspace_bytes("rngd_kv4_attn_workspace", _DT[dt], B, T, NH, NKV, HD, width, window,
+                                 sinks)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr() if need else None
+    _check(_attn(qp, qs, op, os, _DT[dt], pool.data_ptr(), P, NKV, HD, _i32("table", table, (B, width), dev), width,
+                 _i32("lens", lens, (B,), dev), B, T, NH, window, sinks,
+                 HD ** -0.5 if scale is None else scale, ws, need, _lib.raw_stream(dev.index)))
     return out
 
 
@@ -172,16 +183,18 @@ def fork(pool, ref, table, lens, parents=None, room=0):
     L, P, NKV, HD, layer = _pool_dims(pool, True)
     dev = pool.device
     R, width = table.shape
-    with _lib.device_of(dev):
-        rp, tp, lp = _i32("ref", ref, (P,), dev), _i32("table", table, (R, width), dev), _i32("lens", lens, (R,), dev)
-        new_ref, new_table, new_lens = torch.empty_like(ref), torch.empty_like(table), torch.empty_like(lens)
-        short = torch.empty(1, dtype=torch.int32, device=dev)
-        need = _lib.workspace_bytes("rngd_kv4_fork_workspace", R, width)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _check(_fork(pool.data_ptr(), layer, L, P, NKV, HD, rp, tp, width, lp, R,
-                     None if parents is None else _i32("parents", parents, (R,), dev), room, new_ref.data_ptr(),
-                     new_table.data_ptr(), new_lens.data_ptr(), short.data_ptr(), ws.data_ptr(), need,
-                     _lib.raw_stream(dev.index)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return fork(pool, ref, table, lens, parents, room)
+    rp, tp, lp = _i32("ref", ref, (P,), dev), _i32("table", table, (R, width), dev), _i32("lens", lens, (R,), dev)
+    new_ref, new_table, new_lens = torch.empty_like(ref), torch.empty_like(table), torch.empty_like(lens)
+    short = torch.empty(1, dtype=torch.int32, device=dev)
+    need = _lib.workspace_bytes("rngd_kv4_fork_workspace", R, width)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _check(_fork(pool.data_ptr(), layer, L, P, NKV, HD, rp, tp, width, lp, R,
+                 None if parents is None else _i32("parents", parents, (R,), dev), room, new_ref.data_ptr(),
+                 new_table.data_ptr(), new_lens.data_ptr(), short.data_ptr(), ws.data_ptr(), need,
+                 _lib.raw_stream(dev.index)))
     return new_ref, new_table, new_lens, short
 
 
@@ -192,12 +205,14 @@ def compact(pool, ref, table):
     L, P, NKV, HD, layer = _pool_dims(pool, True)
     dev = pool.device
     R, width = table.shape
-    with _lib.device_of(dev):
-        rp, tp = _i32("ref", ref, (P,), dev), _i32("table", table, (R, width), dev)
-        new_ref, new_table = torch.empty_like(ref), torch.empty_like(table)
-        live = torch.empty(1, dtype=torch.int32, device=dev)
-        need = _lib.workspace_bytes("rngd_kv4_compact_workspace", P)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _check(_compact(pool.data_ptr(), layer, L, P, NKV, HD, rp, tp, width, R, new_ref.data_ptr(),
-                        new_table.data_ptr(), live.data_ptr(), ws.data_ptr(), need, _lib.raw_stream(dev.index)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return compact(pool, ref, table)
+    rp, tp = _i32("ref", ref, (P,), dev), _i32("table", table, (R, width), dev)
+    new_ref, new_table = torch.empty_like(ref), torch.empty_like(table)
+    live = torch.empty(1, dtype=torch.int32, device=dev)
+    need = _lib.workspace_bytes("rngd_kv4_compact_workspace", P)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _check(_compact(pool.data_ptr(), layer, L, P, NKV, HD, rp, tp, width, R, new_ref.data_ptr(),
+                    new_table.data_ptr(), live.data_ptr(), ws.data_ptr(), need, _lib.raw_stream(dev.index)))
     return new_ref, new_table, live

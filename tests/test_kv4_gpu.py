@@ -205,6 +205,61 @@ def test_attention_without_pages():
     assert np.all(_check(q, pool, narrow, lens, "fp32") == 0)
 
 
+@pytest.mark.parametrize("HD,NH", [(64, 4), (64, 16), (128, 4), (128, 16)])
+def test_attention_keeps_unseen_nans_out(HD, NH):
+    """NaN in keys or values outside the window, and in what a later token alone sees."""
+    from rngd_pd import kv4
+    g = torch.Generator().manual_seed(21)
+    T, n, W = 3, 150, 60
+    k, v = torch.randn(2, 1, 1, n, 2, HD, generator=g)
+    k[0, 0, 7, 0, 3] = v[0, 0, 9, 1, 40] = v[0, 0, n - T - W, 0, 0] = float("nan")   # before any window
+    v[0, 0, n - 1, 0, 5] = k[0, 0, n - 2, 1, 5] = float("nan")                       # the last tokens' own
+    pool, table = _pool_of(1, 4, 2, HD), torch.tensor([[3, 1, 0]], dtype=torch.int32, device="cuda")
+    kv4.store(pool, table, torch.zeros(1, dtype=torch.int32, device="cuda"), k.cuda(), v.cuda())
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, T, NH, HD, generator=g).cuda()
+    got = _np(kv4.attention(q, pool[0], table, lens, window=W))[0]
+    G = NH // 2
+    assert np.isfinite(got[0]).all() and np.isfinite(got[1, :G]).all()
+    assert np.isnan(got[1, G:]).all() and np.isnan(got[2, :G]).any() and np.isnan(got[2, G:]).all()
+    # what is finite is what it would be without the NaNs
+    clean = k.nan_to_num(1.0), v.nan_to_num(1.0)
+    kv4.store(pool, table, torch.zeros(1, dtype=torch.int32, device="cuda"), clean[0].cuda(), clean[1].cuda())
+    want = _np(kv4.attention(q, pool[0], table, lens, window=W))[0]
+    np.testing.assert_allclose(got[0], want[0], rtol=0, atol=1e-6)
+
+
+def test_attention_of_more_streams_than_a_launch_takes():
+    B = 1030
+    lens = [(7 * b) % 60 for b in range(B)]
+    pool, table = _cache(B, 1, 1, 64, lens, 22)
+    q = torch.randn(B, 1, 2, 64, generator=torch.Generator().manual_seed(9)).cuda()
+    _check(q, pool, table, lens, "fp32")
+
+
+def test_offsets_beyond_32_bits():
+    """Pages, and layers of a pool, more than 4 GB apart."""
+    from rngd_pd import kv4
+    P, NKV, HD, n = 30000, 8, 128, 130
+    g = torch.Generator().manual_seed(23)
+    k, v = (torch.randn(2, 1, n, NKV, HD, generator=g).to(torch.bfloat16).cuda() for _ in (0, 1))
+    q = torch.randn(1, 1, 32, HD, generator=g).cuda()
+    zero, lens = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.tensor([n], dtype=torch.int32, device="cuda")
+    near, far = kv4.alloc_pool(2, 3, NKV, HD), kv4.alloc_pool(2, P, NKV, HD)
+    tn = torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda")
+    tf = torch.tensor([[P - 1, 3, P - 2]], dtype=torch.int32, device="cuda")
+    kv4.store(near, tn, zero, k, v)
+    kv4.store(far, tf, zero, k, v)
+    for l in range(2):
+        assert torch.equal(kv4.attention(q, near[l], tn, lens), kv4.attention(q, far[l], tf, lens))
+    assert all(torch.equal(a, b) for a, b in zip(kv4.load(near, tn, zero, n), kv4.load(far, tf, zero, n)))
+    ref0 = torch.zeros(P, dtype=torch.int32, device="cuda")
+    ref0[tf[0].long()] = 1
+    _, t2, live = kv4.compact(far, ref0, tf)
+    assert live.item() == 3 and sorted(t2[0].tolist()) == [0, 1, 2]
+    assert all(torch.equal(a, b) for a, b in zip(kv4.load(near, tn, zero, n), kv4.load(far, t2, zero, n)))
+
+
 def test_attention_takes_any_strides_and_writes_into_out():
     lens = [77, 130]
     pool, table = _cache(2, 3, 2, 64, lens, 15)
