@@ -16,6 +16,12 @@
 // neither ties nor the order in which threads run can show.  A second kernel, one CTA per group, joins
 // the parts' sums into log-sum-exps and selects among the rows' candidates in the same way, by (score,
 // place).
+//
+// Bytes would allow 20 us for 64 groups of 8 beams by 128256 bf16 logits; the two kernels take 49 (in a
+// graph, logits from memory): an exponential and its sum cost three to four instructions an element on
+// top of the maximum and the copy, so instruction issue bounds the row kernel, then the barriers where a
+// row ends.  1 x 5 x 32003 fp32: 7.7 us, two launches' latency; 16 x 32 x 128256 fp32: 81 us (3.3 TB/s).
+// Four threads rank each set's key: with one, 50.1, 8.1 and 81.5 us.
 #include "kv4.cuh"
 
 namespace rngd {
@@ -57,18 +63,20 @@ struct BeamArgs {
 constexpr int kSets = 64;
 
 // The W-th largest of the sets' keys (each unique, or 0), 0 if there are fewer: every key counts those
-// above it.  s_keys holds the sets' keys; all threads call.
+// above it, four threads to a key.  s_keys holds the sets' keys; all threads call.
 __device__ __forceinline__ u64 nth_key(int W, const u64* s_keys, u64* s_nth) {
   if (threadIdx.x == 0) *s_nth = 0;
   __syncthreads();
-  if (threadIdx.x < kSets) {
-    const u64 mine = s_keys[threadIdx.x];
+  if (threadIdx.x < 4 * kSets) {
+    const u64 mine = s_keys[threadIdx.x >> 2];
     int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < kSets; i += 2) {
-      const ulonglong2 k = *(const ulonglong2*)(s_keys + i);
+#pragma unroll
+    for (int i = 0; i < kSets / 4; i += 2) {
+      const ulonglong2 k = *(const ulonglong2*)(s_keys + 2 * (threadIdx.x & 3) + 4 * i);
       above += (k.x > mine) + (k.y > mine);
     }
+    above += __shfl_xor_sync(0xffffffffu, above, 1);
+    above += __shfl_xor_sync(0xffffffffu, above, 2);
     if (above == W - 1 && mine != 0) *s_nth = mine;
   }
   __syncthreads();
@@ -329,14 +337,19 @@ __global__ void __launch_bounds__(kRowThreads, 3) beam_row_kernel(BeamArgs a) {
       for (int o = 1; o < PER; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (tid % PER == 0) s_set[tid / PER] = m;
       __syncthreads();
-      if (tid < kSets) {
-        const float mine = s_set[tid];
+      if (tid < 4 * kSets) {  // four threads to a set
+        const float mine = s_set[tid >> 2];
         int above = 0, same = 0;
 #pragma unroll
-        for (int i = 0; i < kSets; i += 4) {
-          const float4 q = *(const float4*)(s_set + i);
+        for (int i = 0; i < kSets / 16; i++) {
+          const float4 q = *(const float4*)(s_set + 4 * (tid & 3) + 16 * i);
           above += (q.x > mine) + (q.y > mine) + (q.z > mine) + (q.w > mine);
           same += (q.x == mine) + (q.y == mine) + (q.z == mine) + (q.w == mine);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          above += __shfl_xor_sync(0xffffffffu, above, o);
+          same += __shfl_xor_sync(0xffffffffu, same, o);
         }
         if (above < a.W && above + same >= a.W) {  // one value, however many say so
           s_bound = mine;
@@ -439,6 +452,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) beam_row_kernel(BeamArgs a) {
 // One CTA per group.  per: candidates of a thread; with `rounds` the best are taken one after the other
 // instead (where the list of a very large vocabulary would not fit shared memory).
 constexpr int kGroupThreads = 512;
+static_assert(kRowThreads >= 4 * kSets && kGroupThreads >= 4 * kSets, "sets are ranked by four threads each");
 __global__ void __launch_bounds__(kGroupThreads) beam_group_kernel(BeamArgs a, int rounds) {
   constexpr int PER = kGroupThreads / kSets;
   __shared__ __align__(16) u64 s_keys[kSets];
