@@ -17,10 +17,10 @@
 // the parts' sums into log-sum-exps and selects among the rows' candidates in the same way, by (score,
 // place).
 //
-// Bytes would allow 20 us for 64 groups of 8 beams by 128256 bf16 logits; the two kernels take 49 (in a
-// graph, logits from memory): an exponential and its sum cost three to four instructions an element on
-// top of the maximum and the copy, so instruction issue bounds the row kernel, then the barriers where a
-// row ends.  1 x 5 x 32003 fp32: 7.7 us, two launches' latency; 16 x 32 x 128256 fp32: 81 us (3.3 TB/s).
+// Bytes would allow 20 us for 64 groups of 8 beams by 128256 bf16 logits; the two kernels take 48 to 49 (in a
+// graph, logits from memory, 2.7 TB/s).  Instruction issue (0.65 a cycle and scheduler) and the barriers where
+// a row ends bound the row kernel; the group kernel's 8 us are latency.  1 x 5 x 32003 fp32: 7.7 us, two
+// launches' latency; 16 x 32 x 128256 fp32: 81 us (3.3 TB/s).
 // Four threads rank each set's key: with one, 50.1, 8.1 and 81.5 us.
 #include "kv4.cuh"
 
