@@ -164,27 +164,17 @@ __device__ __forceinline__ Unit look_up(int x, const AttnArgs& a, const int* len
   return u;
 }
 
-// Eight consecutive elements of q as fp32.
-__device__ __forceinline__ void load_q8(const AttnArgs& a, size_t at, float* x) {
-  if (!a.qvec) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = load1(a.q, at + e, a.dt);
-  } else if (a.dt == DT_F32) {
-    const float4 u = __ldg((const float4*)((const float*)a.q + at)), v = __ldg((const float4*)((const float*)a.q + at) + 1);
-    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-    x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+// Eight consecutive elements of 16-bit q as fp32.
+__device__ __forceinline__ void unpack_q8(const uint4& u, int dt, float* x) {
+  if (dt == DT_BF16) {
+    unpack8(u, x);
   } else {
-    const uint4 u = __ldg((const uint4*)((const uint16_t*)a.q + at));
-    if (a.dt == DT_BF16) {
-      unpack8(u, x);
-    } else {
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float2 f = __half22float2(u2h(w[e]));
-        x[2 * e] = f.x;
-        x[2 * e + 1] = f.y;
-      }
+    for (int e = 0; e < 4; e++) {
+      const float2 f = __half22float2(u2h(w[e]));
+      x[2 * e] = f.x;
+      x[2 * e + 1] = f.y;
     }
   }
 }
@@ -224,22 +214,74 @@ struct Rows {
           for (int k = 0; k < 4; k++) f(acc[(((nt * NG + j) * 2 + q) * 4 + k) * 32], o[nt][j][q][k], nt, k & 1);
   }
 
-  __device__ __forceinline__ void begin(const AttnArgs& a, int seg, int n) {
+  // A segment's q as it lies in memory: this lane's eight elements of each row and 32 dimensions.  All loads
+  // are issued before any is used (one after the other they cost a memory latency each: 1x387 took 8.1 us in a graph, 7.3
+  // so; 16x1000 with 20 rows of 128 16.3 and 13.8).
+  static constexpr int QV = FLUSH ? 2 : 1;  // 16-byte vectors of eight elements
+  struct Query {
+    uint4 v[NT][NG][QV];
+  };
+  __device__ __forceinline__ void fetch(const AttnArgs& a, int seg, Query& q) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV;
     const int R = a.T * a.G;
+    size_t at[NT];
+    bool there[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int r = (rt * NT + nt) * CPT + (SPLIT ? g & 3 : g);
+      there[nt] = r < R;
+      at[nt] = (size_t)(b * a.qs[0] + r / a.G * a.qs[1] + (kvh * a.G + r % a.G) * a.qs[2]) + 8 * t;
+    }
+    if (a.qvec) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+#pragma unroll
+          for (int h = 0; h < QV; h++) {
+            q.v[nt][j][h] = make_uint4(0u, 0u, 0u, 0u);
+            if (there[nt]) q.v[nt][j][h] = __ldg((const uint4*)((const uint8_t*)a.q + (at[nt] + 32 * j) * (2 * QV)) + h);
+          }
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+#pragma unroll
+          for (int h = 0; h < QV; h++) {
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+            if (there[nt]) {
+              const size_t i0 = at[nt] + 32 * j + 4 * h;
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                if constexpr (FLUSH)
+                  w[e] = ((const uint32_t*)a.q)[i0 + e];
+                else
+                  w[e] = (uint32_t)((const uint16_t*)a.q)[i0 + 2 * e] | (uint32_t)((const uint16_t*)a.q)[i0 + 2 * e + 1] << 16;
+              }
+            }
+            q.v[nt][j][h] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+    }
+  }
+
+  __device__ __forceinline__ void begin(const AttnArgs& a, int seg, int n, const Query& q) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rt = seg % a.RT, R = a.T * a.G;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
       float x[NG][8];
       float mx = 0.0f;
 #pragma unroll
       for (int j = 0; j < NG; j++) {
-        if (r < R) {
-          load_q8(a, (size_t)(b * a.qs[0] + r / a.G * a.qs[1] + (kvh * a.G + r % a.G) * a.qs[2]) + 32 * j + 8 * t, x[j]);
-        } else {
+        if constexpr (FLUSH) {
+          const uint4 u = q.v[nt][j][0], v = q.v[nt][j][QV - 1];
+          const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int e = 0; e < 8; e++) x[j][e] = 0.0f;
+          for (int e = 0; e < 8; e++) x[j][e] = __uint_as_float(w[e]);
+        } else {
+          unpack_q8(q.v[nt][j][0], a.dt, x[j]);
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[j][e]));
@@ -569,8 +611,8 @@ __host__ __device__ constexpr int attn_smem(int B, int NT, int mode) {
   return attn_stages<HD>() * 2 * kv4_block_bytes(HD) + sum_bytes(HD, NT, mode) + 64 + (2 * B + 1) * 4;
 }
 
-// 8 streams of 65001 positions, 32 query and 8 kv heads of 128, bf16: 127 us in a graph with the joining
-// (5.2 TB/s); from 20480 positions (51 us) on, more of them arrive at 5.9 TB/s, 0.92 of the copy bandwidth, so
+// 8 streams of 65001 positions, 32 query and 8 kv heads of 128, bf16: 126 us in a graph with the joining
+// (5.3 TB/s); from 20480 positions (49 us) on, more of them arrive at 5.9 TB/s, 0.92 of the copy bandwidth, so
 // that about 15 us are fixed: the launches, the first copies of a ring and the joining (4 us).  The decoding of
 // the codes is what comes after memory: 0.60 instructions a cycle and scheduler, the integer pipe at 57%, the
 // tensor pipe at 17% (8x20480).  16 warps an SM is what 128 registers allow.
@@ -634,7 +676,9 @@ __global__ void __launch_bounds__(32, HD == 128 ? (NT == 1 ? (MODE == COLS ? 16 
       seg0 = s_pre[b] + seg % per * ub;
       seg1 = seg0 + ub;
       held = min(s_len[b], a.ld_table * kPage);
-      rows.begin(a, seg, s_len[b]);
+      typename Rows<HD, NT, MODE>::Query q;
+      rows.fetch(a, seg, q);
+      rows.begin(a, seg, s_len[b], q);
     }
     if (ok) ok = mbar_wait(bar + k % ST, (k / ST) & 1, ST_TMA_WAIT, &g_status_kv4);
     ok = __all_sync(0xffffffffu, ok);
@@ -748,7 +792,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(AttnArgs a, i
 
 // The same for sequences that are known to be short: one CTA holds a segment, its warps take the units
 // in turn and join through shared memory, so that one launch is all there is.  Latency bounds it: one stream of
-// 387 positions takes 8.0 us in a graph, 16 of 384 with fp32 q 7.6, 64 of 300 12.3 (2.0 TB/s).
+// 387 positions takes 7.3 us in a graph, 16 of 384 with fp32 q 6.8, 64 of 300 10.9 (2.3 TB/s).
 template <int HD, int NT, int MODE>
 __host__ __device__ constexpr int whole_warps() {  // as many as the registers allow
   return HD == 128 && NT == 2 ? 8 : (NT == 2 || (HD == 128 && (MODE == Q32 || MODE == COLS32)) ? 12 : 16);
@@ -773,10 +817,12 @@ __global__ void __launch_bounds__(32 * whole_warps<HD, NT, MODE>()) kv4_attn_who
   grid_dep_launch();
   const int seg = blockIdx.x;
   const int rt = seg % a.RT, kvh = seg / a.RT % a.NKV, b = seg / a.RT / a.NKV;
+  Rows<HD, NT, MODE> rows;
+  typename Rows<HD, NT, MODE>::Query q;
+  rows.fetch(a, seg, q);  // ahead of the length, the table and the copies, which come one after the other
   const int n = a.lens[b] + a.len_add, held = min(max(n, 0), a.ld_table * kPage);
   const Span sp = span_of(n, a);
   const int U = sp.units(), mine = U > w ? (U - w + warps - 1) / warps : 0;
-  Rows<HD, NT, MODE> rows;
   rows.acc = (float*)(tail + w * sum_bytes(HD, NT, MODE)) + lane;
   Unit next = {}, cur;  // of this warp's units (k & ~31) + lane, for the issuer and for the reader
   auto issue = [&](int k) {
@@ -789,7 +835,7 @@ __global__ void __launch_bounds__(32 * whole_warps<HD, NT, MODE>()) kv4_attn_who
   };
   for (int k = 0; k < min(mine, 2); k++) issue(k);
   cur = next;
-  rows.begin(a, seg, n);
+  rows.begin(a, seg, n, q);
   bool ok = true;
   int k = 0;
   for (; k < mine; k++) {
@@ -820,6 +866,7 @@ __global__ void __launch_bounds__(32 * whole_warps<HD, NT, MODE>()) kv4_attn_who
     if (r >= a.T * a.G) break;
     Joined<4> x;
     x.clear();
+#pragma unroll 4
     for (int k = 0; k < parts; k++) {
       const float* rc = rec + ((size_t)k * RPT + rl) * (HD + 4);
       const float4 u = *(const float4*)(rc + d);
