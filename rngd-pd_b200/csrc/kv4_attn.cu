@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(AttnArgs a, i
 // 387 positions takes 7.3 us in a graph, 16 of 384 with fp32 q 6.8, 64 of 300 10.9 (2.3 TB/s).
 template <int HD, int NT, int MODE>
 __host__ __device__ constexpr int whole_warps() {  // as many as the registers allow
-  return HD == 128 && NT == 2 ? 8 : (NT == 2 || (HD == 128 && (MODE == Q32 || MODE == COLS32)) ? 12 : 16);
+  return HD == 128 && NT > 1 ? 8 : (NT > 1 || (HD == 128 && (MODE == Q32 || MODE == COLS32)) ? 12 : 16);
 }
 template <int HD, int NT, int MODE>
 __host__ __device__ constexpr int whole_smem(int warps) {
@@ -908,7 +908,10 @@ static int launch_whole(const AttnArgs& a, const AttnPlan& p, cudaStream_t s) {
   if (p.mode == COLS) return launch_whole<HD, 1, COLS>(a, p.whole, s);
   if (p.mode == COLS32) return launch_whole<HD, 1, COLS32>(a, p.whole, s);
   if (p.mode == Q16)
-    return p.NT == 1 ? launch_whole<HD, 1, Q16>(a, p.whole, s) : launch_whole<HD, 2, Q16>(a, p.whole, s);
+    return p.NT == 1 ? launch_whole<HD, 1, Q16>(a, p.whole, s)
+                     : (p.NT == 2 ? launch_whole<HD, 2, Q16>(a, p.whole, s) : launch_whole<HD, 3, Q16>(a, p.whole, s));
+  if constexpr (HD == 64)
+    if (p.NT == 3) return launch_whole<HD, 3, Q32>(a, p.whole, s);
   return p.NT == 1 ? launch_whole<HD, 1, Q32>(a, p.whole, s) : launch_whole<HD, 2, Q32>(a, p.whole, s);
 }
 
@@ -951,17 +954,30 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
     const long w = ((long)window + T - 2) / kUnit + 2 + ((long)sinks + kUnit - 1) / kUnit;
     most_u = most_u < w ? most_u : w;
   }
-  const int cap = HD == 128 && p->NT == 2 ? 8 : (p->NT == 2 || (HD == 128 && (p->mode == Q32 || p->mode == COLS32)) ? 12 : 16);
   // One CTA per segment saves the joining kernel (and its launch) but leaves a long stream to one SM.  Streams
-  // of one length, 32/8 heads of 128, us in a graph, whole against runs: 1x387 8.2 and 9.9, 1x1000 10.8 and
+  // of one length, 32/8 heads of 128, us in a graph, whole against runs (before q was fetched at once): 1x387 8.2 and 9.9, 1x1000 10.8 and
   // 10.3, 1x2000 14.7 and 10.4; 16x300 7.8 and 15.3, 16x4000 23.6 and 31.9; 64x1000 23.5 and 34.6, 64x5000
   // 90.5 and 91.2.  A CTA has no more warps than let all CTAs run at once (64x300: 12.0 us, 28.7 without).
-  const long segs = (long)Bl * NKV * p->RT;
+  long segs = (long)Bl * NKV * p->RT;
   p->whole = 0;
   if (most_u <= 48 || (most_u <= 128 && segs >= 64)) {
+    // Three column tiles a warp decode a unit once for 24 rows instead of 16, but halve the CTAs: worth it where
+    // those still fill the GPU and no tile stays empty.  us in a graph, two tiles against three: 24 rows of 64,
+    // 16x1000 (32 segments) 9.8 and 12.1, 64x1500 (128) 17.7 and 14.7; 24 rows of 128, 64x1500 26.9 and 22.4;
+    // 49 rows of 128, 64x1500 49.2 and 84.0.  fp32 q of 128 has no registers for it.
+    if (tiles % 3 == 0 && (p->mode == Q16 || HD == 64) && (long)Bl * NKV * (tiles / 3) * 4 >= 3l * num_sms()) {
+      p->NT = 3;
+      p->RT = (int)(tiles / 3);
+      segs = (long)Bl * NKV * p->RT;
+    }
+    const int cap = HD == 128 && p->NT > 1 ? 8 : (p->NT > 1 || (HD == 128 && (p->mode == Q32 || p->mode == COLS32)) ? 12 : 16);
     long w = segs < 1 ? 1 : (long)num_sms() * cap / segs;  // cap warps fill an SM
     w = w < 2 ? 2 : (w < cap ? w : cap);
     p->whole = (int)(most_u < 1 ? 1 : (most_u < w ? most_u : w));
+    p->warps = 0;
+    p->pre_bytes = p->bytes = 0;
+    RNGD_REQUIRE(segs < (1l << 31), "kv4_attn: %ld segments", segs);
+    return RNGD_OK;
   }
   const long units = (long)Bl * NKV * p->RT * most_u;
   RNGD_REQUIRE(units < (1l << 31) && (long)Bl * NKV * p->RT < (1l << 31), "kv4_attn: %ld units of work", units);
@@ -970,7 +986,7 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
   const long most = (long)num_sms() * per;
   p->warps = (int)(units < 1 ? 1 : (units < most ? units : most));
   p->pre_bytes = ((size_t)(Bl + 1) * 4 + 15) / 16 * 16;
-  p->bytes = p->whole ? 0 : p->pre_bytes + (size_t)p->warps * 2 * p->rows * (HD + 4) * 4;
+  p->bytes = p->pre_bytes + (size_t)p->warps * 2 * p->rows * (HD + 4) * 4;
   return RNGD_OK;
 }
 

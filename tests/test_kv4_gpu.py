@@ -192,6 +192,19 @@ def test_attention_of_several_tokens(HD, T):
     _check(q, pool, table, lens, "fp32", window=T // 2 + 1, sinks=2)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("HD", [64, 128])
+@pytest.mark.parametrize("T", [5, 6, 12])
+def test_attention_of_many_streams_and_rows(dt, HD, T):
+    """20, 24 and 48 query rows of a kv head, in enough streams to fill the GPU."""
+    lens = [0, 1, T - 1, T, 63, 64, 65, 128] + [(37 * i) % 150 for i in range(32)]
+    pool, table = _cache(len(lens), 3, 4, HD, lens, 31)
+    q = torch.randn(len(lens), T, 16, HD, generator=torch.Generator().manual_seed(HD + T)).to(DT[dt]).cuda()
+    got = _check(q, pool, table, lens, dt)
+    assert np.all(got[0] == 0)
+    _check(q, pool, table, lens, dt, window=33, sinks=3)
+
+
 def test_attention_without_pages():
     """-1, ids outside the pool and a table too narrow for the length: those positions are not seen."""
     lens = [200, 200, 130, 64, 1000]
