@@ -17,10 +17,11 @@
 // the parts' sums into log-sum-exps and selects among the rows' candidates in the same way, by (score,
 // place).
 //
-// Bytes would allow 20 us for 64 groups of 8 beams by 128256 bf16 logits; the two kernels take 48 to 49 (in a
-// graph, logits from memory, 2.7 TB/s).  Instruction issue (0.65 a cycle and scheduler) and the barriers where
-// a row ends bound the row kernel; the group kernel's 8 us are latency.  1 x 5 x 32003 fp32: 7.7 us, two
-// launches' latency; 16 x 32 x 128256 fp32: 81 us (3.3 TB/s).
+// Bytes would allow 20 us for 64 groups of 8 beams by 128256 bf16 logits; the two kernels take 47 (in a
+// graph, logits from memory, 2.8 TB/s; 49 with the exponentials' sums one by one instead of in pairs).
+// Instruction issue (0.65 a cycle and scheduler) and the barriers where a row ends bound the row kernel; the
+// group kernel's 8 us are latency.  1 x 5 x 32003 fp32: 7.7 us, two launches' latency; 16 x 32 x 128256
+// fp32: 81 us (3.3 TB/s).
 // Four threads rank each set's key: with one, 50.1, 8.1 and 81.5 us.
 #include "kv4.cuh"
 
@@ -303,6 +304,11 @@ __global__ void __launch_bounds__(kRowThreads, 3) beam_row_kernel(BeamArgs a) {
   };
   for (int f = 0; f < runs; f++) {
     fetch(f + ST - 1);
+    if (now.V == 0) {  // a beam that is done: nothing to read, and nothing of it is asked for
+      stage = stage + 1 == ST ? 0 : stage + 1;
+      step(now);
+      continue;
+    }
     asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
     uint4 u[NV];
     {
@@ -385,15 +391,25 @@ __global__ void __launch_bounds__(kRowThreads, 3) beam_row_kernel(BeamArgs a) {
       }
       top = best;
     }
-    float zz[4] = {};
+    f32x2 zz[2] = {};
+    const f32x2 off = pair(-ref, -ref), log2e = pair(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
     for (int k = 0; k < NV; k++) {
       float x[VL];
       unpack_vec<DT>(u[k], x);
 #pragma unroll
-      for (int i = 0; i < VL; i++) zz[i & 3] += exp2_fast((x[i] - ref) * 1.4426950408889634f);
+      for (int i = 0; i < VL; i += 2) {
+        float y0, y1;
+        unpair(mul_pair(add_pair(pair(x[i], x[i + 1]), off), log2e), y0, y1);
+        zz[i >> 1 & 1] = add_pair(zz[i >> 1 & 1], pair(exp2_fast(y0), exp2_fast(y1)));
+      }
     }
-    z += (zz[0] + zz[1]) + (zz[2] + zz[3]);
+    {
+      float z0, z1, z2, z3;
+      unpair(zz[0], z0, z1);
+      unpair(zz[1], z2, z3);
+      z += (z0 + z1) + (z2 + z3);
+    }
     // noted are the vectors that reach the bound; of -inf (and NaN) only the lowest places can be wanted,
     // after fewer than W others: they lie in the first vectors
     uint32_t word = 0;
