@@ -63,9 +63,9 @@ __device__ __forceinline__ void cluster_sync() {
 
 // One cluster: its CTAs share the tables (counts go up and down by whole-number atomics), the first one
 // then decides row by row, a thread to each.  Latency is what it takes: two rounds of dependent loads over
-// the tables and a walk through the free pages.  With the copies it takes 11.2 us in a graph for 16 rows (14 MB
-// moved, 2.2 us of it by the bytes) and 17.5 us for 256 rows.  Of 16 us for 256 rows, profiled cold, most is spent at
-// barriers and waiting for the atomics to be seen.
+// the tables and a walk through the free pages.  With the copies it takes 10.9 us in a graph for 16 rows (14 MB
+// moved, 2.2 us of it by the bytes) and 16.8 us for 256 rows, most of it at barriers.  The barriers order what the
+// CTAs write for one another; fences before them took 0.7 and 0.9 us more.
 __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads) kv4_fork_kernel(ForkArgs a) {
   __shared__ int s_warp[32];
   __shared__ __align__(16) int s_tail[kMetaThreads];
@@ -101,7 +101,6 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads
       }
     }
   }
-  __threadfence();
   cluster_sync();
   if (blockIdx.x != 0) return;
   const int r = tid;
@@ -153,7 +152,6 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads
       }
     have += got;
   }
-  __threadfence();
   __syncthreads();
   have = min(have, need);
   Move mv = {0, 0, 0};
@@ -191,20 +189,18 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads
 
 struct CompactArgs {
   const int32_t* ref;
-  const int32_t* table;
   int32_t* new_ref;
-  int32_t* new_table;
   int32_t* live_out;
   int* n_moves;
   Move* moves;    // [P]
   int32_t* map;   // [P]
   int P;
-  int cells;
 };
 
 // One CTA: counts the live pages (n), pairs the k-th live page from n on with the k-th free place below n,
-// and rewrites counts and tables.  A thread has a run of pages of its own, so that one prefix sum counts
-// them all.  Latency again: 11.5 us for 2048 pages and 64 tables, profiled cold.
+// and rewrites the counts; the tables are rewritten by the copying kernel's many threads.  A thread has a run of pages of its own, so that one prefix sum counts
+// them all.  Latency again: with
+// the copies 6.2 us in a graph for 12 pages moved of 300 (7.7 with fences, and the tables rewritten here).
 __global__ void __launch_bounds__(kMetaThreads) kv4_compact_kernel(CompactArgs a) {
   __shared__ int s_warp[32];
   const int tid = threadIdx.x, run = (a.P + kMetaThreads - 1) / kMetaThreads;
@@ -228,7 +224,6 @@ __global__ void __launch_bounds__(kMetaThreads) kv4_compact_kernel(CompactArgs a
     a.map[p] = p;
     a.new_ref[p] = rf;
   }
-  __threadfence();
   __syncthreads();
   for (int k = tid; k < srcs; k += kMetaThreads) {
     const int s = __ldcg(&a.moves[k].src), d = __ldcg(&a.moves[k].dst);
@@ -241,26 +236,28 @@ __global__ void __launch_bounds__(kMetaThreads) kv4_compact_kernel(CompactArgs a
     *a.n_moves = srcs;
     *a.live_out = n;
   }
-  __threadfence();
-  __syncthreads();
-  grid_dep_launch();
-#pragma unroll 4
-  for (int i = tid; i < a.cells; i += kMetaThreads) {
-    const int p = a.table[i];
-    a.new_table[i] = p >= 0 && p < a.P ? __ldcg(a.map + p) : -1;
-  }
 }
 
 // Copies pages: a warp takes 2560 bytes of a (move, layer, head) at a time, five loads in flight a lane.
 // 600 pages of 4 layers, 8 heads of 128 (393 MB read and written): 60 us, 6.5 TB/s, the copy bandwidth; with the
-// kernel above 74 us in a graph.
+// kernel above 71 us in a graph.
 constexpr int kCopyVecs = 160;
+struct Tables {  // to rewrite beside the copies: page p becomes map[p]
+  const int32_t* table;
+  int32_t* new_table;
+  const int32_t* map;
+  int cells, P;
+};
 __global__ void __launch_bounds__(256) kv4_copy_kernel(uint8_t* pool, size_t layer_bytes, int L, int NKV, int blk_bytes,
-                                                       const Move* moves, const int* n_moves) {
+                                                       const Move* moves, const int* n_moves, Tables t) {
   const int lane = threadIdx.x & 31;
   const long warp = ((long)blockIdx.x * 256 + threadIdx.x) >> 5, warps = (long)gridDim.x * 8;
   const int blk_vecs = blk_bytes / 16, subs = 4 * blk_vecs / kCopyVecs;
   grid_dep_wait();
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < t.cells; i += gridDim.x * 256) {
+    const int p = t.table[i];
+    t.new_table[i] = p >= 0 && p < t.P ? t.map[p] : -1;
+  }
   const long units = (long)*n_moves * L * NKV * subs;
   for (long u = warp; u < units; u += warps) {
     uint32_t x = (uint32_t)(u % ((long)L * NKV * subs));
@@ -294,11 +291,11 @@ static int check_pages(const char* what, const void* pool, size_t layer_bytes, i
 
 // The copies of up to `most` moves; how many there are is known on the device alone.
 static int launch_copy(uint8_t* pool, size_t layer_bytes, int L, int NKV, int HD, const Move* moves, const int* n_moves,
-                       int most, cudaStream_t s) {
+                       int most, const Tables& t, cudaStream_t s) {
   const long units = (long)most * L * NKV * (4 * kv4_block_bytes(HD) / 16 / kCopyVecs), blocks = (units + 7) / 8;
   const long cap = (long)num_sms() * 8;
   return launch_pdl(kv4_copy_kernel, dim3((unsigned)(blocks < cap ? blocks : cap)), dim3(256), 0, s, "kv4_copy_kernel", pool,
-                    layer_bytes, L, NKV, kv4_block_bytes(HD), moves, n_moves);
+                    layer_bytes, L, NKV, kv4_block_bytes(HD), moves, n_moves, t);
 }
 
 }  // namespace rngd
@@ -331,7 +328,7 @@ extern "C" int rngd_kv4_fork(void* pool, size_t layer_bytes, int L, int P, int N
   cudaStream_t s = (cudaStream_t)stream;
   RNGD_TRY(launch_pdl(kv4_fork_kernel, dim3(kForkCtas), dim3(kMetaThreads), 0, s, "kv4_fork_kernel", a));
   if (R == 0) return RNGD_OK;
-  return launch_copy((uint8_t*)pool, layer_bytes, L, NKV, HD, moves, n_moves, R, s);
+  return launch_copy((uint8_t*)pool, layer_bytes, L, NKV, HD, moves, n_moves, R, Tables{}, s);
 }
 
 extern "C" int rngd_kv4_compact_workspace(int P, size_t* bytes) {
@@ -354,8 +351,8 @@ extern "C" int rngd_kv4_compact(void* pool, size_t layer_bytes, int L, int P, in
   int* n_moves = (int*)workspace;
   Move* moves = (Move*)((uint8_t*)workspace + 16);
   int32_t* map = (int32_t*)(moves + P);
-  CompactArgs a = {ref, table, new_ref, new_table, live, n_moves, moves, map, P, (int)cells};
+  CompactArgs a = {ref, new_ref, live, n_moves, moves, map, P};
   cudaStream_t s = (cudaStream_t)stream;
   RNGD_TRY(launch_pdl(kv4_compact_kernel, dim3(1), dim3(kMetaThreads), 0, s, "kv4_compact_kernel", a));
-  return launch_copy((uint8_t*)pool, layer_bytes, L, NKV, HD, moves, n_moves, P, s);
+  return launch_copy((uint8_t*)pool, layer_bytes, L, NKV, HD, moves, n_moves, P, Tables{table, new_table, map, (int)cells, P}, s);
 }
