@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) beam_row_kernel(BeamArgs a) {
         noted = 0;
         __syncthreads();
       } else {
+        if (direct) __syncthreads();  // settle() clears s_k, by which the others still decide
         settle();
       }
       const int slot = (int)blockIdx.x - owner_of((long)now.r * a.n, total, a.grid);

@@ -181,3 +181,26 @@ def test_select_refusals():
         with pytest.raises(ValueError):
             f()
     assert beam.select(x[:0], s[:0], d[:0], 2)[0].shape == (0, 2)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("R", [40, 80, 160])
+@pytest.mark.parametrize("W", [1, 2, 4])
+def test_few_sets_hold_many_of_the_best(dt, R, W):
+    """Logits that repeat with a chunk's stride: the W sets that reach the bound hold more logits than are listed at
+    once.  Rows of one chunk (or parts of one) with 2, 4 and 8 vectors a thread."""
+    vl = 8 if dt == "bf16" else 4
+    step, run = 256 * vl, 4 * vl                            # logits of a vector per thread, and of a set
+    V = 8 * step - 3 * vl
+    logits = torch.zeros(R, V)
+    at = torch.arange(V) % step // run                      # the set that a place falls to
+    for i in range(W):
+        logits[:, at == (37 * i + 5) % 64] = 3.0 + i        # a value of its own for each of W sets
+    logits += torch.arange(R).view(R, 1) % 3                # the same order, other values
+    logits = logits.to(DT[dt])
+    scores = -0.01 * torch.arange(R).float()
+    got, _, _ = _check(logits, scores, torch.zeros(R, dtype=torch.bool), W, 1)
+    if W == 1:
+        assert np.array_equal(got[2][:, 0], logits.float().numpy().argmax(1))  # the first of the equal ones
+    noise = logits + (torch.rand(R, V, generator=torch.Generator().manual_seed(R)) * 0.25).to(DT[dt])
+    _check(noise, scores, torch.arange(R) % 7 == 3, W, 1)
