@@ -216,4 +216,4 @@ class BeamDecodeEngine:
             ref, table, live = kv4.compact(self.pool, self.ref, self.table)
             self.ref.copy_(ref)
             self.table.copy_(table)
-        return int(live.item())
+            return int(live.item())  # on the engine's stream, after what is queued there

@@ -177,3 +177,18 @@ def test_eos_ends_beams_and_refusals(model):
     small.step(2)
     with pytest.raises(RuntimeError):
         small.result(0)                     # two pages do not hold three beams
+
+
+def test_compact_waits_for_the_steps_before_it(model):
+    """Called with steps still queued and nothing synchronised, the count is that of the state after them."""
+    cfg, pre, m = model
+    prompt = [(5 * j + 1) % SMALL.V for j in range(70)]
+    eng = _engine(model, beams=4, groups=2, pages=40, width=4)
+    for n in (40, 20, 1):
+        for g in (0, 1):
+            _begin(eng, pre, g, prompt)
+        eng.step(n)
+        live = eng.compact()
+        assert live == int((eng.ref > 0).sum()) == int(eng.table.max()) + 1 and live >= 5
+        eng.end(1)
+        assert eng.compact() == int((eng.ref > 0).sum()) < live
