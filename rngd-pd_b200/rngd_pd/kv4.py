@@ -164,10 +164,11 @@ def attention(q, pool, table, lens, window=0, sinks=0, scale=None, out=None):
     op, os = _rows("out", out, 4)
     need = _lib.workspace_bytes("rngd_kv4_attn_workspace", _DT[dt], B, T, NH, NKV, HD, width, window,
                                  sinks)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr() if need else None
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # held until the launches are queued
     _check(_attn(qp, qs, op, os, _DT[dt], pool.data_ptr(), P, NKV, HD, _i32("table", table, (B, width), dev), width,
                  _i32("lens", lens, (B,), dev), B, T, NH, window, sinks,
-                 HD ** -0.5 if scale is None else scale, ws, need, _lib.raw_stream(dev.index)))
+                 HD ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need,
+                 _lib.raw_stream(dev.index)))
     return out
 
 

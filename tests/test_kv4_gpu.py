@@ -344,6 +344,26 @@ def test_attention_on_another_stream_and_in_a_graph():
     assert torch.equal(out, kv4.attention(q, pool, table, lens))
 
 
+def test_attention_keeps_its_workspace_through_the_call(monkeypatch):
+    """What another thread allocates on the stream while the call runs is not the call's workspace."""
+    from rngd_pd import kv4
+    q = torch.zeros(1, 1, 8, 128, dtype=torch.bfloat16, device="cuda")
+    table = torch.full((1, 65), -1, dtype=torch.int32, device="cuda")
+    lens, pool = torch.zeros(1, dtype=torch.int32, device="cuda"), kv4.alloc_pool(1, 2, 2, 128)[0]
+    seen = []
+
+    def entry(*a):                                          # in place of the C entry: nothing is launched
+        ws, need = a[18], a[19]
+        others = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in range(3)]
+        seen.append((ws, need, [t.data_ptr() for t in others]))
+        return 0
+
+    monkeypatch.setattr(kv4, "_attn", entry)
+    kv4.attention(q, pool, table, lens)
+    (ws, need, others), = seen
+    assert need > 0 and all(p + need <= ws or ws + need <= p for p in others)
+
+
 # -------------------------------------------------------------------------------------------- pages
 def _run_fork(ref0, table, lens, parents, room, L=2, NKV=2, HD=64):
     from rngd_pd import kv4
