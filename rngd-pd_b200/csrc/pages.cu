@@ -28,6 +28,9 @@ struct ForkArgs {
   int P, R, ld, room;
 };
 
+// Pages that n positions take, for any n (a sum with kPage - 1 would pass 32 bits).
+__device__ __forceinline__ int pages_of(int n) { return n > 0 ? (n - 1) / kPage + 1 : 0; }
+
 constexpr int kMetaThreads = 1024;
 constexpr int kForkCtas = 8;  // one cluster
 
@@ -84,7 +87,7 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads
         const int r = i / a.ld, col = i - r * a.ld;
         old[k] = a.table[i];
         const int par = a.parents != nullptr ? a.parents[r] : r;
-        if (par >= 0 && par < a.R && col < (a.lens[par] + kPage - 1) / kPage) now[k] = a.table[par * a.ld + col];
+        if (par >= 0 && par < a.R && col < pages_of(a.lens[par])) now[k] = a.table[par * a.ld + col];
       }
     }
 #pragma unroll
@@ -110,11 +113,11 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads
     const bool on = par >= 0 && par < a.R;
     len = on ? max(a.lens[par], 0) : 0;
     a.new_lens[r] = len;
-    n = min((len + kPage - 1) / kPage, a.ld);
+    n = min(pages_of(len), a.ld);
     const int want = on ? (int)(((long)len + a.room + kPage - 1) / kPage) : 0;
     last = max(n, min(want, a.ld));
     over = max(want - last, 0);
-    if (on && len % kPage != 0 && n > 0 && (len + kPage - 1) / kPage <= a.ld) tail = __ldcg(a.new_table + r * a.ld + n - 1);
+    if (on && len % kPage != 0 && n > 0 && pages_of(len) <= a.ld) tail = __ldcg(a.new_table + r * a.ld + n - 1);
   }
   s_tail[tid] = tail;
   __syncthreads();

@@ -427,6 +427,23 @@ def test_fork_of_random_states(R, width, seed):
     _run_fork(ref0, table, lens, parents, int(g.integers(0, 3)), L=1, NKV=1)
 
 
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 63, 2 ** 31 - 64])
+def test_fork_of_lengths_near_the_largest_number(n):
+    """A length far beyond the table keeps the table's pages; what is missing beyond them is counted."""
+    from rngd_pd import kv4
+    pool = kv4.alloc_pool(1, 8, 1, 64)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    ref0, table, lens = i32([1, 1, 1, 1, 0, 0, 0, 0]), i32([[2, 0], [1, 3]]), i32([n, 70])
+    for room in (0, 100):
+        new_ref, new_table, new_lens, short = kv4.fork(pool, ref0, table, lens, i32([0, 1]), room=room)
+        assert new_table.tolist() == [[2, 0], [1, 3]] and new_lens.tolist() == [n, 70]
+        assert new_ref.tolist() == ref0.tolist()
+        assert short.item() == -(-(n + room) // 64) - 2 + (1 if room else 0)
+    new_ref, new_table, _, short = kv4.fork(pool, ref0, table, lens, i32([0, 0]))
+    assert new_table.tolist() == [[2, 0], [2, 0]] and new_ref.tolist() == [2, 0, 2, 0, 0, 0, 0, 0]
+    assert short.item() == 2 * (-(-n // 64) - 2)
+
+
 @pytest.mark.parametrize("P,live,seed", [(1, 0, 0), (1, 1, 1), (5, 5, 2), (100, 60, 3), (3000, 10, 4), (5000, 2600, 5)])
 def test_compact(P, live, seed):
     from rngd_pd import kv4
