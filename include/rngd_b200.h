@@ -330,7 +330,7 @@ int rngd_kv4_load(const void* pool, size_t layer_bytes, int P, int NKV, int HD, 
  * lens[b]: positions held, the T tokens' own among them: token t is at i = lens[b] - T + t and sees
  * positions j <= i that lie in the window (j > i - window; 0: no window) or are sinks (j < sinks).
  * A token that sees nothing gives zeros.  workspace: rngd_kv4_attn_workspace() bytes, 16-byte aligned,
- * any content, not shared by calls that may overlap. */
+ * any content, not shared by calls that may overlap.  ld_table < 2^25: positions are 32-bit numbers. */
 int rngd_kv4_attn(const void* q, const int64_t* q_strides, void* out, const int64_t* out_strides, int dtype,
                   const void* pool, int P, int NKV, int HD, const int32_t* table, int ld_table, const int32_t* lens,
                   int B, int T, int NH, int window, int sinks, float scale, void* workspace, size_t workspace_bytes,

@@ -940,6 +940,8 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
   RNGD_REQUIRE(B >= 0 && T >= 0 && NKV >= 1 && NH >= 1 && NH % NKV == 0 && ld_table >= 0,
                "kv4_attn: B=%d T=%d NH=%d must be a multiple of NKV=%d, table width %d", B, T, NH, NKV, ld_table);
   RNGD_REQUIRE(window >= 0 && sinks >= 0, "kv4_attn: window=%d sinks=%d", window, sinks);
+  // positions are 32-bit numbers, up to the end of the table and of the unit that holds it
+  RNGD_REQUIRE(ld_table <= 0x7FFFFFFF / kPage, "kv4_attn: table of %d pages, at most %d", ld_table, 0x7FFFFFFF / kPage);
   const int Bl = B < kAttnStreams ? B : kAttnStreams;  // streams of one launch
   const long R = (long)T * (NH / NKV);
   p->mode = R <= 4 ? (dtype == DT_F32 ? COLS32 : COLS) : (dtype == DT_F32 ? Q32 : Q16);

@@ -70,3 +70,15 @@ def test_plain_forms_on_small_cases():
     best, parent, token, done, _ = ref.select(np.log(np.array([[.5, .3, .2], [.1, .1, .8]])), np.array([0.0, -1.0]),
                                               np.array([False, False]), 2, 2)
     assert parent.tolist() == [[0, 0]] and token.tolist() == [[0, 1]] and not done.any()
+
+
+def test_tables_wider_than_positions_are_refused():
+    """Positions are 32-bit numbers: 2^25 pages of 64 are one too many."""
+    lib, p, i3 = _lib.lib, ctypes.c_void_p(4096), (ctypes.c_int64 * 3)(1, 1, 1)
+    need = ctypes.c_size_t(0)
+    for ld in (2 ** 25, 2 ** 31 - 1):
+        for window in (0, 100):
+            assert lib.rngd_kv4_attn_workspace(0, 1, 1, 4, 2, 64, ld, window, 0, ctypes.byref(need)) == _lib.RNGD_ERR_ARG
+            assert f"table of {ld} pages" in _lib.last_error()
+        assert lib.rngd_kv4_attn(p, i3, p, i3, 0, p, 1, 2, 64, p, ld, p, 1, 1, 4, 0, 0, 1.0, p, 1 << 40, None) == _lib.RNGD_ERR_ARG
+        assert f"table of {ld} pages" in _lib.last_error()
