@@ -318,12 +318,13 @@ extern "C" int rngd_kv4_fork(void* pool, size_t layer_bytes, int L, int P, int N
   RNGD_TRY(check_pages("kv4_fork", pool, layer_bytes, L, P, NKV, HD, R, ld_table));
   RNGD_REQUIRE(R <= kMetaThreads, "kv4_fork: %d rows, at most %d", R, kMetaThreads);
   RNGD_REQUIRE(room >= 0 && room <= (1 << 30), "kv4_fork: room=%d", room);
-  RNGD_REQUIRE(ref && new_ref && short_out && ref != new_ref && (R == 0 || (lens && new_lens && workspace)) &&
+  RNGD_REQUIRE(ref && new_ref && short_out && workspace && ref != new_ref && (R == 0 || (lens && new_lens)) &&
                    (R == 0 || ld_table == 0 || (table && new_table)) && (table != new_table || table == nullptr),
                "kv4_fork: null pointer, or new state in place of the old");
   size_t need;
   RNGD_TRY(rngd_kv4_fork_workspace(R, ld_table, &need));
-  RNGD_REQUIRE(workspace_bytes >= need, "kv4_fork: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  RNGD_REQUIRE(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need,
+               "kv4_fork: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
   int* n_moves = (int*)workspace;
   Move* moves = (Move*)((uint8_t*)workspace + 16);
   ForkArgs a = {ref, table, lens, parents, new_ref, new_table, new_lens, short_out, n_moves, moves, (int*)(moves + R),
@@ -350,7 +351,8 @@ extern "C" int rngd_kv4_compact(void* pool, size_t layer_bytes, int L, int P, in
                "kv4_compact: null pointer, or new state in place of the old");
   size_t need;
   RNGD_TRY(rngd_kv4_compact_workspace(P, &need));
-  RNGD_REQUIRE(workspace_bytes >= need, "kv4_compact: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  RNGD_REQUIRE(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need,
+               "kv4_compact: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
   int* n_moves = (int*)workspace;
   Move* moves = (Move*)((uint8_t*)workspace + 16);
   int32_t* map = (int32_t*)(moves + P);

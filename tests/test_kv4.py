@@ -82,3 +82,16 @@ def test_tables_wider_than_positions_are_refused():
             assert f"table of {ld} pages" in _lib.last_error()
         assert lib.rngd_kv4_attn(p, i3, p, i3, 0, p, 1, 2, 64, p, ld, p, 1, 1, 4, 0, 0, 1.0, p, 1 << 40, None) == _lib.RNGD_ERR_ARG
         assert f"table of {ld} pages" in _lib.last_error()
+
+
+def test_missing_workspaces_and_those_off_their_alignment_are_refused():
+    lib, p, odd, r = _lib.lib, ctypes.c_void_p(4096), ctypes.c_void_p(4097), ctypes.c_void_p(8192)
+    for name, st in (("kv4_fork", lib.rngd_kv4_fork(p, 0, 1, 1, 1, 64, p, p, 1, p, 1, None, 0, r, r, r, r, odd, 1 << 20, None)),
+                     ("kv4_compact", lib.rngd_kv4_compact(p, 0, 1, 1, 1, 64, p, p, 1, 1, r, r, r, odd, 1 << 20, None))):
+        assert st == _lib.RNGD_ERR_ARG, name
+    # none at all, with no rows to fork: the count of copies is written all the same
+    assert lib.rngd_kv4_fork(p, 0, 1, 1, 1, 64, p, None, 0, None, 0, None, 0, r, None, None, r, None, 16, None) == _lib.RNGD_ERR_ARG
+    for f in (lambda: lib.rngd_kv4_fork(p, 0, 1, 1, 1, 64, p, p, 1, p, 1, None, 0, r, r, r, r, odd, 1 << 20, None),
+              lambda: lib.rngd_kv4_compact(p, 0, 1, 1, 1, 64, p, p, 1, 1, r, r, r, odd, 1 << 20, None)):
+        f()
+        assert "aligned" in _lib.last_error()
