@@ -359,7 +359,7 @@ int rngd_decode_kv4_workspace(const rngd_model_t* m, int B, int ld_table, int wi
  * these rows hold it, the others get a copy (all L layers, the filled blocks).  Then each row gets pages
  * for `room` more positions.  Free pages are given lowest first, in the order of rows.  The new state
  * goes to new_ref / new_table / new_lens (other buffers); the pool changes in pages that were free or
- * were let go.  *short_out: pages that could not be given (-1 in the table).  R <= 1024. */
+ * were let go.  *short_out: pages that could not be given (-1 in the table), at most 2^31 - 1.  R <= 1024. */
 int rngd_kv4_fork(void* pool, size_t layer_bytes, int L, int P, int NKV, int HD, const int32_t* ref,
                   const int32_t* table, int ld_table, const int32_t* lens, int R, const int32_t* parents, int room,
                   int32_t* new_ref, int32_t* new_table, int32_t* new_lens, int32_t* short_out, void* workspace,

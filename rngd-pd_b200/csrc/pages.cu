@@ -72,6 +72,7 @@ __device__ __forceinline__ void cluster_sync() {
 __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads) kv4_fork_kernel(ForkArgs a) {
   __shared__ int s_warp[32];
   __shared__ __align__(16) int s_tail[kMetaThreads];
+  __shared__ unsigned long long s_over;  // pages that could not be given
   const int tid = threadIdx.x, all = kForkCtas * kMetaThreads, me = blockIdx.x * kMetaThreads + tid;
   grid_dep_wait();
   for (int p = me; p < a.P; p += all) a.new_ref[p] = a.ref[p];
@@ -120,6 +121,7 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads
     if (on && len % kPage != 0 && n > 0 && pages_of(len) <= a.ld) tail = __ldcg(a.new_table + r * a.ld + n - 1);
   }
   s_tail[tid] = tail;
+  if (tid == 0) s_over = 0;
   __syncthreads();
   bool copy = false;
   if (tail >= 0) {
@@ -183,10 +185,11 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kMetaThreads
   }
   const int m = block_scan(mv.blocks > 0, s_warp, &got);
   if (mv.blocks > 0) a.moves[m] = mv;
-  block_scan(over, s_warp, &over);
+  if (over > 0) atomicAdd(&s_over, (unsigned long long)over);  // up to 2^36 of 1024 rows
+  __syncthreads();
   if (tid == 0) {
     *a.n_moves = got;
-    *a.short_out = over;
+    *a.short_out = (int)min(s_over, 0x7FFFFFFFull);
   }
 }
 

@@ -178,7 +178,8 @@ def fork(pool, ref, table, lens, parents=None, room=0):
 
     Full pages are shared.  A partly filled last page belongs to one row alone afterwards: the lowest row keeps it
     if only such rows hold it, the others get copies of its filled blocks, in all layers.  Free pages are given
-    lowest first, in the order of rows; short (int32 [1]) counts those that could not be given (-1 in the table).
+    lowest first, in the order of rows; short (int32 [1]) counts those that could not be given (-1 in the table), up
+    to 2^31 - 1.
     The old state is left as it is; the pool changes only in pages that were free or were let go, so the old
     state's own pages stay valid until a later call hands them out."""
     L, P, NKV, HD, layer = _pool_dims(pool, True)

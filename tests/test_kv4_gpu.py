@@ -444,6 +444,17 @@ def test_fork_of_lengths_near_the_largest_number(n):
     assert short.item() == 2 * (-(-n // 64) - 2)
 
 
+@pytest.mark.parametrize("R,room", [(1024, 2 ** 30), (130, 2 ** 30), (3, 2 ** 30), (1024, 2 ** 26)])
+def test_fork_counts_more_missing_pages_than_a_number_holds(R, room):
+    """`short` stays at 2^31 - 1 where more pages are missing."""
+    from rngd_pd import kv4
+    pool = kv4.alloc_pool(1, 2, 1, 64)
+    ref0, table, lens = kv4.empty_state(R, 1, 2)
+    new_ref, new_table, _, short = kv4.fork(pool, ref0, table, lens, room=room)
+    assert short.item() == min(R * (room // 64) - 2, 2 ** 31 - 1)
+    assert new_table[:, 0].tolist() == [0, 1] + [-1] * (R - 2) and new_ref.tolist() == [1, 1]
+
+
 @pytest.mark.parametrize("P,live,seed", [(1, 0, 0), (1, 1, 1), (5, 5, 2), (100, 60, 3), (3000, 10, 4), (5000, 2600, 5)])
 def test_compact(P, live, seed):
     from rngd_pd import kv4
