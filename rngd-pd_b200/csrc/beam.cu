@@ -518,6 +518,10 @@ __global__ void __launch_bounds__(kGroupThreads) beam_group_kernel(BeamArgs a, i
       const int v = !carry ? k : k == 0 ? a.eos : (k - 1 < a.eos ? k - 1 : k);
       return order_key(carry && k == 0 ? cum : -INFINITY, (uint32_t)w * (uint32_t)a.V + (uint32_t)v);
     }
+    if (!(cum > -INFINITY) || !(fabsf(s_lse[w]) < INFINITY)) {  // a row that is lost: all -inf, whatever its logits
+      const int k = i - w * per_row;
+      return k < a.W ? order_key(-INFINITY, (uint32_t)w * (uint32_t)a.V + (uint32_t)k) : 0;
+    }
     if (i - w * per_row >= s_parts[w] * a.W) return 0;
     const u64 k = cand[i];
     if (k == 0) return 0;

@@ -204,3 +204,25 @@ def test_few_sets_hold_many_of_the_best(dt, R, W):
         assert np.array_equal(got[2][:, 0], logits.float().numpy().argmax(1))  # the first of the equal ones
     noise = logits + (torch.rand(R, V, generator=torch.Generator().manual_seed(R)) * 0.25).to(DT[dt])
     _check(noise, scores, torch.arange(R) % 7 == 3, W, 1)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("V", [50, 9000])
+def test_rows_that_are_lost_offer_their_lowest_tokens(dt, V):
+    """A row whose scores are all -inf (by a NaN or +inf logit, by its own score) ranks by place, whatever its logits."""
+    from rngd_pd import beam
+    W = 4
+    logits = torch.randn(4 * W, V, generator=torch.Generator().manual_seed(9)).to(DT[dt])
+    scores = torch.zeros(4 * W)
+    logits[:W, V // 2] = float("nan")                       # group 0: lost by NaN
+    logits[W:2 * W, V // 2] = float("inf")                  # 1: by +inf
+    scores[2 * W:3 * W] = -np.inf                           # 2: by their own scores
+    scores[3 * W:] = torch.tensor([-np.inf, 0.0, np.nan, -np.inf])
+    logits[3 * W + 1, 2:] = -np.inf                         # 3: two continuations, then the lowest places of row 0
+    done = torch.zeros(4 * W, dtype=torch.bool)
+    out = beam.select(logits.cuda(), scores.cuda(), done.cuda(), W)
+    assert torch.isinf(out[0][:3]).all() and out[2][:3].tolist() == [[0, 1, 2, 3]] * 3
+    assert out[1][:3].tolist() == [[0] * 4, [W] * 4, [2 * W] * 4]
+    assert torch.isinf(out[0][3]).tolist() == [False, False, True, True]
+    assert sorted(out[2][3, :2].tolist()) == [0, 1] and out[1][3, :2].tolist() == [3 * W + 1] * 2
+    assert out[2][3, 2:].tolist() == [0, 1] and out[1][3, 2:].tolist() == [3 * W] * 2
