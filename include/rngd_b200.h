@@ -375,9 +375,9 @@ int rngd_kv4_compact_workspace(int P, size_t* bytes);
 /* ------------------------------------------------------------ beam search
  * The reference decodes greedily (greedy_tokens, src/rngd_pd/engines/decode_batch.py:162-171).  Selection
  * of a search: rows are groups of W beams; of a group's W*V continuations the W with the largest
- * scores[r] + log_softmax(logits[r])[v], equal ones by the lowest r*V + v (within a row by the larger
- * logit first).  A beam that is done has one continuation, eos, at its own score.  NaN scores count as
- * -inf.  logits: [R] rows of V, ld elements apart.  Out, best first, [R/W][W]: scores, parents (rows),
+ * scores[r] + log_softmax(logits[r])[v], equal ones by the lowest r*V + v.  A row takes part with its W
+ * largest logits alone (equal ones: the lowest v), which shows only where logits that differ round to one
+ * score.  A beam that is done has one continuation, eos, at its own score.  NaN scores count as -inf.  logits: [R] rows of V, ld elements apart.  Out, best first, [R/W][W]: scores, parents (rows),
  * tokens, done (the parent's, or token == eos; eos < 0: none).  W <= 32, W <= V. */
 int rngd_beam_select(const void* logits, int dtype, int64_t ld, int R, int V, int W, const float* scores,
                      const uint8_t* done, int eos, float* out_scores, int32_t* parents, int32_t* tokens,

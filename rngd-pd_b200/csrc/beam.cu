@@ -4,18 +4,18 @@
 // The reference decodes greedily (greedy_tokens, src/rngd_pd/engines/decode_batch.py:162-171); this is
 // the same step for a search over several beams of one prompt.
 //
-// Within a row the order of scores is the order of logits, so one pass over the logits finds both what
-// the log-sum-exp needs and the row's W best.  The rows' chunks lie end to end and every CTA takes an
-// equal run of them through a ring in shared memory, every thread copying (asynchronously, ahead) and
-// reading its own vectors of 16 bytes, so that nothing makes the warps wait for one another.  In the first
-// chunk of a row (or of its part of one) the threads form 64 sets; the W-th largest of the sets' largest
-// logits is a bound that at least W logits reach, and few others do.  A bit per vector notes those that
-// hold a logit which reaches it.  At the row's end the noted vectors are read again and the W best of
-// their logits kept, once more by way of 64 sets and then by counting, for each that is left, those above
-// it.  Equal logits are told apart by their places, as keys (logit, place) in one 64-bit number, so
-// neither ties nor the order in which threads run can show.  A second kernel, one CTA per group, joins
-// the parts' sums into log-sum-exps and selects among the rows' candidates in the same way, by (score,
-// place).
+// Within a row the order of scores is the order of logits (but for logits that differ and round to one
+// score: of those the largest W take part), so one pass over the logits finds both what the log-sum-exp
+// needs and the row's W best.  The rows' chunks lie end to end and every CTA takes an equal run of them
+// through a ring in shared memory, every thread copying (asynchronously, ahead) and reading its own vectors
+// of 16 bytes, so that nothing makes the warps wait for one another.  In the first chunk of a row (or of
+// its part of one) the threads form 64 sets; the W-th largest of the sets' largest logits is a bound that
+// at least W logits reach, and few others do.  A bit per vector notes those that hold a logit which reaches
+// it.  At the row's end the noted vectors are read again and the W best of their logits kept, once more by
+// way of 64 sets and then by counting, for each that is left, those above it.  Equal logits are told apart
+// by their places, as keys (logit, place) in one 64-bit number, so neither ties nor the order in which
+// threads run can show.  A second kernel, one CTA per group, joins the parts' sums into log-sum-exps and
+// selects among the rows' candidates in the same way, by (score, place).
 //
 // Bytes would allow 20 us for 64 groups of 8 beams by 128256 bf16 logits; the two kernels take 47 (in a
 // graph, logits from memory, 2.8 TB/s; 49 with the exponentials' sums one by one instead of in pairs).

@@ -23,8 +23,9 @@ def select(logits, scores, done, beams, eos=-1):
 
     logits: [R, V] bfloat16, float16 or float32 (rows may lie apart), rows g * beams .. of group g;
     scores: float32 [R], the beams' own; done: bool [R].  A beam that is done goes on with `eos` alone, at its own
-    score (eos < 0: none ends, and a beam that is done is lost).  Equal scores: the lowest row, then the lowest
-    token (within a row the larger logit first).  NaN counts as -inf.
+    score (eos < 0: none ends, and a beam that is done is lost).  NaN counts as -inf.  Equal scores: the lowest row,
+    then the lowest token; but a row takes part with its `beams` largest logits alone (equal ones: the lowest
+    tokens), so where logits that differ round to one score, its smaller ones may stay behind.
     Returns, best first, [R / beams, beams]: scores float32, parents int32 (rows), tokens int32, done bool."""
     if logits.dim() != 2 or logits.dtype not in _DT or not logits.is_cuda:
         raise ValueError(f"logits must be a CUDA matrix of bfloat16, float16 or float32, got {tuple(logits.shape)} "

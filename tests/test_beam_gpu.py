@@ -226,3 +226,15 @@ def test_rows_that_are_lost_offer_their_lowest_tokens(dt, V):
     assert torch.isinf(out[0][3]).tolist() == [False, False, True, True]
     assert sorted(out[2][3, :2].tolist()) == [0, 1] and out[1][3, :2].tolist() == [3 * W + 1] * 2
     assert out[2][3, 2:].tolist() == [0, 1] and out[1][3, 2:].tolist() == [3 * W] * 2
+
+
+def test_logits_that_round_to_one_score():
+    """At -1000 scores lie 2^-14 apart: a row offers its largest logits, and of those equal scores go by the token."""
+    from rngd_pd import beam
+    logits = torch.zeros(2, 100)
+    logits[:, 50], logits[:, 20], logits[:, 80] = 1.000002, 1.0, 1.000004
+    args = lambda s: (torch.tensor(s, device="cuda"), torch.zeros(len(s), dtype=torch.bool, device="cuda"))
+    one = beam.select(logits[:1].cuda(), *args([-1000.0]), 1)
+    assert one[2].tolist() == [[80]]
+    two = beam.select(logits.cuda(), *args([-1000.0, -np.inf]), 2)
+    assert two[2].tolist() == [[50, 80]] and two[1].tolist() == [[0, 0]] and two[0][0, 0] == two[0][0, 1]
