@@ -41,6 +41,8 @@ class BeamDecodeEngine:
             self.done = torch.ones(B, dtype=torch.bool, device=d)
             self.toks = self._e._toks
             self.short = torch.zeros(1, **i32)                  # pages that could not be given, of all steps
+            self.missed = torch.zeros(groups, **i32)            # of each group's search: positions without a page
+            self._first = width * torch.arange(B, **i32)        # each row's first entry of the table
             self._rows = torch.zeros((2, MAXB, cfg.n_kv, cfg.head_dim), dtype=BF, device=d)
             need = ctypes.c_size_t(0)
             _lib.call("rngd_decode_kv4_workspace", self._e._m, B, width, window, sinks, ctypes.byref(need))
@@ -88,6 +90,7 @@ class BeamDecodeEngine:
             self.ref.copy_(ref)
             self.table[r0] = table[0]
             self.short.add_(short)
+            self.missed[group:group + 1].add_(short)
             k, v = (kv[:, i, :, :P].transpose(1, 2).unsqueeze(1) for i in (0, 1))
             kv4.store(self.pool, table, zero, k, v)
             self.lens[r0] = P
@@ -113,12 +116,17 @@ class BeamDecodeEngine:
         self.parents[rows] = -1
         self.scores[rows] = float("-inf")
         self.done[rows] = True
+        self.missed[r0 // self.W] = 0
 
     # ------------------------------------------------------------------- step
     def _step(self):
         """Fork as selected, one decode step, select: all queued on the current stream."""
         e, m, h = self._e, self._e._m, _lib.stream_handle()
         self._fork(self.parents, 1)
+        # a beam without a page for the position that comes now lost it in this fork: its group's search is spoilt
+        live = self.lens > 0
+        page = self.table.view(-1).index_select(0, self._first + self.lens // kv4.PAGE)
+        self.missed.add_(((page < 0) & live).view(self.G, self.W).sum(1, dtype=torch.int32))
         e._pos.copy_(self.lens)
         io = e._io(self._rows[0], self._rows[1])
         cache = _lib.Kv4(pool=self.pool.data_ptr(), layer_bytes=self.pool.stride(0), P=self.pool.shape[1],
@@ -127,7 +135,7 @@ class BeamDecodeEngine:
         _lib.call("rngd_decode_embed", m, io, h)
         _lib.call("rngd_decode_layers_kv4", m, io, cache, 0, self.cfg.n_layers, h)
         _lib.call("rngd_decode_lmhead", m, io, h)
-        self.lens.add_((self.lens > 0).to(torch.int32))
+        self.lens.add_(live)
         sc, pa, tk, dn = beam.select(e._logits, self.scores, self.done, self.W, self.eos)
         self.scores.copy_(sc.view(-1))
         # a beam without continuation lets go of its pages
@@ -147,7 +155,7 @@ class BeamDecodeEngine:
             for _ in range(n):
                 if self._graph is None and self._e.use_graph:
                     # one plain run on a copy of the state loads the kernels; then the step is captured
-                    names = ("ref", "table", "lens", "parents", "scores", "done", "toks", "short")
+                    names = ("ref", "table", "lens", "parents", "scores", "done", "toks", "short", "missed")
                     keep = [getattr(self, x).clone() for x in names]
                     self._step()
                     for x, t in zip(names, keep):
@@ -170,12 +178,13 @@ class BeamDecodeEngine:
     @_lib.on_device
     def result(self, group):
         """The group's beams that have a continuation, best first: [(score, tokens)], tokens up to and with the
-        first eos."""
+        first eos.  Raises where the pool ran out of pages during the group's search (others are not concerned)."""
         if self._begun[group] is None:
             raise ValueError(f"group {group} has no search")
         self.stream.synchronize()
-        if int(self.short.item()):
-            raise RuntimeError(f"the pool ran out: {int(self.short.item())} pages could not be given")
+        missed = int(self.missed[group].item())
+        if missed:
+            raise RuntimeError(f"the pool ran out in this search: {missed} times a page could not be given")
         if _lib.device_status():
             raise RuntimeError("a device wait ran out")
         start, first = self._begun[group]

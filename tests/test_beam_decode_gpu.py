@@ -192,3 +192,41 @@ def test_compact_waits_for_the_steps_before_it(model):
         assert live == int((eng.ref > 0).sum()) == int(eng.table.max()) + 1 and live >= 5
         eng.end(1)
         assert eng.compact() == int((eng.ref > 0).sum()) < live
+
+
+def _same(a, b):
+    """Equal sequences; scores as close as another make-up of the batch leaves them."""
+    return [t for _, t in a] == [t for _, t in b] and np.allclose([s for s, _ in a], [s for s, _ in b], rtol=0, atol=1e-4)
+
+
+def test_a_shortage_concerns_its_own_search_alone(model):
+    """A search that ran out of pages cannot give a result; others can, and the group can after a new begin."""
+    cfg, pre, m = model
+    prompt = [(3 * j + 2) % SMALL.V for j in range(30)]
+    one = _engine(model, beams=3, groups=1, pages=12, width=2)
+    _begin(one, pre, 0, prompt)
+    one.step(5)
+    want = one.result(0)
+    eng = _engine(model, beams=3, groups=2, pages=4, width=2)
+    _begin(eng, pre, 0, prompt)
+    eng.step(1)                             # three pages held
+    _begin(eng, pre, 1, prompt)             # the fourth: its beams cannot part
+    eng.step(4)
+    assert _same(eng.result(0), want)
+    with pytest.raises(RuntimeError):
+        eng.result(1)
+    eng.step(2)
+    with pytest.raises(RuntimeError):
+        eng.result(1)                       # for good
+    eng.result(0)
+    eng.end(0)
+    _begin(eng, pre, 1, prompt)
+    eng.step(5)
+    assert _same(eng.result(1), want)
+    # a prompt that the pool cannot hold
+    tiny = _engine(model, beams=2, groups=2, pages=2, width=4)
+    _begin(tiny, pre, 0, [1] * 30)
+    _begin(tiny, pre, 1, [1] * 90)
+    assert len(tiny.result(0)) == 2
+    with pytest.raises(RuntimeError):
+        tiny.result(1)
