@@ -48,8 +48,9 @@ class BeamDecodeEngine:
             _lib.call("rngd_decode_kv4_workspace", self._e._m, B, width, window, sinks, ctypes.byref(need))
             self._ws = torch.zeros(max(need.value, 16), dtype=torch.uint8, device=d)
         self._graph = None
-        self._steps = []                                        # (tokens, parents) of each step, on the device
-        self._begun = [None] * groups                           # first step of each group's search
+        self._steps = []                                        # (tokens, parents) of the steps that are kept
+        self._past = 0                                          # steps before them: no search reaches back so far
+        self._begun = [None] * groups                           # first step of each group's search, first tokens
         self._held = [0] * groups                               # positions its beams hold
         torch.cuda.synchronize(self.dev)
 
@@ -77,8 +78,6 @@ class BeamDecodeEngine:
         if logits.shape != (c.vocab,) or logits.device != self.dev or kv.device != self.dev:
             raise ValueError(f"logits must be [{c.vocab}] on {self.dev}")
         s, W, r0 = self.stream, self.W, group * self.W
-        if not any(self._begun):
-            self._steps.clear()
         s.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.cuda.stream(s):
             kv.record_stream(s)
@@ -104,8 +103,16 @@ class BeamDecodeEngine:
             self.parents[rows] = torch.where(sc[0] > float("-inf"), pa[0] + r0, -1)
             first = tk[0].clone()
         torch.cuda.current_stream(self.dev).wait_stream(s)
-        self._begun[group] = (len(self._steps), first)
+        self._begun[group] = (self._past + len(self._steps), first)
         self._held[group] = P
+        self._forget()
+
+    def _forget(self):
+        """Drop the steps that came before the oldest search."""
+        now = self._past + len(self._steps)
+        oldest = min((b[0] for b in self._begun if b is not None), default=now)
+        del self._steps[:oldest - self._past]
+        self._past = oldest
 
     def _release(self, r0):
         """Empty the rows of the group whose first one is r0 (on the current stream)."""
@@ -169,7 +176,8 @@ class BeamDecodeEngine:
                     self._graph.replay()
                 else:
                     self._step()
-                self._steps.append((self.toks.clone(), self.parents.clone()))
+                if any(b is not None for b in self._begun):
+                    self._steps.append((self.toks.clone(), self.parents.clone()))
         for g in range(self.G):
             if self._begun[g] is not None:
                 self._held[g] += n
@@ -189,7 +197,7 @@ class BeamDecodeEngine:
             raise RuntimeError("a device wait ran out")
         start, first = self._begun[group]
         r0 = group * self.W
-        hist = [(t.tolist(), p.tolist()) for t, p in self._steps[start:]]
+        hist = [(t.tolist(), p.tolist()) for t, p in self._steps[start - self._past:]]
         scores, first = self.scores.tolist(), first.tolist()
         out = []
         for r in range(r0, r0 + self.W):
@@ -217,6 +225,7 @@ class BeamDecodeEngine:
             self._release(group * self.W)
         self._begun[group] = None
         self._held[group] = 0
+        self._forget()
 
     @_lib.on_device
     def compact(self):

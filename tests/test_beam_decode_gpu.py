@@ -230,3 +230,34 @@ def test_a_shortage_concerns_its_own_search_alone(model):
     assert len(tiny.result(0)) == 2
     with pytest.raises(RuntimeError):
         tiny.result(1)
+
+
+def test_history_is_as_long_as_the_oldest_search(model):
+    """Searches that overlap: steps before the oldest one still alive are forgotten, results are not."""
+    cfg, pre, m = model
+    prompt = [(5 * j + 1) % SMALL.V for j in range(20)]
+    alone = _engine(model, beams=2, groups=1, pages=12, width=3)
+    _begin(alone, pre, 0, prompt)
+    alone.step(9)
+    want = alone.result(0)
+    eng = _engine(model, beams=2, groups=2, pages=24, width=3)
+    _begin(eng, pre, 0, prompt)
+    for i in range(6):                      # the groups in turn: one begins three steps after the other
+        eng.step(3)
+        _begin(eng, pre, (i + 1) % 2, prompt)
+        eng.step(6)
+        assert _same(eng.result(i % 2), want)
+        assert len(eng.result((i + 1) % 2)[0][1]) == 7
+        assert len(eng._steps) <= 9
+        eng.end(i % 2)
+        assert len(eng._steps) <= 6
+        _begin(eng, pre, i % 2, prompt)     # begun anew without an end in between
+        eng.step(9 - 6)
+        assert _same(eng.result((i + 1) % 2), want)
+        eng.end(i % 2)
+        _begin(eng, pre, (i + 1) % 2, prompt)
+        assert len(eng._steps) == 0
+    eng.end(0)
+    eng.end(1)
+    eng.step(4)
+    assert len(eng._steps) == 0
