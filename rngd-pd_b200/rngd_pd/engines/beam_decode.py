@@ -69,8 +69,7 @@ class BeamDecodeEngine:
         held is let go."""
         c = self.cfg
         P, n = len(tokens), self.width * kv4.PAGE
-        if not 0 <= group < self.G:
-            raise IndexError(f"group {group} outside 0..{self.G - 1}")
+        self._check_group(group)
         if not 1 <= P < n:
             raise ValueError(f"a prompt of {P} tokens: 1..{n - 1}")
         if kv.dim() != 5 or kv.shape[:3] != (c.n_layers, 2, c.n_kv) or kv.shape[3] < P or kv.shape[4] != c.head_dim:
@@ -106,6 +105,10 @@ class BeamDecodeEngine:
         self._begun[group] = (self._past + len(self._steps), first)
         self._held[group] = P
         self._forget()
+
+    def _check_group(self, group):
+        if not 0 <= group < self.G:
+            raise IndexError(f"group {group} outside 0..{self.G - 1}")
 
     def _forget(self):
         """Drop the steps that came before the oldest search."""
@@ -153,6 +156,8 @@ class BeamDecodeEngine:
     @_lib.on_device
     def step(self, n=1):
         """n steps of every search.  Queued on the engine's stream; nothing is read back."""
+        if n < 0:
+            raise ValueError(f"{n} steps")
         for g in range(self.G):
             if self._begun[g] is not None and self._held[g] + n > self.width * kv4.PAGE:
                 raise ValueError(f"group {g} holds {self._held[g]} positions: {n} more do not fit {self.width} pages")
@@ -187,6 +192,7 @@ class BeamDecodeEngine:
     def result(self, group):
         """The group's beams that have a continuation, best first: [(score, tokens)], tokens up to and with the
         first eos.  Raises where the pool ran out of pages during the group's search (others are not concerned)."""
+        self._check_group(group)
         if self._begun[group] is None:
             raise ValueError(f"group {group} has no search")
         self.stream.synchronize()
@@ -217,8 +223,7 @@ class BeamDecodeEngine:
     @_lib.on_device
     def end(self, group):
         """Let go of the group's pages and beams."""
-        if not 0 <= group < self.G:
-            raise IndexError(f"group {group} outside 0..{self.G - 1}")
+        self._check_group(group)
         s = self.stream
         s.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.cuda.stream(s):

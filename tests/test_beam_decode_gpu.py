@@ -261,3 +261,15 @@ def test_history_is_as_long_as_the_oldest_search(model):
     eng.end(1)
     eng.step(4)
     assert len(eng._steps) == 0
+
+
+def test_engine_refuses_groups_and_steps_out_of_range(model):
+    cfg, pre, m = model
+    eng = _engine(model, beams=2, groups=2, pages=8, width=2)
+    prompt = [1, 2, 3]
+    _begin(eng, pre, 1, prompt)
+    for bad in (lambda: eng.result(-1), lambda: eng.result(2), lambda: eng.end(-1), lambda: eng.step(-1)):
+        with pytest.raises((ValueError, IndexError)):
+            bad()
+    eng.step(0)
+    assert len(eng.result(1)) == 2 and len(eng.result(1)[0][1]) == 1
