@@ -52,6 +52,7 @@ class BeamDecodeEngine:
         self._past = 0                                          # steps before them: no search reaches back so far
         self._begun = [None] * groups                           # first step of each group's search, first tokens
         self._held = [0] * groups                               # positions its beams hold
+        self._broken = set()                                    # groups whose search a device wait spoilt
         torch.cuda.synchronize(self.dev)
 
     # ------------------------------------------------------------------ pages
@@ -127,6 +128,7 @@ class BeamDecodeEngine:
         self.scores[rows] = float("-inf")
         self.done[rows] = True
         self.missed[r0 // self.W] = 0
+        self._broken.discard(r0 // self.W)
 
     # ------------------------------------------------------------------- step
     def _step(self):
@@ -199,8 +201,10 @@ class BeamDecodeEngine:
         missed = int(self.missed[group].item())
         if missed:
             raise RuntimeError(f"the pool ran out in this search: {missed} times a page could not be given")
-        if _lib.device_status():
-            raise RuntimeError("a device wait ran out")
+        if _lib.device_status():  # reading clears it
+            self._broken.update(g for g in range(self.G) if self._begun[g] is not None)
+        if group in self._broken:
+            raise RuntimeError("a device wait ran out during this search")
         start, first = self._begun[group]
         r0 = group * self.W
         hist = [(t.tolist(), p.tolist()) for t, p in self._steps[start - self._past:]]

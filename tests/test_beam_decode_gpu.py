@@ -273,3 +273,23 @@ def test_engine_refuses_groups_and_steps_out_of_range(model):
             bad()
     eng.step(0)
     assert len(eng.result(1)) == 2 and len(eng.result(1)[0][1]) == 1
+
+
+def test_a_device_wait_that_ran_out_spoils_every_search_alive(model, monkeypatch):
+    """The library's status is read and cleared once; each search that was alive then has no result."""
+    from rngd_pd import _lib
+    cfg, pre, m = model
+    eng = _engine(model, beams=2, groups=2, pages=8, width=2)
+    for g in (0, 1):
+        _begin(eng, pre, g, [1, 2, 3])
+    eng.step(2)
+    codes = [7, 0, 0, 0, 0, 0]              # as if a wait had run out in one of the steps
+    monkeypatch.setattr(_lib, "device_status", lambda reset=True: codes.pop(0))
+    for g in (0, 1, 0):
+        with pytest.raises(RuntimeError):
+            eng.result(g)
+    _begin(eng, pre, 1, [1, 2, 3])
+    eng.step(2)
+    assert len(eng.result(1)) == 2
+    with pytest.raises(RuntimeError):
+        eng.result(0)
