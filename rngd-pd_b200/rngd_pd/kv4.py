@@ -64,6 +64,8 @@ def _pool_dims(pool, layers):
         raise ValueError(f"pool {tuple(shape)}: the last dimensions must be [pages, kv heads, 4, 20 * head_dim]")
     if not pool.is_contiguous() and pool.stride()[-4:] != (NKV * 4 * blk, 4 * blk, blk, 1):
         raise ValueError("pool: a layer's pages must be contiguous")
+    if layers and shape[0] > 1 and pool.stride(0) < P * NKV * 4 * blk:
+        raise ValueError(f"pool: layers {pool.stride(0)} bytes apart lie on one another")
     return (shape[0], P, NKV, HD, pool.stride(0)) if layers else (1, P, NKV, HD, 0)
 
 
@@ -161,6 +163,8 @@ def attention(q, pool, table, lens, window=0, sinks=0, scale=None, out=None):
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype is not dt or out.device != dev:
         raise ValueError(f"out must be {tuple(q.shape)} {dt} on {dev}, got {tuple(out.shape)} {out.dtype}")
+    elif any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError(f"out {tuple(out.shape)} strides {out.stride()}: rows lie on one another")
     op, os = _rows("out", out, 4)
     need = _lib.workspace_bytes("rngd_kv4_attn_workspace", _DT[dt], B, T, NH, NKV, HD, width, window,
                                  sinks)

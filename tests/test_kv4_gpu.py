@@ -548,3 +548,27 @@ def test_refusals_on_the_gpu():
         kv4.fork(pool, ref0, table, lens, room=-1)
     with pytest.raises(_lib.RngdError):
         kv4.fork(pool, *kv4.empty_state(1025, 1, 4))
+
+
+def test_memory_that_would_be_written_twice_is_refused():
+    """Pools whose layers lie on one another, and outputs whose rows do."""
+    from rngd_pd import kv4
+    pool = kv4.alloc_pool(1, 4, 2, 64)
+    two = pool.expand(2, 4, 2, 4, 1280)
+    near = kv4.alloc_pool(1, 5, 2, 64).view(-1).as_strided((2, 4, 2, 4, 1280), (10240, 10240, 5120, 1280, 1))
+    ref0, table, lens = kv4.empty_state(2, 2, 4)
+    k = torch.zeros(2, 2, 1, 2, 64, device="cuda")
+    for bad in (two, near):
+        for f in (lambda: kv4.store(bad, table, lens, k, k), lambda: kv4.fork(bad, ref0, table, lens),
+                  lambda: kv4.compact(bad, ref0, table), lambda: kv4.load(bad, table, lens, 1)):
+            with pytest.raises(ValueError):
+                f()
+    part = kv4.alloc_pool(3, 6, 2, 64)[:, 1:5]              # pages of a larger pool: layers lie apart
+    kv4.store(part, table, lens, torch.zeros(3, 2, 1, 2, 64, device="cuda"), torch.zeros(3, 2, 1, 2, 64, device="cuda"))
+    one = kv4.alloc_pool(1, 4, 2, 64)[0].unsqueeze(0)
+    kv4.load(one, table, lens, 1)
+    q = torch.zeros(2, 3, 8, 64, device="cuda")
+    for shape in ((1, 3, 8, 64), (2, 1, 8, 64), (2, 3, 1, 64)):
+        with pytest.raises(ValueError):
+            kv4.attention(q, pool[0], table, lens, out=torch.zeros(shape, device="cuda").expand(q.shape))
+    kv4.attention(q[:1, :1].expand(2, 3, 8, 64), pool[0], table, lens)   # q may be read twice
