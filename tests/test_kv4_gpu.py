@@ -364,6 +364,89 @@ def test_attention_keeps_its_workspace_through_the_call(monkeypatch):
     assert need > 0 and all(p + need <= ws or ws + need <= p for p in others)
 
 
+# ------------------------------------- attention split over warps: tables wide enough for long sequences
+def _shared(B, width, NKV, HD, lens, seed, P=90):
+    """P full pages, and a table of them in which sequences share pages; entries past a length hold none."""
+    from rngd_pd import kv4
+    g = torch.Generator().manual_seed(seed)
+    pool = _pool_of(1, P, NKV, HD)
+    rows = torch.randn(2, 1, P, 64, NKV, HD, generator=g)
+    rows[0] += torch.randn(1, 1, 1, NKV, HD, generator=g)
+    kv4.store(pool, torch.arange(P, dtype=torch.int32, device="cuda").view(P, 1),
+              torch.zeros(P, dtype=torch.int32, device="cuda"), *rows.cuda())
+    table = torch.randint(0, P, (B, width), generator=g).to(torch.int32)
+    for b, n in enumerate(lens):
+        table[b, -(-n // 64):] = -1
+    return pool[0], table.cuda()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("HD", [64, 128])
+@pytest.mark.parametrize("G,T", [(1, 1), (4, 1), (7, 1), (4, 4), (4, 5), (3, 11)])
+def test_runs_over_rows_and_types(dt, HD, G, T):
+    """1 to 33 query rows of a kv head: every layout of q and P, over lengths from none to 4401."""
+    lens = [0, 1, 33, 700, 4401, 2050]
+    pool, table = _shared(len(lens), 70, 2, HD, lens, 41)
+    q = torch.randn(len(lens), T, 2 * G, HD, generator=torch.Generator().manual_seed(HD + G + T)).to(DT[dt]).cuda()
+    got = _check(q, pool, table, lens, dt)
+    assert np.all(got[0] == 0) and np.all(got[1, :T - 1] == 0)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("HD", [64, 128])
+@pytest.mark.parametrize("G,T,window,sinks", [(4, 1, 4100, 70), (4, 1, 2000, 5), (4, 5, 4097, 1), (7, 1, 4200, 0), (4, 4, 2500, 200)])
+def test_runs_with_windows_and_sinks(dt, HD, G, T, window, sinks):
+    """Units of sinks and of the window, in segments that are cut."""
+    lens = [5100, 4100, 0, 130, 4801]
+    pool, table = _shared(len(lens), 80, 2, HD, lens, 42)
+    q = torch.randn(len(lens), T, 2 * G, HD, generator=torch.Generator().manual_seed(HD + G + T)).to(DT[dt]).cuda()
+    _check(q, pool, table, lens, dt, window, sinks)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("HD", [64, 128])
+@pytest.mark.parametrize("G,T", [(4, 1), (4, 4), (2, 3)])
+def test_runs_of_many_segments(dt, HD, G, T):
+    """160 segments, most of them cut in two or not at all: the join takes all rows of one at a time."""
+    lens = [(617 * b) % 900 for b in range(38)] + [4480, 3001]
+    pool, table = _shared(len(lens), 70, 4, HD, lens, 43)
+    q = torch.randn(len(lens), T, 4 * G, HD, generator=torch.Generator().manual_seed(HD + G + T)).to(DT[dt]).cuda()
+    got = _check(q, pool, table, lens, dt)
+    from rngd_pd import kv4
+    again = kv4.attention(q, pool, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    assert np.array_equal(_np(again), got)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("HD,G,T", [(64, 4, 1), (128, 4, 1), (64, 4, 4), (128, 4, 4), (128, 5, 4)])
+def test_runs_over_missing_pages_and_unseen_nans(dt, HD, G, T):
+    """No page, ids that are none, a table too narrow, and NaN before the window: none of it has a part."""
+    from rngd_pd import kv4
+    lens = [4400, 4400, 2100, 5000, 4000]
+    pool, table = _shared(len(lens), 70, 2, HD, lens, 44, P=95)
+    table[0, 3], table[0, 40], table[1, 0], table[1, 68], table[2, 20:] = -1, 95, -7, 2 ** 31 - 1, -1
+    table[4] = -1
+    lost = torch.full((1, 1, 64, 2, HD), float("nan"), device="cuda")
+    kv4.store(pool.unsqueeze(0), torch.tensor([[94]], dtype=torch.int32, device="cuda"),
+              torch.zeros(1, dtype=torch.int32, device="cuda"), lost, lost)
+    window, sinks = 4150, 3
+    table[table == 94] = 93
+    table[0, 1] = table[1, 2] = 94                          # positions 64..191, past the sinks and before the window
+    q = torch.randn(len(lens), T, 2 * G, HD, generator=torch.Generator().manual_seed(HD + G)).to(DT[dt]).cuda()
+    got = _check(q, pool, table, lens, dt, window, sinks)
+    assert np.all(got[4] == 0)
+
+
+def test_runs_of_more_streams_than_a_launch_takes():
+    """Records and prefix sums are used again by the second launch."""
+    B = 1030
+    lens = [(37 * b) % 150 for b in range(B)]
+    lens[3], lens[500], lens[1026], lens[1029] = 4160, 3000, 4100, 2999
+    pool, table = _shared(B, 65, 1, 64, lens, 45, P=70)
+    q = torch.randn(B, 1, 2, 64, generator=torch.Generator().manual_seed(9)).cuda()
+    _check(q, pool, table, lens, "fp32")
+
+
 # -------------------------------------------------------------------------------------------- pages
 def _run_fork(ref0, table, lens, parents, room, L=2, NKV=2, HD=64):
     from rngd_pd import kv4
