@@ -118,6 +118,39 @@ def test_store_of_special_values(HD):
         assert np.isnan(y[2, 32:64]).all() and np.isfinite(np.delete(y[2], np.arange(32, 64))).all()
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("HD", [64, 128])
+def test_store_of_groups_far_from_zero(dt, HD):
+    """Means of 0 to 2^13 steps: c's rounding comes to count for more than a step, and codes are held to 0..15."""
+    from rngd_pd import kv4
+    far = [0.0, 10.0, 100.0, 400.0, 520.0, 700.0, 2000.0, 8192.0]
+    x = 15 * torch.rand(len(far), 2, HD, generator=torch.Generator().manual_seed(HD))
+    x += torch.tensor(far).view(-1, 1, 1)
+    x[:, 1] *= -0.03                                        # and small steps below zero
+    x = x.to(DT[dt])
+    pool, z = _pool_of(1, 1, 2, HD, 0), torch.zeros(1, dtype=torch.int32, device="cuda")
+    rows = x.view(1, 1, len(far), 2, HD).cuda()
+    kv4.store(pool, z.view(1, 1), z, rows, rows)
+    X = _np(x)
+    u, s, c, tie = ref.encode(X)
+    want, step, base = ref.values(u, s, c), np.repeat(s, 32, -1), np.repeat(np.abs(c), 32, -1)
+    for y in kv4.load(pool, z.view(1, 1), z, len(far), dtype=torch.float32):
+        y = _np(y)[0, 0]
+        # the quotient in fp32 is off by 2^-18 of a step at most (two roundings of up to 32 steps)
+        assert np.all((y == want) | ((tie < 2.0 ** -16) & (np.abs(y - want) <= 1.01 * step)))
+        # half a step, s rounded (31 times), c and the value rounded to 11 bits
+        assert np.all(np.abs(y - X) <= step * (0.5 + 31 * 2.0 ** -11) + 2.0 ** -11 * (base + np.abs(y)))
+    # the scales themselves against 64 bits: s to a place of fp16, c the nearest to min - 16 s but for fp32's rounding
+    raw = pool[0, 0].cpu().numpy()[:, 0, 16 * HD:18 * HD]   # first block, K's scales [heads][16 keys][HD / 32][s, c]
+    sc = np.ascontiguousarray(raw).view(np.float16).astype(np.float64).reshape(2, 16, HD // 32, 2)
+    g = X.reshape(len(far), 2, -1, 32)
+    for i in range(len(far)):
+        s64 = (g[i].max(-1) - g[i].min(-1)) / 15
+        assert np.all(np.abs(sc[:, i, :, 0] - s64) <= 2.0 ** -10 * s64)
+        c64 = g[i].min(-1) - 16 * sc[:, i, :, 0]
+        assert np.all(np.abs(sc[:, i, :, 1] - c64) <= 2.0 ** -11 * np.abs(c64) * (1 + 2.0 ** -10) + 2.0 ** -24)
+
+
 def test_store_takes_any_strides():
     """The prefill engine's layout [L][2][NKV][S][HD], odd strides and odd addresses store the same bytes."""
     from rngd_pd import kv4
