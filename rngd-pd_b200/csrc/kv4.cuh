@@ -64,8 +64,8 @@ __device__ __forceinline__ f32x2 mul_pair(f32x2 a, f32x2 b) {
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 
-// (a & m) | o as one instruction: left to itself the compiler moves the mask ahead of the shift and
-// takes a third one (15% of the kernel's time).
+// (a & m) | o by one lop3.  Attention over 8 x (9001..65001) positions takes 79.8 us in a graph so, 93.1 with the
+// expression written in C; a window of 1000 in 32 x (901..15001) 13.1 and 13.4.
 __device__ __forceinline__ uint32_t lop_ao(uint32_t a, uint32_t m, uint32_t o) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(m), "r"(o));
