@@ -11,8 +11,9 @@
 // K words sit where lane t of a matrix fragment row reads its NG words with one load, V half words
 // where lane (g, t) reads keys 2t and 2t + 1 with one load and all rows of a fragment share a group.
 // The 16 in the value comes from the decoding: a code or-ed into the upper mantissa bits of fp16 16.0
-// is 16 + u exactly, so one fused multiply-add per pair of values finishes it, and c = fp16(min - 16 s)
-// is held to s / 64.  5 bits a value in all.
+// is 16 + u exactly, so one fused multiply-add per pair of values finishes it.  c is held to 2^-11 of itself:
+// to s / 64 for groups around zero, to more the farther their mean lies (a step at 2048 of them).  5 bits a
+// value in all.
 #pragma once
 #include <cuda_fp16.h>
 

@@ -27,8 +27,10 @@ namespace rngd {
 // the result keeps fp32 accuracy.  With up to 4 rows the lo halves take the columns that would stay
 // empty (COLS: hi in columns 0..3, lo in 4..7, one matrix instruction for both); with more they are
 // products of their own into the same accumulators.  Probabilities are held as 2^(x - m + 8), x the
-// score in units of log 2 and m a running maximum that is only moved when a score exceeds it by 6:
-// fp16 then holds them to 2^-35 of the largest, and the output is rescaled rarely.
+// score in units of log 2 and m a running maximum that is only moved when a score exceeds it by 6: the
+// output is rescaled rarely, and hi + lo hold a probability to 2^-23 of itself, or to 2^-33 of the row's
+// largest where that is more.  What is smaller than that is left out of the output and stays in the sum: n
+// such positions take n * 2^-33 off the result at most (65000: 8e-6, where all but one are that small).
 constexpr int kUnit = 32;
 constexpr int kAttnStreams = 1024;  // streams of one launch
 constexpr float kPBias = 8.0f, kPMax = 14.0f;
@@ -957,16 +959,18 @@ static int attn_plan(int dtype, int B, int T, int NH, int NKV, int HD, int ld_ta
     most_u = most_u < w ? most_u : w;
   }
   // One CTA per segment saves the joining kernel (and its launch) but leaves a long stream to one SM.  Streams
-  // of one length, 32/8 heads of 128, us in a graph, whole against runs (before q was fetched at once): 1x387 8.2 and 9.9, 1x1000 10.8 and
-  // 10.3, 1x2000 14.7 and 10.4; 16x300 7.8 and 15.3, 16x4000 23.6 and 31.9; 64x1000 23.5 and 34.6, 64x5000
-  // 90.5 and 91.2.  A CTA has no more warps than let all CTAs run at once (64x300: 12.0 us, 28.7 without).
+  // of one length, 32/8 heads of 128, bf16, us in a graph, whole against runs: 1x387 7.4 and 9.0, 1x1000 9.5
+  // and 9.5, 1x1536 11.0 and 9.2, 1x2000 13.3 and 9.5; 4x1500 11.6 and 11.7; 16x300 6.9 and 14.6, 16x4000 21.4
+  // and 30.1; 64x1000 22.1 and 31.3, 64x4000 70.0 and 71.1, 64x5000 87.1 and 87.8 (fp32 q 97.1 and 93.5).  The
+  // limit of 48 units is put to the table's width, which lengths often stay far below.  A CTA has no more warps
+  // than let all CTAs run at once (64x300: 10.8 us, 28.7 without).
   long segs = (long)Bl * NKV * p->RT;
   p->whole = 0;
   if (most_u <= 48 || (most_u <= 128 && segs >= 64)) {
     // Three column tiles a warp decode a unit once for 24 rows instead of 16, but halve the CTAs: worth it where
-    // those still fill the GPU and no tile stays empty.  us in a graph, two tiles against three: 24 rows of 64,
-    // 16x1000 (32 segments) 9.8 and 12.1, 64x1500 (128) 17.7 and 14.7; 24 rows of 128, 64x1500 26.9 and 22.4;
-    // 49 rows of 128, 64x1500 49.2 and 84.0.  fp32 q of 128 has no registers for it.
+    // those still fill the GPU and no tile stays empty.  us in a graph, 2 kv heads, bf16, two tiles against three:
+    // 24 rows of 64, 16x1000 (32 segments) 9.6 and 11.9, 64x1500 (128) 17.4 and 14.4; 24 rows of 128, 64x1500 26.1
+    // and 21.9; 52 rows of 128 (seven tiles), 64x1500 47.8 and 83.2.  fp32 q of 128 has no registers for it.
     if (tiles % 3 == 0 && (p->mode == Q16 || HD == 64) && (long)Bl * NKV * (tiles / 3) * 4 >= 3l * num_sms()) {
       p->NT = 3;
       p->RT = (int)(tiles / 3);
