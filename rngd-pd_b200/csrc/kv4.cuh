@@ -23,13 +23,11 @@ namespace rngd {
 
 constexpr int kPage = 64;    // positions of a page
 constexpr int kBlk = 16;     // positions of a block
-constexpr int kGrp = 32;     // values that share a scale
 constexpr float kKvMax = 16384.0f;  // magnitudes are held to this, so that c stays finite in fp16
 
 enum : int { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
 
 __host__ __device__ constexpr int kv4_block_bytes(int HD) { return 20 * HD; }
-__host__ __device__ constexpr size_t kv4_page_bytes(int NKV, int HD) { return (size_t)NKV * 4 * 20 * HD; }
 
 // Byte offsets of a scale inside a block.
 template <int HD>
@@ -78,12 +76,6 @@ __device__ __forceinline__ void decode_word(uint32_t w, __half2 s, __half2 c, ui
   v[1] = h2u(__hfma2(u2h(lop_ao(w << 2, 0x03C003C0u, 0x4C004C00u)), s, c));
   v[2] = h2u(__hfma2(u2h(lop_ao(w >> 2, 0x03C003C0u, 0x4C004C00u)), s, c));
   v[3] = h2u(__hfma2(u2h(lop_ao(w >> 6, 0x03C003C0u, 0x4C004C00u)), s, c));
-}
-
-__device__ __forceinline__ float load1(const void* p, size_t i, int dt) {
-  if (dt == DT_F32) return ((const float*)p)[i];
-  if (dt == DT_BF16) return bf2f(((const uint16_t*)p)[i]);
-  return __half2float(((const __half*)p)[i]);
 }
 
 __device__ __forceinline__ void store1(void* p, size_t i, int dt, float v) {

@@ -19,7 +19,6 @@ import torch
 from rngd_pd import _lib
 
 PAGE = 64     # positions of a page
-GROUP = 32    # values that share a scale
 HEAD_DIMS = (64, 128)
 
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
