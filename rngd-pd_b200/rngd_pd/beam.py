@@ -52,6 +52,6 @@ def select(logits, scores, done, beams, eos=-1):
     need = _lib.workspace_bytes("rngd_beam_workspace", _DT[logits.dtype], R, V, beams)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _lib.check(_select(logits.data_ptr(), _DT[logits.dtype], logits.stride(0), R, V, beams, scores.data_ptr(),
-                       done.data_ptr(), eos, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                       done.data_ptr(), max(eos, -1), out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
                        ended.data_ptr(), ws.data_ptr(), need, _lib.raw_stream(dev.index)))
     return out, parents, tokens, ended

@@ -27,7 +27,8 @@ class BeamDecodeEngine:
         if pages < 1 or width < 1 or window < 0 or sinks < 0 or eos >= cfg.vocab:
             raise ValueError(f"pages={pages} width={width} window={window} sinks={sinks} eos={eos}")
         self.cfg, self.W, self.G, self.B = cfg, beams, groups, beams * groups
-        self.eos, self.window, self.sinks, self.width = eos, window, sinks, width
+        self.eos, self.width = eos, width
+        self.window, self.sinks = (min(n, 2 ** 31 - 1) for n in (window, sinks))  # 32 bits in the library
         # the decode step's buffers (its lanes are not used: one group of the least width)
         self._e = BatchDecodeEngine(cfg, sd, B=self.B, S=128, group=cfg.n_layers, chip=chip)
         self.w, self.dev, self.stream = self._e.w, self._e.dev, self._e.stream
@@ -45,7 +46,7 @@ class BeamDecodeEngine:
             self._first = width * torch.arange(B, **i32)        # each row's first entry of the table
             self._rows = torch.zeros((2, MAXB, cfg.n_kv, cfg.head_dim), dtype=BF, device=d)
             need = ctypes.c_size_t(0)
-            _lib.call("rngd_decode_kv4_workspace", self._e._m, B, width, window, sinks, ctypes.byref(need))
+            _lib.call("rngd_decode_kv4_workspace", self._e._m, B, width, self.window, self.sinks, ctypes.byref(need))
             self._ws = torch.zeros(max(need.value, 16), dtype=torch.uint8, device=d)
         self._graph = None
         self._steps = []                                        # (tokens, parents) of the steps that are kept

@@ -192,6 +192,7 @@ def fork(pool, ref, table, lens, parents=None, room=0):
         with torch.cuda.device(dev):
             return fork(pool, ref, table, lens, parents, room)
     rp, tp, lp = _i32("ref", ref, (P,), dev), _i32("table", table, (R, width), dev), _i32("lens", lens, (R,), dev)
+    room = max(-1, min(room, _INT_MAX))  # the library refuses both ends; more would be cut to 32 bits on the way
     new_ref, new_table, new_lens = torch.empty_like(ref), torch.empty_like(table), torch.empty_like(lens)
     short = torch.empty(1, dtype=torch.int32, device=dev)
     need = _lib.workspace_bytes("rngd_kv4_fork_workspace", R, width)

@@ -293,3 +293,21 @@ def test_a_device_wait_that_ran_out_spoils_every_search_alive(model, monkeypatch
     assert len(eng.result(1)) == 2
     with pytest.raises(RuntimeError):
         eng.result(0)
+
+
+def test_engine_takes_windows_sinks_and_eos_beyond_32_bits(model):
+    """They mean what they say (no window, all sinks, no eos), not what their lowest 32 bits do."""
+    cfg, pre, m = model
+    prompt = [(3 * j + 2) % SMALL.V for j in range(40)]
+    res = []
+    for kw in ({}, dict(window=2 ** 32 + 2), dict(window=2, sinks=2 ** 32), dict(window=2 ** 31 + 5, sinks=2 ** 31 + 1)):
+        eng = _engine(model, beams=3, groups=1, pages=12, width=2, **kw)
+        _begin(eng, pre, 0, prompt)
+        eng.step(5)
+        res.append(eng.result(0))
+    assert all(_same(r, res[0]) for r in res)
+    eos = res[0][0][1][2] - 2 ** 32
+    eng = _engine(model, beams=3, groups=1, pages=12, width=2, eos=eos)
+    _begin(eng, pre, 0, prompt)
+    eng.step(5)
+    assert eng.result(0) == res[0]

@@ -238,3 +238,13 @@ def test_logits_that_round_to_one_score():
     assert one[2].tolist() == [[80]]
     two = beam.select(logits.cuda(), *args([-1000.0, -np.inf]), 2)
     assert two[2].tolist() == [[50, 80]] and two[1].tolist() == [[0, 0]] and two[0][0, 0] == two[0][0, 1]
+
+
+def test_eos_below_32_bits_ends_nothing():
+    from rngd_pd import beam
+    logits = torch.randn(2, 100, generator=torch.Generator().manual_seed(2)).cuda()
+    s, d = torch.zeros(2, device="cuda"), torch.zeros(2, dtype=torch.bool, device="cuda")
+    best = int(logits.float().argmax() % 100)
+    for eos in (-1, -5, -2 ** 31 - 1, best - 2 ** 32):
+        out = beam.select(logits, s, d, 2, eos)
+        assert not out[3].any() and best in out[2][0].tolist()

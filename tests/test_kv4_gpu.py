@@ -688,3 +688,12 @@ def test_memory_that_would_be_written_twice_is_refused():
         with pytest.raises(ValueError):
             kv4.attention(q, pool[0], table, lens, out=torch.zeros(shape, device="cuda").expand(q.shape))
     kv4.attention(q[:1, :1].expand(2, 3, 8, 64), pool[0], table, lens)   # q may be read twice
+
+
+def test_rooms_beyond_32_bits_are_refused():
+    """Not taken by their lowest 32 bits."""
+    from rngd_pd import _lib, kv4
+    pool = kv4.alloc_pool(1, 4, 2, 64)
+    for room in (2 ** 30 + 1, 2 ** 32, 2 ** 32 + 64, -2 ** 32, -2 ** 32 + 1):
+        with pytest.raises(_lib.RngdError):
+            kv4.fork(pool, *kv4.empty_state(2, 2, 4), room=room)
