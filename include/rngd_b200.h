@@ -366,7 +366,8 @@ int rngd_kv4_fork(void* pool, size_t layer_bytes, int L, int P, int NKV, int HD,
                   size_t workspace_bytes, rngd_stream_t stream);
 int rngd_kv4_fork_workspace(int R, int ld_table, size_t* bytes);
 /* Compaction: the n pages that are held move into places 0 .. n-1 (the k-th held page from place n on
- * into the k-th free place below n; the rest stay), with their counts and table entries.  *live: n. */
+ * into the k-th free place below n; the rest stay), with their counts and table entries: the table has
+ * to hold every row that goes on using the pool.  *live: n. */
 int rngd_kv4_compact(void* pool, size_t layer_bytes, int L, int P, int NKV, int HD, const int32_t* ref,
                      const int32_t* table, int ld_table, int R, int32_t* new_ref, int32_t* new_table, int32_t* live,
                      void* workspace, size_t workspace_bytes, rngd_stream_t stream);

@@ -183,8 +183,8 @@ def fork(pool, ref, table, lens, parents=None, room=0):
     if only such rows hold it, the others get copies of its filled blocks, in all layers.  Free pages are given
     lowest first, in the order of rows; short (int32 [1]) counts those that could not be given (-1 in the table), up
     to 2^31 - 1.
-    The old state is left as it is; the pool changes only in pages that were free or were let go, so the old
-    state's own pages stay valid until a later call hands them out."""
+    The old state's tensors are left as they are.  The pool changes only in pages that were free or that this call
+    lets go of: pages that the new state holds too keep their content, the others may be handed out at once."""
     L, P, NKV, HD, layer = _pool_dims(pool, True)
     dev = pool.device
     R, width = table.shape
@@ -207,7 +207,9 @@ def fork(pool, ref, table, lens, parents=None, room=0):
 def compact(pool, ref, table):
     """The state with the n held pages in places 0 .. n-1 of the pool: (ref, table, live), live (int32 [1]) being n.
 
-    The k-th held page from place n on moves into the k-th free place below n, in all layers; the rest stay."""
+    The k-th held page from place n on moves into the k-th free place below n, in all layers; the rest stay.  Page
+    ids change: `table` has to hold the rows of every sequence that goes on using the pool.  The old state's
+    tensors are left as they are, but its free places below n now hold pages."""
     L, P, NKV, HD, layer = _pool_dims(pool, True)
     dev = pool.device
     R, width = table.shape
