@@ -385,6 +385,40 @@ int rngd_beam_select(const void* logits, int dtype, int64_t ld, int R, int V, in
                      uint8_t* out_done, void* workspace, size_t workspace_bytes, rngd_stream_t stream);
 int rngd_beam_workspace(int dtype, int R, int V, int W, size_t* bytes);
 
+/* ------------------------------------------------------ 8-bit linear layers
+ * The reference's projections are bf16 (src/rngd_pd/kernels/decode_batch.py:73-109).  These entries hold rows and
+ * weights in e4m3 with fp32 scales: rows [T][K] one for each 128 values from the left, G = ceil(K / 128) a row;
+ * weights [N][K] one for each block of 128 x 128, [ceil(N / 128)][G].  With m = max(amax, 2^-100) of a group,
+ * scale = m / 448 and a value x is held as e4m3(x * (448 / m)); a group with a NaN or an infinity is lost (it reads
+ * as NaN).  8-bit rows start on 16 bytes: q 16-byte aligned, ldq (bytes) a multiple of 16; bytes of a row beyond its
+ * values are neither written nor read.  Row strides are in elements.  All arrays are device memory.
+ * x [T][K] -> q, scale [T][G] (contiguous). */
+int rngd_f8_rows(const void* x, int dtype, int64_t ldx, int64_t T, int K, void* q, int64_t ldq, float* scale,
+                 rngd_stream_t stream);
+/* w [N][K] -> q, scale [ceil(N / 128)][G] (contiguous). */
+int rngd_f8_weight(const void* w, int dtype, int64_t ldw, int N, int K, void* q, int64_t ldq, float* scale,
+                   rngd_stream_t stream);
+/* h = x + residual, rounded to their type and written to total [T][K] (both NULL: h = x, nothing is written);
+ * h / sqrt(mean h^2 + eps) * weight in fp32 -> q, scale [T][G].  weight: of x's type or fp32.  total may not
+ * overlap x or residual. */
+int rngd_f8_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int dtype,
+                     int weight_dtype, int64_t T, int K, float eps, void* total, int64_t ldt, void* q, int64_t ldq,
+                     float* scale, rngd_stream_t stream);
+/* y[m][n] = sum over k of a[m][k] b[n][k] as they stand, plus add[m][n] (of y's type; NULL: nothing), summed in
+ * fp32 and rounded once to dtype.  a: rows [M][K] with scales [M][G]; b: a weight [N][K] with scales
+ * [ceil(N / 128)][G]; strides of the scales' two dimensions in elements.  add may be y. */
+int rngd_f8_matmul(const void* a, int64_t lda, const float* a_scale, const int64_t* a_strides, const void* b,
+                   int64_t ldb, const float* b_scale, const int64_t* b_strides, int M, int N, int K, const void* add,
+                   int64_t ldadd, void* y, int64_t ldy, int dtype, rngd_stream_t stream);
+/* silu(a gate^T) * (a up^T) in fp32 -> q [M][N], scale [M][ceil(N / 128)] (contiguous).  gate, up: weights [N][K] as
+ * in rngd_f8_matmul.  workspace: rngd_f8_swiglu_workspace() bytes, 16-byte aligned, any content, not shared by
+ * calls that may overlap. */
+int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, const int64_t* a_strides, const void* gate,
+                   int64_t ldg, const float* gate_scale, const int64_t* gate_strides, const void* up, int64_t ldu,
+                   const float* up_scale, const int64_t* up_strides, int M, int N, int K, void* q, int64_t ldq,
+                   float* scale, void* workspace, size_t workspace_bytes, rngd_stream_t stream);
+int rngd_f8_swiglu_workspace(int M, int N, int K, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

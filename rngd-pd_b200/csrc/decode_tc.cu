@@ -694,8 +694,8 @@ static EncodeTiledFn get_encode() {
   return fn;
 }
 
-int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
-                     const uint64_t* strides_bytes, const uint32_t* box) {
+static int encode_tmap(CUtensorMapDataType type, CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
+                       const uint64_t* strides_bytes, const uint32_t* box) {
   EncodeTiledFn enc = get_encode();
   RNGD_REQUIRE(enc != nullptr, "cuTensorMapEncodeTiled is unavailable");
   RNGD_REQUIRE(((uintptr_t)base & 15) == 0, "tensor map base must be 16-byte aligned");
@@ -710,7 +710,7 @@ int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_
     RNGD_REQUIRE(strides_bytes[i] % 16 == 0, "tensor map strides must be multiples of 16 bytes");
     st[i] = strides_bytes[i];
   }
-  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, es,
+  CUresult r = enc(out, type, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, es,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -718,6 +718,14 @@ int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_
     return RNGD_ERR_CUDA;
   }
   return RNGD_OK;
+}
+int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
+                     const uint64_t* strides_bytes, const uint32_t* box) {
+  return encode_tmap(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, base, rank, dims, strides_bytes, box);
+}
+int encode_tmap_u8(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
+                   const uint64_t* strides_bytes, const uint32_t* box) {
+  return encode_tmap(CU_TENSOR_MAP_DATA_TYPE_UINT8, out, base, rank, dims, strides_bytes, box);
 }
 
 // cached tensor maps: weights [L][N][K] (3-D) and activation operands [32][K] (2-D)
@@ -1214,11 +1222,12 @@ int rngd::read_status_decode(int* st, int reset) {
 
 extern "C" int rngd_device_status(int* status, int reset) {
   RNGD_REQUIRE(status != nullptr, "device_status: null output");
-  int st = 0, sp = 0, sa = 0, s4 = 0;
+  int st = 0, sp = 0, sa = 0, s4 = 0, s8 = 0;
   RNGD_TRY(read_status_decode(&st, reset));
   RNGD_TRY(read_status_prefill(&sp, reset));
   RNGD_TRY(read_status_attn(&sa, reset));
   RNGD_TRY(read_status_kv4(&s4, reset));
-  *status = st != 0 ? st : (sp != 0 ? sp : (sa != 0 ? sa : s4));
+  RNGD_TRY(read_status_f8(&s8, reset));
+  *status = st != 0 ? st : (sp != 0 ? sp : (sa != 0 ? sa : (s4 != 0 ? s4 : s8)));
   return RNGD_OK;
 }

@@ -1,0 +1,145 @@
+// Rows and weights held in 8 bits (e4m3) with fp32 scales: what the quantisers (fp8.cu) and the products
+// (fp8_mm.cu) share.
+//
+// A row of K values has a scale for each 128 of them from the left (the last group may be shorter), a weight
+// [N][K] one for each 128 x 128 block.  With m = max(amax, 2^-100) of a group's magnitudes,
+//   scale = m / 448,   q = e4m3(x * (448 / m)),   x stands as q * scale.
+// The lower limit keeps 448 / m finite; a group below it (zeros above all) is held in steps of 2^-118, which no
+// sum with ordinary values could show.  The quotient is taken once a group and the values are multiplied with it:
+// one rounding to 24 bits more than a division each, against half a step of e4m3 of 2^-4.  A NaN makes m, the
+// scale and so the whole group NaN; an infinity makes 448 / m zero and the scale infinite, whose products are NaN too.
+#pragma once
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+
+namespace rngd {
+
+constexpr int kGroup = 128;
+
+enum : int { F8_BF16 = 0, F8_F16 = 1, F8_F32 = 2 };
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// m of a group whose magnitudes reach amax
+__device__ __forceinline__ float held_max(float amax) { return max_nan(amax, 7.888609052210118e-31f); }  // 2^-100
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
+}
+__device__ __forceinline__ uint8_t e4m3(float a) { return (uint8_t)e4m3x2(a, 0.f); }
+
+// one value of type DT
+template <int DT>
+__device__ __forceinline__ float load_as_f32(const void* p, long i) {
+  if constexpr (DT == F8_BF16)
+    return bf2f(((const uint16_t*)p)[i]);
+  else if constexpr (DT == F8_F16)
+    return __half2float(((const __half*)p)[i]);
+  else
+    return ((const float*)p)[i];
+}
+template <int DT>
+__device__ __forceinline__ void store_f32_as(void* p, long i, float v) {
+  if constexpr (DT == F8_BF16)
+    ((uint16_t*)p)[i] = f2bf_bits(v);
+  else if constexpr (DT == F8_F16)
+    ((__half*)p)[i] = __float2half_rn(v);
+  else
+    ((float*)p)[i] = v;
+}
+template <int DT>
+__device__ __forceinline__ float rounded_as(float v) {
+  if constexpr (DT == F8_BF16)
+    return bf2f(f2bf_bits(v));
+  else if constexpr (DT == F8_F16)
+    return __half2float(__float2half_rn(v));
+  else
+    return v;
+}
+
+// Eight values from a 16-byte aligned place: the registers that hold them, and their values.
+template <int DT>
+struct Eight {
+  uint4 r[DT == F8_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, long i) {
+    if constexpr (DT == F8_F32) {
+      const uint4* q = (const uint4*)((const float*)p + i);
+      r[0] = ldg_nc_v4(q);
+      r[1] = ldg_nc_v4(q + 1);
+    } else {
+      r[0] = ldg_nc_v4((const uint16_t*)p + i);
+    }
+  }
+  __device__ __forceinline__ void values(float* f) const {
+    if constexpr (DT == F8_F32) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        f[4 * j] = __uint_as_float(r[j].x);
+        f[4 * j + 1] = __uint_as_float(r[j].y);
+        f[4 * j + 2] = __uint_as_float(r[j].z);
+        f[4 * j + 3] = __uint_as_float(r[j].w);
+      }
+    } else if constexpr (DT == F8_BF16) {
+      unpack8(r[0], f);
+    } else {
+      const uint32_t w[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float2 v = __half22float2(*(const __half2*)&w[j]);
+        f[2 * j] = v.x;
+        f[2 * j + 1] = v.y;
+      }
+    }
+  }
+};
+// Eight values to a 16-byte aligned place.
+template <int DT>
+__device__ __forceinline__ void store_eight(void* p, long i, const float* f) {
+  if constexpr (DT == F8_F32) {
+    float4* q = (float4*)((float*)p + i);
+    q[0] = make_float4(f[0], f[1], f[2], f[3]);
+    q[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if constexpr (DT == F8_BF16) {
+        w[j] = (uint32_t)f2bf_bits(f[2 * j]) | ((uint32_t)f2bf_bits(f[2 * j + 1]) << 16);
+      } else {
+        const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+        w[j] = *(const uint32_t*)&h;
+      }
+    }
+    *(uint4*)((uint16_t*)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// The largest magnitude among 16 neighbouring lanes (a group of 128 values, eight a lane).
+__device__ __forceinline__ float amax16(float m) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+__device__ __forceinline__ float amax_of(const float* f, float m = 0.f) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) m = max_nan(m, fabsf(f[e]));
+  return m;
+}
+__device__ __forceinline__ uint2 held8(const float* f, float inv) {
+  return make_uint2(e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                    e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+}
+
+// SwiGLU in fp32: silu(g) * u.  exp(-g) beyond 2^128 gives g / inf = -0, as the function's limit.
+__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+}  // namespace rngd

@@ -256,6 +256,7 @@ int read_status_decode(int* st, int reset);
 int read_status_prefill(int* st, int reset);
 int read_status_attn(int* st, int reset);
 int read_status_kv4(int* st, int reset);
+int read_status_f8(int* st, int reset);
 size_t attn_fused_scratch_units(int Bcap, int NKV, int S);
 
 // Shared host helpers (decode_tc.cu): SM count, cached tensor maps for weight
@@ -277,5 +278,8 @@ __host__ __device__ __forceinline__ int owner_of(long f, long total, int grid) {
 
 int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
                      const uint64_t* strides_bytes, const uint32_t* box);
+// The same of bytes, box[0] = 128.
+int encode_tmap_u8(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                   const uint32_t* box);
 
 }  // namespace rngd

@@ -155,6 +155,15 @@ _sig("rngd_kv4_compact_workspace", _int, _szp)
 _sig("rngd_beam_select", _vp, _int, ctypes.c_int64, _int, _int, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _sz,
      _vp)
 _sig("rngd_beam_workspace", _int, _int, _int, _int, _szp)
+_i64 = ctypes.c_int64
+_sig("rngd_f8_rows", _vp, _int, _i64, _i64, _int, _vp, _i64, _vp, _vp)
+_sig("rngd_f8_weight", _vp, _int, _i64, _int, _int, _vp, _i64, _vp, _vp)
+_sig("rngd_f8_rms_norm", _vp, _i64, _vp, _i64, _vp, _int, _int, _i64, _int, ctypes.c_float, _vp, _i64, _vp, _i64, _vp,
+     _vp)
+_sig("rngd_f8_matmul", _vp, _i64, _vp, _i64p, _vp, _i64, _vp, _i64p, _int, _int, _int, _vp, _i64, _vp, _i64, _int, _vp)
+_sig("rngd_f8_swiglu", _vp, _i64, _vp, _i64p, _vp, _i64, _vp, _i64p, _vp, _i64, _vp, _i64p, _int, _int, _int, _vp,
+     _i64, _vp, _vp, _sz, _vp)
+_sig("rngd_f8_swiglu_workspace", _int, _int, _int, _szp)
 
 
 def last_error():

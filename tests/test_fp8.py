@@ -1,0 +1,84 @@
+"""Argument checks of the 8-bit linear layers that need no GPU, and the plain forms they are tested with."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from rngd_pd import _lib, fp8
+from tests import fp8_ref as ref
+
+
+def test_tensors_off_the_gpu_are_refused():
+    x, w = torch.zeros(4, 256), torch.ones(256)
+    q, s = torch.zeros(4, 256, dtype=torch.float8_e4m3fn), torch.zeros(4, 2)
+    for f in (lambda: fp8.quantize(x), lambda: fp8.quantize_weight(x), lambda: fp8.rms_norm(x, w, 1e-5),
+              lambda: fp8.matmul(q, s, q, s[:1]), lambda: fp8.matmul_swiglu(q, s, q, s[:1], q, s[:1])):
+        with pytest.raises(ValueError):
+            f()
+
+
+def test_c_entries_refuse_bad_arguments():
+    """Refused on the host, with a message, before anything is launched."""
+    lib, p = _lib.lib, ctypes.c_void_p(4096)
+    odd = ctypes.c_void_p(4097)
+    st2 = (ctypes.c_int64 * 2)(2, 1)
+
+    def mm(a=p, lda=256, sa=p, b=p, ldb=256, M=4, N=4, K=256, add=None, y=p, ldy=4, dt=0, ss=st2):
+        return lib.rngd_f8_matmul(a, lda, sa, ss, b, ldb, p, ss, M, N, K, add, 4, y, ldy, dt, None)
+
+    def sw(q=p, ldq=16, ws=p, n=1 << 20, K=256, N=4):
+        return lib.rngd_f8_swiglu(p, 256, p, st2, p, 256, p, st2, p, 256, p, st2, 4, N, K, q, ldq, p, ws, n, None)
+
+    bad = [
+        (lambda: lib.rngd_f8_rows(p, 3, 8, 1, 8, p, 16, p, None), "data type 3"),
+        (lambda: lib.rngd_f8_rows(p, 0, 8, 2, 8, p, 8, p, None), "16 bytes"),
+        (lambda: lib.rngd_f8_rows(p, 0, 8, 2, 32, p, 16, p, None), "16 bytes"),
+        (lambda: lib.rngd_f8_rows(odd, 0, 8, 1, 8, p, 16, p, None), "misaligned"),
+        (lambda: lib.rngd_f8_rows(p, 0, 8, -1, 8, p, 16, p, None), "-1 rows"),
+        (lambda: lib.rngd_f8_rows(p, 0, 8, 1, 8, p, 16, None, None), "null"),
+        (lambda: lib.rngd_f8_weight(p, 0, 8, 2, 8, odd, 16, p, None), "16 bytes"),
+        (lambda: lib.rngd_f8_weight(p, -1, 8, 2, 8, p, 16, p, None), "data type"),
+        (lambda: lib.rngd_f8_rms_norm(p, 8, None, 0, p, 0, 1, 1, 8, 1e-5, None, 0, p, 16, p, None), "weights of data type 1"),
+        (lambda: lib.rngd_f8_rms_norm(p, 8, p, 8, p, 0, 0, 1, 8, 1e-5, None, 0, p, 16, p, None), "place for the sum"),
+        (lambda: lib.rngd_f8_rms_norm(p, 8, p, 8, p, 0, 0, 1, 8, 1e-5, p, 8, p, 16, p, None), "place of its own"),
+        (lambda: lib.rngd_f8_rms_norm(p, 8, None, 0, None, 0, 0, 1, 8, 1e-5, None, 0, p, 16, p, None), "null"),
+        (lambda: mm(dt=5), "data type 5"), (lambda: mm(K=0), "x 0"), (lambda: mm(M=-1), "-1 x"),
+        (lambda: mm(K=2 ** 31 - 2), "K="), (lambda: mm(a=odd), "misaligned"), (lambda: mm(lda=250), "250 apart"),
+        (lambda: mm(ldb=128), "128 apart"), (lambda: mm(b=None), "null"), (lambda: mm(sa=None), "null"),
+        (lambda: mm(y=None), "null"), (lambda: mm(y=odd), "misaligned"), (lambda: mm(add=odd), "misaligned"),
+        (lambda: mm(ldy=3), "lie on one another"), (lambda: mm(ss=None), "null"),
+        (lambda: sw(q=odd), "16 bytes"), (lambda: sw(ldq=8), "16 bytes"), (lambda: sw(K=0), "x 0"),
+        (lambda: sw(N=-4), "-4"), (lambda: sw(q=None), "null"),
+    ]
+    for f, words in bad:
+        assert f() == _lib.RNGD_ERR_ARG, words
+        assert words in _lib.last_error(), (words, _lib.last_error())
+
+
+def test_empty_calls_do_nothing():
+    lib, p = _lib.lib, ctypes.c_void_p(4096)
+    st2 = (ctypes.c_int64 * 2)(2, 1)
+    assert lib.rngd_f8_rows(None, 0, 0, 0, 8, None, 0, None, None) == 0
+    assert lib.rngd_f8_weight(None, 0, 0, 4, 0, None, 0, None, None) == 0
+    assert lib.rngd_f8_rms_norm(None, 0, None, 0, None, 0, 0, 0, 8, 1e-5, None, 0, None, 0, None, None) == 0
+    assert lib.rngd_f8_matmul(None, 0, None, st2, p, 256, p, st2, 0, 4, 256, None, 0, None, 0, 0, None) == 0
+
+
+def test_plain_forms_on_small_cases():
+    assert ref.e4m3([448.0, 500.0, 0.0, 17.0, 19.0, 18.0, 2.0 ** -9, 2.0 ** -10, 1.5 * 2.0 ** -9, -240.0]).tolist() == \
+        [448, 448, 0, 16, 20, 18, 2.0 ** -9, 0, 2.0 ** -8, -240]
+    codes = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    codes = codes[~codes.isnan()].numpy()
+    assert np.array_equal(ref.e4m3(codes), codes)
+    x = np.linspace(-450, 450, 9001)
+    near = codes[np.abs(x[:, None] - codes).argmin(1)]
+    got = ref.e4m3(x)
+    assert np.all(np.abs(got - x) <= np.abs(near - x))
+    y = np.arange(300.0).reshape(1, 300) - 280
+    assert ref.limits(y).tolist() == [[280, 152, 24]]
+    assert ref.block_limits(np.arange(260.0).reshape(130, 2)).tolist() == [[255.0], [259.0]]
+    a, b = np.ones((2, 130)), np.ones((129, 130))
+    sa, sb = np.array([[1.0, 2.0], [3.0, 4.0]]), np.array([[1.0, 1.0], [0.5, 2.0]])
+    y, mag = ref.product(a, sa, b, sb)
+    assert y[0, 0] == 128 + 4 and y[1, 128] == 128 * 1.5 + 2 * 8 and np.array_equal(y, mag)
