@@ -79,6 +79,12 @@ struct Eight {
       r[0] = ldg_nc_v4((const uint16_t*)p + i);
     }
   }
+  // the same of memory that this kernel may write
+  __device__ __forceinline__ void load_any(const void* p, long i) {
+    const uint4* q = (const uint4*)((const char*)p + i * (DT == F8_F32 ? 4 : 2));
+#pragma unroll
+    for (int j = 0; j < (DT == F8_F32 ? 2 : 1); j++) r[j] = q[j];
+  }
   __device__ __forceinline__ void values(float* f) const {
     if constexpr (DT == F8_F32) {
 #pragma unroll

@@ -29,6 +29,123 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// ---------------------------------------------------------------------- pieces of the kernels
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {  // the same place in another CTA
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// A tile load of this GPU's memory into this CTA, counted by a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {  // a warp of both CTAs
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier at this place of both CTAs once every product issued so far has completed.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}\n" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+
+// 32 columns of this warp's 32 lanes, started; tmem_wait() has to come before they are read.
+struct Cols {
+  uint32_t r[32];
+};
+__device__ __forceinline__ void tmem_start(Cols& c, uint32_t taddr) {
+  uint32_t* r = c.r;
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Waits for every load started; the registers pass through, so nothing reads them earlier.
+__device__ __forceinline__ void tmem_wait(Cols& c) {
+  uint32_t* r = c.r;
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 parts_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+// acc[j] += s * v, two columns an instruction
+__device__ __forceinline__ void fma_cols(uint64_t* acc, const Cols& c, uint64_t s) {
+#pragma unroll
+  for (int j = 0; j < 16; j++) {
+    const uint64_t v = pair_of(__uint_as_float(c.r[2 * j]), __uint_as_float(c.r[2 * j + 1]));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[j]) : "l"(v), "l"(s));
+  }
+}
+// acc[0..31] (64 columns from taddr t0) += s0 * them, acc[32..63] (from t1) += s1 * them; the next 32 columns are on
+// their way while the present ones are added.
+__device__ __forceinline__ void scale_add(uint64_t* acc, uint32_t t0, uint32_t t1, float s0, float s1) {
+  const uint64_t p0 = pair_of(s0, s0), p1 = pair_of(s1, s1);
+  Cols x, y;
+  tmem_start(x, t0);
+  tmem_wait(x);
+  tmem_start(y, t0 + 32);
+  fma_cols(acc, x, p0);
+  tmem_wait(y);
+  tmem_start(x, t1);
+  fma_cols(acc + 16, y, p0);
+  tmem_wait(x);
+  tmem_start(y, t1 + 32);
+  fma_cols(acc + 32, x, p1);
+  tmem_wait(y);
+  fma_cols(acc + 48, y, p1);
+}
+
 struct MmArgs {
   int M, N, K, G;
   const float* sa;  // [M][G], strides in elements
@@ -154,6 +271,246 @@ __global__ void __launch_bounds__(kMmThreads, 1) f8_mm_kernel(const __grid_const
   }
 }
 
+// ------------------------------------------------------------------ many rows: pairs of CTAs
+// Two CTAs (a cluster) work on 256 rows x 256 columns: each holds 128 rows of a and 128 of the weight's in shared
+// memory (32 KB a group), one thread of the first issues the products of both, and each ends with its own 128
+// rows x 256 columns.  A persistent grid, one CTA per SM.
+struct PairArgs {
+  MmArgs m;
+  const float* sb1;  // of the second weight (SWIGLU)
+  long sb1_n, sb1_g;
+  int tm, tn;        // tiles
+  int vec;           // rows of y and add are whole 16-byte vectors
+  uint8_t* q;        // SWIGLU: 8-bit rows and their scales [M][NG]
+  long ldq;
+  float* scale;
+};
+constexpr int kPairStages = 6, kPairStage = 2 * kMmTile, kPairThreads = 128 + 256;
+constexpr size_t kPairSmem = 1024 + kPairStages * kPairStage + (2 * kPairStages + 4) * 8 + 16 + 2 * 2 * 128 * 4;
+
+// 128 sums of row m from column n0 on: plus add, rounded, stored.
+template <int DT>
+__device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* acc, int m, int n0) {
+  const MmArgs& a = p.m;
+  const long o = m * a.ldy + n0, oa = m * a.ldadd + n0;
+  if (p.vec && n0 + 128 <= a.N) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      float v[8], w[8];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float2 x = parts_of(acc[4 * j + e]);
+        v[2 * e] = x.x;
+        v[2 * e + 1] = x.y;
+      }
+      if (a.add != nullptr) {
+        Eight<DT> r;
+        r.load_any(a.add, oa + 8 * j);
+        r.values(w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += w[e];
+      }
+      store_eight<DT>(a.y, o + 8 * j, v);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 64; j++) {
+    const float2 x = parts_of(acc[j]);
+    const float v[2] = {x.x, x.y};
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int c = 2 * j + e;
+      if (n0 + c < a.N) store_f32_as<DT>(a.y, o + c, a.add != nullptr ? v[e] + load_as_f32<DT>(a.add, oa + c) : v[e]);
+    }
+  }
+}
+
+// 64 gate sums and 64 up sums of row m, columns n0 ..: the other 64 of the group are another warp's, so the maximum
+// meets in shared memory.
+__device__ __forceinline__ void pair_store_swiglu(const PairArgs& p, const uint64_t* acc, int m, bool row, int n0, int grp,
+                                                  int h, int r, int quarter, float* s_amax) {
+  const int N = p.m.N;
+  float v[64], most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; j++) {
+    const float2 g = parts_of(acc[j]), u = parts_of(acc[32 + j]);
+    v[2 * j] = n0 + 2 * j < N ? swiglu(g.x, u.x) : 0.f;
+    v[2 * j + 1] = n0 + 2 * j + 1 < N ? swiglu(g.y, u.y) : 0.f;
+    most = max_nan(most, max_nan(fabsf(v[2 * j]), fabsf(v[2 * j + 1])));
+  }
+  s_amax[h * 128 + r] = most;
+  asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+  const float lim = held_max(max_nan(most, s_amax[(1 - h) * 128 + r])), inv = 448.0f / lim;
+  if (!row) return;
+  if (h == 0) p.scale[(long)m * ((N + 127) / 128) + grp] = lim / 448.0f;
+  uint8_t* q = p.q + (long)m * p.ldq + n0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float* f = v + 16 * j;
+    if (n0 + 16 * j + 16 <= N) {
+      const uint2 x = held8(f, inv), y = held8(f + 8, inv);
+      *(uint4*)(q + 16 * j) = make_uint4(x.x, x.y, y.x, y.y);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (n0 + 16 * j + e < N) q[16 * j + e] = e4m3(f[e] * inv);
+    }
+  }
+}
+
+// Row tiles are taken eight at a time: the pairs at work at one time then share few rows of a and of the weight.
+__device__ __forceinline__ void pair_tile(int t, int tm, int tn, int* mt, int* nt) {
+  const int band = t / (8 * tn), first = band * 8, rows = tm - first < 8 ? tm - first : 8, in = t - band * 8 * tn;
+  *mt = first + in % rows;
+  *nt = in / rows;
+}
+
+template <int DT, bool SWIGLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmB1, PairArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = (uint64_t*)(base + kPairStages * kPairStage);  // used in the first CTA
+  uint64_t* empty = full + kPairStages;
+  uint64_t* acc_full = empty + kPairStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;        // [2], used in the first CTA
+  uint32_t* slot = (uint32_t*)(acc_empty + 2);
+  float* s_amax = (float*)(slot + 4);        // [2][2][128]
+  const MmArgs& a = p.m;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pairs = gridDim.x >> 1, pair = blockIdx.x >> 1, tiles = p.tm * p.tn;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 16);  // a warp each of both CTAs' eight
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (SWIGLU) tma_prefetch_desc(&tmB1);
+  }
+  if (warp == 1) tmem_alloc_pair(slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the other CTA's barriers are there
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  grid_dep_wait();
+  // The 384 threads start with 168 registers each: 64512.  Four warps give up theirs for the eight that hold the sums:
+  // 128 * (40 + 2 * 224) = 62464.
+  if (warp < 4) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+   if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int mt, nt;
+        pair_tile(t, p.tm, p.tn, &mt, &nt);
+        const CUtensorMap* tb = SWIGLU && rank ? &tmB1 : &tmB;
+        const int n0 = SWIGLU ? nt * 128 : nt * 256 + (int)rank * 128;
+        for (int i = 0; i < a.G; i++, it++) {
+          const int s = it % kPairStages;
+          ok = mbar_wait(&empty[s], ((uint32_t)(it / kPairStages) & 1u) ^ 1u, ST_TMA_WAIT, &g_status_f8);
+          if (!ok) break;
+          uint8_t* st = base + s * kPairStage;
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStage);  // both CTAs' tiles
+          const uint32_t bar = mapa(smem_u32(&full[s]), 0);
+          tma_load_2d_pair(st, &tmA, bar, i * kGroup, mt * 256 + (int)rank * 128);
+          tma_load_2d_pair(st + kMmTile, tb, bar, i * kGroup, n0);
+        }
+      }
+      // what is in flight lands before the blocks may end: the last products' arrivals, or, where a wait ran out, copies
+      if (ok || rank == 0)
+        for (int j = it < kPairStages ? 0 : it - kPairStages; j < it; j++)
+          mbar_wait(ok ? &empty[j % kPairStages] : &full[j % kPairStages], (uint32_t)(j / kPairStages) & 1u, ST_TMA_WAIT,
+                    &g_status_f8);
+      grid_dep_launch();
+    }
+    __syncwarp();
+   } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_e4m3_f32(256, 256);
+      int it = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs)
+        for (int i = 0; i < a.G; i++, it++) {
+          const int s = it % kPairStages, buf = it & 1;
+          ok = mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8) &&
+               mbar_wait(&full[s], (uint32_t)(it / kPairStages) & 1u, ST_MMA_WAIT, &g_status_f8);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(base + s * kPairStage), sb = sa + kMmTile;
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++)
+            umma_e4m3_pair(tmem + buf * 256, sw128_kmajor_desc(sa + kk * 32), sw128_kmajor_desc(sb + kk * 32), idesc, kk != 0);
+          umma_commit_pair(&empty[s]);
+          umma_commit_pair(&acc_full[buf]);
+        }
+    }
+    __syncwarp();
+   }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // Eight warps: the lane quarter warp & 3 (the rows that a warp may read), half h of the columns.  A thread's
+    // 128 sums are two pieces of 64 columns; with SWIGLU the gate's (columns 0..127 of the tile) and the up's.
+    const int h = (warp - 4) >> 2, r = ((warp & 3) << 5) | lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const int c0 = SWIGLU ? 64 * h : 128 * h, c1 = SWIGLU ? 128 + 64 * h : 128 * h + 64;
+    const uint32_t bar_empty = mapa(smem_u32(acc_empty), 0);
+    const int nblocks = (a.N + 127) / 128;
+    int it = 0, round = 0;
+    bool ok = true;  // a wait that ran out ends the work, but no warp leaves the others alone at a barrier
+    for (int t = pair; t < tiles; t += pairs, round++) {
+      int mt, nt;
+      pair_tile(t, p.tm, p.tn, &mt, &nt);
+      const int m = mt * 256 + (int)rank * 128 + r;
+      const bool row = m < a.M;
+      const int nb = SWIGLU ? nt : (2 * nt + h < nblocks ? 2 * nt + h : nblocks - 1);
+      const float* sa = a.sa + (row ? m : 0) * a.sa_m;
+      const float* sb = a.sb + nb * a.sb_n;
+      const float* sb1 = SWIGLU ? p.sb1 + nb * p.sb1_n : nullptr;
+      uint64_t acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; j++) acc[j] = 0ull;
+      float na = row ? __ldg(sa) : 0.f, nb0 = __ldg(sb), nb1 = SWIGLU ? __ldg(sb1) : 0.f;  // the next group's scales
+      for (int i = 0; i < a.G; i++, it++) {
+        const int buf = it & 1;
+        const float s0 = na * nb0, s1 = SWIGLU ? na * nb1 : s0;
+        if (i + 1 < a.G) {
+          na = row ? __ldg(sa + (i + 1) * a.sa_g) : 0.f;
+          nb0 = __ldg(sb + (i + 1) * a.sb_g);
+          if (SWIGLU) nb1 = __ldg(sb1 + (i + 1) * p.sb1_g);
+        }
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (uint32_t)(it >> 1) & 1u, ST_EPI_WAIT, &g_status_f8));
+        if (!ok) continue;
+        tc_fence_after();
+        const uint32_t d = tmem + lane_base + (uint32_t)(buf * 256);
+        scale_add(acc, d + c0, d + c1, s0, s1);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(bar_empty + 8 * buf);
+      }
+      if (SWIGLU) {
+        pair_store_swiglu(p, acc, m, row && ok, nt * 128 + 64 * h, nt, h, r, warp & 3, s_amax + (round & 1) * 256);
+      } else if (row && ok) {
+        pair_store<DT>(p, acc, m, nt * 256 + 128 * h);
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync();  // nothing of this pair's is in flight any more
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+  cluster_sync();
+}
+
 // silu(gate) * up of fp32 rows, quantised by groups: 16 lanes a group, eight values each.
 struct SwigluArgs {
   const float *g, *u;  // [M][N], N a multiple of 4
@@ -222,6 +579,41 @@ static int mm_launch(const Operand& a, const Operand& b, int M, int N, int K, co
   return launch_pdl(kernel, dim3((unsigned)tiles), dim3(kMmThreads), kMmSmem, s, "f8_mm_kernel", ta, tb, g);
 }
 
+// The pairs' launch: one weight, or gate and up (b1) with the 8-bit result (q, scale).
+static int pair_launch(const Operand& a, const Operand& b, const Operand* b1, int M, int N, int K, const void* add,
+                       long ldadd, void* y, long ldy, int dtype, uint8_t* q, long ldq, float* scale, cudaStream_t s) {
+  CUtensorMap ta, tb, tb1;
+  RNGD_TRY(operand_map(a, M, K, 128, &ta));
+  RNGD_TRY(operand_map(b, N, K, 128, &tb));
+  tb1 = tb;
+  if (b1 != nullptr) RNGD_TRY(operand_map(*b1, N, K, 128, &tb1));
+  PairArgs p = {};
+  p.m = {M, N, K, (K + 127) / 128, a.scale, (long)a.s0, (long)a.s1, b.scale, (long)b.s0, (long)b.s1, y, ldy, add, ldadd};
+  if (b1 != nullptr) {
+    p.sb1 = b1->scale;
+    p.sb1_n = (long)b1->s0;
+    p.sb1_g = (long)b1->s1;
+  }
+  p.tm = (M + 255) / 256;
+  p.tn = b1 != nullptr ? (N + 127) / 128 : (N + 255) / 256;
+  RNGD_REQUIRE((long)p.tm * p.tn <= 0x7FFFFFFFl / 2, "f8_matmul: %d x %d results", M, N);
+  const int sz = dtype == F8_F32 ? 4 : 2;
+  p.vec = ((uintptr_t)y & 15) == 0 && ldy * sz % 16 == 0 && ((uintptr_t)add & 15) == 0 && ldadd * sz % 16 == 0;
+  p.q = q;
+  p.ldq = ldq;
+  p.scale = scale;
+  auto kernel = b1 != nullptr       ? f8_pair_kernel<F8_F32, true>
+                : dtype == F8_BF16 ? f8_pair_kernel<F8_BF16, false>
+                : dtype == F8_F16  ? f8_pair_kernel<F8_F16, false>
+                                   : f8_pair_kernel<F8_F32, false>;
+  static std::atomic<unsigned long long> smem_set[4];
+  RNGD_TRY(set_smem_limit_once((const void*)kernel, kPairSmem, &smem_set[b1 != nullptr ? 3 : dtype],
+                               "cudaFuncSetAttribute(f8_pair_kernel)"));
+  const int tiles = p.tm * p.tn, most = num_sms() / 2;
+  return launch_pdl(kernel, dim3(2 * (tiles < most ? tiles : most)), dim3(kPairThreads), kPairSmem, s, "f8_pair_kernel",
+                    ta, tb, tb1, p);
+}
+
 int read_status_f8(int* st, int reset) {
   RNGD_TRY(check_cuda(cudaMemcpyFromSymbol(st, g_status_f8, sizeof(int)), "read device status"));
   if (reset) {
@@ -249,6 +641,9 @@ extern "C" int rngd_f8_matmul(const void* a, int64_t lda, const float* a_scale, 
   const Operand oa = {a, lda, a_scale, a_strides[0], a_strides[1]}, ob = {b, ldb, b_scale, b_strides[0], b_strides[1]};
   RNGD_TRY(check_operand("f8_matmul", oa, M, K));
   RNGD_TRY(check_operand("f8_matmul", ob, N, K));
+  if (M > 128)
+    return pair_launch(oa, ob, nullptr, M, N, K, add, (long)ldadd, y, (long)ldy, dtype, nullptr, 0, nullptr,
+                       (cudaStream_t)stream);
   return mm_launch(oa, ob, M, N, K, add, (long)ldadd, y, (long)ldy, dtype, (cudaStream_t)stream);
 }
 
@@ -257,7 +652,7 @@ static size_t swiglu_pitch(int N) { return ((size_t)N + 3) / 4 * 4; }
 extern "C" int rngd_f8_swiglu_workspace(int M, int N, int K, size_t* bytes) {
   RNGD_REQUIRE(bytes != nullptr, "f8_swiglu_workspace: null output");
   RNGD_REQUIRE(M >= 0 && N >= 0 && K >= 1, "f8_swiglu: %d x %d x %d", M, N, K);
-  *bytes = 2 * (size_t)M * swiglu_pitch(N) * 4;
+  *bytes = M > 128 ? 0 : 2 * (size_t)M * swiglu_pitch(N) * 4;
   return RNGD_OK;
 }
 
@@ -273,7 +668,7 @@ extern "C" int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, 
   RNGD_REQUIRE(q && scale && a_strides && gate_strides && up_strides, "f8_swiglu: null pointer");
   RNGD_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)scale & 3) == 0 && (M <= 1 || (ldq >= N && ldq % 16 == 0)),
                "f8_swiglu: 8-bit rows must start on 16 bytes and not overlap");
-  RNGD_REQUIRE(workspace != nullptr && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need,
+  RNGD_REQUIRE(need == 0 || (workspace != nullptr && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need),
                "f8_swiglu: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
   const Operand oa = {a, lda, a_scale, a_strides[0], a_strides[1]};
   const Operand og = {gate, ldg, gate_scale, gate_strides[0], gate_strides[1]};
@@ -281,6 +676,9 @@ extern "C" int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, 
   RNGD_TRY(check_operand("f8_swiglu", oa, M, K));
   RNGD_TRY(check_operand("f8_swiglu", og, N, K));
   RNGD_TRY(check_operand("f8_swiglu", ou, N, K));
+  if (M > 128)
+    return pair_launch(oa, og, &ou, M, N, K, nullptr, 0, nullptr, 0, F8_F32, (uint8_t*)q, (long)ldq, scale,
+                       (cudaStream_t)stream);
   const long pitch = (long)swiglu_pitch(N);
   float* g = (float*)workspace;
   float* u = g + M * pitch;
