@@ -80,34 +80,25 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
       : "memory");
 }
 
-// 32 columns of this warp's 32 lanes, started; tmem_wait() has to come before they are read.
-struct Cols {
-  uint32_t r[32];
-};
-__device__ __forceinline__ void tmem_start(Cols& c, uint32_t taddr) {
-  uint32_t* r = c.r;
+// 64 columns of this warp's 32 lanes.  The wait is part of the same statement, so nothing reads the registers earlier.
+__device__ __forceinline__ void tmem_ld_x64(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-// Waits for every load started; the registers pass through, so nothing reads them earlier.
-__device__ __forceinline__ void tmem_wait(Cols& c) {
-  uint32_t* r = c.r;
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
-               :
-               : "memory");
-  asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
 }
 __device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
   uint64_t r;
@@ -119,31 +110,16 @@ __device__ __forceinline__ float2 parts_of(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-// acc[j] += s * v, two columns an instruction
-__device__ __forceinline__ void fma_cols(uint64_t* acc, const Cols& c, uint64_t s) {
+// acc[0..31] += s * (64 columns from taddr), two columns an instruction
+__device__ __forceinline__ void scale_add(uint64_t* acc, uint32_t taddr, float s) {
+  uint32_t r[64];
+  tmem_ld_x64(taddr, r);
+  const uint64_t ss = pair_of(s, s);
 #pragma unroll
-  for (int j = 0; j < 16; j++) {
-    const uint64_t v = pair_of(__uint_as_float(c.r[2 * j]), __uint_as_float(c.r[2 * j + 1]));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[j]) : "l"(v), "l"(s));
+  for (int j = 0; j < 32; j++) {
+    const uint64_t v = pair_of(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[j]) : "l"(v), "l"(ss));
   }
-}
-// acc[0..31] (64 columns from taddr t0) += s0 * them, acc[32..63] (from t1) += s1 * them; the next 32 columns are on
-// their way while the present ones are added.
-__device__ __forceinline__ void scale_add(uint64_t* acc, uint32_t t0, uint32_t t1, float s0, float s1) {
-  const uint64_t p0 = pair_of(s0, s0), p1 = pair_of(s1, s1);
-  Cols x, y;
-  tmem_start(x, t0);
-  tmem_wait(x);
-  tmem_start(y, t0 + 32);
-  fma_cols(acc, x, p0);
-  tmem_wait(y);
-  tmem_start(x, t1);
-  fma_cols(acc + 16, y, p0);
-  tmem_wait(x);
-  tmem_start(y, t1 + 32);
-  fma_cols(acc + 32, x, p1);
-  tmem_wait(y);
-  fma_cols(acc + 48, y, p1);
 }
 
 struct MmArgs {
@@ -467,7 +443,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const uint32_t bar_empty = mapa(smem_u32(acc_empty), 0);
     const int nblocks = (a.N + 127) / 128;
     int it = 0, round = 0;
-    bool ok = true;  // a wait that ran out ends the work, but no warp leaves the others alone at a barrier
+    bool ok = true;  // a wait that ran out ends the waiting, but no warp leaves the others alone at a barrier
     for (int t = pair; t < tiles; t += pairs, round++) {
       int mt, nt;
       pair_tile(t, p.tm, p.tn, &mt, &nt);
@@ -480,20 +456,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       uint64_t acc[64];
 #pragma unroll
       for (int j = 0; j < 64; j++) acc[j] = 0ull;
-      float na = row ? __ldg(sa) : 0.f, nb0 = __ldg(sb), nb1 = SWIGLU ? __ldg(sb1) : 0.f;  // the next group's scales
+      // scales a group ahead; a row that is not there takes the first one's, and nothing of it is stored
+      float na = __ldg(sa), nb0 = __ldg(sb), nb1 = SWIGLU ? __ldg(sb1) : 0.f;
       for (int i = 0; i < a.G; i++, it++) {
         const int buf = it & 1;
         const float s0 = na * nb0, s1 = SWIGLU ? na * nb1 : s0;
         if (i + 1 < a.G) {
-          na = row ? __ldg(sa + (i + 1) * a.sa_g) : 0.f;
-          nb0 = __ldg(sb + (i + 1) * a.sb_g);
-          if (SWIGLU) nb1 = __ldg(sb1 + (i + 1) * p.sb1_g);
+          na = __ldg(sa += a.sa_g);
+          nb0 = __ldg(sb += a.sb_g);
+          if (SWIGLU) nb1 = __ldg(sb1 += p.sb1_g);
         }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (uint32_t)(it >> 1) & 1u, ST_EPI_WAIT, &g_status_f8));
-        if (!ok) continue;
+        if (ok) ok = mbar_wait(&acc_full[buf], (uint32_t)(it >> 1) & 1u, ST_EPI_WAIT, &g_status_f8);
+        __syncwarp();
         tc_fence_after();
         const uint32_t d = tmem + lane_base + (uint32_t)(buf * 256);
-        scale_add(acc, d + c0, d + c1, s0, s1);
+        scale_add(acc, d + c0, s0);
+        scale_add(acc + 32, d + c1, s1);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(bar_empty + 8 * buf);
