@@ -35,6 +35,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ bool elect_one() {  // one lane of the warp, all of which are here
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
@@ -412,8 +417,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
    } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    // The whole warp runs the loop and one elected lane issues: with operands that the compiler knows to be the
+    // warp's own, an issue takes a fraction of the time that it takes under a branch on the lane.
+    if (rank == 0) {
       const uint32_t idesc = idesc_e4m3_f32(256, 256);
+      const uint64_t desc = sw128_kmajor_desc(smem_u32(base));
       int it = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs)
@@ -421,17 +429,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           const int s = it % kPairStages, buf = it & 1;
           ok = mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8) &&
                mbar_wait(&full[s], (uint32_t)(it / kPairStages) & 1u, ST_MMA_WAIT, &g_status_f8);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(base + s * kPairStage), sb = sa + kMmTile;
+          const uint64_t da = desc + (uint64_t)(s * (kPairStage >> 4)), db = da + (kMmTile >> 4);
+          const uint32_t d = tmem + (uint32_t)(buf * 256);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; kk++)
-            umma_e4m3_pair(tmem + buf * 256, sw128_kmajor_desc(sa + kk * 32), sw128_kmajor_desc(sb + kk * 32), idesc, kk != 0);
-          umma_commit_pair(&empty[s]);
-          umma_commit_pair(&acc_full[buf]);
+            for (int kk = 0; kk < 4; kk++) umma_e4m3_pair(d, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
+            umma_commit_pair(&empty[s]);
+            umma_commit_pair(&acc_full[buf]);
+          }
+          __syncwarp();
         }
     }
-    __syncwarp();
    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
