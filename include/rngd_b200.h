@@ -411,13 +411,11 @@ int rngd_f8_matmul(const void* a, int64_t lda, const float* a_scale, const int64
                    int64_t ldb, const float* b_scale, const int64_t* b_strides, int M, int N, int K, const void* add,
                    int64_t ldadd, void* y, int64_t ldy, int dtype, rngd_stream_t stream);
 /* silu(a gate^T) * (a up^T) in fp32 -> q [M][N], scale [M][ceil(N / 128)] (contiguous).  gate, up: weights [N][K] as
- * in rngd_f8_matmul.  workspace: rngd_f8_swiglu_workspace() bytes, 16-byte aligned, any content, not shared by
- * calls that may overlap. */
+ * in rngd_f8_matmul. */
 int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, const int64_t* a_strides, const void* gate,
                    int64_t ldg, const float* gate_scale, const int64_t* gate_strides, const void* up, int64_t ldu,
                    const float* up_scale, const int64_t* up_strides, int M, int N, int K, void* q, int64_t ldq,
-                   float* scale, void* workspace, size_t workspace_bytes, rngd_stream_t stream);
-int rngd_f8_swiglu_workspace(int M, int N, int K, size_t* bytes);
+                   float* scale, rngd_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -105,6 +105,16 @@ __device__ __forceinline__ void tmem_ld_x64(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -139,38 +149,105 @@ struct MmArgs {
   long ldadd;
 };
 
-constexpr int kMmStages = 4, kMmTile = 128 * 128, kMmThreads = 192;
-constexpr size_t kMmSmem = 1024 + kMmStages * 2 * kMmTile + (2 * kMmStages + 5) * 8 + 16;
+constexpr int kMmTile = 128 * 128;  // bytes of 128 rows of a group
 
-template <int DT>
-__global__ void __launch_bounds__(kMmThreads, 1) f8_mm_kernel(const __grid_constant__ CUtensorMap tmA,
-                                                              const __grid_constant__ CUtensorMap tmB, MmArgs a) {
+// ------------------------------------------------------------- few rows: the weight's rows as lanes
+// One CTA works on 128 rows of the weight (DUAL: of gate and of up) and NT rows of a: the weight is the products'
+// first operand, so NT may be as small as 16 and the weight's bytes, which bound this, are read once.  The groups of
+// K are cut into `split` runs, one for each CTA of a cluster, whose sums meet in shared memory, in the order of the
+// runs.  A thread holds NT sums of its row of the weight; the scales of 32 groups at a time, each row's times the
+// block's, lie in shared memory.
+template <int NT, bool DUAL>
+struct FewCfg {
+  static constexpr int A = (DUAL ? 2 : 1) * kMmTile, STAGE = A + NT * 128;
+  static constexpr int COLS = (DUAL ? 2 : 1) * NT;     // columns of one buffer in tensor memory
+  static constexpr int BUFS = NT <= 32 ? 4 : 2;
+  static constexpr int CHUNK = 32;                     // groups whose scales are in shared memory
+  static constexpr int SCALES = CHUNK * COLS * 4;
+  static constexpr int FIXED = 1024 + SCALES + 4 * NT * 4 + 256;
+  // two CTAs an SM where three stages of each fit (an SM has 227 KB, a block's own KB taken off), else one
+  static constexpr int PER_SM = (113 * 1024 - FIXED) / STAGE >= 3 ? 2 : 1;
+  static constexpr int MOST = ((PER_SM == 2 ? 113 : 226) * 1024 - FIXED) / STAGE;
+  static constexpr int STAGES = MOST < 8 ? MOST : 8;
+  static constexpr size_t SMEM = FIXED + STAGES * STAGE;
+  static_assert(STAGES * STAGE >= COLS * 128 * 4, "the sums fit where the stages were");
+  static_assert(BUFS * COLS * PER_SM <= 512 && BUFS * COLS >= 32 && ((BUFS * COLS) & (BUFS * COLS - 1)) == 0, "");
+  static_assert((2 * STAGES + 2 * BUFS + 1) * 8 + 16 <= 256, "barriers");
+};
+struct FewArgs {
+  MmArgs m;
+  const float* sb1;  // of the second weight (DUAL)
+  long sb1_n, sb1_g;
+  int tn, split;
+  uint8_t* q;        // DUAL: 8-bit rows and their scales [M][ceil(N / 128)]
+  long ldq;
+  float* scale;
+};
+constexpr int kFewThreads = 192;
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void few_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// acc[0 .. N / 2) += (N columns from taddr) * s[0 .. N), two columns an instruction
+template <int N>
+__device__ __forceinline__ void scale_add_cols(uint64_t* acc, uint32_t taddr, const float* s) {
+#pragma unroll
+  for (int c = 0; c < N; c += 16) {
+    uint32_t r[16];
+    tmem_ld_x16(taddr + c, r);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const ulonglong2 f = *(const ulonglong2*)(s + c + 4 * j);
+      const uint64_t v0 = pair_of(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]));
+      const uint64_t v1 = pair_of(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+      asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[c / 2 + 2 * j]) : "l"(v0), "l"(f.x));
+      asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[c / 2 + 2 * j + 1]) : "l"(v1), "l"(f.y));
+    }
+  }
+}
+
+template <int NT, bool DUAL, int DT>
+__global__ void __launch_bounds__(kFewThreads, FewCfg<NT, DUAL>::PER_SM)
+    f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                  const __grid_constant__ CUtensorMap tmW1, FewArgs p) {
+  using C = FewCfg<NT, DUAL>;
+  constexpr int ST = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = (uint64_t*)(base + kMmStages * 2 * kMmTile);
-  uint64_t* empty = full + kMmStages;
-  uint64_t* acc_full = empty + kMmStages;  // [2]
-  uint64_t* acc_empty = acc_full + 2;      // [2]
-  uint64_t* done = acc_empty + 2;
+  float* s_scale = (float*)(base + ST * C::STAGE);   // [CHUNK][COLS]
+  float* s_red = s_scale + C::CHUNK * C::COLS;       // [NT][4]
+  uint64_t* full = (uint64_t*)(s_red + 4 * NT);
+  uint64_t* empty = full + ST;
+  uint64_t* acc_full = empty + ST;           // [BUFS]
+  uint64_t* acc_empty = acc_full + C::BUFS;  // [BUFS]
+  uint64_t* done = acc_empty + C::BUFS;
   uint32_t* slot = (uint32_t*)(done + 1);
+  const MmArgs& a = p.m;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tn = (a.N + 127) / 128, mt = blockIdx.x / tn, nt = blockIdx.x - mt * tn;
+  const int rank = blockIdx.x % p.split, tile = blockIdx.x / p.split;
+  const int mt = tile / p.tn, nt = tile - mt * p.tn;
+  const int g0 = (int)((long)a.G * rank / p.split), g1 = (int)((long)a.G * (rank + 1) / p.split);
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kMmStages; s++) {
+    for (int s = 0; s < ST; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < C::BUFS; i++) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 128);
+      mbar_init(&acc_empty[i], 4);
     }
-    mbar_init(done, 128);
+    mbar_init(done, 4);
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmW);
+    if (DUAL) tma_prefetch_desc(&tmW1);
   }
   if (warp == 1) {
-    tmem_alloc(slot, 256);
+    tmem_alloc(slot, C::BUFS * C::COLS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -178,78 +255,150 @@ __global__ void __launch_bounds__(kMmThreads, 1) f8_mm_kernel(const __grid_const
   tc_fence_after();
   const uint32_t tmem = *slot;
   grid_dep_wait();
+  grid_dep_launch();
   if (warp == 0) {
     if (lane == 0) {
       int i = 0;
-      for (; i < a.G; i++) {
-        const int s = i % kMmStages;
-        if (!mbar_wait(&empty[s], ((uint32_t)(i / kMmStages) & 1u) ^ 1u, ST_TMA_WAIT, &g_status_f8)) break;
-        uint8_t* st = base + s * 2 * kMmTile;
-        mbar_arrive_expect_tx(&full[s], 2 * kMmTile);
-        tma_load_2d(st, &tmA, &full[s], i * kGroup, mt * 128);
-        tma_load_2d(st + kMmTile, &tmB, &full[s], i * kGroup, nt * 128);
+      bool ok = true;
+      for (int g = g0; g < g1; g++, i++) {
+        const int s = i % ST;
+        ok = mbar_wait(&empty[s], ((uint32_t)(i / ST) & 1u) ^ 1u, ST_TMA_WAIT, &g_status_f8);
+        if (!ok) break;
+        uint8_t* st = base + s * C::STAGE;
+        mbar_arrive_expect_tx(&full[s], C::STAGE);
+        tma_load_2d(st, &tmW, &full[s], g * kGroup, nt * 128);
+        if (DUAL) tma_load_2d(st + kMmTile, &tmW1, &full[s], g * kGroup, nt * 128);
+        tma_load_2d(st + C::A, &tmA, &full[s], g * kGroup, mt * NT);
       }
-      if (i < a.G)  // a wait ran out: the copies in flight land before the block may end
-        for (int j = i < kMmStages ? 0 : i - kMmStages; j < i; j++)
-          mbar_wait(&full[j % kMmStages], (uint32_t)(j / kMmStages) & 1u, ST_TMA_WAIT, &g_status_f8);
-      grid_dep_launch();
+      if (!ok)  // a wait ran out: the copies in flight land before the block may end
+        for (int j = i < ST ? 0 : i - ST; j < i; j++)
+          mbar_wait(&full[j % ST], (uint32_t)(j / ST) & 1u, ST_TMA_WAIT, &g_status_f8);
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_e4m3_f32(128, 128);
-      for (int i = 0; i < a.G; i++) {
-        const int s = i % kMmStages, buf = i & 1;
-        if (!mbar_wait(&acc_empty[buf], ((uint32_t)(i >> 1) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8)) break;
-        if (!mbar_wait(&full[s], (uint32_t)(i / kMmStages) & 1u, ST_MMA_WAIT, &g_status_f8)) break;
-        tc_fence_after();
-        const uint32_t sa = smem_u32(base + s * 2 * kMmTile), sb = sa + kMmTile;
+    const uint32_t idesc = idesc_e4m3_f32(128, NT);
+    const uint64_t desc = sw128_kmajor_desc(smem_u32(base));
+    for (int i = 0; i < g1 - g0; i++) {
+      const int s = i % ST, buf = i % C::BUFS;
+      bool ok = mbar_wait(&acc_empty[buf], ((uint32_t)(i / C::BUFS) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8) &&
+                mbar_wait(&full[s], (uint32_t)(i / ST) & 1u, ST_MMA_WAIT, &g_status_f8);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const uint64_t dw = desc + (uint64_t)(s * (C::STAGE >> 4)), da = dw + (C::A >> 4);
+      const uint32_t d = tmem + (uint32_t)(buf * C::COLS);
+      if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++)
-          umma_e4m3(tmem + buf * 128, sw128_kmajor_desc(sa + kk * 32), sw128_kmajor_desc(sb + kk * 32), idesc, kk != 0);
+        for (int kk = 0; kk < 4; kk++) {
+          umma_e4m3(d, dw + 2 * kk, da + 2 * kk, idesc, kk != 0);
+          if (DUAL) umma_e4m3(d + NT, dw + (kMmTile >> 4) + 2 * kk, da + 2 * kk, idesc, kk != 0);
+        }
         umma_commit(&empty[s]);
         umma_commit(&acc_full[buf]);
       }
-      mbar_wait(done, 0u, ST_EPI_WAIT, &g_status_f8);
-      tc_fence_after();
+      __syncwarp();
     }
+    mbar_wait(done, 0u, ST_EPI_WAIT, &g_status_f8);
+    tc_fence_after();
     __syncwarp();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, C::BUFS * C::COLS);
   } else {
-    const int r = ((warp & 3) << 5) | lane, m = mt * 128 + r;
+    const int r = ((warp & 3) << 5) | lane, et = threadIdx.x - 64;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    float acc[128];
+    uint64_t acc[C::COLS / 2];
 #pragma unroll
-    for (int j = 0; j < 128; j++) acc[j] = 0.f;
-    for (int i = 0; i < a.G; i++) {
-      const int buf = i & 1;
-      const float s = m < a.M ? a.sa[m * a.sa_m + i * a.sa_g] * a.sb[nt * a.sb_n + i * a.sb_g] : 0.f;
-      const bool ok = mbar_wait(&acc_full[buf], (uint32_t)(i >> 1) & 1u, ST_EPI_WAIT, &g_status_f8);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        float v[32];
-        tmem_ld_32x32b_x32(tmem + lane_base + buf * 128 + c * 32, v);
-#pragma unroll
-        for (int j = 0; j < 32; j++) acc[c * 32 + j] = fmaf(s, v[j], acc[c * 32 + j]);
+    for (int j = 0; j < C::COLS / 2; j++) acc[j] = 0ull;
+    bool ok = true;
+    for (int c0 = g0; c0 < g1; c0 += C::CHUNK) {
+      const int n = min(C::CHUNK, g1 - c0);
+      if (c0 != g0) few_bar();  // every warp is past the previous scales
+      for (int e = et; e < n * NT; e += 128) {
+        const int t = e / n, g = c0 + e - t * n, m = mt * NT + t;  // neighbouring threads: groups of one row
+        const float x = m < a.M ? __ldg(a.sa + m * a.sa_m + g * a.sa_g) : 0.f;
+        s_scale[(g - c0) * C::COLS + t] = x * __ldg(a.sb + nt * a.sb_n + g * a.sb_g);
+        if (DUAL) s_scale[(g - c0) * C::COLS + NT + t] = x * __ldg(p.sb1 + nt * p.sb1_n + g * p.sb1_g);
       }
-      tc_fence_before();
-      mbar_arrive(&acc_empty[buf]);
+      few_bar();
+      for (int k = 0; k < n; k++) {
+        const int i = c0 - g0 + k, buf = i % C::BUFS;
+        if (ok) ok = mbar_wait(&acc_full[buf], (uint32_t)(i / C::BUFS) & 1u, ST_EPI_WAIT, &g_status_f8);
+        __syncwarp();
+        tc_fence_after();
+        scale_add_cols<C::COLS>(acc, tmem + lane_base + (uint32_t)(buf * C::COLS), s_scale + k * C::COLS);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      }
     }
-    mbar_arrive(done);
-    if (m < a.M) {
+    if (lane == 0) mbar_arrive(done);
+    const int n = nt * 128 + r;
+    if (p.split == 1 && !DUAL) {
 #pragma unroll
-      for (int j = 0; j < 128; j++) {
-        const int n = nt * 128 + j;
-        if (n < a.N) {
-          float v = acc[j];
-          if (a.add != nullptr) v += load_as_f32<DT>(a.add, m * a.ldadd + n);
-          store_f32_as<DT>(a.y, m * a.ldy + n, v);
+      for (int t = 0; t < NT; t++) {
+        const int m = mt * NT + t;
+        if (m < a.M && n < a.N && ok) {
+          const float2 v = parts_of(acc[t / 2]);
+          const float y = t & 1 ? v.y : v.x;
+          store_f32_as<DT>(a.y, m * a.ldy + n, a.add != nullptr ? y + load_as_f32<DT>(a.add, m * a.ldadd + n) : y);
         }
+      }
+    } else {
+      float* part = (float*)base;  // [COLS][128]: the stages are done with
+      few_bar();                   // (every warp has seen the last products)
+#pragma unroll
+      for (int j = 0; j < C::COLS / 2; j++) {
+        const float2 v = parts_of(acc[j]);
+        part[(2 * j) * 128 + r] = v.x;
+        part[(2 * j + 1) * 128 + r] = v.y;
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(&g_status_f8, 0, ST_EPI_WAIT);
+  }
+  if (p.split == 1 && !DUAL) return;
+  if (p.split > 1)
+    cluster_sync();
+  else if (warp >= 2)
+    few_bar();
+  if (warp >= 2) {
+    // this CTA's rows of a: their sums over the cluster, the result
+    const int r = ((warp & 3) << 5) | lane, n = nt * 128 + r;
+    float* part = (float*)base;
+    const int t0 = NT * rank / p.split, t1 = min(NT * (rank + 1) / p.split, a.M - mt * NT);
+    const uint32_t at = smem_u32(part + r);
+    auto sum = [&](int c) {
+      if (p.split == 1) return part[c * 128 + r];
+      float v = 0.f;
+      for (int k = 0; k < p.split; k++) v += ld_cluster(mapa(at + c * 512, k));
+      return v;
+    };
+    if constexpr (!DUAL) {
+      for (int t = t0; t < t1; t++) {
+        const int m = mt * NT + t;
+        const float y = sum(t);
+        if (n < a.N)
+          store_f32_as<DT>(a.y, m * a.ldy + n, a.add != nullptr ? y + load_as_f32<DT>(a.add, m * a.ldadd + n) : y);
+      }
+    } else {
+      // the values go back to this CTA's own place, which no other reads
+      for (int t = t0; t < t1; t++) {
+        const float g = sum(t), u = sum(NT + t);
+        const float v = n < a.N ? swiglu(g, u) : 0.f;
+        float most = fabsf(v);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+        part[t * 128 + r] = v;
+        if (lane == 0) s_red[t * 4 + (warp & 3)] = most;
+      }
+      few_bar();
+      for (int t = t0; t < t1; t++) {
+        const int m = mt * NT + t;
+        const float4 w = *(const float4*)(s_red + t * 4);
+        const float lim = held_max(max_nan(max_nan(w.x, w.y), max_nan(w.z, w.w))), inv = 448.0f / lim;
+        if (n < a.N) p.q[m * p.ldq + n] = e4m3(part[t * 128 + r] * inv);
+        if (r == 0) p.scale[(long)m * p.tn + nt] = lim / 448.0f;
       }
     }
   }
+  if (p.split > 1) cluster_sync();  // nobody reads this CTA's sums any more
 }
 
 // ------------------------------------------------------------------ many rows: pairs of CTAs
@@ -500,38 +649,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync();
 }
 
-// silu(gate) * up of fp32 rows, quantised by groups: 16 lanes a group, eight values each.
-struct SwigluArgs {
-  const float *g, *u;  // [M][N], N a multiple of 4
-  int N, NG;
-  long total;  // groups
-  int cols;
-  uint8_t* q;
-  long ldq;
-  float* scale;
-};
-__global__ void __launch_bounds__(256) f8_swiglu_kernel(SwigluArgs a) {
-  grid_dep_wait();
-  const int l = threadIdx.x & 15;
-  const long i = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const bool there = i < a.total;
-  const long row = there ? i / a.NG : 0;
-  const int grp = (int)(i - row * a.NG);
-  float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const int n = grp * kGroup + l + 16 * e;
-    v[e] = there && n < a.cols ? swiglu(a.g[row * a.N + n], a.u[row * a.N + n]) : 0.f;
-  }
-  const float m = held_max(amax16(amax_of(v))), inv = 448.0f / m;
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const int n = grp * kGroup + l + 16 * e;
-    if (there && n < a.cols) a.q[row * a.ldq + n] = e4m3(v[e] * inv);
-  }
-  if (there && l == 0) a.scale[row * a.NG + grp] = m / 448.0f;
-}
-
 // -------------------------------------------------------------------------------------------- host
 struct Operand {
   const void* q;
@@ -554,18 +671,70 @@ static int operand_map(const Operand& o, long rows, int K, int box, CUtensorMap*
   return encode_tmap_u8(out, o.q, 2, dims, strides, bx);
 }
 
-static int mm_launch(const Operand& a, const Operand& b, int M, int N, int K, const void* add, long ldadd, void* y,
-                     long ldy, int dtype, cudaStream_t s) {
-  CUtensorMap ta, tb;
-  RNGD_TRY(operand_map(a, M, K, 128, &ta));
-  RNGD_TRY(operand_map(b, N, K, 128, &tb));
-  MmArgs g = {M, N, K, (K + 127) / 128, a.scale, (long)a.s0, (long)a.s1, b.scale, (long)b.s0, (long)b.s1, y, ldy, add, ldadd};
-  const long tiles = ((long)M + 127) / 128 * (((long)N + 127) / 128);
-  RNGD_REQUIRE(tiles <= 0x7FFFFFFFl, "f8_matmul: %d x %d results", M, N);
-  auto kernel = dtype == F8_BF16 ? f8_mm_kernel<F8_BF16> : dtype == F8_F16 ? f8_mm_kernel<F8_F16> : f8_mm_kernel<F8_F32>;
-  static std::atomic<unsigned long long> smem_set[3];
-  RNGD_TRY(set_smem_limit_once((const void*)kernel, kMmSmem, &smem_set[dtype], "cudaFuncSetAttribute(f8_mm_kernel)"));
-  return launch_pdl(kernel, dim3((unsigned)tiles), dim3(kMmThreads), kMmSmem, s, "f8_mm_kernel", ta, tb, g);
+// The few-row kernel's launch: y, or (b1: the second weight) q and its scales.
+template <int NT, bool DUAL, int DT>
+static int few_launch_as(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb1, const FewArgs& p,
+                         unsigned grid, cudaStream_t s) {
+  using C = FewCfg<NT, DUAL>;
+  static std::atomic<unsigned long long> smem_set{0};
+  auto kernel = f8_few_kernel<NT, DUAL, DT>;
+  RNGD_TRY(set_smem_limit_once((const void*)kernel, (int)C::SMEM, &smem_set, "cudaFuncSetAttribute(f8_few_kernel)"));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tb1, p), "f8_few_kernel");
+}
+template <int NT, bool DUAL>
+static int few_launch_nt(const Operand& a, const Operand& b, const Operand* b1, FewArgs& p, int dtype, cudaStream_t s) {
+  CUtensorMap ta, tb, tb1;
+  const MmArgs& m = p.m;
+  RNGD_TRY(operand_map(a, m.M, m.K, NT, &ta));
+  RNGD_TRY(operand_map(b, m.N, m.K, 128, &tb));
+  tb1 = tb;
+  if (DUAL) RNGD_TRY(operand_map(*b1, m.N, m.K, 128, &tb1));
+  p.tn = (m.N + 127) / 128;
+  const long tiles = (long)p.tn * ((m.M + NT - 1) / NT);
+  // as many runs of K as fill the SMs' places, none shorter than two groups
+  p.split = 1;
+  while (p.split < 8 && tiles * p.split * 2 <= (long)num_sms() * FewCfg<NT, DUAL>::PER_SM && p.split * 4 <= m.G) p.split *= 2;
+  RNGD_REQUIRE(tiles * p.split <= 0x7FFFFFFFl, "f8_matmul: %d x %d results", m.M, m.N);
+  const unsigned grid = (unsigned)(tiles * p.split);
+  if constexpr (DUAL) return few_launch_as<NT, true, F8_F32>(ta, tb, tb1, p, grid, s);
+  else {
+    if (dtype == F8_BF16) return few_launch_as<NT, false, F8_BF16>(ta, tb, tb1, p, grid, s);
+    if (dtype == F8_F16) return few_launch_as<NT, false, F8_F16>(ta, tb, tb1, p, grid, s);
+    return few_launch_as<NT, false, F8_F32>(ta, tb, tb1, p, grid, s);
+  }
+}
+static int few_launch(const Operand& a, const Operand& b, const Operand* b1, int M, int N, int K, const void* add,
+                      long ldadd, void* y, long ldy, int dtype, uint8_t* q, long ldq, float* scale, cudaStream_t s) {
+  FewArgs p = {};
+  p.m = {M, N, K, (K + 127) / 128, a.scale, (long)a.s0, (long)a.s1, b.scale, (long)b.s0, (long)b.s1, y, ldy, add, ldadd};
+  p.q = q;
+  p.ldq = ldq;
+  p.scale = scale;
+  if (b1 != nullptr) {
+    p.sb1 = b1->scale;
+    p.sb1_n = (long)b1->s0;
+    p.sb1_g = (long)b1->s1;
+    if (M <= 16) return few_launch_nt<16, true>(a, b, b1, p, dtype, s);
+    if (M <= 32) return few_launch_nt<32, true>(a, b, b1, p, dtype, s);
+    return few_launch_nt<64, true>(a, b, b1, p, dtype, s);
+  }
+  if (M <= 16) return few_launch_nt<16, false>(a, b, b1, p, dtype, s);
+  if (M <= 32) return few_launch_nt<32, false>(a, b, b1, p, dtype, s);
+  if (M <= 64) return few_launch_nt<64, false>(a, b, b1, p, dtype, s);
+  return few_launch_nt<128, false>(a, b, b1, p, dtype, s);
 }
 
 // The pairs' launch: one weight, or gate and up (b1) with the 8-bit result (q, scale).
@@ -603,6 +772,13 @@ static int pair_launch(const Operand& a, const Operand& b, const Operand* b1, in
                     ta, tb, tb1, p);
 }
 
+// Whether the pairs' tiles, 256 rows x 128 * blocks columns, are worth it.
+static bool pairs_pay(int M, int N, int blocks) {
+  static const char* e = getenv("F8_ROWS");
+  if (e) return M > atoi(e);
+  return M > 128;
+}
+
 int read_status_f8(int* st, int reset) {
   RNGD_TRY(check_cuda(cudaMemcpyFromSymbol(st, g_status_f8, sizeof(int)), "read device status"));
   if (reset) {
@@ -630,35 +806,23 @@ extern "C" int rngd_f8_matmul(const void* a, int64_t lda, const float* a_scale, 
   const Operand oa = {a, lda, a_scale, a_strides[0], a_strides[1]}, ob = {b, ldb, b_scale, b_strides[0], b_strides[1]};
   RNGD_TRY(check_operand("f8_matmul", oa, M, K));
   RNGD_TRY(check_operand("f8_matmul", ob, N, K));
-  if (M > 128)
+  if (pairs_pay(M, N, 2))
     return pair_launch(oa, ob, nullptr, M, N, K, add, (long)ldadd, y, (long)ldy, dtype, nullptr, 0, nullptr,
                        (cudaStream_t)stream);
-  return mm_launch(oa, ob, M, N, K, add, (long)ldadd, y, (long)ldy, dtype, (cudaStream_t)stream);
-}
-
-static size_t swiglu_pitch(int N) { return ((size_t)N + 3) / 4 * 4; }
-
-extern "C" int rngd_f8_swiglu_workspace(int M, int N, int K, size_t* bytes) {
-  RNGD_REQUIRE(bytes != nullptr, "f8_swiglu_workspace: null output");
-  RNGD_REQUIRE(M >= 0 && N >= 0 && K >= 1, "f8_swiglu: %d x %d x %d", M, N, K);
-  *bytes = M > 128 ? 0 : 2 * (size_t)M * swiglu_pitch(N) * 4;
-  return RNGD_OK;
+  return few_launch(oa, ob, nullptr, M, N, K, add, (long)ldadd, y, (long)ldy, dtype, nullptr, 0, nullptr,
+                    (cudaStream_t)stream);
 }
 
 extern "C" int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, const int64_t* a_strides,
                               const void* gate, int64_t ldg, const float* gate_scale, const int64_t* gate_strides,
                               const void* up, int64_t ldu, const float* up_scale, const int64_t* up_strides, int M, int N,
-                              int K, void* q, int64_t ldq, float* scale, void* workspace, size_t workspace_bytes,
-                              rngd_stream_t stream) {
-  size_t need = 0;
-  RNGD_TRY(rngd_f8_swiglu_workspace(M, N, K, &need));
+                              int K, void* q, int64_t ldq, float* scale, rngd_stream_t stream) {
+  RNGD_REQUIRE(M >= 0 && N >= 0 && K >= 1, "f8_swiglu: %d x %d x %d", M, N, K);
   RNGD_REQUIRE(K <= 0x7FFFFFFF - 127 && N <= 0x7FFFFFFF - 127, "f8_swiglu: %d x %d x %d", M, N, K);
   if (M == 0 || N == 0) return RNGD_OK;
   RNGD_REQUIRE(q && scale && a_strides && gate_strides && up_strides, "f8_swiglu: null pointer");
   RNGD_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)scale & 3) == 0 && (M <= 1 || (ldq >= N && ldq % 16 == 0)),
                "f8_swiglu: 8-bit rows must start on 16 bytes and not overlap");
-  RNGD_REQUIRE(need == 0 || (workspace != nullptr && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need),
-               "f8_swiglu: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
   const Operand oa = {a, lda, a_scale, a_strides[0], a_strides[1]};
   const Operand og = {gate, ldg, gate_scale, gate_strides[0], gate_strides[1]};
   const Operand ou = {up, ldu, up_scale, up_strides[0], up_strides[1]};
@@ -668,14 +832,6 @@ extern "C" int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, 
   if (M > 128)
     return pair_launch(oa, og, &ou, M, N, K, nullptr, 0, nullptr, 0, F8_F32, (uint8_t*)q, (long)ldq, scale,
                        (cudaStream_t)stream);
-  const long pitch = (long)swiglu_pitch(N);
-  float* g = (float*)workspace;
-  float* u = g + M * pitch;
-  cudaStream_t s = (cudaStream_t)stream;
-  RNGD_TRY(mm_launch(oa, og, M, N, K, nullptr, 0, g, pitch, F8_F32, s));
-  RNGD_TRY(mm_launch(oa, ou, M, N, K, nullptr, 0, u, pitch, F8_F32, s));
-  const int NG = (N + 127) / 128;
-  SwigluArgs w = {g, u, (int)pitch, NG, (long)M * NG, N, (uint8_t*)q, (long)ldq, scale};
-  RNGD_REQUIRE((w.total + 15) / 16 <= 0x7FFFFFFFl, "f8_swiglu: %d x %d results", M, N);
-  return launch_pdl(f8_swiglu_kernel, dim3((unsigned)((w.total + 15) / 16)), dim3(256), 0, s, "f8_swiglu_kernel", w);
+  auto launch = pairs_pay(M, N, 1) ? pair_launch : few_launch;
+  return launch(oa, og, &ou, M, N, K, nullptr, 0, nullptr, 0, F8_F32, (uint8_t*)q, (long)ldq, scale, (cudaStream_t)stream);
 }

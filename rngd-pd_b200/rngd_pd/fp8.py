@@ -180,8 +180,6 @@ def matmul_swiglu(a, a_scale, gate, gate_scale, up, up_scale):
             return matmul_swiglu(a, a_scale, gate, gate_scale, up, up_scale)
     q, ldq = _held(M, N, dev)
     scale = torch.empty((M, (N + GROUP - 1) // GROUP), dtype=_F32, device=dev)
-    need = _lib.workspace_bytes("rngd_f8_swiglu_workspace", M, N, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # held until the launches are queued
     _check(_swiglu(ap, lda, sp, ss, gp, ldg, tp, ts, up_, ldu, vp, vs, M, N, K, q.data_ptr(), ldq, scale.data_ptr(),
-                   None if ws is None else ws.data_ptr(), need, _lib.raw_stream(dev.index)))
+                   _lib.raw_stream(dev.index)))
     return q, scale

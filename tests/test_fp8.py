@@ -27,8 +27,8 @@ def test_c_entries_refuse_bad_arguments():
     def mm(a=p, lda=256, sa=p, b=p, ldb=256, M=4, N=4, K=256, add=None, y=p, ldy=4, dt=0, ss=st2):
         return lib.rngd_f8_matmul(a, lda, sa, ss, b, ldb, p, ss, M, N, K, add, 4, y, ldy, dt, None)
 
-    def sw(q=p, ldq=16, ws=p, n=1 << 20, K=256, N=4):
-        return lib.rngd_f8_swiglu(p, 256, p, st2, p, 256, p, st2, p, 256, p, st2, 4, N, K, q, ldq, p, ws, n, None)
+    def sw(q=p, ldq=16, K=256, N=4):
+        return lib.rngd_f8_swiglu(p, 256, p, st2, p, 256, p, st2, p, 256, p, st2, 4, N, K, q, ldq, p, None)
 
     bad = [
         (lambda: lib.rngd_f8_rows(p, 3, 8, 1, 8, p, 16, p, None), "data type 3"),
