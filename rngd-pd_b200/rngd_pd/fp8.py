@@ -16,6 +16,8 @@ Everything lives on the tensors' GPU; calls are queued on the current stream and
 be captured into a CUDA graph.  As with torch's own operators, a tensor made on another stream has to be
 ordered before the call by the caller (and kept alive with record_stream).  Nothing falls back to the CPU.
 """
+import functools
+
 import torch
 
 from rngd_pd import _lib
@@ -25,80 +27,134 @@ GROUP = 128  # values that share a scale
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _E4M3 = torch.float8_e4m3fn
 _F32 = torch.float32
+_empty = torch.empty_strided  # half of torch.empty's time on the host
 _INT_MAX = 2 ** 31 - GROUP
 _check = _lib.check
 _rows, _weight, _norm = _lib.lib.rngd_f8_rows, _lib.lib.rngd_f8_weight, _lib.lib.rngd_f8_rms_norm
 _matmul, _swiglu = _lib.lib.rngd_f8_matmul, _lib.lib.rngd_f8_swiglu
 
 
+# The operators are called hundreds of times a step, and small ones take less time on the GPU than a call's checks on
+# the host.  So what depends on shapes, strides and types alone is checked once for each set of them.
+
 def _elsewhere(dev):
     """Whether another GPU than the tensors' is current (the calls below then start over with theirs)."""
     return dev.index != torch.cuda.current_device()
 
 
-def _matrix(name, x, dev=None, shape=None, dtype=None):
+def _key(t):
+    return t.shape, t.stride(), t.dtype, t.device
+
+
+def _matrix(name, shape, strides, dtype, dev):
     """Row stride of a matrix of bfloat16, float16 or float32 whose rows are contiguous."""
-    if x.dim() != 2 or x.dtype not in _DT or not x.is_cuda or (x.shape[1] > 1 and x.stride(1) != 1):
+    if len(shape) != 2 or dtype not in _DT or dev.type != "cuda" or (shape[1] > 1 and strides[1] != 1):
         raise ValueError(f"{name} must be a CUDA matrix of bfloat16, float16 or float32 with contiguous rows, got "
-                         f"{tuple(x.shape)} {x.dtype} strides {x.stride()} on {x.device}")
-    if dev is not None and (x.device != dev or x.shape != shape or x.dtype is not dtype):
-        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
-    return x.stride(0)
+                         f"{tuple(shape)} {dtype} strides {strides} on {dev}")
+    return strides[0]
 
 
-def _held(rows, K, dev):
-    """Room for rows of K 8-bit values that start on 16 bytes, and the bytes between them."""
-    if K % 16 == 0:
-        return torch.empty((rows, K), dtype=_E4M3, device=dev), K
-    wide = (K + 15) // 16 * 16
-    return torch.empty((rows, wide), dtype=_E4M3, device=dev)[:, :K], wide
+def _like(name, shape, strides, dtype, dev, want, want_dtype, want_dev):
+    """Row stride of a matrix that has to be of this shape and type."""
+    if shape != want or dtype is not want_dtype or dev != want_dev:
+        raise ValueError(f"{name} must be {tuple(want)} {want_dtype} on {want_dev}, got {tuple(shape)} {dtype} on {dev}")
+    return _matrix(name, shape, strides, dtype, dev)
 
 
-def _operand(name, q, scale, blocks, dev=None, K=None):
-    """(pointer, row stride, pointer of the scales, their strides) of 8-bit rows or, with `blocks`, of a weight."""
-    if q.dim() != 2 or q.dtype is not _E4M3 or not q.is_cuda or (dev is not None and q.device != dev):
-        raise ValueError(f"{name} must be a float8_e4m3fn matrix on {dev or 'a GPU'}, got {tuple(q.shape)} {q.dtype} on "
-                         f"{q.device}")
-    n, k = q.shape
-    if K is not None and k != K:
-        raise ValueError(f"{name} {tuple(q.shape)}: rows of {K} values are needed")
-    ld = q.stride(0)
-    if (k > 1 and q.stride(1) != 1) or q.data_ptr() % 16 or (n > 1 and (ld % 16 or ld < k)):
-        raise ValueError(f"{name} {tuple(q.shape)} strides {q.stride()}: rows must be contiguous, start on 16 bytes and "
-                         "not overlap")
-    want = ((n + GROUP - 1) // GROUP if blocks else n, (k + GROUP - 1) // GROUP)
-    if scale.shape != want or scale.dtype is not _F32 or scale.device != q.device:
-        raise ValueError(f"{name}'s scale must be float32 {want} on {q.device}, got {tuple(scale.shape)} {scale.dtype} on "
-                         f"{scale.device}")
-    return q.data_ptr(), ld, scale.data_ptr(), _lib.i64_array(scale.stride())
+def _groups(n):
+    return (n + GROUP - 1) // GROUP
+
+
+@functools.lru_cache(maxsize=4096)
+def _source(name, shape, strides, dtype, dev):
+    """What quantize and the others take from their input: (row stride, type's number, sizes, the 8-bit rows' strides)."""
+    ld = _matrix(name, shape, strides, dtype, dev)
+    return ld, _DT[dtype], shape[0], shape[1], ((shape[1] + 15) // 16 * 16, 1)
+
+
+def _operand(name, q, scale, blocks):
+    """(n, k, row stride, strides of the scales) of 8-bit rows or, with `blocks`, of a weight, given as _key()s."""
+    shape, strides, dtype, dev = q
+    if len(shape) != 2 or dtype is not _E4M3 or dev.type != "cuda":
+        raise ValueError(f"{name} must be a float8_e4m3fn CUDA matrix, got {tuple(shape)} {dtype} on {dev}")
+    n, k = shape
+    ld = strides[0]
+    if (k > 1 and strides[1] != 1) or (n > 1 and (ld % 16 or ld < k)):
+        raise ValueError(f"{name} {tuple(shape)} strides {strides}: rows must be contiguous, start on 16 bytes and not "
+                         "overlap")
+    if k == 0 or k > _INT_MAX:
+        raise ValueError(f"{name} {tuple(shape)}: nothing to sum, or too much")
+    want = (_groups(n) if blocks else n, _groups(k))
+    if scale[0] != want or scale[2] is not _F32 or scale[3] != dev:
+        raise ValueError(f"{name}'s scale must be float32 {want} on {dev}, got {tuple(scale[0])} {scale[2]} on {scale[3]}")
+    return n, k, ld, _lib.i64_array(scale[1])
+
+
+def _against(name, a, b, b_scale):
+    """_operand() of a weight that rows `a` (a _key()) are multiplied with."""
+    n, k, ld, st = _operand(name, b, b_scale, True)
+    if k != a[0][1] or b[3] != a[3]:
+        raise ValueError(f"{name} {tuple(b[0])} on {b[3]}: rows of {a[0][1]} values on {a[3]} are needed")
+    return n, ld, st
+
+
+@functools.lru_cache(maxsize=4096)
+def _product(dtype, a, a_scale, b, b_scale, add, out):
+    M, K, lda, ast = _operand("a", a, a_scale, False)
+    N, ldb, bst = _against("b", a, b, b_scale)
+    if dtype not in _DT:
+        raise ValueError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+    dev, shape = a[3], (M, N)
+    ldadd = 0 if add is None else _like("add", *add, shape, dtype, dev)
+    ldo = N if out is None else _like("out", *out, shape, dtype, dev)
+    if M > 1 and ldo < N:
+        raise ValueError(f"out {shape} strides {out[1]}: rows lie on one another")
+    return M, N, K, lda, ast, ldb, bst, ldadd, ldo, _DT[dtype], shape, (N, 1)
+
+
+@functools.lru_cache(maxsize=4096)
+def _gated(a, a_scale, gate, gate_scale, up, up_scale):
+    M, K, lda, ast = _operand("a", a, a_scale, False)
+    N, ldg, gst = _against("gate", a, gate, gate_scale)
+    n, ldu, ust = _against("up", a, up, up_scale)
+    if n != N:
+        raise ValueError(f"gate {tuple(gate[0])} and up {tuple(up[0])} must be of one shape")
+    return M, N, K, lda, ast, ldg, gst, ldu, ust, (M, N), ((N + 15) // 16 * 16, 1), (M, _groups(N)), (_groups(N), 1)
+
+
+def _start(name, q):
+    p = q.data_ptr()
+    if p % 16:
+        raise ValueError(f"{name} must start on 16 bytes")
+    return p
 
 
 def quantize(x):
     """Rows in 8 bits: x [T, K] bfloat16, float16 or float32 (rows contiguous) -> (q [T, K], scale [T, G])."""
-    ld = _matrix("x", x)
     dev = x.device
-    T, K = x.shape
+    ld, dt, T, K, st = _source("x", x.shape, x.stride(), x.dtype, dev)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return quantize(x)
-    q, ldq = _held(T, K, dev)
-    scale = torch.empty((T, (K + GROUP - 1) // GROUP), dtype=_F32, device=dev)
-    _check(_rows(x.data_ptr(), _DT[x.dtype], ld, T, K, q.data_ptr(), ldq, scale.data_ptr(), _lib.raw_stream(dev.index)))
+    G = _groups(K)
+    q = _empty((T, K), st, dtype=_E4M3, device=dev)
+    scale = _empty((T, G), (G, 1), dtype=_F32, device=dev)
+    _check(_rows(x.data_ptr(), dt, ld, T, K, q.data_ptr(), st[0], scale.data_ptr(), _lib.raw_stream(dev.index)))
     return q, scale
 
 
 def quantize_weight(w):
     """A weight in 8 bits: w [N, K] bfloat16, float16 or float32 (rows contiguous) -> (q [N, K], scale
     [ceil(N / 128), G])."""
-    ld = _matrix("w", w)
     dev = w.device
-    N, K = w.shape
+    ld, dt, N, K, st = _source("w", w.shape, w.stride(), w.dtype, dev)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return quantize_weight(w)
-    q, ldq = _held(N, K, dev)
-    scale = torch.empty(((N + GROUP - 1) // GROUP, (K + GROUP - 1) // GROUP), dtype=_F32, device=dev)
-    _check(_weight(w.data_ptr(), _DT[w.dtype], ld, N, K, q.data_ptr(), ldq, scale.data_ptr(), _lib.raw_stream(dev.index)))
+    G = _groups(K)
+    q = _empty((N, K), st, dtype=_E4M3, device=dev)
+    scale = _empty((_groups(N), G), (G, 1), dtype=_F32, device=dev)
+    _check(_weight(w.data_ptr(), dt, ld, N, K, q.data_ptr(), st[0], scale.data_ptr(), _lib.raw_stream(dev.index)))
     return q, scale
 
 
@@ -108,27 +164,27 @@ def rms_norm(x, weight, eps, residual=None):
     x, residual: [T, K] of one type (rows contiguous); weight: [K] of that type or float32.  total = x + residual
     rounded to their type, the residual stream as it goes on (None without a residual); the norm is of the rounded
     sum, total / sqrt(mean(total^2) + eps) * weight, worked out in fp32 and rounded to 8 bits alone."""
-    ld = _matrix("x", x)
-    dev, dt = x.device, x.dtype
-    T, K = x.shape
-    if weight.shape != (K,) or (weight.dtype is not dt and weight.dtype is not _F32) or weight.device != dev or \
-            not weight.is_contiguous():
-        raise ValueError(f"weight must be a contiguous {dt} or float32 [{K}] tensor on {dev}, got {tuple(weight.shape)} "
-                         f"{weight.dtype} on {weight.device}")
+    dev, dtype = x.device, x.dtype
+    ld, dt, T, K, st = _source("x", x.shape, x.stride(), dtype, dev)
+    wt = weight.dtype
+    if weight.shape != (K,) or (wt is not dtype and wt is not _F32) or weight.device != dev or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous {dtype} or float32 [{K}] tensor on {dev}, got "
+                         f"{tuple(weight.shape)} {wt} on {weight.device}")
     if residual is not None:
-        ldr = _matrix("residual", residual, dev, x.shape, dt)
+        ldr = _like("residual", residual.shape, residual.stride(), residual.dtype, residual.device, x.shape, dtype, dev)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return rms_norm(x, weight, eps, residual)
-    q, ldq = _held(T, K, dev)
-    scale = torch.empty((T, (K + GROUP - 1) // GROUP), dtype=_F32, device=dev)
+    G = _groups(K)
+    q = _empty((T, K), st, dtype=_E4M3, device=dev)
+    scale = _empty((T, G), (G, 1), dtype=_F32, device=dev)
     if residual is None:
         total, r, t, ldr = None, None, None, 0
     else:
-        total = torch.empty((T, K), dtype=dt, device=dev)
+        total = _empty((T, K), (K, 1), dtype=dtype, device=dev)
         r, t = residual.data_ptr(), total.data_ptr()
-    _check(_norm(x.data_ptr(), ld, r, ldr, weight.data_ptr(), _DT[dt], _DT[weight.dtype], T, K, eps, t, K,
-                 q.data_ptr(), ldq, scale.data_ptr(), _lib.raw_stream(dev.index)))
+    _check(_norm(x.data_ptr(), ld, r, ldr, weight.data_ptr(), dt, _DT[wt], T, K, eps, t, K, q.data_ptr(), st[0],
+                 scale.data_ptr(), _lib.raw_stream(dev.index)))
     return q, scale, total
 
 
@@ -138,48 +194,31 @@ def matmul(a, a_scale, b, b_scale, dtype=torch.bfloat16, add=None, out=None):
     Sums are held in fp32, `add` ([M, N] of `dtype`, rows contiguous) is added there, and the result is rounded once
     to `dtype` (bfloat16, float16 or float32).  out: [M, N] of `dtype`, rows contiguous; it may be `add` itself, but
     must not overlap it in part, nor the operands."""
-    ap, lda, sp, ss = _operand("a", a, a_scale, False)
-    dev = a.device
-    M, K = a.shape
-    bp, ldb, tp, ts = _operand("b", b, b_scale, True, dev, K)
-    N = b.shape[0]
-    if dtype not in _DT:
-        raise ValueError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-    if K == 0 or K > _INT_MAX:
-        raise ValueError(f"a {tuple(a.shape)}: nothing to sum, or too much")
-    p, lda_ = (None, 0) if add is None else (add.data_ptr(), _matrix("add", add, dev, (M, N), dtype))
+    M, N, K, lda, ast, ldb, bst, ldadd, ldo, dt, shape, st = _product(
+        dtype, _key(a), _key(a_scale), _key(b), _key(b_scale), None if add is None else _key(add),
+        None if out is None else _key(out))
+    ap, bp, dev = _start("a", a), _start("b", b), a.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return matmul(a, a_scale, b, b_scale, dtype, add, out)
     if out is None:
-        out, ldo = torch.empty((M, N), dtype=dtype, device=dev), N
-    else:
-        ldo = _matrix("out", out, dev, (M, N), dtype)
-        if M > 1 and ldo < N:
-            raise ValueError(f"out {tuple(out.shape)} strides {out.stride()}: rows lie on one another")
-    _check(_matmul(ap, lda, sp, ss, bp, ldb, tp, ts, M, N, K, p, lda_, out.data_ptr(), ldo, _DT[dtype],
-                   _lib.raw_stream(dev.index)))
+        out = _empty(shape, st, dtype=dtype, device=dev)
+    _check(_matmul(ap, lda, a_scale.data_ptr(), ast, bp, ldb, b_scale.data_ptr(), bst, M, N, K,
+                   None if add is None else add.data_ptr(), ldadd, out.data_ptr(), ldo, dt, _lib.raw_stream(dev.index)))
     return out
 
 
 def matmul_swiglu(a, a_scale, gate, gate_scale, up, up_scale):
     """silu(a gate^T) * (a up^T) of 8-bit rows a [M, K] and 8-bit weights gate, up [N, K], in 8 bits again:
     (q [M, N], scale [M, ceil(N / 128)]), what the down projection takes.  Nothing is rounded in between."""
-    ap, lda, sp, ss = _operand("a", a, a_scale, False)
-    dev = a.device
-    M, K = a.shape
-    gp, ldg, tp, ts = _operand("gate", gate, gate_scale, True, dev, K)
-    up_, ldu, vp, vs = _operand("up", up, up_scale, True, dev, K)
-    N = gate.shape[0]
-    if up.shape[0] != N:
-        raise ValueError(f"gate {tuple(gate.shape)} and up {tuple(up.shape)} must be of one shape")
-    if K == 0 or K > _INT_MAX:
-        raise ValueError(f"a {tuple(a.shape)}: nothing to sum, or too much")
+    M, N, K, lda, ast, ldg, gst, ldu, ust, shape, st, s_shape, s_st = _gated(
+        _key(a), _key(a_scale), _key(gate), _key(gate_scale), _key(up), _key(up_scale))
+    ap, gp, up_, dev = _start("a", a), _start("gate", gate), _start("up", up), a.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return matmul_swiglu(a, a_scale, gate, gate_scale, up, up_scale)
-    q, ldq = _held(M, N, dev)
-    scale = torch.empty((M, (N + GROUP - 1) // GROUP), dtype=_F32, device=dev)
-    _check(_swiglu(ap, lda, sp, ss, gp, ldg, tp, ts, up_, ldu, vp, vs, M, N, K, q.data_ptr(), ldq, scale.data_ptr(),
-                   _lib.raw_stream(dev.index)))
+    q = _empty(shape, st, dtype=_E4M3, device=dev)
+    scale = _empty(s_shape, s_st, dtype=_F32, device=dev)
+    _check(_swiglu(ap, lda, a_scale.data_ptr(), ast, gp, ldg, gate_scale.data_ptr(), gst, up_, ldu, up_scale.data_ptr(),
+                   ust, M, N, K, q.data_ptr(), st[0], scale.data_ptr(), _lib.raw_stream(dev.index)))
     return q, scale
