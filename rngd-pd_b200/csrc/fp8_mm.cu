@@ -440,7 +440,7 @@ __device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* ac
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += w[e];
       }
-      store_eight<DT>(a.y, o + 8 * j, v);
+      store_eight<DT>(a.y, o + 8 * j, eight_of<DT>(v));
     }
     return;
   }
