@@ -115,6 +115,19 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -161,10 +174,14 @@ template <int NT, bool DUAL>
 struct FewCfg {
   static constexpr int A = (DUAL ? 2 : 1) * kMmTile, STAGE = A + NT * 128;
   static constexpr int COLS = (DUAL ? 2 : 1) * NT;     // columns of one buffer in tensor memory
+  static constexpr int GROUPS = NT >= 64 ? 2 : 1;      // warpgroups that share them, by rows of a
+  static constexpr int SUMMERS = 128 * GROUPS, THREADS = 64 + SUMMERS, TN = NT / GROUPS;
+  static constexpr int STEP = NT == 16 || NT == 64 ? 16 : 32;  // columns read at a time (32 spill registers with 64)
   static constexpr int BUFS = NT <= 32 ? 4 : 2;
   static constexpr int CHUNK = 32;                     // groups whose scales are in shared memory
-  static constexpr int SCALES = CHUNK * COLS * 4;
-  static constexpr int FIXED = 1024 + SCALES + 4 * NT * 4 + 256;
+  static constexpr int PITCH = COLS + 4;               // floats of a group's; fewer of the stores' banks meet
+  static constexpr int SCALES = CHUNK * PITCH * 4;
+  static constexpr int FIXED = 1024 + SCALES + 256;
   // two CTAs an SM where three stages of each fit (an SM has 227 KB, a block's own KB taken off), else one
   static constexpr int PER_SM = (113 * 1024 - FIXED) / STAGE >= 3 ? 2 : 1;
   static constexpr int MOST = ((PER_SM == 2 ? 113 : 226) * 1024 - FIXED) / STAGE;
@@ -179,28 +196,76 @@ struct FewArgs {
   const float* sb1;  // of the second weight (DUAL)
   long sb1_n, sb1_g;
   int tn, split;
+  int vec;           // rows of y and add are whole 16-byte vectors
   uint8_t* q;        // DUAL: 8-bit rows and their scales [M][ceil(N / 128)]
   long ldq;
   float* scale;
 };
-constexpr int kFewThreads = 192;
-
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+// Eight neighbouring sums at this place of each CTA of the cluster, added in the CTAs' order.
+__device__ __forceinline__ void few_sum(float* y, uint32_t at, int split) {
+  float4 v[8][2];
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    v[k][0] = v[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (k < split) {
+      const uint32_t from = mapa(at, k);
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[k][c].x), "=f"(v[k][c].y), "=f"(v[k][c].z), "=f"(v[k][c].w)
+                     : "r"(from + 16 * c));
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; c++) {
+    float* z = y + 4 * c;
+    z[0] = z[1] = z[2] = z[3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      z[0] += v[k][c].x;
+      z[1] += v[k][c].y;
+      z[2] += v[k][c].z;
+      z[3] += v[k][c].w;
+    }
+  }
 }
-__device__ __forceinline__ void few_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// Eight sums of row m from column n on: plus add, rounded, stored.
+template <int DT>
+__device__ __forceinline__ void store_sums(const MmArgs& a, float* v, long m, int n, int vec) {
+  const long o = m * a.ldy + n, oa = m * a.ldadd + n;
+  if (vec && n + 8 <= a.N) {
+    if (a.add != nullptr) {
+      Eight<DT> r;
+      float w[8];
+      r.load_any(a.add, oa);
+      r.values(w);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += w[e];
+    }
+    store_eight<DT>(a.y, o, eight_of<DT>(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (n + e < a.N) store_f32_as<DT>(a.y, o + e, a.add != nullptr ? v[e] + load_as_f32<DT>(a.add, oa + e) : v[e]);
+  }
+}
+template <int THREADS>
+__device__ __forceinline__ void few_bar() {
+  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
 
 // acc[0 .. N / 2) += (N columns from taddr) * s[0 .. N), two columns an instruction
-template <int N>
+template <int N, int STEP>
 __device__ __forceinline__ void scale_add_cols(uint64_t* acc, uint32_t taddr, const float* s) {
 #pragma unroll
-  for (int c = 0; c < N; c += 16) {
-    uint32_t r[16];
-    tmem_ld_x16(taddr + c, r);
+  for (int c = 0; c < N; c += STEP) {
+    uint32_t r[STEP];
+    if constexpr (STEP == 16)
+      tmem_ld_x16(taddr + c, r);
+    else
+      tmem_ld_x32(taddr + c, r);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < STEP / 4; j++) {
       const ulonglong2 f = *(const ulonglong2*)(s + c + 4 * j);
       const uint64_t v0 = pair_of(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]));
       const uint64_t v1 = pair_of(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
@@ -211,16 +276,15 @@ __device__ __forceinline__ void scale_add_cols(uint64_t* acc, uint32_t taddr, co
 }
 
 template <int NT, bool DUAL, int DT>
-__global__ void __launch_bounds__(kFewThreads, FewCfg<NT, DUAL>::PER_SM)
+__global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::PER_SM)
     f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                   const __grid_constant__ CUtensorMap tmW1, FewArgs p) {
   using C = FewCfg<NT, DUAL>;
   constexpr int ST = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* s_scale = (float*)(base + ST * C::STAGE);   // [CHUNK][COLS]
-  float* s_red = s_scale + C::CHUNK * C::COLS;       // [NT][4]
-  uint64_t* full = (uint64_t*)(s_red + 4 * NT);
+  float* s_scale = (float*)(base + ST * C::STAGE);   // [CHUNK][PITCH]
+  uint64_t* full = (uint64_t*)(s_scale + C::CHUNK * C::PITCH);
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;           // [BUFS]
   uint64_t* acc_empty = acc_full + C::BUFS;  // [BUFS]
@@ -238,9 +302,9 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<NT, DUAL>::PER_SM)
     }
     for (int i = 0; i < C::BUFS; i++) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4);
+      mbar_init(&acc_empty[i], C::SUMMERS / 32);
     }
-    mbar_init(done, 4);
+    mbar_init(done, C::SUMMERS / 32);
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
@@ -302,99 +366,102 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<NT, DUAL>::PER_SM)
     __syncwarp();
     tmem_dealloc(tmem, C::BUFS * C::COLS);
   } else {
-    const int r = ((warp & 3) << 5) | lane, et = threadIdx.x - 64;
+    // thread: row r of the weight's 128, rows wt .. wt + TN - 1 of a's NT
+    constexpr int TN = C::TN;
+    const int r = ((warp & 3) << 5) | lane, et = threadIdx.x - 64, wt = (et >> 7) * TN;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    uint64_t acc[C::COLS / 2];
+    uint64_t acc[(DUAL ? 2 : 1) * TN / 2];
 #pragma unroll
-    for (int j = 0; j < C::COLS / 2; j++) acc[j] = 0ull;
+    for (int j = 0; j < (DUAL ? 2 : 1) * TN / 2; j++) acc[j] = 0ull;
     bool ok = true;
     for (int c0 = g0; c0 < g1; c0 += C::CHUNK) {
       const int n = min(C::CHUNK, g1 - c0);
-      if (c0 != g0) few_bar();  // every warp is past the previous scales
-      for (int e = et; e < n * NT; e += 128) {
-        const int t = e / n, g = c0 + e - t * n, m = mt * NT + t;  // neighbouring threads: groups of one row
-        const float x = m < a.M ? __ldg(a.sa + m * a.sa_m + g * a.sa_g) : 0.f;
-        s_scale[(g - c0) * C::COLS + t] = x * __ldg(a.sb + nt * a.sb_n + g * a.sb_g);
-        if (DUAL) s_scale[(g - c0) * C::COLS + NT + t] = x * __ldg(p.sb1 + nt * p.sb1_n + g * p.sb1_g);
+      if (c0 != g0) few_bar<C::SUMMERS>();  // every warp is past the previous scales
+      // a row's scales by neighbouring threads, eight loads a thread at a time, so that their latencies overlap
+      for (int e0 = et; e0 < NT * C::CHUNK; e0 += 8 * C::SUMMERS) {
+        const int g = et % C::CHUNK, gg = c0 + min(g, n - 1);
+        const float b = __ldg(a.sb + nt * a.sb_n + gg * a.sb_g), b1 = DUAL ? __ldg(p.sb1 + nt * p.sb1_n + gg * p.sb1_g) : 0.f;
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const int t = (e0 + u * C::SUMMERS) / C::CHUNK, m = mt * NT + t;
+          x[u] = t < NT && m < a.M ? __ldg(a.sa + m * a.sa_m + gg * a.sa_g) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const int t = (e0 + u * C::SUMMERS) / C::CHUNK;
+          if (t < NT) {
+            s_scale[g * C::PITCH + t] = x[u] * b;
+            if (DUAL) s_scale[g * C::PITCH + NT + t] = x[u] * b1;
+          }
+        }
       }
-      few_bar();
+      few_bar<C::SUMMERS>();
       for (int k = 0; k < n; k++) {
         const int i = c0 - g0 + k, buf = i % C::BUFS;
         if (ok) ok = mbar_wait(&acc_full[buf], (uint32_t)(i / C::BUFS) & 1u, ST_EPI_WAIT, &g_status_f8);
         __syncwarp();
         tc_fence_after();
-        scale_add_cols<C::COLS>(acc, tmem + lane_base + (uint32_t)(buf * C::COLS), s_scale + k * C::COLS);
+        const uint32_t d = tmem + lane_base + (uint32_t)(buf * C::COLS + wt);
+        const float* s = s_scale + k * C::PITCH + wt;
+        scale_add_cols<TN, C::STEP>(acc, d, s);
+        if (DUAL) scale_add_cols<TN, C::STEP>(acc + TN / 2, d + NT, s + NT);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[buf]);
       }
     }
     if (lane == 0) mbar_arrive(done);
-    const int n = nt * 128 + r;
-    if (p.split == 1 && !DUAL) {
+    float* part = (float*)base;  // [COLS][128]: the stages are done with
+    few_bar<C::SUMMERS>();       // (every warp has seen the last products)
 #pragma unroll
-      for (int t = 0; t < NT; t++) {
-        const int m = mt * NT + t;
-        if (m < a.M && n < a.N && ok) {
-          const float2 v = parts_of(acc[t / 2]);
-          const float y = t & 1 ? v.y : v.x;
-          store_f32_as<DT>(a.y, m * a.ldy + n, a.add != nullptr ? y + load_as_f32<DT>(a.add, m * a.ldadd + n) : y);
-        }
-      }
-    } else {
-      float* part = (float*)base;  // [COLS][128]: the stages are done with
-      few_bar();                   // (every warp has seen the last products)
-#pragma unroll
-      for (int j = 0; j < C::COLS / 2; j++) {
-        const float2 v = parts_of(acc[j]);
-        part[(2 * j) * 128 + r] = v.x;
-        part[(2 * j + 1) * 128 + r] = v.y;
-      }
+    for (int j = 0; j < (DUAL ? 2 : 1) * TN / 2; j++) {
+      const float2 v = parts_of(acc[j]);
+      const int c = wt + 2 * j + (DUAL && j >= TN / 2 ? NT - TN : 0);
+      part[c * 128 + r] = v.x;
+      part[(c + 1) * 128 + r] = v.y;
     }
-    if (!ok && lane == 0) atomicCAS(&g_status_f8, 0, ST_EPI_WAIT);
   }
-  if (p.split == 1 && !DUAL) return;
   if (p.split > 1)
     cluster_sync();
   else if (warp >= 2)
-    few_bar();
+    few_bar<C::SUMMERS>();
   if (warp >= 2) {
-    // this CTA's rows of a: their sums over the cluster, the result
-    const int r = ((warp & 3) << 5) | lane, n = nt * 128 + r;
-    float* part = (float*)base;
+    // This CTA's rows of a: their sums over the cluster, in the order of the runs, and the result.  16 threads have a
+    // row's 128 columns, eight each.  (A short loop: code that runs once costs its way from memory.)
+    const int et = threadIdx.x - 64, l = et & 15, n = nt * 128 + 8 * l;
     const int t0 = NT * rank / p.split, t1 = min(NT * (rank + 1) / p.split, a.M - mt * NT);
-    const uint32_t at = smem_u32(part + r);
-    auto sum = [&](int c) {
-      if (p.split == 1) return part[c * 128 + r];
-      float v = 0.f;
-      for (int k = 0; k < p.split; k++) v += ld_cluster(mapa(at + c * 512, k));
-      return v;
-    };
-    if constexpr (!DUAL) {
-      for (int t = t0; t < t1; t++) {
-        const int m = mt * NT + t;
-        const float y = sum(t);
-        if (n < a.N)
-          store_f32_as<DT>(a.y, m * a.ldy + n, a.add != nullptr ? y + load_as_f32<DT>(a.add, m * a.ldadd + n) : y);
-      }
-    } else {
-      // the values go back to this CTA's own place, which no other reads
-      for (int t = t0; t < t1; t++) {
-        const float g = sum(t), u = sum(NT + t);
-        const float v = n < a.N ? swiglu(g, u) : 0.f;
-        float most = fabsf(v);
+    const uint32_t at = smem_u32(base) + l * 32;
+    for (int tb = t0; tb < t1; tb += C::SUMMERS / 16) {
+      const int t = tb + (et >> 4);
+      const bool there = t < t1;
+      const long m = mt * NT + t;
+      float y[8], u[8];
+      few_sum(y, at + (there ? t : t0) * 512, p.split);
+      if constexpr (DUAL) {
+        few_sum(u, at + (NT + (there ? t : t0)) * 512, p.split);
+        float most = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-        part[t * 128 + r] = v;
-        if (lane == 0) s_red[t * 4 + (warp & 3)] = most;
-      }
-      few_bar();
-      for (int t = t0; t < t1; t++) {
-        const int m = mt * NT + t;
-        const float4 w = *(const float4*)(s_red + t * 4);
-        const float lim = held_max(max_nan(max_nan(w.x, w.y), max_nan(w.z, w.w))), inv = 448.0f / lim;
-        if (n < a.N) p.q[m * p.ldq + n] = e4m3(part[t * 128 + r] * inv);
-        if (r == 0) p.scale[(long)m * p.tn + nt] = lim / 448.0f;
+        for (int e = 0; e < 8; e++) {
+          y[e] = n + e < a.N ? swiglu(y[e], u[e]) : 0.f;
+          most = max_nan(most, fabsf(y[e]));
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float lim = held_max(most), inv = 448.0f / lim;
+        if (there) {
+          uint8_t* q = p.q + m * p.ldq + n;
+          if (n + 8 <= a.N) {
+            *(uint2*)q = held8(y, inv);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              if (n + e < a.N) q[e] = e4m3(y[e] * inv);
+          }
+          if (l == 0) p.scale[m * p.tn + nt] = lim / 448.0f;
+        }
+      } else if (there) {
+        store_sums<DT>(a, y, m, n, p.vec);
       }
     }
   }
@@ -417,44 +484,6 @@ struct PairArgs {
 };
 constexpr int kPairStages = 6, kPairStage = 2 * kMmTile, kPairThreads = 128 + 256;
 constexpr size_t kPairSmem = 1024 + kPairStages * kPairStage + (2 * kPairStages + 4) * 8 + 16 + 2 * 2 * 128 * 4;
-
-// 128 sums of row m from column n0 on: plus add, rounded, stored.
-template <int DT>
-__device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* acc, int m, int n0) {
-  const MmArgs& a = p.m;
-  const long o = m * a.ldy + n0, oa = m * a.ldadd + n0;
-  if (p.vec && n0 + 128 <= a.N) {
-#pragma unroll
-    for (int j = 0; j < 16; j++) {
-      float v[8], w[8];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float2 x = parts_of(acc[4 * j + e]);
-        v[2 * e] = x.x;
-        v[2 * e + 1] = x.y;
-      }
-      if (a.add != nullptr) {
-        Eight<DT> r;
-        r.load_any(a.add, oa + 8 * j);
-        r.values(w);
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += w[e];
-      }
-      store_eight<DT>(a.y, o + 8 * j, eight_of<DT>(v));
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 64; j++) {
-    const float2 x = parts_of(acc[j]);
-    const float v[2] = {x.x, x.y};
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int c = 2 * j + e;
-      if (n0 + c < a.N) store_f32_as<DT>(a.y, o + c, a.add != nullptr ? v[e] + load_as_f32<DT>(a.add, oa + c) : v[e]);
-    }
-  }
-}
 
 // 64 gate sums and 64 up sums of row m, columns n0 ..: the other 64 of the group are another warp's, so the maximum
 // meets in shared memory.
@@ -639,7 +668,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (SWIGLU) {
         pair_store_swiglu(p, acc, m, row && ok, nt * 128 + 64 * h, nt, h, r, warp & 3, s_amax + (round & 1) * 256);
       } else if (row && ok) {
-        pair_store<DT>(p, acc, m, nt * 256 + 128 * h);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float2 x = parts_of(acc[4 * j + e]);
+            v[2 * e] = x.x;
+            v[2 * e + 1] = x.y;
+          }
+          store_sums<DT>(a, v, m, nt * 256 + 128 * h + 8 * j, p.vec);
+        }
       }
     }
   }
@@ -671,6 +710,11 @@ static int operand_map(const Operand& o, long rows, int K, int box, CUtensorMap*
   return encode_tmap_u8(out, o.q, 2, dims, strides, bx);
 }
 
+static int whole_rows(const void* y, long ldy, const void* add, long ldadd, int dtype) {
+  const int sz = dtype == F8_F32 ? 4 : 2;
+  return (((uintptr_t)y | (uintptr_t)add) & 15) == 0 && ldy * sz % 16 == 0 && ldadd * sz % 16 == 0;
+}
+
 // The few-row kernel's launch: y, or (b1: the second weight) q and its scales.
 template <int NT, bool DUAL, int DT>
 static int few_launch_as(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb1, const FewArgs& p,
@@ -681,7 +725,7 @@ static int few_launch_as(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
   RNGD_TRY(set_smem_limit_once((const void*)kernel, (int)C::SMEM, &smem_set, "cudaFuncSetAttribute(f8_few_kernel)"));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kFewThreads);
+  cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -704,9 +748,9 @@ static int few_launch_nt(const Operand& a, const Operand& b, const Operand* b1, 
   if (DUAL) RNGD_TRY(operand_map(*b1, m.N, m.K, 128, &tb1));
   p.tn = (m.N + 127) / 128;
   const long tiles = (long)p.tn * ((m.M + NT - 1) / NT);
-  // as many runs of K as fill the SMs' places, none shorter than two groups
+  // as many runs of K as fill the SMs' places, none shorter than four groups
   p.split = 1;
-  while (p.split < 8 && tiles * p.split * 2 <= (long)num_sms() * FewCfg<NT, DUAL>::PER_SM && p.split * 4 <= m.G) p.split *= 2;
+  while (p.split < 8 && tiles * p.split * 2 <= (long)num_sms() * FewCfg<NT, DUAL>::PER_SM && p.split * 8 <= m.G) p.split *= 2;
   RNGD_REQUIRE(tiles * p.split <= 0x7FFFFFFFl, "f8_matmul: %d x %d results", m.M, m.N);
   const unsigned grid = (unsigned)(tiles * p.split);
   if constexpr (DUAL) return few_launch_as<NT, true, F8_F32>(ta, tb, tb1, p, grid, s);
@@ -720,6 +764,7 @@ static int few_launch(const Operand& a, const Operand& b, const Operand* b1, int
                       long ldadd, void* y, long ldy, int dtype, uint8_t* q, long ldq, float* scale, cudaStream_t s) {
   FewArgs p = {};
   p.m = {M, N, K, (K + 127) / 128, a.scale, (long)a.s0, (long)a.s1, b.scale, (long)b.s0, (long)b.s1, y, ldy, add, ldadd};
+  p.vec = whole_rows(y, ldy, add, ldadd, dtype);
   p.q = q;
   p.ldq = ldq;
   p.scale = scale;
@@ -755,8 +800,7 @@ static int pair_launch(const Operand& a, const Operand& b, const Operand* b1, in
   p.tm = (M + 255) / 256;
   p.tn = b1 != nullptr ? (N + 127) / 128 : (N + 255) / 256;
   RNGD_REQUIRE((long)p.tm * p.tn <= 0x7FFFFFFFl / 2, "f8_matmul: %d x %d results", M, N);
-  const int sz = dtype == F8_F32 ? 4 : 2;
-  p.vec = ((uintptr_t)y & 15) == 0 && ldy * sz % 16 == 0 && ((uintptr_t)add & 15) == 0 && ldadd * sz % 16 == 0;
+  p.vec = whole_rows(y, ldy, add, ldadd, dtype);
   p.q = q;
   p.ldq = ldq;
   p.scale = scale;
@@ -829,9 +873,6 @@ extern "C" int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, 
   RNGD_TRY(check_operand("f8_swiglu", oa, M, K));
   RNGD_TRY(check_operand("f8_swiglu", og, N, K));
   RNGD_TRY(check_operand("f8_swiglu", ou, N, K));
-  if (M > 128)
-    return pair_launch(oa, og, &ou, M, N, K, nullptr, 0, nullptr, 0, F8_F32, (uint8_t*)q, (long)ldq, scale,
-                       (cudaStream_t)stream);
   auto launch = pairs_pay(M, N, 1) ? pair_launch : few_launch;
   return launch(oa, og, &ou, M, N, K, nullptr, 0, nullptr, 0, F8_F32, (uint8_t*)q, (long)ldq, scale, (cudaStream_t)stream);
 }
