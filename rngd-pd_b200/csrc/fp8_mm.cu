@@ -202,13 +202,14 @@ struct FewArgs {
   float* scale;
 };
 // Eight neighbouring sums at this place of each CTA of the cluster, added in the CTAs' order.
-__device__ __forceinline__ void few_sum(float* y, uint32_t at, int split) {
+// self: -1, or the CTA whose own place stands for all of them.
+__device__ __forceinline__ void few_sum(float* y, uint32_t at, int split, int self) {
   float4 v[8][2];
 #pragma unroll
   for (int k = 0; k < 8; k++) {
     v[k][0] = v[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (k < split) {
-      const uint32_t from = mapa(at, k);
+      const uint32_t from = mapa(at, self < 0 ? k : self);
 #pragma unroll
       for (int c = 0; c < 2; c++)
         asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -318,9 +319,9 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *slot;
-  grid_dep_wait();
-  grid_dep_launch();
   if (warp == 0) {
+    grid_dep_wait();
+    grid_dep_launch();
     if (lane == 0) {
       int i = 0;
       bool ok = true;
@@ -340,6 +341,8 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
     }
     __syncwarp();
   } else if (warp == 1) {
+    grid_dep_wait();
+    grid_dep_launch();
     const uint32_t idesc = idesc_e4m3_f32(128, NT);
     const uint64_t desc = sw128_kmajor_desc(smem_u32(base));
     for (int i = 0; i < g1 - g0; i++) {
@@ -370,102 +373,113 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
     constexpr int TN = C::TN;
     const int r = ((warp & 3) << 5) | lane, et = threadIdx.x - 64, wt = (et >> 7) * TN;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    uint64_t acc[(DUAL ? 2 : 1) * TN / 2];
+    // The end of the kernel runs once in front without storing anything: its code, which would come from memory at
+    // the end while everything waits, comes while the data do.  (Not where a block has the SM for itself, and so starts
+    // after the launch before it: nothing is gained there.)
+#pragma unroll 1
+    for (int work = C::PER_SM == 1; work < 2; work++) {
+      if (work) {
+        grid_dep_wait();
+        grid_dep_launch();
+        uint64_t acc[(DUAL ? 2 : 1) * TN / 2];
 #pragma unroll
-    for (int j = 0; j < (DUAL ? 2 : 1) * TN / 2; j++) acc[j] = 0ull;
-    bool ok = true;
-    for (int c0 = g0; c0 < g1; c0 += C::CHUNK) {
-      const int n = min(C::CHUNK, g1 - c0);
-      if (c0 != g0) few_bar<C::SUMMERS>();  // every warp is past the previous scales
-      // a row's scales by neighbouring threads, eight loads a thread at a time, so that their latencies overlap
-      for (int e0 = et; e0 < NT * C::CHUNK; e0 += 8 * C::SUMMERS) {
-        const int g = et % C::CHUNK, gg = c0 + min(g, n - 1);
-        const float b = __ldg(a.sb + nt * a.sb_n + gg * a.sb_g), b1 = DUAL ? __ldg(p.sb1 + nt * p.sb1_n + gg * p.sb1_g) : 0.f;
-        float x[8];
+        for (int j = 0; j < (DUAL ? 2 : 1) * TN / 2; j++) acc[j] = 0ull;
+        bool ok = true;
+        for (int c0 = g0; c0 < g1; c0 += C::CHUNK) {
+          const int n = min(C::CHUNK, g1 - c0);
+          if (c0 != g0) few_bar<C::SUMMERS>();  // every warp is past the previous scales
+          // a row's scales by neighbouring threads, eight loads a thread at a time, so that their latencies overlap
+          for (int e0 = et; e0 < NT * C::CHUNK; e0 += 8 * C::SUMMERS) {
+            const int g = et % C::CHUNK, gg = c0 + min(g, n - 1);
+            const float b = __ldg(a.sb + nt * a.sb_n + gg * a.sb_g), b1 = DUAL ? __ldg(p.sb1 + nt * p.sb1_n + gg * p.sb1_g) : 0.f;
+            float x[8];
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const int t = (e0 + u * C::SUMMERS) / C::CHUNK, m = mt * NT + t;
-          x[u] = t < NT && m < a.M ? __ldg(a.sa + m * a.sa_m + gg * a.sa_g) : 0.f;
-        }
+            for (int u = 0; u < 8; u++) {
+              const int t = (e0 + u * C::SUMMERS) / C::CHUNK, m = mt * NT + t;
+              x[u] = t < NT && m < a.M ? __ldg(a.sa + m * a.sa_m + gg * a.sa_g) : 0.f;
+            }
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const int t = (e0 + u * C::SUMMERS) / C::CHUNK;
-          if (t < NT) {
-            s_scale[g * C::PITCH + t] = x[u] * b;
-            if (DUAL) s_scale[g * C::PITCH + NT + t] = x[u] * b1;
+            for (int u = 0; u < 8; u++) {
+              const int t = (e0 + u * C::SUMMERS) / C::CHUNK;
+              if (t < NT) {
+                s_scale[g * C::PITCH + t] = x[u] * b;
+                if (DUAL) s_scale[g * C::PITCH + NT + t] = x[u] * b1;
+              }
+            }
+          }
+          few_bar<C::SUMMERS>();
+          for (int k = 0; k < n; k++) {
+            const int i = c0 - g0 + k, buf = i % C::BUFS;
+            if (ok) ok = mbar_wait(&acc_full[buf], (uint32_t)(i / C::BUFS) & 1u, ST_EPI_WAIT, &g_status_f8);
+            __syncwarp();
+            tc_fence_after();
+            const uint32_t d = tmem + lane_base + (uint32_t)(buf * C::COLS + wt);
+            const float* s = s_scale + k * C::PITCH + wt;
+            scale_add_cols<TN, C::STEP>(acc, d, s);
+            if (DUAL) scale_add_cols<TN, C::STEP>(acc + TN / 2, d + NT, s + NT);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
           }
         }
-      }
-      few_bar<C::SUMMERS>();
-      for (int k = 0; k < n; k++) {
-        const int i = c0 - g0 + k, buf = i % C::BUFS;
-        if (ok) ok = mbar_wait(&acc_full[buf], (uint32_t)(i / C::BUFS) & 1u, ST_EPI_WAIT, &g_status_f8);
-        __syncwarp();
-        tc_fence_after();
-        const uint32_t d = tmem + lane_base + (uint32_t)(buf * C::COLS + wt);
-        const float* s = s_scale + k * C::PITCH + wt;
-        scale_add_cols<TN, C::STEP>(acc, d, s);
-        if (DUAL) scale_add_cols<TN, C::STEP>(acc + TN / 2, d + NT, s + NT);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
-      }
-    }
-    if (lane == 0) mbar_arrive(done);
-    float* part = (float*)base;  // [COLS][128]: the stages are done with
-    few_bar<C::SUMMERS>();       // (every warp has seen the last products)
+        if (lane == 0) mbar_arrive(done);
+        float* part = (float*)base;  // [COLS][128]: the stages are done with
+        few_bar<C::SUMMERS>();       // (every warp has seen the last products)
 #pragma unroll
-    for (int j = 0; j < (DUAL ? 2 : 1) * TN / 2; j++) {
-      const float2 v = parts_of(acc[j]);
-      const int c = wt + 2 * j + (DUAL && j >= TN / 2 ? NT - TN : 0);
-      part[c * 128 + r] = v.x;
-      part[(c + 1) * 128 + r] = v.y;
-    }
-  }
-  if (p.split > 1)
-    cluster_sync();
-  else if (warp >= 2)
-    few_bar<C::SUMMERS>();
-  if (warp >= 2) {
-    // This CTA's rows of a: their sums over the cluster, in the order of the runs, and the result.  16 threads have a
-    // row's 128 columns, eight each.  (A short loop: code that runs once costs its way from memory.)
-    const int et = threadIdx.x - 64, l = et & 15, n = nt * 128 + 8 * l;
-    const int t0 = NT * rank / p.split, t1 = min(NT * (rank + 1) / p.split, a.M - mt * NT);
-    const uint32_t at = smem_u32(base) + l * 32;
-    for (int tb = t0; tb < t1; tb += C::SUMMERS / 16) {
-      const int t = tb + (et >> 4);
-      const bool there = t < t1;
-      const long m = mt * NT + t;
-      float y[8], u[8];
-      few_sum(y, at + (there ? t : t0) * 512, p.split);
-      if constexpr (DUAL) {
-        few_sum(u, at + (NT + (there ? t : t0)) * 512, p.split);
-        float most = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          y[e] = n + e < a.N ? swiglu(y[e], u[e]) : 0.f;
-          most = max_nan(most, fabsf(y[e]));
+        for (int j = 0; j < (DUAL ? 2 : 1) * TN / 2; j++) {
+          const float2 v = parts_of(acc[j]);
+          const int c = wt + 2 * j + (DUAL && j >= TN / 2 ? NT - TN : 0);
+          part[c * 128 + r] = v.x;
+          part[(c + 1) * 128 + r] = v.y;
         }
+        if (p.split > 1)
+          cluster_sync();
+        else
+          few_bar<C::SUMMERS>();
+      }
+      // This CTA's rows of a: their sums over the cluster, in the order of the runs, and the result.  16 threads have a
+      // row's 128 columns, eight each.  (A short loop: code that runs once costs its way from memory.)
+      const int l = et & 15, n = nt * 128 + 8 * l;
+      const int t0 = NT * rank / p.split, t1 = min(NT * (rank + 1) / p.split, a.M - mt * NT);
+      const uint32_t at = smem_u32(base) + l * 32;
+      for (int tb = t0; tb < (work ? t1 : t0 + 1); tb += C::SUMMERS / 16) {
+        const int t = tb + (et >> 4);
+        const bool there = work && t < t1;
+        const long m = mt * NT + t;
+        float y[8], u[8];
+        few_sum(y, at + (there ? t : 0) * 512, p.split, there ? -1 : (int)rank);
+        if constexpr (DUAL) {
+          few_sum(u, at + (NT + (there ? t : 0)) * 512, p.split, there ? -1 : (int)rank);
+          float most = 0.f;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const float lim = held_max(most), inv = 448.0f / lim;
-        if (there) {
-          uint8_t* q = p.q + m * p.ldq + n;
-          if (n + 8 <= a.N) {
-            *(uint2*)q = held8(y, inv);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-              if (n + e < a.N) q[e] = e4m3(y[e] * inv);
+          for (int e = 0; e < 8; e++) {
+            y[e] = n + e < a.N ? swiglu(y[e], u[e]) : 0.f;
+            most = max_nan(most, fabsf(y[e]));
           }
-          if (l == 0) p.scale[m * p.tn + nt] = lim / 448.0f;
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+          const float lim = held_max(most), inv = 448.0f / lim;
+          if (there) {
+            uint8_t* q = p.q + m * p.ldq + n;
+            if (n + 8 <= a.N) {
+              *(uint2*)q = held8(y, inv);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (n + e < a.N) q[e] = e4m3(y[e] * inv);
+            }
+            if (l == 0) p.scale[m * p.tn + nt] = lim / 448.0f;
+          }
+        } else if (there) {
+          store_sums<DT>(a, y, m, n, p.vec);
         }
-      } else if (there) {
-        store_sums<DT>(a, y, m, n, p.vec);
       }
     }
   }
-  if (p.split > 1) cluster_sync();  // nobody reads this CTA's sums any more
+  if (p.split > 1) {
+    if (warp < 2) cluster_sync();
+    cluster_sync();  // nobody reads this CTA's sums any more
+  }
 }
 
 // ------------------------------------------------------------------ many rows: pairs of CTAs
