@@ -496,8 +496,67 @@ struct PairArgs {
   long ldq;
   float* scale;
 };
-constexpr int kPairStages = 6, kPairStage = 2 * kMmTile, kPairThreads = 128 + 256;
-constexpr size_t kPairSmem = 1024 + kPairStages * kPairStage + (2 * kPairStages + 4) * 8 + 16 + 2 * 2 * 128 * 4;
+constexpr int kPairStages = 5, kPairStage = 2 * kMmTile, kPairThreads = 128 + 256;
+constexpr int kPairPitch = 36;  // floats of a row of 32 on its way out: 16-byte accesses meet in no bank
+constexpr size_t kPairSmem =
+    1024 + kPairStages * kPairStage + (2 * kPairStages + 4) * 8 + 16 + 2 * 2 * 128 * 4 + 8 * 32 * kPairPitch * 4;
+
+// A warp's 32 rows x 128 sums (row m0 + lane, from column n0 on) go out 32 columns at a time through shared memory, so
+// that the stores of a row lie together whatever its alignment.
+template <int DT>
+__device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* acc, long m0, int n0, float* room, bool ok) {
+  const MmArgs& a = p.m;
+  const int lane = threadIdx.x & 31;
+  constexpr bool AHEAD = DT != F8_F32;  // what is added comes while the sums are laid out; registers do not reach in fp32
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    const int n = n0 + 32 * c, n8 = n + (lane & 3) * 8;
+    const bool whole = p.vec && n + 32 <= a.N, plus = whole && a.add != nullptr;
+    Eight<DT> add[AHEAD ? 4 : 1];
+    auto fetch = [&](Eight<DT>& to, int i) {
+      const long m = m0 + 8 * i + (lane >> 2);
+      if (plus && m < a.M) to.load_any(a.add, m * a.ldadd + n8);
+    };
+    if (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) fetch(add[i], i);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float2 x = parts_of(acc[16 * c + 2 * j]), y = parts_of(acc[16 * c + 2 * j + 1]);
+      *(float4*)(room + lane * kPairPitch + 4 * j) = make_float4(x.x, x.y, y.x, y.y);
+    }
+    __syncwarp();
+    if (whole) {
+#pragma unroll(AHEAD ? 4 : 1)
+      for (int i = 0; i < 4; i++) {
+        const int r = 8 * i + (lane >> 2);
+        const float* f = room + r * kPairPitch + (lane & 3) * 8;
+        float v[8];
+        *(float4*)v = *(const float4*)f;
+        *(float4*)(v + 4) = *(const float4*)(f + 4);
+        if (plus) {
+          float w[8];
+          if (!AHEAD) fetch(add[0], i);
+          add[AHEAD ? i : 0].values(w);
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[e] += w[e];
+        }
+        if (m0 + r < a.M && ok) store_eight<DT>(a.y, (m0 + r) * a.ldy + n8, eight_of<DT>(v));
+      }
+    } else if (n + lane < a.N && ok) {
+#pragma unroll 2
+      for (int r = 0; r < 32; r++) {
+        const long m = m0 + r;
+        const float v = room[r * kPairPitch + lane];
+        if (m < a.M)
+          store_f32_as<DT>(a.y, m * a.ldy + n + lane,
+                           a.add != nullptr ? v + load_as_f32<DT>(a.add, m * a.ldadd + n + lane) : v);
+      }
+    }
+    __syncwarp();
+  }
+}
 
 // 64 gate sums and 64 up sums of row m, columns n0 ..: the other 64 of the group are another warp's, so the maximum
 // meets in shared memory.
@@ -551,6 +610,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint64_t* acc_empty = acc_full + 2;        // [2], used in the first CTA
   uint32_t* slot = (uint32_t*)(acc_empty + 2);
   float* s_amax = (float*)(slot + 4);        // [2][2][128]
+  float* s_room = s_amax + 2 * 2 * 128;      // [8 warps][32][kPairPitch]
   const MmArgs& a = p.m;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -577,7 +637,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem = *slot;
   grid_dep_wait();
   // The 384 threads start with 168 registers each: 64512.  Four warps give up theirs for the eight that hold the sums:
-  // 128 * (40 + 2 * 224) = 62464.
+  // 128 * (40 + 2 * 232) = 64512.
   if (warp < 4) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
    if (warp == 0) {
@@ -637,7 +697,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // Eight warps: the lane quarter warp & 3 (the rows that a warp may read), half h of the columns.  A thread's
     // 128 sums are two pieces of 64 columns; with SWIGLU the gate's (columns 0..127 of the tile) and the up's.
     const int h = (warp - 4) >> 2, r = ((warp & 3) << 5) | lane;
@@ -681,18 +741,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       if (SWIGLU) {
         pair_store_swiglu(p, acc, m, row && ok, nt * 128 + 64 * h, nt, h, r, warp & 3, s_amax + (round & 1) * 256);
-      } else if (row && ok) {
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float2 x = parts_of(acc[4 * j + e]);
-            v[2 * e] = x.x;
-            v[2 * e + 1] = x.y;
-          }
-          store_sums<DT>(a, v, m, nt * 256 + 128 * h + 8 * j, p.vec);
-        }
+      } else {
+        pair_store<DT>(p, acc, mt * 256 + (int)rank * 128 + (warp & 3) * 32, nt * 256 + 128 * h,
+                       s_room + (warp - 4) * 32 * kPairPitch, ok);
       }
     }
   }
@@ -729,6 +780,26 @@ static int whole_rows(const void* y, long ldy, const void* add, long ldadd, int 
   return (((uintptr_t)y | (uintptr_t)add) & 15) == 0 && ldy * sz % 16 == 0 && ldadd * sz % 16 == 0;
 }
 
+// The few-row kernel's tiles: rows of a in each, and the runs that K is cut into, as many as fill the SMs' places, none
+// shorter than four groups.
+struct FewPlan {
+  long tiles, waves;
+  int split;
+};
+static int few_rows(int M, bool dual) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 || dual ? 64 : 128; }
+static FewPlan few_plan(int M, int N, int G, bool dual) {
+  const int rows = few_rows(M, dual);
+  const bool two = rows == 16 || (rows <= 64 && !dual);
+  const long places = (long)num_sms() * (two ? 2 : 1);
+  static_assert(FewCfg<16, true>::PER_SM == 2 && FewCfg<32, true>::PER_SM == 1 && FewCfg<64, true>::PER_SM == 1, "");
+  static_assert(FewCfg<16, false>::PER_SM == 2 && FewCfg<32, false>::PER_SM == 2 && FewCfg<64, false>::PER_SM == 2 &&
+                    FewCfg<128, false>::PER_SM == 1, "");
+  FewPlan f = {((long)N + 127) / 128 * (((long)M + rows - 1) / rows), 0, 1};
+  while (f.split < 8 && f.tiles * f.split * 2 <= places && f.split * 8 <= G) f.split *= 2;
+  f.waves = (f.tiles * f.split + places - 1) / places;
+  return f;
+}
+
 // The few-row kernel's launch: y, or (b1: the second weight) q and its scales.
 template <int NT, bool DUAL, int DT>
 static int few_launch_as(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb1, const FewArgs& p,
@@ -760,11 +831,10 @@ static int few_launch_nt(const Operand& a, const Operand& b, const Operand* b1, 
   RNGD_TRY(operand_map(b, m.N, m.K, 128, &tb));
   tb1 = tb;
   if (DUAL) RNGD_TRY(operand_map(*b1, m.N, m.K, 128, &tb1));
+  const FewPlan plan = few_plan(m.M, m.N, m.G, DUAL);
   p.tn = (m.N + 127) / 128;
-  const long tiles = (long)p.tn * ((m.M + NT - 1) / NT);
-  // as many runs of K as fill the SMs' places, none shorter than four groups
-  p.split = 1;
-  while (p.split < 8 && tiles * p.split * 2 <= (long)num_sms() * FewCfg<NT, DUAL>::PER_SM && p.split * 8 <= m.G) p.split *= 2;
+  p.split = plan.split;
+  const long tiles = plan.tiles;
   RNGD_REQUIRE(tiles * p.split <= 0x7FFFFFFFl, "f8_matmul: %d x %d results", m.M, m.N);
   const unsigned grid = (unsigned)(tiles * p.split);
   if constexpr (DUAL) return few_launch_as<NT, true, F8_F32>(ta, tb, tb1, p, grid, s);
@@ -786,14 +856,18 @@ static int few_launch(const Operand& a, const Operand& b, const Operand* b1, int
     p.sb1 = b1->scale;
     p.sb1_n = (long)b1->s0;
     p.sb1_g = (long)b1->s1;
-    if (M <= 16) return few_launch_nt<16, true>(a, b, b1, p, dtype, s);
-    if (M <= 32) return few_launch_nt<32, true>(a, b, b1, p, dtype, s);
-    return few_launch_nt<64, true>(a, b, b1, p, dtype, s);
+    switch (few_rows(M, true)) {
+      case 16: return few_launch_nt<16, true>(a, b, b1, p, dtype, s);
+      case 32: return few_launch_nt<32, true>(a, b, b1, p, dtype, s);
+      default: return few_launch_nt<64, true>(a, b, b1, p, dtype, s);
+    }
   }
-  if (M <= 16) return few_launch_nt<16, false>(a, b, b1, p, dtype, s);
-  if (M <= 32) return few_launch_nt<32, false>(a, b, b1, p, dtype, s);
-  if (M <= 64) return few_launch_nt<64, false>(a, b, b1, p, dtype, s);
-  return few_launch_nt<128, false>(a, b, b1, p, dtype, s);
+  switch (few_rows(M, false)) {
+    case 16: return few_launch_nt<16, false>(a, b, b1, p, dtype, s);
+    case 32: return few_launch_nt<32, false>(a, b, b1, p, dtype, s);
+    case 64: return few_launch_nt<64, false>(a, b, b1, p, dtype, s);
+    default: return few_launch_nt<128, false>(a, b, b1, p, dtype, s);
+  }
 }
 
 // The pairs' launch: one weight, or gate and up (b1) with the 8-bit result (q, scale).
@@ -830,11 +904,15 @@ static int pair_launch(const Operand& a, const Operand& b, const Operand* b1, in
                     ta, tb, tb1, p);
 }
 
-// Whether the pairs' tiles, 256 rows x 128 * blocks columns, are worth it.
-static bool pairs_pay(int M, int N, int blocks) {
-  static const char* e = getenv("F8_ROWS");
-  if (e) return M > atoi(e);
-  return M > 128;
+// Which of the two kernels: a wave of either takes about 7 us and 0.4 us for each of its groups (256 rows a tile of the
+// pairs', 64 or 128 of the other, whose K may be cut).  Measured over 65 to 2000 rows, N from 300 to 28000 and K from 300
+// to 8192 this takes the faster one but for ties within a tenth.
+static bool pairs_pay(int M, int N, int K, bool dual) {
+  const int G = (K + 127) / 128;
+  const FewPlan f = few_plan(M, N, G, dual);
+  const long tiles = ((long)M + 255) / 256 * (((long)N + (dual ? 127 : 255)) / (dual ? 128 : 256));
+  const long pairs = num_sms() / 2, waves = (tiles + pairs - 1) / pairs;
+  return waves * (18 + G) <= f.waves * (18 + (G + f.split - 1) / f.split);
 }
 
 int read_status_f8(int* st, int reset) {
@@ -864,7 +942,7 @@ extern "C" int rngd_f8_matmul(const void* a, int64_t lda, const float* a_scale, 
   const Operand oa = {a, lda, a_scale, a_strides[0], a_strides[1]}, ob = {b, ldb, b_scale, b_strides[0], b_strides[1]};
   RNGD_TRY(check_operand("f8_matmul", oa, M, K));
   RNGD_TRY(check_operand("f8_matmul", ob, N, K));
-  if (pairs_pay(M, N, 2))
+  if (pairs_pay(M, N, K, false))
     return pair_launch(oa, ob, nullptr, M, N, K, add, (long)ldadd, y, (long)ldy, dtype, nullptr, 0, nullptr,
                        (cudaStream_t)stream);
   return few_launch(oa, ob, nullptr, M, N, K, add, (long)ldadd, y, (long)ldy, dtype, nullptr, 0, nullptr,
@@ -887,6 +965,6 @@ extern "C" int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, 
   RNGD_TRY(check_operand("f8_swiglu", oa, M, K));
   RNGD_TRY(check_operand("f8_swiglu", og, N, K));
   RNGD_TRY(check_operand("f8_swiglu", ou, N, K));
-  auto launch = pairs_pay(M, N, 1) ? pair_launch : few_launch;
+  auto launch = pairs_pay(M, N, K, true) ? pair_launch : few_launch;
   return launch(oa, og, &ou, M, N, K, nullptr, 0, nullptr, 0, F8_F32, (uint8_t*)q, (long)ldq, scale, (cudaStream_t)stream);
 }
