@@ -29,18 +29,14 @@ _E4M3 = torch.float8_e4m3fn
 _F32 = torch.float32
 _empty = torch.empty_strided  # half of torch.empty's time on the host
 _INT_MAX = 2 ** 31 - GROUP
-_check = _lib.check
+_check, _stream = _lib.check, torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice  # the calls start over with the tensors' GPU where another is current
 _rows, _weight, _norm = _lib.lib.rngd_f8_rows, _lib.lib.rngd_f8_weight, _lib.lib.rngd_f8_rms_norm
 _matmul, _swiglu = _lib.lib.rngd_f8_matmul, _lib.lib.rngd_f8_swiglu
 
 
 # The operators are called hundreds of times a step, and small ones take less time on the GPU than a call's checks on
 # the host.  So what depends on shapes, strides and types alone is checked once for each set of them.
-
-def _elsewhere(dev):
-    """Whether another GPU than the tensors' is current (the calls below then start over with theirs)."""
-    return dev.index != torch.cuda.current_device()
-
 
 def _key(t):
     return t.shape, t.stride(), t.dtype, t.device
@@ -67,9 +63,11 @@ def _groups(n):
 
 @functools.lru_cache(maxsize=4096)
 def _source(name, shape, strides, dtype, dev):
-    """What quantize and the others take from their input: (row stride, type's number, sizes, the 8-bit rows' strides)."""
+    """What the quantisers take from their input: (row stride, type's number, sizes, strides of the 8-bit rows and of
+    the scales, their number a row)."""
     ld = _matrix(name, shape, strides, dtype, dev)
-    return ld, _DT[dtype], shape[0], shape[1], ((shape[1] + 15) // 16 * 16, 1)
+    T, K = shape
+    return ld, _DT[dtype], T, K, ((K + 15) // 16 * 16, 1), (_groups(K), 1), _groups(K)
 
 
 def _operand(name, q, scale, blocks):
@@ -132,14 +130,13 @@ def _start(name, q):
 def quantize(x):
     """Rows in 8 bits: x [T, K] bfloat16, float16 or float32 (rows contiguous) -> (q [T, K], scale [T, G])."""
     dev = x.device
-    ld, dt, T, K, st = _source("x", x.shape, x.stride(), x.dtype, dev)
-    if _elsewhere(dev):
+    ld, dt, T, K, st, s_st, G = _source("x", x.shape, x.stride(), x.dtype, dev)
+    if dev.index != _current():
         with torch.cuda.device(dev):
             return quantize(x)
-    G = _groups(K)
     q = _empty((T, K), st, dtype=_E4M3, device=dev)
-    scale = _empty((T, G), (G, 1), dtype=_F32, device=dev)
-    _check(_rows(x.data_ptr(), dt, ld, T, K, q.data_ptr(), st[0], scale.data_ptr(), _lib.raw_stream(dev.index)))
+    scale = _empty((T, G), s_st, dtype=_F32, device=dev)
+    _check(_rows(x.data_ptr(), dt, ld, T, K, q.data_ptr(), st[0], scale.data_ptr(), _stream(dev.index)))
     return q, scale
 
 
@@ -147,14 +144,13 @@ def quantize_weight(w):
     """A weight in 8 bits: w [N, K] bfloat16, float16 or float32 (rows contiguous) -> (q [N, K], scale
     [ceil(N / 128), G])."""
     dev = w.device
-    ld, dt, N, K, st = _source("w", w.shape, w.stride(), w.dtype, dev)
-    if _elsewhere(dev):
+    ld, dt, N, K, st, s_st, G = _source("w", w.shape, w.stride(), w.dtype, dev)
+    if dev.index != _current():
         with torch.cuda.device(dev):
             return quantize_weight(w)
-    G = _groups(K)
     q = _empty((N, K), st, dtype=_E4M3, device=dev)
-    scale = _empty((_groups(N), G), (G, 1), dtype=_F32, device=dev)
-    _check(_weight(w.data_ptr(), dt, ld, N, K, q.data_ptr(), st[0], scale.data_ptr(), _lib.raw_stream(dev.index)))
+    scale = _empty((_groups(N), G), s_st, dtype=_F32, device=dev)
+    _check(_weight(w.data_ptr(), dt, ld, N, K, q.data_ptr(), st[0], scale.data_ptr(), _stream(dev.index)))
     return q, scale
 
 
@@ -165,26 +161,28 @@ def rms_norm(x, weight, eps, residual=None):
     rounded to their type, the residual stream as it goes on (None without a residual); the norm is of the rounded
     sum, total / sqrt(mean(total^2) + eps) * weight, worked out in fp32 and rounded to 8 bits alone."""
     dev, dtype = x.device, x.dtype
-    ld, dt, T, K, st = _source("x", x.shape, x.stride(), dtype, dev)
+    ld, dt, T, K, st, s_st, G = _source("x", x.shape, x.stride(), dtype, dev)
     wt = weight.dtype
     if weight.shape != (K,) or (wt is not dtype and wt is not _F32) or weight.device != dev or not weight.is_contiguous():
         raise ValueError(f"weight must be a contiguous {dtype} or float32 [{K}] tensor on {dev}, got "
                          f"{tuple(weight.shape)} {wt} on {weight.device}")
     if residual is not None:
-        ldr = _like("residual", residual.shape, residual.stride(), residual.dtype, residual.device, x.shape, dtype, dev)
-    if _elsewhere(dev):
+        if residual.shape != x.shape or residual.dtype is not dtype or residual.device != dev:
+            raise ValueError(f"residual must be {tuple(x.shape)} {dtype} on {dev}, got {tuple(residual.shape)} "
+                             f"{residual.dtype} on {residual.device}")
+        ldr = _source("residual", x.shape, residual.stride(), dtype, dev)[0]
+    if dev.index != _current():
         with torch.cuda.device(dev):
             return rms_norm(x, weight, eps, residual)
-    G = _groups(K)
     q = _empty((T, K), st, dtype=_E4M3, device=dev)
-    scale = _empty((T, G), (G, 1), dtype=_F32, device=dev)
+    scale = _empty((T, G), s_st, dtype=_F32, device=dev)
     if residual is None:
         total, r, t, ldr = None, None, None, 0
     else:
         total = _empty((T, K), (K, 1), dtype=dtype, device=dev)
         r, t = residual.data_ptr(), total.data_ptr()
     _check(_norm(x.data_ptr(), ld, r, ldr, weight.data_ptr(), dt, _DT[wt], T, K, eps, t, K, q.data_ptr(), st[0],
-                 scale.data_ptr(), _lib.raw_stream(dev.index)))
+                 scale.data_ptr(), _stream(dev.index)))
     return q, scale, total
 
 
@@ -198,13 +196,13 @@ def matmul(a, a_scale, b, b_scale, dtype=torch.bfloat16, add=None, out=None):
         dtype, _key(a), _key(a_scale), _key(b), _key(b_scale), None if add is None else _key(add),
         None if out is None else _key(out))
     ap, bp, dev = _start("a", a), _start("b", b), a.device
-    if _elsewhere(dev):
+    if dev.index != _current():
         with torch.cuda.device(dev):
             return matmul(a, a_scale, b, b_scale, dtype, add, out)
     if out is None:
         out = _empty(shape, st, dtype=dtype, device=dev)
     _check(_matmul(ap, lda, a_scale.data_ptr(), ast, bp, ldb, b_scale.data_ptr(), bst, M, N, K,
-                   None if add is None else add.data_ptr(), ldadd, out.data_ptr(), ldo, dt, _lib.raw_stream(dev.index)))
+                   None if add is None else add.data_ptr(), ldadd, out.data_ptr(), ldo, dt, _stream(dev.index)))
     return out
 
 
@@ -214,11 +212,11 @@ def matmul_swiglu(a, a_scale, gate, gate_scale, up, up_scale):
     M, N, K, lda, ast, ldg, gst, ldu, ust, shape, st, s_shape, s_st = _gated(
         _key(a), _key(a_scale), _key(gate), _key(gate_scale), _key(up), _key(up_scale))
     ap, gp, up_, dev = _start("a", a), _start("gate", gate), _start("up", up), a.device
-    if _elsewhere(dev):
+    if dev.index != _current():
         with torch.cuda.device(dev):
             return matmul_swiglu(a, a_scale, gate, gate_scale, up, up_scale)
     q = _empty(shape, st, dtype=_E4M3, device=dev)
     scale = _empty(s_shape, s_st, dtype=_F32, device=dev)
     _check(_swiglu(ap, lda, a_scale.data_ptr(), ast, gp, ldg, gate_scale.data_ptr(), gst, up_, ldu, up_scale.data_ptr(),
-                   ust, M, N, K, q.data_ptr(), st[0], scale.data_ptr(), _lib.raw_stream(dev.index)))
+                   ust, M, N, K, q.data_ptr(), st[0], scale.data_ptr(), _stream(dev.index)))
     return q, scale
