@@ -138,10 +138,8 @@ __device__ __forceinline__ float2 parts_of(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-// acc[0..31] += s * (64 columns from taddr), two columns an instruction
-__device__ __forceinline__ void scale_add(uint64_t* acc, uint32_t taddr, float s) {
-  uint32_t r[64];
-  tmem_ld_x64(taddr, r);
+// acc[0..31] += s * 64 columns, two an instruction
+__device__ __forceinline__ void scale_add(uint64_t* acc, const uint32_t* r, float s) {
   const uint64_t ss = pair_of(s, s);
 #pragma unroll
   for (int j = 0; j < 32; j++) {
@@ -679,8 +677,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int t = pair; t < tiles && ok; t += pairs)
         for (int i = 0; i < a.G; i++, it++) {
           const int s = it % kPairStages, buf = it & 1;
-          ok = mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8) &&
-               mbar_wait(&full[s], (uint32_t)(it / kPairStages) & 1u, ST_MMA_WAIT, &g_status_f8);
+          ok = mbar_wait(&full[s], (uint32_t)(it / kPairStages) & 1u, ST_MMA_WAIT, &g_status_f8) &&
+               mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -733,11 +731,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         tc_fence_after();
         const uint32_t d = tmem + lane_base + (uint32_t)(buf * 256);
-        scale_add(acc, d + c0, s0);
-        scale_add(acc + 32, d + c1, s1);
+        uint32_t v[64];
+        tmem_ld_x64(d + c0, v);
+        scale_add(acc, v, s0);
+        tmem_ld_x64(d + c1, v);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(bar_empty + 8 * buf);
+        if (lane == 0) mbar_arrive_cluster(bar_empty + 8 * buf);  // before the rest is added: the products wait for it
+        scale_add(acc + 32, v, s1);
       }
       if (SWIGLU) {
         pair_store_swiglu(p, acc, m, row && ok, nt * 128 + 64 * h, nt, h, r, warp & 3, s_amax + (round & 1) * 256);
