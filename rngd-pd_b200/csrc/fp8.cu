@@ -6,6 +6,8 @@
 #include "fp8.cuh"
 #include "tc.cuh"
 
+#include <type_traits>
+
 namespace rngd {
 
 struct RowsArgs {
@@ -20,7 +22,7 @@ struct RowsArgs {
 
 constexpr int kRowsThreads = 256, kRowsPer = 2;  // neighbouring groups of a row that eight lanes take
 
-// VEC: rows of whole 16-byte vectors.
+// VEC: rows of whole 16-byte vectors; else they start anywhere.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads) f8_rows_kernel(RowsArgs a) {
   grid_dep_wait();
@@ -32,36 +34,47 @@ __global__ void __launch_bounds__(kRowsThreads) f8_rows_kernel(RowsArgs a) {
   const bool there = row < a.T;
   const long k0 = (long)g0 * kGroup, in0 = row * a.ldx + k0;
   const int left = there ? (int)min((long)a.K - k0, (long)kRowsPer * kGroup) : 0;  // values of this run
-  Eight<DT> in[kRowsPer][2];
+  const char* end = end_of<DT>(a.x, a.T, a.ldx, a.K);
+  std::conditional_t<VEC, Eight<DT>, EightAt<DT>> in[kRowsPer][2];
   float v[kRowsPer][16], m[kRowsPer], inv[kRowsPer];
+#pragma unroll
+  for (int j = 0; j < kRowsPer; j++)
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      const int k = j * kGroup + 64 * c + 8 * l;
+      if (k < left) {
+        if constexpr (VEC)
+          in[j][c].load(a.x, in0 + k);
+        else
+          in[j][c].fetch(a.x, in0 + k, end);
+      }
+    }
+  grid_dep_launch();
 #pragma unroll
   for (int j = 0; j < kRowsPer; j++) {
 #pragma unroll
     for (int e = 0; e < 16; e++) v[j][e] = 0.f;
-    if (VEC) {
 #pragma unroll
-      for (int c = 0; c < 2; c++)
-        if (j * kGroup + 64 * c + 8 * l < left) in[j][c].load(a.x, in0 + j * kGroup + 64 * c + 8 * l);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; e++)
-        if (j * kGroup + l + 8 * e < left) v[j][e] = load_as_f32<DT>(a.x, in0 + j * kGroup + l + 8 * e);
-    }
-  }
-  grid_dep_launch();
-#pragma unroll
-  for (int j = 0; j < kRowsPer; j++) {
-    if (VEC) {
-#pragma unroll
-      for (int c = 0; c < 2; c++)
-        if (j * kGroup + 64 * c + 8 * l < left) in[j][c].values(v[j] + 8 * c);
+    for (int c = 0; c < 2; c++) {
+      const int k = j * kGroup + 64 * c + 8 * l;
+      if (k < left) {
+        if constexpr (VEC)
+          in[j][c].values(v[j] + 8 * c);
+        else
+          in[j][c].get(a.x, in0 + k, left - k, end).values(v[j] + 8 * c);
+      }
     }
     m[j] = held_max(amax_lanes(amax_of<16>(v[j])));
   }
   const float scale = quotients<kRowsPer>(m, inv);
   uint8_t* dst = a.q + (long)row * a.ldq + k0;
 #pragma unroll
-  for (int j = 0; j < kRowsPer; j++) store_held<VEC>(dst + j * kGroup, l, left - j * kGroup, v[j], inv[j]);
+  for (int j = 0; j < kRowsPer; j++)
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      const int k = j * kGroup + 64 * c + 8 * l;
+      store_held<VEC>(dst + k, left - k, v[j] + 8 * c, inv[j]);
+    }
   if (l < kRowsPer && l * kGroup < left) a.scale[(long)row * a.G + g0 + l] = scale;
 }
 
@@ -84,29 +97,32 @@ __global__ void __launch_bounds__(256) f8_weight_kernel(WeightArgs a) {
   const int b = blockIdx.x, nb = b / a.G, kb = b - nb * a.G;
   const int l = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   const int k0 = kb * kGroup;
+  const int k = k0 + 8 * l;
+  const char* end = end_of<DT>(a.w, a.N, a.ldw, a.K);
+  std::conditional_t<VEC, Eight<DT>, EightAt<DT>> raw[8];
   Eight<DT> in[8];
   float most = 0.f, v[8];
+  auto there = [&](int j) { return nb * kGroup + r0 + 16 * j < a.N && k < a.K; };
+  auto at = [&](int j) { return (long)(nb * kGroup + r0 + 16 * j) * a.ldw + k; };
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const int n = nb * kGroup + r0 + 16 * j;
-    if (VEC && n < a.N && k0 + 8 * l < a.K) in[j].load(a.w, (long)n * a.ldw + k0 + 8 * l);
-  }
+  for (int j = 0; j < 8; j++)
+    if (there(j)) {
+      if constexpr (VEC)
+        raw[j].load(a.w, at(j));
+      else
+        raw[j].fetch(a.w, at(j), end);
+    }
   grid_dep_launch();
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const int n = nb * kGroup + r0 + 16 * j;
-    if (n >= a.N) continue;
-    if (VEC) {
-      if (k0 + 8 * l < a.K) {
-        in[j].values(v);
-        most = amax_of<8>(v, most);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (k0 + l + 16 * e < a.K) most = max_nan(most, fabsf(load_as_f32<DT>(a.w, (long)n * a.ldw + k0 + l + 16 * e)));
+  for (int j = 0; j < 8; j++)
+    if (there(j)) {
+      if constexpr (VEC)
+        in[j] = raw[j];
+      else
+        in[j] = raw[j].get(a.w, at(j), a.K - k, end);
+      in[j].values(v);
+      most = amax_of<8>(v, most);
     }
-  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
   if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = most;
@@ -116,22 +132,11 @@ __global__ void __launch_bounds__(256) f8_weight_kernel(WeightArgs a) {
   const float m = held_max(most), inv = 448.0f / m;
   if (threadIdx.x == 0) a.scale[b] = m / 448.0f;
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const int n = nb * kGroup + r0 + 16 * j;
-    if (n >= a.N) continue;
-    uint8_t* dst = a.q + (long)n * a.ldq + k0;
-    if (VEC) {
-      if (k0 + 8 * l < a.K) {
-        in[j].values(v);
-        *(uint2*)(dst + 8 * l) = held8(v, inv);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (k0 + l + 16 * e < a.K)
-          dst[l + 16 * e] = e4m3(load_as_f32<DT>(a.w, (long)n * a.ldw + k0 + l + 16 * e) * inv);
+  for (int j = 0; j < 8; j++)
+    if (there(j)) {
+      in[j].values(v);
+      store_held<VEC>(a.q + (long)(nb * kGroup + r0 + 16 * j) * a.ldq + k, a.K - k, v, inv);
     }
-  }
 }
 
 // --------------------------------------------------------------------------------------------- norm
@@ -144,6 +149,7 @@ struct NormArgs {
   int K, G;
   float eps;
   long T;
+  int stage;    // rows of the sum go out through shared memory
   void* total;  // [T][K] of x's type, rows ldt apart
   long ldt;
   uint8_t* q;
@@ -154,59 +160,57 @@ struct NormArgs {
 // A lane's 16 values of x and the residual in the group from k0 on, as they are loaded.
 template <int DT, bool VEC>
 struct NormIn {
-  Eight<DT> x[2], r[2];
-  float h[VEC ? 1 : 16];
+  std::conditional_t<VEC, Eight<DT>, EightAt<DT>> x[2], r[2];
   __device__ __forceinline__ void load(const NormArgs& a, long row, int k0, int l) {
-    if constexpr (VEC) {
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        const int k = k0 + 64 * c + 8 * l;
-        if (k < a.K) {
-          x[c].load(a.x, row * a.ldx + k);
-          if (a.res != nullptr) r[c].load(a.res, row * a.ldr + k);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int k = k0 + l + 8 * e;
-        h[e] = 0.f;
-        if (k < a.K) {
-          h[e] = load_as_f32<DT>(a.x, row * a.ldx + k);
-          if (a.res != nullptr) h[e] = rounded_as<DT>(h[e] + load_as_f32<DT>(a.res, row * a.ldr + k));
-        }
+    for (int c = 0; c < 2; c++) {
+      const int k = k0 + 64 * c + 8 * l;
+      if (k >= a.K) continue;
+      if constexpr (VEC) {
+        x[c].load(a.x, row * a.ldx + k);
+        if (a.res != nullptr) r[c].load(a.res, row * a.ldr + k);
+      } else {
+        x[c].fetch(a.x, row * a.ldx + k, end_of<DT>(a.x, a.T, a.ldx, a.K));
+        if (a.res != nullptr) r[c].fetch(a.res, row * a.ldr + k, end_of<DT>(a.res, a.T, a.ldr, a.K));
       }
     }
   }
-  // their sum as it is kept (zeros beyond the row), written to total where that is asked for
-  __device__ __forceinline__ void sum(const NormArgs& a, long row, int k0, int l, bool write, float* f) const {
-    if constexpr (VEC) {
+  // their sum as it is kept (zeros beyond the row), written to total where that is asked for, or to `room` (VEC: null)
+  __device__ __forceinline__ void sum(const NormArgs& a, long row, int k0, int l, bool write, float* f, char* room) const {
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        const int k = k0 + 64 * c + 8 * l;
-        float* fc = f + 8 * c;
-        if (k < a.K) {
+    for (int c = 0; c < 2; c++) {
+      const int k = k0 + 64 * c + 8 * l;
+      float* fc = f + 8 * c;
+      if (k < a.K) {
+        if constexpr (VEC)
           x[c].values(fc);
-          if (a.res != nullptr) {
-            float g[8];
+        else
+          x[c].get(a.x, row * a.ldx + k, a.K - k, end_of<DT>(a.x, a.T, a.ldx, a.K)).values(fc);
+        if (a.res != nullptr) {
+          float g[8];
+          if constexpr (VEC)
             r[c].values(g);
+          else
+            r[c].get(a.res, row * a.ldr + k, a.K - k, end_of<DT>(a.res, a.T, a.ldr, a.K)).values(g);
 #pragma unroll
-            for (int e = 0; e < 8; e++) fc[e] += g[e];
-            const Eight<DT> kept = eight_of<DT>(fc);
-            kept.values(fc);
-            if (write) store_eight<DT>(a.total, row * a.ldt + k, kept);
+          for (int e = 0; e < 8; e++) fc[e] += g[e];
+          const Eight<DT> kept = eight_of<DT>(fc);
+          kept.values(fc);
+          if (write) {
+            if constexpr (VEC) {
+              store_eight<DT>(a.total, row * a.ldt + k, kept);
+            } else if (room != nullptr) {
+              store_eight<DT>(room, k, kept);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (k + e < a.K) store_f32_as<DT>(a.total, row * a.ldt + k + e, fc[e]);
+            }
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e++) fc[e] = 0.f;
         }
-      }
-    } else {
+      } else {
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int k = k0 + l + 8 * e;
-        f[e] = h[e];
-        if (a.res != nullptr && write && k < a.K) store_f32_as<DT>(a.total, row * a.ldt + k, f[e]);
+        for (int e = 0; e < 8; e++) fc[e] = 0.f;
       }
     }
   }
@@ -216,29 +220,47 @@ struct NormWeight {  // the weights of the same 16
   Eight<WT> w[2];
   __device__ __forceinline__ void load(const NormArgs& a, int k0, int l) {
 #pragma unroll
-    for (int c = 0; c < 2; c++)
-      if (VEC && k0 + 64 * c + 8 * l < a.K) w[c].load(a.w, k0 + 64 * c + 8 * l);
-  }
-  __device__ __forceinline__ void scale(const NormArgs& a, int k0, int l, float r, float* f) const {
-    if (VEC) {
-#pragma unroll
-      for (int c = 0; c < 2; c++) {
-        if (k0 + 64 * c + 8 * l < a.K) {
-          float g[8];
-          w[c].values(g);
-#pragma unroll
-          for (int e = 0; e < 8; e++) f[8 * c + e] = f[8 * c + e] * r * g[e];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int k = k0 + l + 8 * e;
-        if (k < a.K) f[e] = f[e] * r * load_as_f32<WT>(a.w, k);
+    for (int c = 0; c < 2; c++) {
+      const int k = k0 + 64 * c + 8 * l;
+      if (k >= a.K) continue;
+      if constexpr (VEC) {
+        w[c].load(a.w, k);
+      } else {
+        const char* end = end_of<WT>(a.w, 1, 0, a.K);
+        EightAt<WT> raw;
+        raw.fetch(a.w, k, end);
+        w[c] = raw.get(a.w, k, a.K - k, end);
       }
     }
   }
+  __device__ __forceinline__ void scale(const NormArgs& a, int k0, int l, float r, float* f) const {
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+      if (k0 + 64 * c + 8 * l < a.K) {
+        float g[8];
+        w[c].values(g);
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[8 * c + e] = f[8 * c + e] * r * g[e];
+      }
+  }
 };
+
+// A row of the sum from shared memory to a place of any alignment, four bytes a thread at a time.
+template <int DT>
+__device__ __forceinline__ void norm_row_out(const NormArgs& a, long row, const char* room) {
+  if constexpr (DT == F8_F32) {
+    float* to = (float*)a.total + row * a.ldt;
+    for (int i = threadIdx.x; i < a.K; i += blockDim.x) to[i] = ((const float*)room)[i];
+  } else {
+    uint16_t* to = (uint16_t*)a.total + row * a.ldt;
+    const uint16_t* from = (const uint16_t*)room;
+    const int head = (int)((uintptr_t)to >> 1) & 1, pairs = (a.K - head) >> 1;
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x)
+      ((uint32_t*)(to + head))[i] = from[head + 2 * i] | (uint32_t)from[head + 2 * i + 1] << 16;
+    if (threadIdx.x == 0 && head) to[0] = from[0];
+    if (threadIdx.x == 0 && ((a.K - head) & 1)) to[a.K - 1] = from[a.K - 1];
+  }
+}
 
 // 1 / sqrt(mean + eps) of the block's sums of squares
 __device__ __forceinline__ float norm_factor(float ss, float* s_sum, const NormArgs& a) {
@@ -257,16 +279,24 @@ __device__ __forceinline__ void norm_store(const NormArgs& a, long row, int g0, 
   const float scale = quotients<PER>(m, inv);
 #pragma unroll
   for (int j = 0; j < PER; j++) {
-    const int k0 = (g0 + j * gs) * kGroup;
-    store_held<VEC>(a.q + row * a.ldq + k0, l, a.K - k0, f[j], inv[j]);
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      const int k = (g0 + j * gs) * kGroup + 64 * c + 8 * l;
+      store_held<VEC>(a.q + row * a.ldq + k, a.K - k, f[j] + 8 * c, inv[j]);
+    }
   }
   if (l < PER && g0 + l * gs < a.G) a.scale[row * a.G + g0 + l * gs] = scale;
 }
 
-// The next row is on its way while the present one is summed and rounded; the weights stay in registers.
+template <bool VEC>
+constexpr int kNormThreads = VEC ? 512 : 384;  // 384: at 80 registers two blocks' warps fit an SM's quarters
+// The next row is on its way while the present one is summed and rounded (where rows are whole vectors: the others'
+// registers go further as a second block an SM; 8000 x 4097 bf16 with a residual 98 us, ahead of time 121); the weights stay in registers.
 template <int DT, int WT, bool VEC, int PER>
-__global__ void __launch_bounds__(512) f8_norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads<VEC>, VEC ? 0 : 2) f8_norm_kernel(NormArgs a) {
   __shared__ float s_sum[2][32];  // for each of two rows in turn
+  extern __shared__ uint4 s_row[];
+  char* room = !VEC && a.stage ? (char*)s_row : nullptr;
   grid_dep_wait();
   const int l = threadIdx.x & (kLanes - 1), g0 = threadIdx.x / kLanes, gs = blockDim.x / kLanes;
   NormIn<DT, VEC> in[PER];
@@ -274,26 +304,32 @@ __global__ void __launch_bounds__(512) f8_norm_kernel(NormArgs a) {
   long row = blockIdx.x;
 #pragma unroll
   for (int j = 0; j < PER; j++) {
-    in[j].load(a, row, (g0 + j * gs) * kGroup, l);
+    if (VEC) in[j].load(a, row, (g0 + j * gs) * kGroup, l);
     w[j].load(a, (g0 + j * gs) * kGroup, l);
   }
   grid_dep_launch();
   for (int half = 0; row < a.T; row += gridDim.x, half ^= 1) {
     float f[PER][16], ss = 0.f;
+    if (!VEC) {
+#pragma unroll
+      for (int j = 0; j < PER; j++) in[j].load(a, row, (g0 + j * gs) * kGroup, l);
+    }
 #pragma unroll
     for (int j = 0; j < PER; j++) {
-      in[j].sum(a, row, (g0 + j * gs) * kGroup, l, true, f[j]);
+      in[j].sum(a, row, (g0 + j * gs) * kGroup, l, true, f[j], room);
 #pragma unroll
       for (int e = 0; e < 16; e++) ss = fmaf(f[j][e], f[j][e], ss);
     }
-    if (row + gridDim.x < a.T) {
+    if (VEC && row + gridDim.x < a.T) {
 #pragma unroll
       for (int j = 0; j < PER; j++) in[j].load(a, row + gridDim.x, (g0 + j * gs) * kGroup, l);
     }
     const float r = norm_factor(ss, s_sum[half], a);
+    if (room != nullptr) norm_row_out<DT>(a, row, room);
 #pragma unroll
     for (int j = 0; j < PER; j++) w[j].scale(a, (g0 + j * gs) * kGroup, l, r, f[j]);
     norm_store<DT, VEC, PER>(a, row, g0, gs, l, f);
+    if (room != nullptr) __syncthreads();  // the next row's sum goes to the same place
   }
 }
 
@@ -310,7 +346,7 @@ __global__ void __launch_bounds__(512) f8_norm_wide_kernel(NormArgs a) {
   const int rounds = (a.G + gs - 1) / gs;
   for (int j = 0, g = threadIdx.x / kLanes; j < rounds; j++, g += gs) {
     in.load(a, row, g * kGroup, l);
-    in.sum(a, row, g * kGroup, l, true, f[0]);
+    in.sum(a, row, g * kGroup, l, true, f[0], nullptr);
 #pragma unroll
     for (int e = 0; e < 16; e++) ss = fmaf(f[0][e], f[0][e], ss);
   }
@@ -319,7 +355,7 @@ __global__ void __launch_bounds__(512) f8_norm_wide_kernel(NormArgs a) {
   for (int j = 0, g = threadIdx.x / kLanes; j < rounds; j++, g += gs) {
     in.load(a, row, g * kGroup, l);
     w.load(a, g * kGroup, l);
-    in.sum(a, row, g * kGroup, l, false, f[0]);
+    in.sum(a, row, g * kGroup, l, false, f[0], nullptr);
     w.scale(a, g * kGroup, l, r, f[0]);
     norm_store<DT, VEC, 1>(a, row, g, gs, l, f);
   }
@@ -359,6 +395,7 @@ struct WeightLaunch {
                       "f8_weight_kernel", a);
   }
 };
+constexpr int kSmSmem = 200 * 1024;  // what the blocks of an SM may have of its shared memory
 template <int DT, bool VEC>
 struct NormLaunch {
   static int go(const NormArgs& a, bool w32, cudaStream_t s) {
@@ -379,11 +416,13 @@ struct NormLaunch {
         if (n < 1) n = 1;
         known[per][warps].store(n, std::memory_order_relaxed);
       }
+      const int smem = a.stage ? a.G * kGroup * dtype_size(DT) : 0;
+      if (smem > 0 && n > kSmSmem / smem) n = kSmSmem / smem;
       const long most = (long)num_sms() * n;
-      return launch_pdl(kernel, dim3((unsigned)(a.T < most ? a.T : most)), dim3(warps * 32), 0, s, "f8_norm_kernel", a);
+      return launch_pdl(kernel, dim3((unsigned)(a.T < most ? a.T : most)), dim3(warps * 32), smem, s, "f8_norm_kernel", a);
     };
-    if (lanes <= 512) return run(f8_norm_kernel<DT, WT, VEC, 1>, 1);
-    if (lanes <= 1024) return run(f8_norm_kernel<DT, WT, VEC, 2>, 2);
+    if (lanes <= kNormThreads<VEC>) return run(f8_norm_kernel<DT, WT, VEC, 1>, 1);
+    if (lanes <= 2 * kNormThreads<VEC>) return run(f8_norm_kernel<DT, WT, VEC, 2>, 2);
     return launch_pdl(f8_norm_wide_kernel<DT, WT, VEC>, dim3((unsigned)a.T), dim3(512), 0, s, "f8_norm_wide_kernel", a);
   }
 };
@@ -435,9 +474,10 @@ extern "C" int rngd_f8_rms_norm(const void* x, int64_t ldx, const void* residual
   RNGD_REQUIRE(total == nullptr || (total != x && total != residual), "f8_rms_norm: the sum needs a place of its own");
   RNGD_REQUIRE(total == nullptr || ldt >= K || T <= 1, "f8_rms_norm: rows of the sum lie on one another");
   RNGD_TRY(check_held("f8_rms_norm", (uint8_t*)q, ldq, T, K, scale));
-  NormArgs a = {x, residual, weight, (long)ldx, (long)ldr, K, G, eps, (long)T,
+  NormArgs a = {x, residual, weight, (long)ldx, (long)ldr, K, G, eps, (long)T, 0,
                 total, (long)ldt, (uint8_t*)q, (long)ldq, scale};
   const bool vec = whole_vectors(x, ldx, K, dtype) && whole_vectors(weight, 0, K, weight_dtype) &&
                    (residual == nullptr || (whole_vectors(residual, ldr, K, dtype) && whole_vectors(total, ldt, K, dtype)));
+  a.stage = !vec && total != nullptr && (long)G * kGroup * sz <= 48 * 1024;
   return by_type<NormLaunch>(dtype, vec, a, weight_dtype == F8_F32, (cudaStream_t)stream);
 }

@@ -79,7 +79,7 @@ struct Eight {
       r[0] = ldg_nc_v4((const uint16_t*)p + i);
     }
   }
-  // the same of memory that this kernel may write
+  // an aligned eight of memory that this kernel may write
   __device__ __forceinline__ void load_any(const void* p, long i) {
     const uint4* q = (const uint4*)((const char*)p + i * (DT == F8_F32 ? 4 : 2));
 #pragma unroll
@@ -107,6 +107,80 @@ struct Eight {
     }
   }
 };
+// The first n of eight values, zeros for the others, from any place of a matrix that ends before `end`.  They come as the
+// aligned vectors around them (neighbouring rows' values may come along), fetched first and shifted into place when they
+// are needed, so that several are on their way at a time; where the vectors would reach beyond the matrix, value by value.
+template <int DT>
+struct EightAt {
+  static constexpr int SZ = DT == F8_F32 ? 4 : 2, V = 8 * SZ / 16;  // vectors where the place is aligned, else one more
+  uint4 v[V + 1];
+  __device__ __forceinline__ static bool inside(const void* p, long i, const char* end) {
+    const char* at = (const char*)p + i * SZ;
+    const int s = (int)((uintptr_t)at & 15);
+    return at - s >= (const char*)p && at - s + 16 * (V + (s != 0)) <= end;
+  }
+  __device__ __forceinline__ void fetch(const void* p, long i, const char* end) {
+    const char* at = (const char*)p + i * SZ;
+    const int s = (int)((uintptr_t)at & 15);
+    if (inside(p, i, end)) {
+#pragma unroll
+      for (int j = 0; j < V; j++) v[j] = ldg_nc_v4(at - s + 16 * j);
+      if (s != 0) v[V] = ldg_nc_v4(at - s + 16 * V);
+    }
+  }
+  __device__ __forceinline__ Eight<DT> get(const void* p, long i, int n, const char* end) const {
+    Eight<DT> r;
+    const char* at = (const char*)p + i * SZ;
+    uint32_t w[4 * V + 4];
+    if (inside(p, i, end)) {
+      const int s = (int)((uintptr_t)at & 15);
+#pragma unroll
+      for (int j = 0; j <= V; j++) {
+        const uint4 x = v[j];
+        w[4 * j] = x.x;
+        w[4 * j + 1] = x.y;
+        w[4 * j + 2] = x.z;
+        w[4 * j + 3] = x.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4 * V + 2; j++) w[j] = s & 8 ? w[j + 2] : w[j];
+#pragma unroll
+      for (int j = 0; j < 4 * V + 1; j++) w[j] = s & 4 ? w[j + 1] : w[j];
+      if constexpr (SZ == 2) {
+#pragma unroll
+        for (int j = 0; j < 4 * V; j++) w[j] = __funnelshift_r(w[j], w[j + 1], (s & 2) * 8);
+      }
+      if (n < 8) {
+#pragma unroll
+        for (int j = 0; j < 4 * V; j++) {
+          if constexpr (SZ == 4)
+            w[j] = j < n ? w[j] : 0u;
+          else
+            w[j] = 2 * j + 1 < n ? w[j] : 2 * j < n ? w[j] & 0xFFFFu : 0u;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4 * V; j++) {
+        if constexpr (SZ == 4) {
+          w[j] = j < n ? __float_as_uint(((const float*)at)[j]) : 0u;
+        } else {
+          const uint32_t l = 2 * j < n ? ((const uint16_t*)at)[2 * j] : 0u, h = 2 * j + 1 < n ? ((const uint16_t*)at)[2 * j + 1] : 0u;
+          w[j] = l | h << 16;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) r.r[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    return r;
+  }
+};
+// one past a matrix of rows ld apart
+template <int DT>
+__device__ __forceinline__ const char* end_of(const void* p, long rows, long ld, int K) {
+  return (const char*)p + ((rows - 1) * ld + K) * (DT == F8_F32 ? 4 : 2);
+}
+
 // Eight values rounded to DT.
 template <int DT>
 __device__ __forceinline__ Eight<DT> eight_of(const float* f) {
@@ -139,8 +213,7 @@ __device__ __forceinline__ void store_eight(void* p, long i, const Eight<DT>& v)
   for (int j = 0; j < (DT == F8_F32 ? 2 : 1); j++) q[j] = v.r[j];
 }
 
-// A group lies in 8 neighbouring lanes, 16 values each: lane l has the vectors of eight at 8 l and at 64 + 8 l, or,
-// where rows are no whole vectors, the values l, l + 8, ..  (16 lanes with eight each take a third more steps to the
+// A group lies in 8 neighbouring lanes, 16 values each: lane l has the vectors of eight at 8 l and at 64 + 8 l.  (16 lanes with eight each take a third more steps to the
 // group's maximum, and the quotients twice as often a value: rows of 8191 x 4096 bf16 then take 22.7 us, not 17.6.)
 constexpr int kLanes = 8;
 __device__ __forceinline__ float amax_lanes(float m) {
@@ -174,16 +247,15 @@ __device__ __forceinline__ uint2 held8(const float* f, float inv) {
   return make_uint2(e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
                     e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
 }
-// This lane's 16 values of a group, rounded, to dst (the group's first byte); `left` values of the group exist.
-template <bool VEC>
-__device__ __forceinline__ void store_held(uint8_t* dst, int l, int left, const float* f, float inv) {
-  if (VEC) {
-    if (8 * l < left) *(uint2*)(dst + 8 * l) = held8(f, inv);
-    if (64 + 8 * l < left) *(uint2*)(dst + 64 + 8 * l) = held8(f + 8, inv);
-  } else {
+// Eight values rounded to dst, 8-byte aligned; `left` of them exist (whole: all or none).
+template <bool WHOLE>
+__device__ __forceinline__ void store_held(uint8_t* dst, int left, const float* f, float inv) {
+  if (WHOLE ? left > 0 : left >= 8) {
+    *(uint2*)dst = held8(f, inv);
+  } else if (!WHOLE) {
 #pragma unroll
-    for (int e = 0; e < 16; e++)
-      if (l + 8 * e < left) dst[l + 8 * e] = e4m3(f[e] * inv);
+    for (int e = 0; e < 8; e++)
+      if (e < left) dst[e] = e4m3(f[e] * inv);
   }
 }
 
