@@ -1,8 +1,11 @@
 // Quantisers to e4m3: rows, weights, and the RMS norm that adds the residual (fp8.cuh gives the format).
 //
-// All three read each value once and write it once in 8 bits; the memory bounds them where there are many
-// rows, the launch where there are few.  The rows of the result start on 16 bytes whatever their width (the caller's row stride), as the
-// products' tile loads want them.
+// All three read each value once and write it once in 8 bits; the memory bounds them where there are many rows, the
+// launch where there are few.  The rows of the result start on 16 bytes whatever their width (the caller's row stride),
+// as the products' tile loads want them.  Measured, inputs larger than the L2 cache: rows 8191 x 4096 bf16 16.4 us, 6.2
+// TB/s; weight 14336 x 4096 bf16 28.6 us, 6.2 TB/s; norm 8192 x 4096 bf16 with a residual 38.3 us, 6.2 TB/s (the copy
+// rate is 6.55).  Rows of 4097 values, which start anywhere: 8000 of them in bf16 25 us, the norm with a residual 98:
+// more instructions a value, and fewer blocks an SM.
 #include "fp8.cuh"
 #include "tc.cuh"
 

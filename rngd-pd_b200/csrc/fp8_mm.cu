@@ -2,9 +2,13 @@
 //
 //   y[m][n] = sum_g sa[m][g] * sb[n / 128][g] * d_g[m][n],   d_g[m][n] = sum_{k in group g} a[m][k] b[n][k]
 //
-// The tensor cores hold d_g of one group of 128 (four steps of kind::f8f6f4, exact products, fp32 sums) in tensor
-// memory; the epilogue's threads multiply it with the two scales and add it to sums in their registers while the
-// next group's products run into the other half of the tensor memory.
+// The tensor cores hold d_g of one group of 128 (four steps of kind::f8f6f4: exact products, fp32 sums) in tensor
+// memory; threads multiply it with the two scales and add it to sums in their registers while the next groups'
+// products run into other columns of the tensor memory.  Results in fp32 are within 1.1e-7 of 64 bits
+// (16 x 128256 x 4096, 2-norm), a tenth of what sums in plain fp32 are off.
+//
+// Two kernels: pairs of CTAs with tiles of 256 x 256 where there are many rows, and one whose tiles have the weight's
+// rows as lanes and 16 to 128 rows of a where there are few; pairs_pay() below chooses.
 #include "fp8.cuh"
 #include "tc.cuh"
 
@@ -50,6 +54,12 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {  // the
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Starts a tile's way from this GPU's memory into its L2 cache.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* tm, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(tm)),
+               "r"(c0), "r"(c1)
+               : "memory");
 }
 // A tile load of this GPU's memory into this CTA, counted by a barrier of the pair's first CTA.
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
@@ -166,8 +176,13 @@ constexpr int kMmTile = 128 * 128;  // bytes of 128 rows of a group
 // One CTA works on 128 rows of the weight (DUAL: of gate and of up) and NT rows of a: the weight is the products'
 // first operand, so NT may be as small as 16 and the weight's bytes, which bound this, are read once.  The groups of
 // K are cut into `split` runs, one for each CTA of a cluster, whose sums meet in shared memory, in the order of the
-// runs.  A thread holds NT sums of its row of the weight; the scales of 32 groups at a time, each row's times the
-// block's, lie in shared memory.
+// runs: the same bits every time, one launch, no workspace.  A thread holds NT sums of its row of the weight (NT / 2
+// from 64 on); the scales of 32 groups at a time, each row's times the block's, lie in shared memory.
+//
+// 16 x 128256 x 4096 with an fp32 result: 83 us, 6.4 TB/s, 0.98 of the copy rate.  16 x 14336 x 4096 gate and up: 24.5 us,
+// 4.8 TB/s; 18 at the copy rate, the rest is the way in (scales, first copies) and out (cluster, code that runs once).
+// 1 x 4096 x 4096: 6.7 us, latency.  With 128 rows of a a tile's operands come from the L2 cache at 11 TB/s, which bounds
+// 512 x 4096 x 4096 (19 us).
 template <int NT, bool DUAL>
 struct FewCfg {
   static constexpr int A = (DUAL ? 2 : 1) * kMmTile, STAGE = A + NT * 128;
@@ -318,6 +333,14 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
   tc_fence_after();
   const uint32_t tmem = *slot;
   if (warp == 0) {
+    // The weight's first eight groups are on their way into the L2 cache while the launch before this one ends: gate and
+    // up 16 x 14336 x 4096 25.3 -> 24.5 us, 16 x 4096 x 14336 14.1 -> 13.2 (with 16 groups 28.7 and 13.9).  Should that
+    // launch write them, the cache has what it wrote: only copies into shared memory have to wait.
+    if (lane == 0)
+      for (int g = g0; g < g1 && g < g0 + 8; g++) {
+        tma_prefetch_2d(&tmW, g * kGroup, nt * 128);
+        if (DUAL) tma_prefetch_2d(&tmW1, g * kGroup, nt * 128);
+      }
     grid_dep_wait();
     grid_dep_launch();
     if (lane == 0) {
@@ -484,6 +507,15 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
 // Two CTAs (a cluster) work on 256 rows x 256 columns: each holds 128 rows of a and 128 of the weight's in shared
 // memory (32 KB a group), one thread of the first issues the products of both, and each ends with its own 128
 // rows x 256 columns.  A persistent grid, one CTA per SM.
+//
+// 8192 x 4096 x 14336: 426 us, 2260 TFLOP/s; 4096 x 14336 x 4096 gate and up with SwiGLU and its rounding: 490 us, 1960
+// TFLOP/s (bursts of 30 ms; in longer runs the power limit takes the clock to 1.48 GHz, and they take 510 and 575).  A
+// group's products take 512 cycles, and 780 to 900 pass for each: the way from them through the eight warps that add
+// them up (two tensor memory reads of 85 cycles and 128 multiply-adds each, two warps a quarter of the SM) and back is
+// longer than the other buffer's products.  Tried: products of 128 columns with barriers of their own (they run at half
+// the rate, by shared memory's bandwidth: 472 us where this took 457), sixteen warps of 64 columns (518 where eight
+// took 467), multiply-adds of one column (509 where two at a time took 463).  The sums and what is read take 192
+// registers; with 224 a thread instead of 232 the compiler moves them about (484 us where 232 took 427).
 struct PairArgs {
   MmArgs m;
   const float* sb1;  // of the second weight (SWIGLU)
@@ -907,7 +939,8 @@ static int pair_launch(const Operand& a, const Operand& b, const Operand* b1, in
 
 // Which of the two kernels: a wave of either takes about 7 us and 0.4 us for each of its groups (256 rows a tile of the
 // pairs', 64 or 128 of the other, whose K may be cut).  Measured over 65 to 2000 rows, N from 300 to 28000 and K from 300
-// to 8192 this takes the faster one but for ties within a tenth.
+// to 8192 this takes the faster one but for ties within a tenth: 200 x 4096 x 4096 20 us by pairs, 14 by the other;
+// 1000 x 4096 x 4096 21 and 40.
 static bool pairs_pay(int M, int N, int K, bool dual) {
   const int G = (K + 127) / 128;
   const FewPlan f = few_plan(M, N, G, dual);

@@ -207,6 +207,23 @@ def test_products_follow_the_definition(dt, M, N, K):
     assert np.all(np.abs(_np(got) - y) <= _tol(y, mag + np.abs(_np(add)), K, dt))
 
 
+# K cut over clusters of 2, 4 and 8, more than 32 groups in one run, several tiles a block
+WIDE = [(1, 900, 2100), (16, 4096, 4096), (30, 1000, 4096), (60, 2000, 2048), (128, 1000, 8192), (100, 640, 1536),
+        (7, 39000, 4300), (40, 19100, 4352), (16, 60000, 260), (4100, 5000, 300), (2048, 4096, 512)]
+
+
+@pytest.mark.parametrize("M,N,K", WIDE)
+def test_products_cut_and_tiled_in_every_way(M, N, K):
+    from rngd_pd import fp8
+    ops, y, mag = _simple(M, N, K)
+    add = torch.randn(M, N, generator=torch.Generator().manual_seed(9)).bfloat16()
+    got = fp8.matmul(*ops, dtype=torch.float32)
+    assert np.all(np.abs(_np(got) - y) <= _tol(y, mag, K, "fp32"))
+    got = fp8.matmul(*ops, dtype=torch.bfloat16, add=add.cuda())
+    y, mag = y + _np(add), mag + np.abs(_np(add))
+    assert np.all(np.abs(_np(got) - y) <= _tol(y, mag, K, "bf16"))
+
+
 def _simple(M, N, K, seed=0):
     a, av = _held(M, K, seed + 1)
     b, bv = _held(N, K, seed + 2)
@@ -268,7 +285,8 @@ def test_lost_groups_spoil_their_rows_alone(M):
 
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 128, 256), (16, 512, 1024), (5, 100, 300), (3, 129, 17), (33, 260, 640),
                                    (70, 384, 200), (128, 256, 128), (200, 330, 1000), (520, 640, 384), (1030, 200, 260),
-                                   (260, 1100, 500)])
+                                   (260, 1100, 500), (16, 1000, 4096), (30, 1000, 4096), (64, 500, 4096), (3, 19100, 4352),
+                                   (2100, 3001, 260), (700, 5000, 140)])
 def test_gate_and_up_follow_the_definition(M, N, K):
     from rngd_pd import fp8
     a, av = _held(M, K, M)
@@ -363,6 +381,41 @@ def test_graph_replays_and_other_streams_give_the_same():
             torch.cuda.synchronize()
             assert all(torch.equal(a.float(), b) for a, b in zip(got, want[i]))
             assert all(torch.equal(a.float(), b) for a, b in zip(other, want[0]))
+
+
+def test_weights_written_by_the_launch_before():
+    """A weight quantised into memory that held another one, and multiplied with at once, over and over."""
+    from rngd_pd import fp8
+    g = torch.Generator().manual_seed(4)
+    a = fp8.quantize(torch.randn(5, 4096, generator=g).cuda())
+    ws = [(torch.randn(2048, 4096, generator=g) * 0.02).cuda() for _ in range(3)]
+    want = []
+    for w in ws:
+        b = fp8.quantize_weight(w)
+        torch.cuda.synchronize()
+        want.append((fp8.matmul(*a, *b, dtype=torch.float32), fp8.matmul_swiglu(*a, *b, *b)[0].float()))
+        torch.cuda.synchronize()
+    got = []
+    for i in range(60):
+        b = fp8.quantize_weight(ws[i % 3])
+        got.append((fp8.matmul(*a, *b, dtype=torch.float32), fp8.matmul_swiglu(*a, *b, *b)[0]))
+        del b  # the next one gets its memory
+    for i, (y, q) in enumerate(got):
+        assert torch.equal(y, want[i % 3][0]) and torch.equal(q.float(), want[i % 3][1])
+
+
+def test_calls_on_two_streams_at_once():
+    from rngd_pd import fp8
+    cases = [_simple(*d)[0] for d in ((3, 3000, 4096), (300, 1500, 2048), (40, 2000, 1000), (1000, 2000, 512))]
+    want = [fp8.matmul(*c, dtype=torch.float32) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(40):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((i * 3 % 4, fp8.matmul(*cases[i * 3 % 4], dtype=torch.float32)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[c]) for c, y in got)
 
 
 def test_the_same_call_twice_gives_the_same_bits():
