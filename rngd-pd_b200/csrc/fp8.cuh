@@ -249,7 +249,19 @@ __device__ __forceinline__ void store_held(uint8_t* dst, int left, const float* 
   }
 }
 
-// SwiGLU in fp32: silu(g) * u.  exp(-g) beyond 2^128 gives g / inf = -0, as the function's limit.
-__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+// SwiGLU in fp32: silu(g) * u, g / (1 + 2^(-g log2 e)) by the machine's power of two and reciprocal (2 and 1 units in the
+// last place; the exponent's rounding is |g| / 2 of them).  A power beyond the range gives a reciprocal of 0, the limit.
+__device__ __forceinline__ float swiglu(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
+// the largest magnitude of three, NaN if any is
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 }  // namespace rngd

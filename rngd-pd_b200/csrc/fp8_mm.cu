@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
           float most = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            y[e] = n + e < a.N ? swiglu(y[e], u[e]) : 0.f;
+            y[e] = swiglu(y[e], u[e]);  // (zeros beyond N: the tile loads filled the weights' rows with them)
             most = max_nan(most, fabsf(y[e]));
           }
 #pragma unroll
@@ -589,7 +589,8 @@ __device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* ac
 }
 
 // 64 gate sums and 64 up sums of row m, columns n0 ..: the other 64 of the group are another warp's, so the maximum
-// meets in shared memory.
+// meets in shared memory.  (Columns beyond N come last in a row, and their sums are zeros: the tile loads filled the
+// weights' rows with them.  A row that is not there may hold anything.)
 __device__ __forceinline__ void pair_store_swiglu(const PairArgs& p, const uint64_t* acc, int m, bool row, int n0, int grp,
                                                   int h, int r, int quarter, float* s_amax) {
   const int N = p.m.N;
@@ -597,9 +598,9 @@ __device__ __forceinline__ void pair_store_swiglu(const PairArgs& p, const uint6
 #pragma unroll
   for (int j = 0; j < 32; j++) {
     const float2 g = parts_of(acc[j]), u = parts_of(acc[32 + j]);
-    v[2 * j] = n0 + 2 * j < N ? swiglu(g.x, u.x) : 0.f;
-    v[2 * j + 1] = n0 + 2 * j + 1 < N ? swiglu(g.y, u.y) : 0.f;
-    most = max_nan(most, max_nan(fabsf(v[2 * j]), fabsf(v[2 * j + 1])));
+    v[2 * j] = swiglu(g.x, u.x);
+    v[2 * j + 1] = swiglu(g.y, u.y);
+    most = max3_abs(most, v[2 * j], v[2 * j + 1]);
   }
   s_amax[h * 128 + r] = most;
   asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
@@ -607,17 +608,15 @@ __device__ __forceinline__ void pair_store_swiglu(const PairArgs& p, const uint6
   if (!row) return;
   if (h == 0) p.scale[(long)m * ((N + 127) / 128) + grp] = lim / 448.0f;
   uint8_t* q = p.q + (long)m * p.ldq + n0;
+  if (n0 + 64 <= N) {
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const float* f = v + 16 * j;
-    if (n0 + 16 * j + 16 <= N) {
-      const uint2 x = held8(f, inv), y = held8(f + 8, inv);
+    for (int j = 0; j < 4; j++) {
+      const uint2 x = held8(v + 16 * j, inv), y = held8(v + 16 * j + 8, inv);
       *(uint4*)(q + 16 * j) = make_uint4(x.x, x.y, y.x, y.y);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; e++)
-        if (n0 + 16 * j + e < N) q[16 * j + e] = e4m3(f[e] * inv);
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) store_held<false>(q + 8 * j, N - n0 - 8 * j, v + 8 * j, inv);
   }
 }
 
@@ -737,20 +736,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int nblocks = (a.N + 127) / 128;
     int it = 0, round = 0;
     bool ok = true;  // a wait that ran out ends the waiting, but no warp leaves the others alone at a barrier
-    for (int t = pair; t < tiles; t += pairs, round++) {
-      int mt, nt;
+    // Scales are fetched a group ahead, a tile's first before the last one's results go out.  A row that is not there
+    // takes the first one's, and nothing of it is stored.
+    int mt, nt;
+    const float *sa, *sb, *sb1;
+    float na, nb0, nb1;
+    auto begin = [&](int t) {
       pair_tile(t, p.tm, p.tn, &mt, &nt);
-      const int m = mt * 256 + (int)rank * 128 + r;
-      const bool row = m < a.M;
-      const int nb = SWIGLU ? nt : (2 * nt + h < nblocks ? 2 * nt + h : nblocks - 1);
-      const float* sa = a.sa + (row ? m : 0) * a.sa_m;
-      const float* sb = a.sb + nb * a.sb_n;
-      const float* sb1 = SWIGLU ? p.sb1 + nb * p.sb1_n : nullptr;
+      const int m = mt * 256 + (int)rank * 128 + r, nb = SWIGLU ? nt : min(2 * nt + h, nblocks - 1);
+      sa = a.sa + (m < a.M ? m : 0) * a.sa_m;
+      sb = a.sb + nb * a.sb_n;
+      sb1 = SWIGLU ? p.sb1 + nb * p.sb1_n : nullptr;
+      na = __ldg(sa);
+      nb0 = __ldg(sb);
+      nb1 = SWIGLU ? __ldg(sb1) : 0.f;
+    };
+    begin(pair);
+    for (int t = pair; t < tiles; t += pairs, round++) {
       uint64_t acc[64];
 #pragma unroll
       for (int j = 0; j < 64; j++) acc[j] = 0ull;
-      // scales a group ahead; a row that is not there takes the first one's, and nothing of it is stored
-      float na = __ldg(sa), nb0 = __ldg(sb), nb1 = SWIGLU ? __ldg(sb1) : 0.f;
       for (int i = 0; i < a.G; i++, it++) {
         const int buf = it & 1;
         const float s0 = na * nb0, s1 = SWIGLU ? na * nb1 : s0;
@@ -772,12 +777,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (lane == 0) mbar_arrive_cluster(bar_empty + 8 * buf);  // before the rest is added: the products wait for it
         scale_add(acc + 32, v, s1);
       }
-      if (SWIGLU) {
-        pair_store_swiglu(p, acc, m, row && ok, nt * 128 + 64 * h, nt, h, r, warp & 3, s_amax + (round & 1) * 256);
-      } else {
-        pair_store<DT>(p, acc, mt * 256 + (int)rank * 128 + (warp & 3) * 32, nt * 256 + 128 * h,
-                       s_room + (warp - 4) * 32 * kPairPitch, ok);
-      }
+      const int m = mt * 256 + (int)rank * 128 + r, n = nt;
+      if (t + pairs < tiles) begin(t + pairs);
+      if (SWIGLU)
+        pair_store_swiglu(p, acc, m, m < a.M && ok, n * 128 + 64 * h, n, h, r, warp & 3, s_amax + (round & 1) * 256);
+      else
+        pair_store<DT>(p, acc, m - lane, n * 256 + 128 * h, s_room + (warp - 4) * 32 * kPairPitch, ok);
     }
   }
   tc_fence_before();
