@@ -508,9 +508,10 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
 // memory (32 KB a group), one thread of the first issues the products of both, and each ends with its own 128
 // rows x 256 columns.  A persistent grid, one CTA per SM.
 //
-// 8192 x 4096 x 14336: 426 us, 2260 TFLOP/s; 4096 x 14336 x 4096 gate and up with SwiGLU and its rounding: 490 us, 1960
-// TFLOP/s (bursts of 30 ms; in longer runs the power limit takes the clock to 1.48 GHz, and they take 510 and 575).  A
-// group's products take 512 cycles, and 780 to 900 pass for each: the way from them through the eight warps that add
+// 8192 x 4096 x 14336: 426 us, 2260 TFLOP/s; 4096 x 14336 x 4096 gate and up with SwiGLU and its rounding: 436 us, 2205
+// TFLOP/s (bursts of 30 ms; in longer runs the power limit takes the clock to 1.48 GHz, and they take 510 and 520).  A
+// tile's results take 4000 to 8000 cycles to go out, while the products run two groups ahead.  A
+// group's products take 512 cycles, and 780 to 800 pass for each: the way from them through the eight warps that add
 // them up (two tensor memory reads of 85 cycles and 128 multiply-adds each, two warps a quarter of the SM) and back is
 // longer than the other buffer's products.  Tried: products of 128 columns with barriers of their own (they run at half
 // the rate, by shared memory's bandwidth: 472 us where this took 457), sixteen warps of 64 columns (518 where eight
@@ -537,12 +538,12 @@ template <int DT>
 __device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* acc, long m0, int n0, float* room, bool ok) {
   const MmArgs& a = p.m;
   const int lane = threadIdx.x & 31;
-  constexpr bool AHEAD = DT != F8_F32;  // what is added comes while the sums are laid out; registers do not reach in fp32
+  constexpr bool AHEAD = DT != F8_F32;  // what is added comes while the sums are laid out; in fp32 registers reach for two rows at a time
 #pragma unroll
   for (int c = 0; c < 4; c++) {
     const int n = n0 + 32 * c, n8 = n + (lane & 3) * 8;
     const bool whole = p.vec && n + 32 <= a.N, plus = whole && a.add != nullptr;
-    Eight<DT> add[AHEAD ? 4 : 1];
+    Eight<DT> add[AHEAD ? 4 : 2];
     auto fetch = [&](Eight<DT>& to, int i) {
       const long m = m0 + 8 * i + (lane >> 2);
       if (plus && m < a.M) to.load_any(a.add, m * a.ldadd + n8);
@@ -558,7 +559,7 @@ __device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* ac
     }
     __syncwarp();
     if (whole) {
-#pragma unroll(AHEAD ? 4 : 1)
+#pragma unroll(AHEAD ? 4 : 2)
       for (int i = 0; i < 4; i++) {
         const int r = 8 * i + (lane >> 2);
         const float* f = room + r * kPairPitch + (lane & 3) * 8;
@@ -567,8 +568,11 @@ __device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* ac
         *(float4*)(v + 4) = *(const float4*)(f + 4);
         if (plus) {
           float w[8];
-          if (!AHEAD) fetch(add[0], i);
-          add[AHEAD ? i : 0].values(w);
+          if (!AHEAD && i % 2 == 0) {
+            fetch(add[0], i);
+            fetch(add[1], i + 1);
+          }
+          add[AHEAD ? i : i % 2].values(w);
 #pragma unroll
           for (int e = 0; e < 8; e++) v[e] += w[e];
         }
