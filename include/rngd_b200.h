@@ -391,7 +391,7 @@ int rngd_beam_workspace(int dtype, int R, int V, int W, size_t* bytes);
  * weights [N][K] one for each block of 128 x 128, [ceil(N / 128)][G].  With m = max(amax, 2^-100) of a group,
  * scale = m / 448 and a value x is held as e4m3(x * (448 / m)); a group with a NaN or an infinity is lost (it reads
  * as NaN).  8-bit rows start on 16 bytes: q 16-byte aligned, ldq (bytes) a multiple of 16; bytes of a row beyond its
- * values are neither written nor read.  Row strides are in elements.  All arrays are device memory.
+ * values are neither written nor read.  Row strides are in elements.  All arrays are device memory.  K is at most 2^30.
  * x [T][K] -> q, scale [T][G] (contiguous). */
 int rngd_f8_rows(const void* x, int dtype, int64_t ldx, int64_t T, int K, void* q, int64_t ldq, float* scale,
                  rngd_stream_t stream);

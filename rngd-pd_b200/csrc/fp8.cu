@@ -293,8 +293,9 @@ __device__ __forceinline__ void norm_store(const NormArgs& a, long row, int g0, 
 
 template <bool VEC>
 constexpr int kNormThreads = VEC ? 512 : 384;  // 384: at 80 registers two blocks' warps fit an SM's quarters
-// The next row is on its way while the present one is summed and rounded (where rows are whole vectors: the others'
-// registers go further as a second block an SM; 8000 x 4097 bf16 with a residual 98 us, ahead of time 121); the weights stay in registers.
+// The next row is on its way while the present one is summed and rounded, and the weights stay in registers.  (Only where
+// rows are whole vectors: the others' registers go further as a second block an SM; 8000 x 4097 bf16 with a residual
+// takes 98 us, 121 with the next row on its way.)
 template <int DT, int WT, bool VEC, int PER>
 __global__ void __launch_bounds__(kNormThreads<VEC>, VEC ? 0 : 2) f8_norm_kernel(NormArgs a) {
   __shared__ float s_sum[2][32];  // for each of two rows in turn
@@ -387,7 +388,8 @@ template <int DT, bool VEC>
 struct RowsLaunch {
   static int go(const RowsArgs& a, cudaStream_t s) {
     const long runs = a.T * ((a.G + kRowsPer - 1) / kRowsPer);
-    return launch_pdl(f8_rows_kernel<DT, VEC>, dim3((unsigned)((runs + kRowsThreads / kLanes - 1) / (kRowsThreads / kLanes))), dim3(kRowsThreads), 0, s,
+    constexpr int per = kRowsThreads / kLanes;
+    return launch_pdl(f8_rows_kernel<DT, VEC>, dim3((unsigned)((runs + per - 1) / per)), dim3(kRowsThreads), 0, s,
                       "f8_rows_kernel", a);
   }
 };
@@ -437,7 +439,7 @@ using namespace rngd;
 extern "C" int rngd_f8_rows(const void* x, int dtype, int64_t ldx, int64_t T, int K, void* q, int64_t ldq, float* scale,
                             rngd_stream_t stream) {
   RNGD_REQUIRE(dtype >= F8_BF16 && dtype <= F8_F32, "f8_rows: data type %d", dtype);
-  RNGD_REQUIRE(T >= 0 && K >= 0, "f8_rows: %ld rows of %d", (long)T, K);
+  RNGD_REQUIRE(T >= 0 && K >= 0 && K <= kMostK, "f8_rows: %ld rows of %d", (long)T, K);
   if (T == 0 || K == 0) return RNGD_OK;
   const int G = (int)(((long)K + kGroup - 1) / kGroup);
   RNGD_REQUIRE(T <= 0x7FFFFFFFl && T * ((G + kRowsPer - 1) / kRowsPer) <= 0x7FFFFFFFl, "f8_rows: %ld rows of %d", (long)T, K);
@@ -450,7 +452,7 @@ extern "C" int rngd_f8_rows(const void* x, int dtype, int64_t ldx, int64_t T, in
 extern "C" int rngd_f8_weight(const void* w, int dtype, int64_t ldw, int N, int K, void* q, int64_t ldq, float* scale,
                               rngd_stream_t stream) {
   RNGD_REQUIRE(dtype >= F8_BF16 && dtype <= F8_F32, "f8_weight: data type %d", dtype);
-  RNGD_REQUIRE(N >= 0 && K >= 0, "f8_weight: %d x %d", N, K);
+  RNGD_REQUIRE(N >= 0 && N <= kMostRows && K >= 0 && K <= kMostK, "f8_weight: %d x %d", N, K);
   if (N == 0 || K == 0) return RNGD_OK;
   const int G = (int)(((long)K + kGroup - 1) / kGroup);
   RNGD_REQUIRE(((long)N + 127) / 128 * G <= 0x7FFFFFFFl, "f8_weight: %d x %d", N, K);
@@ -466,7 +468,7 @@ extern "C" int rngd_f8_rms_norm(const void* x, int64_t ldx, const void* residual
   RNGD_REQUIRE(dtype >= F8_BF16 && dtype <= F8_F32, "f8_rms_norm: data type %d", dtype);
   RNGD_REQUIRE(weight_dtype == dtype || weight_dtype == F8_F32, "f8_rms_norm: weights of data type %d with rows of %d",
                weight_dtype, dtype);
-  RNGD_REQUIRE(T >= 0 && T <= 0x7FFFFFFFl && K >= 0, "f8_rms_norm: %ld rows of %d", (long)T, K);
+  RNGD_REQUIRE(T >= 0 && T <= 0x7FFFFFFFl && K >= 0 && K <= kMostK, "f8_rms_norm: %ld rows of %d", (long)T, K);
   if (T == 0 || K == 0) return RNGD_OK;
   const int sz = dtype_size(dtype), G = (int)(((long)K + kGroup - 1) / kGroup);
   RNGD_REQUIRE(x != nullptr && weight != nullptr, "f8_rms_norm: null pointer");

@@ -16,6 +16,7 @@
 namespace rngd {
 
 constexpr int kGroup = 128;
+constexpr int kMostK = 1 << 30, kMostRows = 0x7FFFFFFF - 255;  // places within a row, and tiles' ends, are 32-bit numbers
 
 enum : int { F8_BF16 = 0, F8_F16 = 1, F8_F32 = 2 };
 
@@ -155,7 +156,8 @@ struct EightAt {
         if constexpr (SZ == 4) {
           w[j] = j < n ? __float_as_uint(((const float*)at)[j]) : 0u;
         } else {
-          const uint32_t l = 2 * j < n ? ((const uint16_t*)at)[2 * j] : 0u, h = 2 * j + 1 < n ? ((const uint16_t*)at)[2 * j + 1] : 0u;
+          const uint16_t* half = (const uint16_t*)at;
+          const uint32_t l = 2 * j < n ? half[2 * j] : 0u, h = 2 * j + 1 < n ? half[2 * j + 1] : 0u;
           w[j] = l | h << 16;
         }
       }
@@ -203,8 +205,9 @@ __device__ __forceinline__ void store_eight(void* p, long i, const Eight<DT>& v)
   for (int j = 0; j < (DT == F8_F32 ? 2 : 1); j++) q[j] = v.r[j];
 }
 
-// A group lies in 8 neighbouring lanes, 16 values each: lane l has the vectors of eight at 8 l and at 64 + 8 l.  (16 lanes with eight each take a third more steps to the
-// group's maximum, and the quotients twice as often a value: rows of 8191 x 4096 bf16 then take 22.7 us, not 17.6.)
+// A group lies in 8 neighbouring lanes, 16 values each: lane l has the vectors of eight at 8 l and at 64 + 8 l.  (16 lanes
+// with eight each take a third more steps to the group's maximum, and the quotients twice as often a value: rows of
+// 8191 x 4096 bf16 then take 17.6 us, not 16.4.)
 constexpr int kLanes = 8;
 __device__ __forceinline__ float amax_lanes(float m) {
 #pragma unroll

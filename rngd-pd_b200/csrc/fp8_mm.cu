@@ -189,7 +189,7 @@ struct FewCfg {
   static constexpr int COLS = (DUAL ? 2 : 1) * NT;     // columns of one buffer in tensor memory
   static constexpr int GROUPS = NT >= 64 ? 2 : 1;      // warpgroups that share them, by rows of a
   static constexpr int SUMMERS = 128 * GROUPS, THREADS = 64 + SUMMERS, TN = NT / GROUPS;
-  static constexpr int STEP = NT == 16 || NT == 64 ? 16 : 32;  // columns read at a time (32 spill registers with 64)
+  static constexpr int STEP = NT == 16 || NT == 64 ? 16 : 32;  // columns read at a time (with NT = 64 reads of 32 would spill)
   static constexpr int BUFS = NT <= 32 ? 4 : 2;
   static constexpr int CHUNK = 32;                     // groups whose scales are in shared memory
   static constexpr int PITCH = COLS + 4;               // floats of a group's; fewer of the stores' banks meet
@@ -412,7 +412,8 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
           // a row's scales by neighbouring threads, eight loads a thread at a time, so that their latencies overlap
           for (int e0 = et; e0 < NT * C::CHUNK; e0 += 8 * C::SUMMERS) {
             const int g = et % C::CHUNK, gg = c0 + min(g, n - 1);
-            const float b = __ldg(a.sb + nt * a.sb_n + gg * a.sb_g), b1 = DUAL ? __ldg(p.sb1 + nt * p.sb1_n + gg * p.sb1_g) : 0.f;
+            const float b = __ldg(a.sb + nt * a.sb_n + gg * a.sb_g);
+            const float b1 = DUAL ? __ldg(p.sb1 + nt * p.sb1_n + gg * p.sb1_g) : 0.f;
             float x[8];
 #pragma unroll
             for (int u = 0; u < 8; u++) {
@@ -538,7 +539,8 @@ template <int DT>
 __device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* acc, long m0, int n0, float* room, bool ok) {
   const MmArgs& a = p.m;
   const int lane = threadIdx.x & 31;
-  constexpr bool AHEAD = DT != F8_F32;  // what is added comes while the sums are laid out; in fp32 registers reach for two rows at a time
+  // What is added comes while the sums are laid out; in fp32 the registers reach for two rows at a time only.
+  constexpr bool AHEAD = DT != F8_F32;
 #pragma unroll
   for (int c = 0; c < 4; c++) {
     const int n = n0 + 32 * c, n8 = n + (lane & 3) * 8;
@@ -672,63 +674,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   // The 384 threads start with 168 registers each: 64512.  Four warps give up theirs for the eight that hold the sums:
   // 128 * (40 + 2 * 232) = 64512.
   if (warp < 4) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-   if (warp == 0) {
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        int mt, nt;
-        pair_tile(t, p.tm, p.tn, &mt, &nt);
-        const CUtensorMap* tb = SWIGLU && rank ? &tmB1 : &tmB;
-        const int n0 = SWIGLU ? nt * 128 : nt * 256 + (int)rank * 128;
-        for (int i = 0; i < a.G; i++, it++) {
-          const int s = it % kPairStages;
-          ok = mbar_wait(&empty[s], ((uint32_t)(it / kPairStages) & 1u) ^ 1u, ST_TMA_WAIT, &g_status_f8);
-          if (!ok) break;
-          uint8_t* st = base + s * kPairStage;
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStage);  // both CTAs' tiles
-          const uint32_t bar = mapa(smem_u32(&full[s]), 0);
-          tma_load_2d_pair(st, &tmA, bar, i * kGroup, mt * 256 + (int)rank * 128);
-          tma_load_2d_pair(st + kMmTile, tb, bar, i * kGroup, n0);
-        }
-      }
-      // what is in flight lands before the blocks may end: the last products' arrivals, or, where a wait ran out, copies
-      if (ok || rank == 0)
-        for (int j = it < kPairStages ? 0 : it - kPairStages; j < it; j++)
-          mbar_wait(ok ? &empty[j % kPairStages] : &full[j % kPairStages], (uint32_t)(j / kPairStages) & 1u, ST_TMA_WAIT,
-                    &g_status_f8);
-      grid_dep_launch();
-    }
-    __syncwarp();
-   } else if (warp == 1) {
-    // The whole warp runs the loop and one elected lane issues: with operands that the compiler knows to be the
-    // warp's own, an issue takes a fraction of the time that it takes under a branch on the lane.
-    if (rank == 0) {
-      const uint32_t idesc = idesc_e4m3_f32(256, 256);
-      const uint64_t desc = sw128_kmajor_desc(smem_u32(base));
-      int it = 0;
-      bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs)
-        for (int i = 0; i < a.G; i++, it++) {
-          const int s = it % kPairStages, buf = it & 1;
-          ok = mbar_wait(&full[s], (uint32_t)(it / kPairStages) & 1u, ST_MMA_WAIT, &g_status_f8) &&
-               mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t da = desc + (uint64_t)(s * (kPairStage >> 4)), db = da + (kMmTile >> 4);
-          const uint32_t d = tmem + (uint32_t)(buf * 256);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++) umma_e4m3_pair(d, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
-            umma_commit_pair(&empty[s]);
-            umma_commit_pair(&acc_full[buf]);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      if (lane == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int t = pair; t < tiles && ok; t += pairs) {
+          int mt, nt;
+          pair_tile(t, p.tm, p.tn, &mt, &nt);
+          const CUtensorMap* tb = SWIGLU && rank ? &tmB1 : &tmB;
+          const int n0 = SWIGLU ? nt * 128 : nt * 256 + (int)rank * 128;
+          for (int i = 0; i < a.G; i++, it++) {
+            const int s = it % kPairStages;
+            ok = mbar_wait(&empty[s], ((uint32_t)(it / kPairStages) & 1u) ^ 1u, ST_TMA_WAIT, &g_status_f8);
+            if (!ok) break;
+            uint8_t* st = base + s * kPairStage;
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStage);  // both CTAs' tiles
+            const uint32_t bar = mapa(smem_u32(&full[s]), 0);
+            tma_load_2d_pair(st, &tmA, bar, i * kGroup, mt * 256 + (int)rank * 128);
+            tma_load_2d_pair(st + kMmTile, tb, bar, i * kGroup, n0);
           }
-          __syncwarp();
         }
+        // what is in flight lands before the blocks may end: the last products' arrivals, or, where a wait ran out, copies
+        if (ok || rank == 0)
+          for (int j = it < kPairStages ? 0 : it - kPairStages; j < it; j++)
+            mbar_wait(ok ? &empty[j % kPairStages] : &full[j % kPairStages], (uint32_t)(j / kPairStages) & 1u, ST_TMA_WAIT,
+                      &g_status_f8);
+        grid_dep_launch();
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      // The whole warp runs the loop and one elected lane issues: with operands that the compiler knows to be the
+      // warp's own, an issue takes a fraction of the time that it takes under a branch on the lane.
+      if (rank == 0) {
+        const uint32_t idesc = idesc_e4m3_f32(256, 256);
+        const uint64_t desc = sw128_kmajor_desc(smem_u32(base));
+        int it = 0;
+        bool ok = true;
+        for (int t = pair; t < tiles && ok; t += pairs)
+          for (int i = 0; i < a.G; i++, it++) {
+            const int s = it % kPairStages, buf = it & 1;
+            ok = mbar_wait(&full[s], (uint32_t)(it / kPairStages) & 1u, ST_MMA_WAIT, &g_status_f8) &&
+                 mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t da = desc + (uint64_t)(s * (kPairStage >> 4)), db = da + (kMmTile >> 4);
+            const uint32_t d = tmem + (uint32_t)(buf * 256);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < 4; kk++) umma_e4m3_pair(d, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
+              umma_commit_pair(&empty[s]);
+              umma_commit_pair(&acc_full[buf]);
+            }
+            __syncwarp();
+          }
+      }
     }
-   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // Eight warps: the lane quarter warp & 3 (the rows that a warp may read), half h of the columns.  A thread's
@@ -976,7 +978,7 @@ extern "C" int rngd_f8_matmul(const void* a, int64_t lda, const float* a_scale, 
                               const void* add, int64_t ldadd, void* y, int64_t ldy, int dtype, rngd_stream_t stream) {
   RNGD_REQUIRE(dtype >= F8_BF16 && dtype <= F8_F32, "f8_matmul: data type %d", dtype);
   RNGD_REQUIRE(M >= 0 && N >= 0 && K >= 1, "f8_matmul: %d x %d x %d", M, N, K);
-  RNGD_REQUIRE(K <= 0x7FFFFFFF - 127, "f8_matmul: K=%d", K);
+  RNGD_REQUIRE(M <= kMostRows && N <= kMostRows && K <= kMostK, "f8_matmul: %d x %d x %d is too much", M, N, K);
   if (M == 0 || N == 0) return RNGD_OK;
   const uintptr_t mis = dtype == F8_F32 ? 3 : 1;
   RNGD_REQUIRE(y != nullptr && a_strides != nullptr && b_strides != nullptr, "f8_matmul: null pointer");
@@ -997,7 +999,7 @@ extern "C" int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, 
                               const void* up, int64_t ldu, const float* up_scale, const int64_t* up_strides, int M, int N,
                               int K, void* q, int64_t ldq, float* scale, rngd_stream_t stream) {
   RNGD_REQUIRE(M >= 0 && N >= 0 && K >= 1, "f8_swiglu: %d x %d x %d", M, N, K);
-  RNGD_REQUIRE(K <= 0x7FFFFFFF - 127 && N <= 0x7FFFFFFF - 127, "f8_swiglu: %d x %d x %d", M, N, K);
+  RNGD_REQUIRE(M <= kMostRows && N <= kMostRows && K <= kMostK, "f8_swiglu: %d x %d x %d is too much", M, N, K);
   if (M == 0 || N == 0) return RNGD_OK;
   RNGD_REQUIRE(q && scale && a_strides && gate_strides && up_strides, "f8_swiglu: null pointer");
   RNGD_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)scale & 3) == 0 && (M <= 1 || (ldq >= N && ldq % 16 == 0)),

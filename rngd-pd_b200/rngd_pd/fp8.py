@@ -28,7 +28,7 @@ _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _E4M3 = torch.float8_e4m3fn
 _F32 = torch.float32
 _empty = torch.empty_strided  # half of torch.empty's time on the host
-_INT_MAX = 2 ** 31 - GROUP
+_MOST_K = 2 ** 30
 _check, _stream = _lib.check, torch._C._cuda_getCurrentRawStream
 _current = torch._C._cuda_getDevice  # the calls start over with the tensors' GPU where another is current
 _rows, _weight, _norm = _lib.lib.rngd_f8_rows, _lib.lib.rngd_f8_weight, _lib.lib.rngd_f8_rms_norm
@@ -80,7 +80,7 @@ def _operand(name, q, scale, blocks):
     if (k > 1 and strides[1] != 1) or (n > 1 and (ld % 16 or ld < k)):
         raise ValueError(f"{name} {tuple(shape)} strides {strides}: rows must be contiguous, start on 16 bytes and not "
                          "overlap")
-    if k == 0 or k > _INT_MAX:
+    if k == 0 or k > _MOST_K:
         raise ValueError(f"{name} {tuple(shape)}: nothing to sum, or too much")
     want = (_groups(n) if blocks else n, _groups(k))
     if scale[0] != want or scale[2] is not _F32 or scale[3] != dev:

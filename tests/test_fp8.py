@@ -44,7 +44,9 @@ def test_c_entries_refuse_bad_arguments():
         (lambda: lib.rngd_f8_rms_norm(p, 8, p, 8, p, 0, 0, 1, 8, 1e-5, p, 8, p, 16, p, None), "place of its own"),
         (lambda: lib.rngd_f8_rms_norm(p, 8, None, 0, None, 0, 0, 1, 8, 1e-5, None, 0, p, 16, p, None), "null"),
         (lambda: mm(dt=5), "data type 5"), (lambda: mm(K=0), "x 0"), (lambda: mm(M=-1), "-1 x"),
-        (lambda: mm(K=2 ** 31 - 2), "K="), (lambda: mm(a=odd), "misaligned"), (lambda: mm(lda=250), "250 apart"),
+        (lambda: mm(K=2 ** 31 - 2), "too much"), (lambda: mm(N=2 ** 31 - 2), "too much"), (lambda: sw(K=2 ** 30 + 1), "too much"),
+        (lambda: lib.rngd_f8_rows(p, 0, 8, 1, 2 ** 30 + 1, p, 16, p, None), "1073741825"),
+        (lambda: lib.rngd_f8_rows(p, 0, 8, 2 ** 33, 8, p, 16, p, None), "8589934592 rows"), (lambda: mm(a=odd), "misaligned"), (lambda: mm(lda=250), "250 apart"),
         (lambda: mm(ldb=128), "128 apart"), (lambda: mm(b=None), "null"), (lambda: mm(sa=None), "null"),
         (lambda: mm(y=None), "null"), (lambda: mm(y=odd), "misaligned"), (lambda: mm(add=odd), "misaligned"),
         (lambda: mm(ldy=3), "lie on one another"), (lambda: mm(ss=None), "null"),
