@@ -259,8 +259,11 @@ __device__ __forceinline__ void store_sums(const MmArgs& a, float* v, long m, in
     store_eight<DT>(a.y, o, eight_of<DT>(v));
   } else {
 #pragma unroll
+    for (int e = 0; e < 8; e++)  // (all loads before the first store, which might be to the same place)
+      if (a.add != nullptr && n + e < a.N) v[e] += load_as_f32<DT>(a.add, oa + e);
+#pragma unroll
     for (int e = 0; e < 8; e++)
-      if (n + e < a.N) store_f32_as<DT>(a.y, o + e, a.add != nullptr ? v[e] + load_as_f32<DT>(a.add, oa + e) : v[e]);
+      if (n + e < a.N) store_f32_as<DT>(a.y, o + e, v[e]);
   }
 }
 template <int THREADS>
@@ -580,14 +583,24 @@ __device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* ac
         }
         if (m0 + r < a.M && ok) store_eight<DT>(a.y, (m0 + r) * a.ldy + n8, eight_of<DT>(v));
       }
-    } else if (n + lane < a.N && ok) {
+    } else if (n + lane < a.N && ok && a.add == nullptr) {  // a column a lane
 #pragma unroll 2
-      for (int r = 0; r < 32; r++) {
-        const long m = m0 + r;
-        const float v = room[r * kPairPitch + lane];
-        if (m < a.M)
-          store_f32_as<DT>(a.y, m * a.ldy + n + lane,
-                           a.add != nullptr ? v + load_as_f32<DT>(a.add, m * a.ldadd + n + lane) : v);
+      for (int r = 0; r < 32; r++)
+        if (m0 + r < a.M) store_f32_as<DT>(a.y, (m0 + r) * a.ldy + n + lane, room[r * kPairPitch + lane]);
+    } else if (n + lane < a.N && ok) {
+      // with what is added, eight rows at a time: 6206 x 1423 x 4519 fp32 93 us, 219 two at a time
+      for (int r0 = 0; r0 < 32 && m0 + r0 < a.M; r0 += 8) {
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const long m = m0 + r0 + i;
+          w[i] = m < a.M ? load_as_f32<DT>(a.add, m * a.ldadd + n + lane) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const long m = m0 + r0 + i;
+          if (m < a.M) store_f32_as<DT>(a.y, m * a.ldy + n + lane, room[(r0 + i) * kPairPitch + lane] + w[i]);
+        }
       }
     }
     __syncwarp();
