@@ -401,6 +401,7 @@ struct WeightLaunch {
   }
 };
 constexpr int kSmSmem = 200 * 1024;  // what the blocks of an SM may have of its shared memory
+constexpr int kStageSmem = 47 * 1024;  // what a block may have for its row beside the kernel's own, without asking
 template <int DT, bool VEC>
 struct NormLaunch {
   static int go(const NormArgs& a, bool w32, cudaStream_t s) {
@@ -483,6 +484,6 @@ extern "C" int rngd_f8_rms_norm(const void* x, int64_t ldx, const void* residual
                 total, (long)ldt, (uint8_t*)q, (long)ldq, scale};
   const bool vec = whole_vectors(x, ldx, K, dtype) && whole_vectors(weight, 0, K, weight_dtype) &&
                    (residual == nullptr || (whole_vectors(residual, ldr, K, dtype) && whole_vectors(total, ldt, K, dtype)));
-  a.stage = !vec && total != nullptr && (long)G * kGroup * sz <= 48 * 1024;
+  a.stage = !vec && total != nullptr && (long)G * kGroup * sz <= kStageSmem;
   return by_type<NormLaunch>(dtype, vec, a, weight_dtype == F8_F32, (cudaStream_t)stream);
 }

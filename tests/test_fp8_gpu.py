@@ -149,6 +149,15 @@ def test_norm_follows_the_definition(dt, T, K):
             _check_norm(x, weight, 1e-5, res, got)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("K", [6143, 6145, 12159, 12161, 12287, 12289, 16383, 16384])
+def test_norm_at_the_widths_where_its_layout_changes(dt, K):
+    """Rows that one, two and no registers' worth of groups hold, the sum's row in shared memory and not."""
+    from rngd_pd import fp8
+    x, r, w = _rows(3, K, dt, K), _rows(3, K, dt, K + 1, spread=3.0), torch.rand(K) + 0.5
+    _check_norm(x, w, 1e-5, r, fp8.rms_norm(x.cuda(), w.cuda(), 1e-5, r.cuda()))
+
+
 def test_norm_of_zero_rows_and_lost_ones():
     from rngd_pd import fp8
     x = torch.randn(4, 300)
