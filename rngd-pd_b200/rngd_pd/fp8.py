@@ -28,7 +28,9 @@ _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _E4M3 = torch.float8_e4m3fn
 _F32 = torch.float32
 _empty = torch.empty_strided  # half of torch.empty's time on the host
+# what the library counts with 32 bits; ctypes would cut greater numbers to their lowest 32
 _MOST_K = 2 ** 30
+_MOST_ROWS = 2 ** 31 - 256  # of a weight, and of a product's operands
 _check, _stream = _lib.check, torch._C._cuda_getCurrentRawStream
 _current = torch._C._cuda_getDevice  # the calls start over with the tensors' GPU where another is current
 _rows, _weight, _norm = _lib.lib.rngd_f8_rows, _lib.lib.rngd_f8_weight, _lib.lib.rngd_f8_rms_norm
@@ -64,9 +66,11 @@ def _groups(n):
 @functools.lru_cache(maxsize=4096)
 def _source(name, shape, strides, dtype, dev):
     """What the quantisers take from their input: (row stride, type's number, sizes, strides of the 8-bit rows and of
-    the scales, their number a row)."""
+    the scales, their number a row).  name: "w" of a weight, whose rows are counted with 32 bits too."""
     ld = _matrix(name, shape, strides, dtype, dev)
     T, K = shape
+    if K > _MOST_K or (name == "w" and T > _MOST_ROWS):
+        raise ValueError(f"{name} {tuple(shape)} is too much: {_MOST_ROWS} rows of a weight, {_MOST_K} values a row")
     return ld, _DT[dtype], T, K, ((K + 15) // 16 * 16, 1), (_groups(K), 1), _groups(K)
 
 
@@ -80,8 +84,8 @@ def _operand(name, q, scale, blocks):
     if (k > 1 and strides[1] != 1) or (n > 1 and (ld % 16 or ld < k)):
         raise ValueError(f"{name} {tuple(shape)} strides {strides}: rows must be contiguous, start on 16 bytes and not "
                          "overlap")
-    if k == 0 or k > _MOST_K:
-        raise ValueError(f"{name} {tuple(shape)}: nothing to sum, or too much")
+    if k == 0 or k > _MOST_K or n > _MOST_ROWS:
+        raise ValueError(f"{name} {tuple(shape)}: nothing to sum, or too much ({_MOST_ROWS} rows of {_MOST_K} values)")
     want = (_groups(n) if blocks else n, _groups(k))
     if scale[0] != want or scale[2] is not _F32 or scale[3] != dev:
         raise ValueError(f"{name}'s scale must be float32 {want} on {dev}, got {tuple(scale[0])} {scale[2]} on {scale[3]}")

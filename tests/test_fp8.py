@@ -84,3 +84,47 @@ def test_plain_forms_on_small_cases():
     sa, sb = np.array([[1.0, 2.0], [3.0, 4.0]]), np.array([[1.0, 1.0], [0.5, 2.0]])
     y, mag = ref.product(a, sa, b, sb)
     assert y[0, 0] == 128 + 4 and y[1, 128] == 128 * 1.5 + 2 * 8 and np.array_equal(y, mag)
+
+
+def _huge(shape, dtype=torch.bfloat16, ld=None):
+    """A tensor on the GPU by its shape and type alone: nothing is allocated, any launch would fail here."""
+    return torch.empty_strided(shape, (ld or shape[1], 1), dtype=dtype, device="cuda")
+
+
+@pytest.mark.parametrize("n", [2 ** 30 + 1, 2 ** 32, 2 ** 32 + 8])
+def test_widths_that_32_bits_do_not_hold_are_refused(n):
+    """Not cut to their lowest 32 bits: 2^32 values a row would pass for none, 2^32 + 8 for eight."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    e4m3, f32, G = torch.float8_e4m3fn, torch.float32, -(-n // 128)
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        x, w, v = _huge((1, n)), _huge((2, n)), torch.empty(n, dtype=torch.bfloat16, device="cuda")
+        q, s = _huge((1, n), e4m3, n + -n % 16), _huge((1, G), f32)
+        for f in (lambda: fp8.quantize(x), lambda: fp8.quantize_weight(w), lambda: fp8.rms_norm(x, v, 1e-5),
+                  lambda: fp8.rms_norm(x, v, 1e-5, residual=x), lambda: fp8.matmul(q, s, q, s),
+                  lambda: fp8.matmul_swiglu(q, s, q, s, q, s)):
+            with pytest.raises(ValueError, match=str(n)):
+                f()
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 255, 2 ** 32, 2 ** 32 + 8])
+def test_rows_that_32_bits_do_not_hold_are_refused(n):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    e4m3, f32, NB = torch.float8_e4m3fn, torch.float32, -(-n // 128)
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        w = _huge((n, 1))
+        many, one, block = (_huge((n, 1), e4m3, 16), _huge((n, 1), f32)), (_huge((1, 1), e4m3, 16), _huge((1, 1), f32)), \
+            _huge((NB, 1), f32)
+        for f in (lambda: fp8.quantize_weight(w), lambda: fp8.matmul(*many, *one), lambda: fp8.matmul(*one, many[0], block),
+                  lambda: fp8.matmul_swiglu(*many, *one, *one),
+                  lambda: fp8.matmul_swiglu(*one, many[0], block, many[0], block)):
+            with pytest.raises(ValueError, match=str(n)):
+                f()
+
+
+def test_the_greatest_sizes_pass_the_checks():
+    """2^30 values a row and 2^31 - 256 rows."""
+    dev, e4m3, f32 = torch.device("cuda", 0), torch.float8_e4m3fn, torch.float32
+    n = 2 ** 30
+    assert fp8._source("x", (1, n), (n, 1), torch.bfloat16, dev)[2:4] == (1, n)
+    n = 2 ** 31 - 256
+    assert fp8._operand("b", ((n, 1), (16, 1), e4m3, dev), ((n // 128, 1), (1, 1), f32, dev), True)[0] == n
