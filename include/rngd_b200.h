@@ -416,6 +416,10 @@ int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, const int64
                    int64_t ldg, const float* gate_scale, const int64_t* gate_strides, const void* up, int64_t ldu,
                    const float* up_scale, const int64_t* up_strides, int M, int N, int K, void* q, int64_t ldq,
                    float* scale, rngd_stream_t stream);
+/* For tests of what a host does when a device wait runs out.  While it is on, every rngd_f8_matmul and rngd_f8_swiglu
+ * that is launched waits for something that never comes: each gives up after the waits' limit (2 s), its results are NaN
+ * as always then, and the status word says so. */
+int rngd_f8_unanswered(int on);
 
 #ifdef __cplusplus
 }

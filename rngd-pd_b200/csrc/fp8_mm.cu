@@ -168,7 +168,13 @@ struct MmArgs {
   long ldy;
   const void* add;  // of y's type, or null
   long ldadd;
+  int unanswered;   // rngd_f8_unanswered: the sums wait for a barrier that nothing completes
 };
+
+// When a wait runs out.  Whoever gave up waits for nothing more, but comes to every barrier that the others wait at, and
+// its sums are NaN from there on, so that no result can pass for a good one.  It no longer says that it has read the
+// tensor memory: the products then stop (by their own wait), instead of going on into columns that slower warps still read.
+__device__ __forceinline__ float lost() { return __int_as_float(0x7FFFFFFF); }
 
 constexpr int kMmTile = 128 * 128;  // bytes of 128 rows of a group
 
@@ -202,7 +208,7 @@ struct FewCfg {
   static constexpr size_t SMEM = FIXED + STAGES * STAGE;
   static_assert(STAGES * STAGE >= COLS * 128 * 4, "the sums fit where the stages were");
   static_assert(BUFS * COLS * PER_SM <= 512 && BUFS * COLS >= 32 && ((BUFS * COLS) & (BUFS * COLS - 1)) == 0, "");
-  static_assert((2 * STAGES + 2 * BUFS + 1) * 8 + 16 <= 256, "barriers");
+  static_assert((2 * STAGES + 3 * BUFS + 2) * 8 + 16 <= 256, "barriers");
 };
 struct FewArgs {
   MmArgs m;
@@ -306,7 +312,9 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
   uint64_t* acc_full = empty + ST;           // [BUFS]
   uint64_t* acc_empty = acc_full + C::BUFS;  // [BUFS]
   uint64_t* done = acc_empty + C::BUFS;
-  uint32_t* slot = (uint32_t*)(done + 1);
+  uint64_t* quiet = done + 1;                // no copy and no product is on its way any more
+  uint64_t* never = quiet + 1;               // [BUFS]
+  uint32_t* slot = (uint32_t*)(never + C::BUFS);
   const MmArgs& a = p.m;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % p.split, tile = blockIdx.x / p.split;
@@ -320,8 +328,10 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
     for (int i = 0; i < C::BUFS; i++) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], C::SUMMERS / 32);
+      mbar_init(&never[i], 1);
     }
     mbar_init(done, C::SUMMERS / 32);
+    mbar_init(quiet, 2);
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
@@ -362,6 +372,7 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
       if (!ok)  // a wait ran out: the copies in flight land before the block may end
         for (int j = i < ST ? 0 : i - ST; j < i; j++)
           mbar_wait(&full[j % ST], (uint32_t)(j / ST) & 1u, ST_TMA_WAIT, &g_status_f8);
+      mbar_arrive(quiet);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -369,7 +380,8 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
     grid_dep_launch();
     const uint32_t idesc = idesc_e4m3_f32(128, NT);
     const uint64_t desc = sw128_kmajor_desc(smem_u32(base));
-    for (int i = 0; i < g1 - g0; i++) {
+    int i = 0;
+    for (; i < g1 - g0; i++) {
       const int s = i % ST, buf = i % C::BUFS;
       bool ok = mbar_wait(&acc_empty[buf], ((uint32_t)(i / C::BUFS) & 1u) ^ 1u, ST_MMA_WAIT, &g_status_f8) &&
                 mbar_wait(&full[s], (uint32_t)(i / ST) & 1u, ST_MMA_WAIT, &g_status_f8);
@@ -388,6 +400,11 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
       }
       __syncwarp();
     }
+    // The last product has completed before the tensor memory goes, or anything is written where the tiles were.  (Where no
+    // wait ran out, the sums have seen it.)
+    if (i > 0) mbar_wait(&acc_full[(i - 1) % C::BUFS], (uint32_t)((i - 1) / C::BUFS) & 1u, ST_MMA_WAIT, &g_status_f8);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(quiet);
     mbar_wait(done, 0u, ST_EPI_WAIT, &g_status_f8);
     tc_fence_after();
     __syncwarp();
@@ -409,6 +426,7 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
 #pragma unroll
         for (int j = 0; j < (DUAL ? 2 : 1) * TN / 2; j++) acc[j] = 0ull;
         bool ok = true;
+        uint64_t* seen = a.unanswered ? never : acc_full;
         for (int c0 = g0; c0 < g1; c0 += C::CHUNK) {
           const int n = min(C::CHUNK, g1 - c0);
           if (c0 != g0) few_bar<C::SUMMERS>();  // every warp is past the previous scales
@@ -435,7 +453,7 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
           few_bar<C::SUMMERS>();
           for (int k = 0; k < n; k++) {
             const int i = c0 - g0 + k, buf = i % C::BUFS;
-            if (ok) ok = mbar_wait(&acc_full[buf], (uint32_t)(i / C::BUFS) & 1u, ST_EPI_WAIT, &g_status_f8);
+            if (ok) ok = mbar_wait(&seen[buf], (uint32_t)(i / C::BUFS) & 1u, ST_EPI_WAIT, &g_status_f8);
             __syncwarp();
             tc_fence_after();
             const uint32_t d = tmem + lane_base + (uint32_t)(buf * C::COLS + wt);
@@ -444,10 +462,15 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
             if (DUAL) scale_add_cols<TN, C::STEP>(acc + TN / 2, d + NT, s + NT);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            if (lane == 0 && ok) mbar_arrive(&acc_empty[buf]);
           }
         }
         if (lane == 0) mbar_arrive(done);
+        if (!ok) {
+          mbar_wait(quiet, 0u, ST_EPI_WAIT, &g_status_f8);
+#pragma unroll
+          for (int j = 0; j < (DUAL ? 2 : 1) * TN / 2; j++) acc[j] = pair_of(lost(), lost());
+        }
         float* part = (float*)base;  // [COLS][128]: the stages are done with
         few_bar<C::SUMMERS>();       // (every warp has seen the last products)
 #pragma unroll
@@ -534,12 +557,12 @@ struct PairArgs {
 constexpr int kPairStages = 5, kPairStage = 2 * kMmTile, kPairThreads = 128 + 256;
 constexpr int kPairPitch = 36;  // floats of a row of 32 on its way out: 16-byte accesses meet in no bank
 constexpr size_t kPairSmem =
-    1024 + kPairStages * kPairStage + (2 * kPairStages + 4) * 8 + 16 + 2 * 2 * 128 * 4 + 8 * 32 * kPairPitch * 4;
+    1024 + kPairStages * kPairStage + (2 * kPairStages + 6) * 8 + 16 + 2 * 2 * 128 * 4 + 8 * 32 * kPairPitch * 4;
 
 // A warp's 32 rows x 128 sums (row m0 + lane, from column n0 on) go out 32 columns at a time through shared memory, so
 // that the stores of a row lie together whatever its alignment.
 template <int DT>
-__device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* acc, long m0, int n0, float* room, bool ok) {
+__device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* acc, long m0, int n0, float* room) {
   const MmArgs& a = p.m;
   const int lane = threadIdx.x & 31;
   // What is added comes while the sums are laid out; in fp32 the registers reach for two rows at a time only.
@@ -581,13 +604,13 @@ __device__ __forceinline__ void pair_store(const PairArgs& p, const uint64_t* ac
 #pragma unroll
           for (int e = 0; e < 8; e++) v[e] += w[e];
         }
-        if (m0 + r < a.M && ok) store_eight<DT>(a.y, (m0 + r) * a.ldy + n8, eight_of<DT>(v));
+        if (m0 + r < a.M) store_eight<DT>(a.y, (m0 + r) * a.ldy + n8, eight_of<DT>(v));
       }
-    } else if (n + lane < a.N && ok && a.add == nullptr) {  // a column a lane
+    } else if (n + lane < a.N && a.add == nullptr) {  // a column a lane
 #pragma unroll 2
       for (int r = 0; r < 32; r++)
         if (m0 + r < a.M) store_f32_as<DT>(a.y, (m0 + r) * a.ldy + n + lane, room[r * kPairPitch + lane]);
-    } else if (n + lane < a.N && ok) {
+    } else if (n + lane < a.N) {
       // with what is added, eight rows at a time: 6206 x 1423 x 4519 fp32 93 us, 219 two at a time
       for (int r0 = 0; r0 < 32 && m0 + r0 < a.M; r0 += 8) {
         float w[8];
@@ -656,7 +679,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint64_t* empty = full + kPairStages;
   uint64_t* acc_full = empty + kPairStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;        // [2], used in the first CTA
-  uint32_t* slot = (uint32_t*)(acc_empty + 2);
+  uint64_t* never = acc_empty + 2;           // [2]
+  uint32_t* slot = (uint32_t*)(never + 2);
   float* s_amax = (float*)(slot + 4);        // [2][2][128]
   float* s_room = s_amax + 2 * 2 * 128;      // [8 warps][32][kPairPitch]
   const MmArgs& a = p.m;
@@ -671,6 +695,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     for (int i = 0; i < 2; i++) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 16);  // a warp each of both CTAs' eight
+      mbar_init(&never[i], 1);
     }
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
@@ -754,7 +779,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const uint32_t bar_empty = mapa(smem_u32(acc_empty), 0);
     const int nblocks = (a.N + 127) / 128;
     int it = 0, round = 0;
-    bool ok = true;  // a wait that ran out ends the waiting, but no warp leaves the others alone at a barrier
+    bool ok = true;
+    uint64_t* seen = a.unanswered ? never : acc_full;
     // Scales are fetched a group ahead, a tile's first before the last one's results go out.  A row that is not there
     // takes the first one's, and nothing of it is stored.
     int mt, nt;
@@ -777,13 +803,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int j = 0; j < 64; j++) acc[j] = 0ull;
       for (int i = 0; i < a.G; i++, it++) {
         const int buf = it & 1;
-        const float s0 = na * nb0, s1 = SWIGLU ? na * nb1 : s0;
+        float s0 = na * nb0, s1 = SWIGLU ? na * nb1 : s0;
         if (i + 1 < a.G) {
           na = __ldg(sa += a.sa_g);
           nb0 = __ldg(sb += a.sb_g);
           if (SWIGLU) nb1 = __ldg(sb1 += p.sb1_g);
         }
-        if (ok) ok = mbar_wait(&acc_full[buf], (uint32_t)(it >> 1) & 1u, ST_EPI_WAIT, &g_status_f8);
+        if (ok) ok = mbar_wait(&seen[buf], (uint32_t)(it >> 1) & 1u, ST_EPI_WAIT, &g_status_f8);
+        if (!ok) s0 = s1 = lost();
         __syncwarp();
         tc_fence_after();
         const uint32_t d = tmem + lane_base + (uint32_t)(buf * 256);
@@ -793,15 +820,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         tmem_ld_x64(d + c1, v);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(bar_empty + 8 * buf);  // before the rest is added: the products wait for it
+        if (lane == 0 && ok) mbar_arrive_cluster(bar_empty + 8 * buf);  // before the rest is added: the products wait for it
         scale_add(acc + 32, v, s1);
       }
       const int m = mt * 256 + (int)rank * 128 + r, n = nt;
       if (t + pairs < tiles) begin(t + pairs);
       if (SWIGLU)
-        pair_store_swiglu(p, acc, m, m < a.M && ok, n * 128 + 64 * h, n, h, r, warp & 3, s_amax + (round & 1) * 256);
+        pair_store_swiglu(p, acc, m, m < a.M, n * 128 + 64 * h, n, h, r, warp & 3, s_amax + (round & 1) * 256);
       else
-        pair_store<DT>(p, acc, m - lane, n * 256 + 128 * h, s_room + (warp - 4) * 32 * kPairPitch, ok);
+        pair_store<DT>(p, acc, m - lane, n * 256 + 128 * h, s_room + (warp - 4) * 32 * kPairPitch);
     }
   }
   tc_fence_before();
@@ -824,6 +851,8 @@ static int check_operand(const char* what, const Operand& o, long rows, int K) {
                "%s: rows of %d bytes, %ld apart (a multiple of 16)", what, K, (long)o.ld);
   return RNGD_OK;
 }
+static std::atomic<int> g_unanswered{0};  // rngd_f8_unanswered
+
 // rows x K bytes, rows ld apart, read in boxes of 128 bytes x `box` rows; zeros beyond the edges
 static int operand_map(const Operand& o, long rows, int K, int box, CUtensorMap* out) {
   const uint64_t dims[2] = {(uint64_t)K, (uint64_t)rows};
@@ -905,7 +934,8 @@ static int few_launch_nt(const Operand& a, const Operand& b, const Operand* b1, 
 static int few_launch(const Operand& a, const Operand& b, const Operand* b1, int M, int N, int K, const void* add,
                       long ldadd, void* y, long ldy, int dtype, uint8_t* q, long ldq, float* scale, cudaStream_t s) {
   FewArgs p = {};
-  p.m = {M, N, K, (K + 127) / 128, a.scale, (long)a.s0, (long)a.s1, b.scale, (long)b.s0, (long)b.s1, y, ldy, add, ldadd};
+  p.m = {M, N, K, (K + 127) / 128, a.scale, (long)a.s0, (long)a.s1, b.scale, (long)b.s0, (long)b.s1, y, ldy, add, ldadd,
+         g_unanswered.load(std::memory_order_relaxed)};
   p.vec = whole_rows(y, ldy, add, ldadd, dtype);
   p.q = q;
   p.ldq = ldq;
@@ -937,7 +967,8 @@ static int pair_launch(const Operand& a, const Operand& b, const Operand* b1, in
   tb1 = tb;
   if (b1 != nullptr) RNGD_TRY(operand_map(*b1, N, K, 128, &tb1));
   PairArgs p = {};
-  p.m = {M, N, K, (K + 127) / 128, a.scale, (long)a.s0, (long)a.s1, b.scale, (long)b.s0, (long)b.s1, y, ldy, add, ldadd};
+  p.m = {M, N, K, (K + 127) / 128, a.scale, (long)a.s0, (long)a.s1, b.scale, (long)b.s0, (long)b.s1, y, ldy, add, ldadd,
+         g_unanswered.load(std::memory_order_relaxed)};
   if (b1 != nullptr) {
     p.sb1 = b1->scale;
     p.sb1_n = (long)b1->s0;
@@ -986,6 +1017,11 @@ int read_status_f8(int* st, int reset) {
 }  // namespace rngd
 
 using namespace rngd;
+
+extern "C" int rngd_f8_unanswered(int on) {
+  g_unanswered.store(on != 0, std::memory_order_relaxed);
+  return RNGD_OK;
+}
 
 extern "C" int rngd_f8_matmul(const void* a, int64_t lda, const float* a_scale, const int64_t* a_strides, const void* b,
                               int64_t ldb, const float* b_scale, const int64_t* b_strides, int M, int N, int K,
