@@ -105,7 +105,8 @@ int rngd_decode_workspace(const rngd_model_t* m, int S, size_t* partial_floats, 
 /* Size of io->attn_part for streams 0..Bcap-1 (Bcap <= 16) of S cache positions: chunk
  * records of the fused decode attention plus an epoch per (stream, kv head). */
 int rngd_decode_attn_workspace(const rngd_model_t* m, int Bcap, int S, size_t* attn_units);
-/* Device status word of the bounded waits (0 = none timed out); reset clears it. */
+/* Device status word of the bounded waits (0 = none timed out); reset clears it.  The 8-bit products have their own
+ * (rngd_f8_status). */
 int rngd_device_status(int* status, int reset);
 
 /* x = embed[toks] (engines/decode_batch.py:432), plus the first layer's
@@ -416,6 +417,9 @@ int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, const int64
                    int64_t ldg, const float* gate_scale, const int64_t* gate_strides, const void* up, int64_t ldu,
                    const float* up_scale, const int64_t* up_strides, int M, int N, int K, void* q, int64_t ldq,
                    float* scale, rngd_stream_t stream);
+/* Device status word of the 8-bit products' bounded waits (0 = none timed out), apart from rngd_device_status; reset
+ * clears it.  Results of a call whose wait timed out are NaN. */
+int rngd_f8_status(int* status, int reset);
 /* For tests of what a host does when a device wait runs out.  While it is on, every rngd_f8_matmul and rngd_f8_swiglu
  * that is launched waits for something that never comes: each gives up after the waits' limit (2 s), its results are NaN
  * as always then, and the status word says so. */

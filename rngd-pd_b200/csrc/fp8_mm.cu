@@ -1005,18 +1005,20 @@ static bool pairs_pay(int M, int N, int K, bool dual) {
   return waves * (18 + G) <= f.waves * (18 + (G + f.split - 1) / f.split);
 }
 
-int read_status_f8(int* st, int reset) {
-  RNGD_TRY(check_cuda(cudaMemcpyFromSymbol(st, g_status_f8, sizeof(int)), "read device status"));
+}  // namespace rngd
+
+using namespace rngd;
+
+// A word of its own: whoever uses the engines reads and clears theirs (rngd_device_status).
+extern "C" int rngd_f8_status(int* status, int reset) {
+  RNGD_REQUIRE(status != nullptr, "f8_status: null output");
+  RNGD_TRY(check_cuda(cudaMemcpyFromSymbol(status, g_status_f8, sizeof(int)), "read device status"));
   if (reset) {
     const int zero = 0;
     RNGD_TRY(check_cuda(cudaMemcpyToSymbol(g_status_f8, &zero, sizeof(int)), "reset device status"));
   }
   return RNGD_OK;
 }
-
-}  // namespace rngd
-
-using namespace rngd;
 
 extern "C" int rngd_f8_unanswered(int on) {
   g_unanswered.store(on != 0, std::memory_order_relaxed);

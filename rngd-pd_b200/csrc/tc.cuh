@@ -256,7 +256,6 @@ int read_status_decode(int* st, int reset);
 int read_status_prefill(int* st, int reset);
 int read_status_attn(int* st, int reset);
 int read_status_kv4(int* st, int reset);
-int read_status_f8(int* st, int reset);
 size_t attn_fused_scratch_units(int Bcap, int NKV, int S);
 
 // Shared host helpers (decode_tc.cu): SM count, cached tensor maps for weight

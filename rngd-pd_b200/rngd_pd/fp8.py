@@ -15,7 +15,11 @@ be laid out like that too.
 Everything lives on the tensors' GPU; calls are queued on the current stream and wait for nothing, so they can
 be captured into a CUDA graph.  As with torch's own operators, a tensor made on another stream has to be
 ordered before the call by the caller (and kept alive with record_stream).  Nothing falls back to the CPU.
+
+The products' kernels wait for their own copies, 2 s at most.  Where such a wait runs out the call's results are NaN and
+device_status() says so, whatever the engines' own status (BeamDecodeEngine.result) reads and clears.
 """
+import ctypes
 import functools
 
 import torch
@@ -224,3 +228,12 @@ def matmul_swiglu(a, a_scale, gate, gate_scale, up, up_scale):
     _check(_swiglu(ap, lda, a_scale.data_ptr(), ast, gp, ldg, gate_scale.data_ptr(), gst, up_, ldu, up_scale.data_ptr(),
                    ust, M, N, K, q.data_ptr(), st[0], scale.data_ptr(), _stream(dev.index)))
     return q, scale
+
+
+def device_status(reset=True):
+    """Status word of the products' device waits on the current GPU: 0, or the code of the first one that ran out since it
+    was last cleared (reset: by this call).  Waits for the GPU; not for use under graph capture."""
+    st = ctypes.c_int(0)
+    torch.cuda.synchronize()
+    _lib.call("rngd_f8_status", ctypes.byref(st), 1 if reset else 0)
+    return st.value

@@ -128,3 +128,7 @@ def test_the_greatest_sizes_pass_the_checks():
     assert fp8._source("x", (1, n), (n, 1), torch.bfloat16, dev)[2:4] == (1, n)
     n = 2 ** 31 - 256
     assert fp8._operand("b", ((n, 1), (16, 1), e4m3, dev), ((n // 128, 1), (1, 1), f32, dev), True)[0] == n
+
+
+def test_status_entries_refuse_null():
+    assert _lib.lib.rngd_f8_status(None, 1) == _lib.RNGD_ERR_ARG and "null" in _lib.last_error()
