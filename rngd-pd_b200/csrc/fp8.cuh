@@ -57,6 +57,15 @@ __device__ __forceinline__ void store_f32_as(void* p, long i, float v) {
   else
     ((float*)p)[i] = v;
 }
+template <int DT>
+__device__ __forceinline__ float rounded_to(float v) {
+  if constexpr (DT == F8_BF16)
+    return bf2f(f2bf_bits(v));
+  else if constexpr (DT == F8_F16)
+    return __half2float(__float2half_rn(v));
+  else
+    return v;
+}
 // Eight values from a 16-byte aligned place: the registers that hold them, and their values.
 template <int DT>
 struct Eight {

@@ -167,7 +167,8 @@ def rms_norm(x, weight, eps, residual=None):
 
     x, residual: [T, K] of one type (rows contiguous); weight: [K] of that type or float32.  total = x + residual
     rounded to their type, the residual stream as it goes on (None without a residual); the norm is of the rounded
-    sum, total / sqrt(mean(total^2) + eps) * weight, worked out in fp32 and rounded to 8 bits alone."""
+    sum, total / sqrt(mean(total^2) + eps) * weight, worked out in fp32 (rows whose squares leave its range by values times
+    a power of two) and rounded to 8 bits alone."""
     dev, dtype = x.device, x.dtype
     ld, dt, T, K, st, s_st, G = _source("x", x.shape, x.stride(), dtype, dev)
     wt = weight.dtype
