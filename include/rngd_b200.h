@@ -417,6 +417,9 @@ int rngd_f8_swiglu(const void* a, int64_t lda, const float* a_scale, const int64
                    int64_t ldg, const float* gate_scale, const int64_t* gate_strides, const void* up, int64_t ldu,
                    const float* up_scale, const int64_t* up_strides, int M, int N, int K, void* q, int64_t ldq,
                    float* scale, rngd_stream_t stream);
+/* Rows of a in the tiles of the kernel that a product of these sizes takes (gated: rngd_f8_swiglu's), for profiles and
+ * tests: 256 of pairs of CTAs, 16, 32, 64 or 128 of the kernel for few rows. */
+int rngd_f8_tile_rows(int M, int N, int K, int gated, int* rows);
 /* Device status word of the 8-bit products' bounded waits (0 = none timed out), apart from rngd_device_status; reset
  * clears it.  Results of a call whose wait timed out are NaN. */
 int rngd_f8_status(int* status, int reset);

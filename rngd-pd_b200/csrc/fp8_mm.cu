@@ -872,6 +872,7 @@ static int whole_rows(const void* y, long ldy, const void* add, long ldadd, int 
 struct FewPlan {
   long tiles, waves;
   int split;
+  bool two;  // blocks an SM
 };
 static int few_rows(int M, bool dual) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 || dual ? 64 : 128; }
 static FewPlan few_plan(int M, int N, int G, bool dual) {
@@ -881,7 +882,7 @@ static FewPlan few_plan(int M, int N, int G, bool dual) {
   static_assert(FewCfg<16, true>::PER_SM == 2 && FewCfg<32, true>::PER_SM == 1 && FewCfg<64, true>::PER_SM == 1, "");
   static_assert(FewCfg<16, false>::PER_SM == 2 && FewCfg<32, false>::PER_SM == 2 && FewCfg<64, false>::PER_SM == 2 &&
                     FewCfg<128, false>::PER_SM == 1, "");
-  FewPlan f = {((long)N + 127) / 128 * (((long)M + rows - 1) / rows), 0, 1};
+  FewPlan f = {((long)N + 127) / 128 * (((long)M + rows - 1) / rows), 0, 1, two};
   while (f.split < 8 && f.tiles * f.split * 2 <= places && f.split * 8 <= G) f.split *= 2;
   f.waves = (f.tiles * f.split + places - 1) / places;
   return f;
@@ -995,19 +996,30 @@ static int pair_launch(const Operand& a, const Operand& b, const Operand* b1, in
 
 // Which of the two kernels: a wave of either takes about 7 us and 0.4 us for each of its groups (256 rows a tile of the
 // pairs', 64 or 128 of the other, whose K may be cut).  Measured over 65 to 2000 rows, N from 300 to 28000 and K from 300
-// to 8192 this takes the faster one but for ties within a tenth: 200 x 4096 x 4096 20 us by pairs, 14 by the other;
-// 1000 x 4096 x 4096 21 and 40.
+// to 8192 this takes the faster one but for ties within a fifth: 200 x 4096 x 4096 20 us by pairs, 14 by the other;
+// 1000 x 4096 x 4096 21 and 40.  With so few rows that two blocks fit an SM the other kernel's wave is shorter, and a tie
+// is its: 1 x 4864 x 896 8.2 us by pairs, 3.9 by the other; 64 x 896 x 512 6.6 and 5.2; gate and up 16 x 4864 x 896 8.0
+// and 5.9 (32 rows, one block an SM, 8.1 and 7.5, but 32 x 128 x 512 5.5 and 5.8).
 static bool pairs_pay(int M, int N, int K, bool dual) {
   const int G = (K + 127) / 128;
   const FewPlan f = few_plan(M, N, G, dual);
   const long tiles = ((long)M + 255) / 256 * (((long)N + (dual ? 127 : 255)) / (dual ? 128 : 256));
   const long pairs = num_sms() / 2, waves = (tiles + pairs - 1) / pairs;
-  return waves * (18 + G) <= f.waves * (18 + (G + f.split - 1) / f.split);
+  const long by_pairs = waves * (18 + G), by_few = f.waves * (18 + (G + f.split - 1) / f.split);
+  return by_pairs < by_few || (by_pairs == by_few && !f.two);
 }
 
 }  // namespace rngd
 
 using namespace rngd;
+
+extern "C" int rngd_f8_tile_rows(int M, int N, int K, int gated, int* rows) {
+  RNGD_REQUIRE(rows != nullptr, "f8_tile_rows: null output");
+  RNGD_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M <= kMostRows && N <= kMostRows && K <= kMostK, "f8_tile_rows: %d x %d x %d",
+               M, N, K);
+  *rows = pairs_pay(M, N, K, gated != 0) ? 256 : few_rows(M, gated != 0);
+  return RNGD_OK;
+}
 
 // A word of its own: whoever uses the engines reads and clears theirs (rngd_device_status).
 extern "C" int rngd_f8_status(int* status, int reset) {

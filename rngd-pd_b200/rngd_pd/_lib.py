@@ -163,6 +163,7 @@ _sig("rngd_f8_rms_norm", _vp, _i64, _vp, _i64, _vp, _int, _int, _i64, _int, ctyp
 _sig("rngd_f8_matmul", _vp, _i64, _vp, _i64p, _vp, _i64, _vp, _i64p, _int, _int, _int, _vp, _i64, _vp, _i64, _int, _vp)
 _sig("rngd_f8_swiglu", _vp, _i64, _vp, _i64p, _vp, _i64, _vp, _i64p, _vp, _i64, _vp, _i64p, _int, _int, _int, _vp,
      _i64, _vp, _vp)
+_sig("rngd_f8_tile_rows", _int, _int, _int, _int, ctypes.POINTER(_int))
 _sig("rngd_f8_status", ctypes.POINTER(_int), _int)
 _sig("rngd_f8_unanswered", _int)
 

@@ -130,5 +130,25 @@ def test_the_greatest_sizes_pass_the_checks():
     assert fp8._operand("b", ((n, 1), (16, 1), e4m3, dev), ((n // 128, 1), (1, 1), f32, dev), True)[0] == n
 
 
+def _tile_rows(M, N, K, gated=0):
+    n = ctypes.c_int(0)
+    assert _lib.lib.rngd_f8_tile_rows(M, N, K, gated, ctypes.byref(n)) == 0
+    return n.value
+
+
+def test_few_rows_take_the_kernel_for_few_rows():
+    """Also where K is too short to be cut, so that either kernel has one wave."""
+    for N in (1, 128, 896, 4864, 18944):
+        for K in (1, 128, 512, 896, 1100, 4096):
+            assert [_tile_rows(M, N, K) for M in (1, 16, 17, 32, 33, 64)] == [16, 16, 32, 32, 64, 64]
+            assert [_tile_rows(M, N, K, 1) for M in (1, 16)] == [16, 16]
+    assert _tile_rows(128, 4096, 4096) == 128 and _tile_rows(33, 14336, 4096, 1) == 64
+    assert _tile_rows(333, 6144, 4096) == 256 and _tile_rows(8192, 4096, 14336) == 256
+    n = ctypes.c_int(0)
+    for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, 2 ** 30 + 1)):
+        assert _lib.lib.rngd_f8_tile_rows(*bad, 0, ctypes.byref(n)) == _lib.RNGD_ERR_ARG
+    assert _lib.lib.rngd_f8_tile_rows(1, 1, 1, 0, None) == _lib.RNGD_ERR_ARG and "null" in _lib.last_error()
+
+
 def test_status_entries_refuse_null():
     assert _lib.lib.rngd_f8_status(None, 1) == _lib.RNGD_ERR_ARG and "null" in _lib.last_error()
