@@ -407,7 +407,8 @@ int rngd_f8_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t l
                      float* scale, rngd_stream_t stream);
 /* y[m][n] = sum over k of a[m][k] b[n][k] as they stand, plus add[m][n] (of y's type; NULL: nothing), summed in
  * fp32 and rounded once to dtype.  a: rows [M][K] with scales [M][G]; b: a weight [N][K] with scales
- * [ceil(N / 128)][G]; strides of the scales' two dimensions in elements.  add may be y. */
+ * [ceil(N / 128)][G]; strides of the scales' two dimensions in elements.  A row's scale times a block's is held in fp32
+ * and should be one of its normal numbers.  add may be y. */
 int rngd_f8_matmul(const void* a, int64_t lda, const float* a_scale, const int64_t* a_strides, const void* b,
                    int64_t ldb, const float* b_scale, const int64_t* b_strides, int M, int N, int K, const void* add,
                    int64_t ldadd, void* y, int64_t ldy, int dtype, rngd_stream_t stream);

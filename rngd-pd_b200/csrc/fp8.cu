@@ -4,8 +4,9 @@
 // launch where there are few.  The rows of the result start on 16 bytes whatever their width (the caller's row stride),
 // as the products' tile loads want them.  Measured, inputs larger than the L2 cache: rows 8191 x 4096 bf16 16.4 us, 6.2
 // TB/s; weight 14336 x 4096 bf16 28.6 us, 6.2 TB/s; norm 8192 x 4096 bf16 with a residual 38.3 us, 6.2 TB/s (the copy
-// rate is 6.55).  Rows of 4097 values, which start anywhere: 8000 of them in bf16 25 us, the norm with a residual 98:
-// more instructions a value, and fewer blocks an SM.
+// rate is 6.55).  Rows of 4097 values, which start anywhere: 8000 of them in bf16 26 us, the norm with a residual 98:
+// eight values come as one aligned vector more than they fill, which the neighbouring lane asks the L2 cache for too, and
+// are shifted into place; more instructions a value, and fewer blocks an SM.
 #include "fp8.cuh"
 #include "tc.cuh"
 
@@ -352,7 +353,9 @@ template <bool VEC>
 constexpr int kNormThreads = VEC ? 512 : 384;  // 384: at 80 registers two blocks' warps fit an SM's quarters
 // The next row is on its way while the present one is summed and rounded, and the weights stay in registers.  (Only where
 // rows are whole vectors: the others' registers go further as a second block an SM; 8000 x 4097 bf16 with a residual
-// takes 98 us, 121 with the next row on its way.)
+// takes 98 us, 121 with the next row on its way.)  What two runs of groups a thread (PER = 2) need is more than the
+// registers: rows that start anywhere keep some 300 bytes a thread in local memory then, fp32 ones 432 (2000 x 12001 fp16
+// with a residual 103 us, 1.6 TB/s), fp32 rows in whole vectors 112 (3000 x 12288 129 us, 3.7 TB/s).
 template <int DT, int WT, bool VEC, int PER>
 __global__ void __launch_bounds__(kNormThreads<VEC>, VEC ? 0 : 2) f8_norm_kernel(NormArgs a) {
   __shared__ float s_sum[2][32];  // for each of two rows in turn

@@ -187,8 +187,8 @@ constexpr int kMmTile = 128 * 128;  // bytes of 128 rows of a group
 //
 // 16 x 128256 x 4096 with an fp32 result: 83 us, 6.4 TB/s, 0.98 of the copy rate.  16 x 14336 x 4096 gate and up: 24.5 us,
 // 4.8 TB/s; 18 at the copy rate, the rest is the way in (scales, first copies) and out (cluster, code that runs once).
-// 1 x 4096 x 4096: 6.7 us, latency.  With 128 rows of a a tile's operands come from the L2 cache at 11 TB/s, which bounds
-// 512 x 4096 x 4096 (19 us).
+// 1 x 4096 x 4096: 6.7 us, latency.  With 128 rows of a every CTA fetches as much of a as of the weight:
+// 128 x 18944 x 4096, one tile an SM, takes 23.8 us, 6.5 TB/s into shared memory; 200 x 4096 x 4096, K cut in two, 14.0 us.
 template <int NT, bool DUAL>
 struct FewCfg {
   static constexpr int A = (DUAL ? 2 : 1) * kMmTile, STAGE = A + NT * 128;
@@ -535,15 +535,15 @@ __global__ void __launch_bounds__(FewCfg<NT, DUAL>::THREADS, FewCfg<NT, DUAL>::P
 // memory (32 KB a group), one thread of the first issues the products of both, and each ends with its own 128
 // rows x 256 columns.  A persistent grid, one CTA per SM.
 //
-// 8192 x 4096 x 14336: 426 us, 2260 TFLOP/s; 4096 x 14336 x 4096 gate and up with SwiGLU and its rounding: 436 us, 2205
-// TFLOP/s (bursts of 30 ms; in longer runs the power limit takes the clock to 1.48 GHz, and they take 510 and 520).  A
-// tile's results take 4000 to 8000 cycles to go out, while the products run two groups ahead.  A
-// group's products take 512 cycles, and 780 to 800 pass for each: the way from them through the eight warps that add
-// them up (two tensor memory reads of 85 cycles and 128 multiply-adds each, two warps a quarter of the SM) and back is
-// longer than the other buffer's products.  Tried: products of 128 columns with barriers of their own (they run at half
-// the rate, by shared memory's bandwidth: 472 us where this took 457), sixteen warps of 64 columns (518 where eight
-// took 467), multiply-adds of one column (509 where two at a time took 463).  The sums and what is read take 192
-// registers; with 224 a thread instead of 232 the compiler moves them about (484 us where 232 took 427).
+// 8192 x 4096 x 14336: 507 to 516 us, 1900 to 1865 TFLOP/s, in runs of a second and more, which the power limit holds to
+// 1.37 to 1.53 GHz; 430 us in bursts of 30 ms.  4096 x 14336 x 4096 gate and up with SwiGLU and its rounding: 516 to 527
+// us, 1865 to 1825 TFLOP/s, and 440 to 460.  A tile's results take 4000 to 8000 cycles to go out, while the products run
+// two groups ahead.  A group's products take 512 cycles, and 780 to 800 pass for each: the way from them through the
+// eight warps that add them up (two tensor memory reads of 85 cycles and 128 multiply-adds each, two warps a quarter of
+// the SM) and back is longer than the other buffer's products.  Tried: products of 128 columns with barriers of their own
+// (they run at half the rate, by shared memory's bandwidth: 472 us in bursts where this took 457), sixteen warps of 64
+// columns (518 where eight took 467), multiply-adds of one column (509 where two at a time took 463).  The sums and what
+// is read take 192 registers; with 224 a thread instead of 232 the compiler moves them about (484 us where 232 took 427).
 struct PairArgs {
   MmArgs m;
   const float* sb1;  // of the second weight (SWIGLU)

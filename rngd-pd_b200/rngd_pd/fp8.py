@@ -8,9 +8,10 @@ what a prompt's goes by.
   weight  float8_e4m3fn [N, K], scale float32 [ceil(N / 128), G]: one for each block of 128 x 128
 
 With m = max(amax, 2^-100) of a group, scale = m / 448 and a value x is held as e4m3(x * (448 / m)).  A group with a
-NaN or an infinity reads as NaN.  Rows start on 16 bytes: where K is no multiple of 16, the tensors that quantize,
-quantize_weight, rms_norm and matmul_swiglu return are views of wider ones, and operands that a caller brings have to
-be laid out like that too.
+NaN or an infinity reads as NaN.  The products hold a row's scale times a block's in fp32: but for groups of zeros the two
+should multiply to one of its normal numbers (magnitudes of a and b to between 1e-32 and 1e43).  Rows start on 16 bytes:
+where K is no multiple of 16, the tensors that quantize, quantize_weight, rms_norm and matmul_swiglu return are views of
+wider ones, and operands that a caller brings have to be laid out like that too.
 
 Everything lives on the tensors' GPU; calls are queued on the current stream and wait for nothing, so they can
 be captured into a CUDA graph.  As with torch's own operators, a tensor made on another stream has to be
